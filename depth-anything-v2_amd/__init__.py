@@ -138,6 +138,73 @@ class ConvF32Args(C.Structure):
                 ("flags", C.c_uint32), ("out", C.c_void_p), ("residual", C.c_void_p)]
 
 
+# the decoder operators' argument blocks (include/dav2_hip.h)
+DTYPE = {"f32": 0, "f16": 1, "bf16": 2}
+ROTARY_LAYOUT = {"halves": 0, "pairs": 1}
+ROTARY_SCALING = {"none": 0, "linear": 1, "base": 2, "wavelength": 3}
+QK_NORM = {"rms": 0, "layer": 1}
+
+
+class RotaryArgs(C.Structure):
+    _fields_ = [("input", C.c_void_p), ("output", C.c_void_p), ("input_stride", C.c_uint64),
+                ("output_stride", C.c_uint64), ("positions", C.c_void_p), ("frequencies", C.c_void_p),
+                ("tokens", C.c_uint32), ("heads", C.c_uint32), ("head_dim", C.c_uint32), ("rotary_dim", C.c_uint32),
+                ("layout", C.c_uint32), ("dtype", C.c_uint32), ("amplitude", C.c_float)]
+
+
+class QkNormRotaryArgs(C.Structure):
+    _fields_ = [("query", C.c_void_p), ("key", C.c_void_p), ("query_out", C.c_void_p), ("key_out", C.c_void_p),
+                ("query_stride", C.c_uint64), ("key_stride", C.c_uint64), ("query_out_stride", C.c_uint64),
+                ("key_out_stride", C.c_uint64), ("query_weight", C.c_void_p), ("key_weight", C.c_void_p),
+                ("positions", C.c_void_p), ("frequencies", C.c_void_p), ("tokens", C.c_uint32),
+                ("query_heads", C.c_uint32), ("key_heads", C.c_uint32), ("head_dim", C.c_uint32),
+                ("rotary_dim", C.c_uint32), ("layout", C.c_uint32), ("dtype", C.c_uint32), ("norm", C.c_uint32),
+                ("epsilon", C.c_float), ("amplitude", C.c_float)]
+
+
+class RotaryScaling(C.Structure):
+    _fields_ = [("kind", C.c_uint32), ("factor", C.c_double), ("original_length", C.c_double),
+                ("low_turns", C.c_double), ("high_turns", C.c_double)]
+
+
+class CacheI8(C.Structure):
+    _fields_ = [("keys", C.c_void_p), ("values", C.c_void_p), ("key_scales", C.c_void_p),
+                ("value_scales", C.c_void_p), ("pages", C.c_uint32), ("kv_heads", C.c_uint32),
+                ("page_size", C.c_uint32), ("head_dim", C.c_uint32)]
+
+
+class CacheStoreI8Args(C.Structure):
+    _fields_ = [("cache", CacheI8), ("keys", C.c_void_p), ("values", C.c_void_p), ("key_stride", C.c_uint64),
+                ("value_stride", C.c_uint64), ("page_table", C.c_void_p), ("starts", C.c_void_p),
+                ("lengths", C.c_void_p), ("sequences", C.c_uint32), ("table_pages", C.c_uint32),
+                ("tokens", C.c_uint32), ("max_new", C.c_uint32), ("dtype", C.c_uint32)]
+
+
+class AttentionCacheI8Args(C.Structure):
+    _fields_ = [("cache", CacheI8), ("query", C.c_void_p), ("output", C.c_void_p), ("query_stride", C.c_uint64),
+                ("output_stride", C.c_uint64), ("page_table", C.c_void_p), ("starts", C.c_void_p),
+                ("lengths", C.c_void_p), ("sequences", C.c_uint32), ("table_pages", C.c_uint32),
+                ("tokens", C.c_uint32), ("heads", C.c_uint32), ("max_query", C.c_uint32), ("max_length", C.c_uint32),
+                ("causal", C.c_uint32), ("dtype", C.c_uint32), ("scale", C.c_float), ("scratch", C.c_void_p),
+                ("scratch_bytes", C.c_uint64)]
+
+
+class CrossAttentionArgs(C.Structure):
+    _fields_ = [("query", C.c_void_p), ("keys", C.c_void_p), ("values", C.c_void_p), ("output", C.c_void_p),
+                ("query_stride", C.c_uint64), ("key_stride", C.c_uint64), ("value_stride", C.c_uint64),
+                ("output_stride", C.c_uint64), ("query_batch_stride", C.c_uint64), ("key_batch_stride", C.c_uint64),
+                ("value_batch_stride", C.c_uint64), ("output_batch_stride", C.c_uint64), ("key_lengths", C.c_void_p),
+                ("key_mask", C.c_void_p), ("batch", C.c_uint32), ("query_tokens", C.c_uint32),
+                ("key_tokens", C.c_uint32), ("heads", C.c_uint32), ("kv_heads", C.c_uint32),
+                ("head_dim", C.c_uint32), ("dtype", C.c_uint32), ("scale", C.c_float), ("scratch", C.c_void_p),
+                ("scratch_bytes", C.c_uint64)]
+
+
+class OpsCacheInt8(C.Structure):
+    _fields_ = [("keys", DeviceBuffer), ("values", DeviceBuffer), ("key_scales", DeviceBuffer),
+                ("value_scales", DeviceBuffer)]
+
+
 CONV_RELU_INPUT, CONV_RELU_OUTPUT, CONV_EMIT_ABSMAX, CONV_EMIT_RELU_MAX = 1, 2, 4, 8
 
 
@@ -235,6 +302,13 @@ PROTOTYPES = {
     "dav2_hip_preprocess_rgba8": (C.c_int, [vp, u32, u32, u64, u32, u32, u32, vp, vp]),
     "dav2_hip_position_bicubic": (C.c_int, [vp, vp, u32, u32, u32, vp]),
     "dav2_hip_finish_tokens": (C.c_int, [vp, vp, vp, vp, u32, u32, u32, u32, vp]),
+    "dav2_hip_rotary": (C.c_int, [vp, vp]),
+    "dav2_hip_qk_norm_rotary": (C.c_int, [vp, vp]),
+    "dav2_hip_cache_store_i8": (C.c_int, [vp, vp]),
+    "dav2_hip_attention_cache_i8_scratch_bytes": (u64, [vp]),
+    "dav2_hip_attention_cache_i8": (C.c_int, [vp, vp]),
+    "dav2_hip_cross_attention_scratch_bytes": (u64, [vp]),
+    "dav2_hip_cross_attention": (C.c_int, [vp, vp]),
     "dav2_hip_error_string": (C.c_char_p, [C.c_int]),
     # operator surface
     "dav2_ops_create": (vp, [i32]),
@@ -262,6 +336,12 @@ PROTOTYPES = {
     "dav2_ops_relu": (C.c_int, [vp, DB, DB, u32]),
     "dav2_ops_add": (C.c_int, [vp, DB, DB, DB, u32]),
     "dav2_ops_gelu": (C.c_int, [vp, DB, DB, u32]),
+    "dav2_ops_rotary_frequencies": (C.c_int, [vp, u32, C.c_double, vp]),
+    "dav2_ops_rotary": (C.c_int, [vp, DB, DB, DB, DB, vp]),
+    "dav2_ops_qk_norm_rotary": (C.c_int, [vp, DB, DB, DB, DB, DB, DB, DB, DB, vp]),
+    "dav2_ops_cache_store_int8": (C.c_int, [vp, OpsCacheInt8, DB, DB, DB, DB, DB, vp]),
+    "dav2_ops_attention_cache_int8": (C.c_int, [vp, DB, DB, OpsCacheInt8, DB, DB, DB, DB, vp]),
+    "dav2_ops_cross_attention": (C.c_int, [vp, DB, DB, DB, DB, DB, DB, DB, vp]),
     "dav2_infer_tensor_f32_device_logits": (C.c_int, [vp, vp, i32, i32, vp, vp, vp]),
 }
 

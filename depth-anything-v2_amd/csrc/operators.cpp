@@ -1007,4 +1007,199 @@ void HipOperators::gelu(DeviceBuffer& output, const DeviceBuffer& input, std::ui
     hip_check(dav2_hip_gelu(output.as<float>(), input.as<float>(), count, stream()), "gelu");
 }
 
+// ---------------------------------------------------------------------------
+// Operators of a decoder behind the encoder (no reference counterpart).
+namespace {
+
+// What the launcher rejects is the caller's argument; anything else is the device's.
+void launch_check(int error, const char* what) {
+    if (error == hipErrorInvalidValue) throw std::invalid_argument(std::string("invalid ") + what + " arguments");
+    hip_check(error, what);
+}
+
+std::uint64_t element_bytes(std::uint32_t dtype) {
+    if (dtype > DAV2_DTYPE_BF16) throw std::invalid_argument("unknown element type");
+    return dtype == DAV2_DTYPE_F32 ? 4 : 2;
+}
+
+// elements of `size` bytes; the product may not leave 64 bits
+void require_size(const DeviceBuffer& buffer, unsigned __int128 elements, std::uint64_t size, const char* name) {
+    if (elements * size > buffer.size()) throw std::invalid_argument(std::string(name) + " device buffer is too small");
+}
+
+// `count` rows of `row` elements, `stride` apart
+unsigned __int128 strided(std::uint64_t count, std::uint64_t stride, std::uint64_t row) {
+    return count == 0 ? 0 : static_cast<unsigned __int128>(count - 1) * stride + row;
+}
+
+void require_cache(const HipOperators::CacheBuffers& b, const dav2_cache_i8& c) {
+    const auto planes = static_cast<unsigned __int128>(c.pages) * c.kv_heads;
+    const std::uint64_t plane = static_cast<std::uint64_t>(c.page_size) * c.head_dim;
+    if (planes == 0 || plane == 0) throw std::invalid_argument("invalid cache dimensions");
+    require_size(b.keys, planes * plane, 1, "cache keys");
+    require_size(b.values, planes * plane, 1, "cache values");
+    require_size(b.key_scales, planes, sizeof(float), "cache key scales");
+    require_size(b.value_scales, planes, sizeof(float), "cache value scales");
+}
+
+dav2_cache_i8 cache_of(const HipOperators::CacheBuffers& b, dav2_cache_i8 c) {
+    c.keys = b.keys.as<int8_t>();
+    c.values = b.values.as<int8_t>();
+    c.key_scales = b.key_scales.as<float>();
+    c.value_scales = b.value_scales.as<float>();
+    return c;
+}
+
+void require_sequences(const DeviceBuffer& page_table, const DeviceBuffer& starts, const DeviceBuffer& lengths,
+                       std::uint32_t sequences, std::uint32_t table_pages) {
+    require_size(page_table, static_cast<unsigned __int128>(sequences) * table_pages, sizeof(std::int32_t),
+                 "page table");
+    require_size(starts, std::uint64_t(sequences) + 1, sizeof(std::int32_t), "starts");
+    require_size(lengths, sequences, sizeof(std::int32_t), "lengths");
+}
+
+}  // namespace
+
+void HipOperators::rotary(DeviceBuffer& output, const DeviceBuffer& input, const DeviceBuffer& positions,
+                          const DeviceBuffer& frequencies, const dav2_rotary_args& sizes) {
+    dav2_rotary_args a = sizes;
+    if (a.tokens == 0 || a.heads == 0 || a.head_dim == 0) throw std::invalid_argument("invalid rotary dimensions");
+    const std::uint64_t size = element_bytes(a.dtype), row = std::uint64_t(a.heads) * a.head_dim;
+    require_size(input, strided(a.tokens, a.input_stride, row), size, "rotary input");
+    require_size(output, strided(a.tokens, a.output_stride, row), size, "rotary output");
+    require_size(positions, a.tokens, sizeof(std::int32_t), "positions");
+    require_size(frequencies, a.rotary_dim / 2, sizeof(double), "frequencies");
+    a.input = input.data();
+    a.output = output.data();
+    a.positions = positions.as<std::int32_t>();
+    a.frequencies = frequencies.as<double>();
+    ProfileScope prof(context_.profiler(), "rotary", 2.0 * size * row * a.tokens, "B", stream());
+    launch_check(dav2_hip_rotary(&a, stream()), "rotary");
+}
+
+void HipOperators::qk_norm_rotary(DeviceBuffer& query_out, DeviceBuffer& key_out, const DeviceBuffer& query,
+                                  const DeviceBuffer& key, const DeviceBuffer& query_weight,
+                                  const DeviceBuffer& key_weight, const DeviceBuffer& positions,
+                                  const DeviceBuffer& frequencies, const dav2_qk_norm_rotary_args& sizes) {
+    dav2_qk_norm_rotary_args a = sizes;
+    if (a.tokens == 0 || (a.query_heads == 0 && a.key_heads == 0) || a.head_dim == 0)
+        throw std::invalid_argument("invalid query/key norm dimensions");
+    const std::uint64_t size = element_bytes(a.dtype);
+    const std::uint64_t q_row = std::uint64_t(a.query_heads) * a.head_dim, k_row = std::uint64_t(a.key_heads) * a.head_dim;
+    if (a.query_heads) {
+        require_size(query, strided(a.tokens, a.query_stride, q_row), size, "query");
+        require_size(query_out, strided(a.tokens, a.query_out_stride, q_row), size, "query output");
+    }
+    if (a.key_heads) {
+        require_size(key, strided(a.tokens, a.key_stride, k_row), size, "key");
+        require_size(key_out, strided(a.tokens, a.key_out_stride, k_row), size, "key output");
+    }
+    if (query_weight) require_size(query_weight, a.head_dim, sizeof(float), "query norm weight");
+    if (key_weight) require_size(key_weight, a.head_dim, sizeof(float), "key norm weight");
+    if (a.rotary_dim) {
+        require_size(positions, a.tokens, sizeof(std::int32_t), "positions");
+        require_size(frequencies, a.rotary_dim / 2, sizeof(double), "frequencies");
+    }
+    a.query = query.data();
+    a.key = key.data();
+    a.query_out = query_out.data();
+    a.key_out = key_out.data();
+    a.query_weight = query_weight.as<float>();
+    a.key_weight = key_weight.as<float>();
+    a.positions = positions.as<std::int32_t>();
+    a.frequencies = frequencies.as<double>();
+    ProfileScope prof(context_.profiler(), "qk_norm_rotary", 2.0 * size * (q_row + k_row) * a.tokens, "B", stream());
+    launch_check(dav2_hip_qk_norm_rotary(&a, stream()), "query/key norm");
+}
+
+void HipOperators::cache_store_int8(const CacheBuffers& cache, const DeviceBuffer& keys, const DeviceBuffer& values,
+                                    const DeviceBuffer& page_table, const DeviceBuffer& starts,
+                                    const DeviceBuffer& lengths, const dav2_cache_store_i8_args& sizes) {
+    dav2_cache_store_i8_args a = sizes;
+    if (a.sequences == 0 || a.tokens == 0 || a.max_new == 0 || a.table_pages == 0)
+        throw std::invalid_argument("invalid cache store dimensions");
+    require_cache(cache, a.cache);
+    require_sequences(page_table, starts, lengths, a.sequences, a.table_pages);
+    const std::uint64_t size = element_bytes(a.dtype), row = std::uint64_t(a.cache.kv_heads) * a.cache.head_dim;
+    require_size(keys, strided(a.tokens, a.key_stride, row), size, "new keys");
+    require_size(values, strided(a.tokens, a.value_stride, row), size, "new values");
+    a.cache = cache_of(cache, a.cache);
+    a.keys = keys.data();
+    a.values = values.data();
+    a.page_table = page_table.as<std::int32_t>();
+    a.starts = starts.as<std::int32_t>();
+    a.lengths = lengths.as<std::int32_t>();
+    ProfileScope prof(context_.profiler(), "cache_store_i8", 2.0 * (size + 1.0) * row * a.tokens, "B", stream());
+    launch_check(dav2_hip_cache_store_i8(&a, stream()), "cache store");
+}
+
+void* HipOperators::attention_scratch(const DeviceBuffer& given, std::uint64_t need, std::uint64_t& bytes) {
+    bytes = need;
+    if (need == 0) return nullptr;
+    if (given) {
+        if (given.size() < need) throw std::invalid_argument("attention scratch device buffer is too small");
+        return given.data();
+    }
+    hipStreamCaptureStatus capture = hipStreamCaptureStatusNone;
+    hip_check(hipStreamIsCapturing(stream(), &capture), "capture status");
+    if (capture != hipStreamCaptureStatusNone)
+        throw std::invalid_argument("attention under graph capture needs a scratch buffer of its own");
+    return grow(decoder_scratch_, need).data();
+}
+
+void HipOperators::attention_cache_int8(DeviceBuffer& output, const DeviceBuffer& query, const CacheBuffers& cache,
+                                        const DeviceBuffer& page_table, const DeviceBuffer& starts,
+                                        const DeviceBuffer& lengths, const DeviceBuffer& scratch,
+                                        const dav2_attention_cache_i8_args& sizes) {
+    dav2_attention_cache_i8_args a = sizes;
+    if (a.sequences == 0 || a.tokens == 0 || a.max_query == 0 || a.table_pages == 0 || a.heads == 0)
+        throw std::invalid_argument("invalid cache attention dimensions");
+    require_cache(cache, a.cache);
+    require_sequences(page_table, starts, lengths, a.sequences, a.table_pages);
+    const std::uint64_t size = element_bytes(a.dtype), row = std::uint64_t(a.heads) * a.cache.head_dim;
+    require_size(query, strided(a.tokens, a.query_stride, row), size, "query");
+    require_size(output, strided(a.tokens, a.output_stride, row), size, "attention output");
+    a.cache = cache_of(cache, a.cache);
+    a.query = query.data();
+    a.output = output.data();
+    a.page_table = page_table.as<std::int32_t>();
+    a.starts = starts.as<std::int32_t>();
+    a.lengths = lengths.as<std::int32_t>();
+    a.scratch = attention_scratch(scratch, dav2_hip_attention_cache_i8_scratch_bytes(&a), a.scratch_bytes);
+    // at most: every row sees max_length tokens
+    ProfileScope prof(context_.profiler(), "attention_cache_i8", 4.0 * row * a.tokens * a.max_length, "FLOP", stream());
+    launch_check(dav2_hip_attention_cache_i8(&a, stream()), "cache attention");
+}
+
+void HipOperators::cross_attention(DeviceBuffer& output, const DeviceBuffer& query, const DeviceBuffer& keys,
+                                   const DeviceBuffer& values, const DeviceBuffer& key_lengths,
+                                   const DeviceBuffer& key_mask, const DeviceBuffer& scratch,
+                                   const dav2_cross_attention_args& sizes) {
+    dav2_cross_attention_args a = sizes;
+    if (a.batch == 0 || a.query_tokens == 0 || a.heads == 0 || a.kv_heads == 0 || a.head_dim == 0)
+        throw std::invalid_argument("invalid cross attention dimensions");
+    const std::uint64_t size = element_bytes(a.dtype);
+    const std::uint64_t row = std::uint64_t(a.heads) * a.head_dim, key_row = std::uint64_t(a.kv_heads) * a.head_dim;
+    auto batched = [&](std::uint64_t tokens, std::uint64_t stride, std::uint64_t batch_stride, std::uint64_t width) {
+        return tokens == 0 ? 0 : static_cast<unsigned __int128>(a.batch - 1) * batch_stride + strided(tokens, stride, width);
+    };
+    require_size(query, batched(a.query_tokens, a.query_stride, a.query_batch_stride, row), size, "query");
+    require_size(output, batched(a.query_tokens, a.output_stride, a.output_batch_stride, row), size,
+                 "attention output");
+    require_size(keys, batched(a.key_tokens, a.key_stride, a.key_batch_stride, key_row), size, "keys");
+    require_size(values, batched(a.key_tokens, a.value_stride, a.value_batch_stride, key_row), size, "values");
+    if (key_lengths) require_size(key_lengths, a.batch, sizeof(std::int32_t), "key lengths");
+    if (key_mask) require_size(key_mask, std::uint64_t(a.batch) * a.key_tokens, 1, "key mask");
+    a.query = query.data();
+    a.output = output.data();
+    a.keys = keys.data();
+    a.values = values.data();
+    a.key_lengths = key_lengths.as<std::int32_t>();
+    a.key_mask = key_mask.as<std::uint8_t>();
+    a.scratch = attention_scratch(scratch, dav2_hip_cross_attention_scratch_bytes(&a), a.scratch_bytes);
+    ProfileScope prof(context_.profiler(), "cross_attention",
+                      4.0 * row * a.query_tokens * double(a.batch) * a.key_tokens, "FLOP", stream());
+    launch_check(dav2_hip_cross_attention(&a, stream()), "cross attention");
+}
+
 }  // namespace dav2

@@ -16,6 +16,7 @@
 // they compute the same arithmetic as the reference's separate passes.
 #pragma once
 
+#include "dav2_hip.h"
 #include "runtime.h"
 
 #include <cstdint>
@@ -186,6 +187,31 @@ public:
     void add(DeviceBuffer& output, const DeviceBuffer& left, const DeviceBuffer& right, std::uint32_t count);
     void gelu(DeviceBuffer& output, const DeviceBuffer& input, std::uint32_t count);
 
+    // ---- operators of a decoder behind the encoder -----------------------
+    // No reference counterpart. The argument block of the kernel carries the
+    // sizes (dav2_hip.h); its pointers are replaced by the buffers, which are
+    // checked against the sizes. An empty optional buffer is left out; an
+    // empty scratch is the operators' own, which a stream under capture
+    // cannot use.
+    struct CacheBuffers {
+        const DeviceBuffer &keys, &values, &key_scales, &value_scales;
+    };
+    void rotary(DeviceBuffer& output, const DeviceBuffer& input, const DeviceBuffer& positions,
+                const DeviceBuffer& frequencies, const dav2_rotary_args& sizes);
+    void qk_norm_rotary(DeviceBuffer& query_out, DeviceBuffer& key_out, const DeviceBuffer& query,
+                        const DeviceBuffer& key, const DeviceBuffer& query_weight, const DeviceBuffer& key_weight,
+                        const DeviceBuffer& positions, const DeviceBuffer& frequencies,
+                        const dav2_qk_norm_rotary_args& sizes);
+    void cache_store_int8(const CacheBuffers& cache, const DeviceBuffer& keys, const DeviceBuffer& values,
+                          const DeviceBuffer& page_table, const DeviceBuffer& starts, const DeviceBuffer& lengths,
+                          const dav2_cache_store_i8_args& sizes);
+    void attention_cache_int8(DeviceBuffer& output, const DeviceBuffer& query, const CacheBuffers& cache,
+                              const DeviceBuffer& page_table, const DeviceBuffer& starts, const DeviceBuffer& lengths,
+                              const DeviceBuffer& scratch, const dav2_attention_cache_i8_args& sizes);
+    void cross_attention(DeviceBuffer& output, const DeviceBuffer& query, const DeviceBuffer& keys,
+                         const DeviceBuffer& values, const DeviceBuffer& key_lengths, const DeviceBuffer& key_mask,
+                         const DeviceBuffer& scratch, const dav2_cross_attention_args& sizes);
+
     // ---- fused variants used by the graph drivers ------------------------
     // LayerNorm whose output row is quantized straight into the workspace
     // (layer_norm + quantize_rows of linear_int8); fp32 row optional.
@@ -251,6 +277,9 @@ private:
                             std::uint32_t output_row_offset, std::uint32_t output_row_stride, bool output_transposed,
                             bool has_bias, const DeviceBuffer* residual = nullptr, bool relu_output = false);
 
+    // The scratch of an attention call: the caller's, or decoder_scratch_.
+    void* attention_scratch(const DeviceBuffer& given, std::uint64_t need, std::uint64_t& bytes);
+
     HipContext& context_;
     hipStream_t stream_ = nullptr;
     Int8Workspace workspace_;
@@ -266,6 +295,7 @@ private:
     DeviceBuffer conv_weights_;    // packed weights of a conv2d_int8 call that brought none
     DeviceBuffer conv_act_;        // ReLU of a conv2d_int8 input on the im2col path
     DeviceBuffer gemm_split_;      // int32 slices of split-K channel-major GEMMs
+    DeviceBuffer decoder_scratch_; // parts of attention_cache_int8 / cross_attention split over the keys
     DeviceBuffer f32_cols_;        // fp32 im2col rows of the fp32 convolutions
     std::uint32_t workspace_ld_ = 0;  // row stride of the int8 rows currently in the workspace
 };

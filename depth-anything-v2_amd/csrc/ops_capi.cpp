@@ -8,6 +8,7 @@
 
 #include <algorithm>
 #include <atomic>
+#include <cmath>
 #include <memory>
 #include <mutex>
 #include <new>
@@ -49,6 +50,12 @@ dav2_status guard(dav2_ops* ops, Function&& f) {
 }
 
 dav2::DeviceBuffer v(const dav2_device_buffer& b) { return dav2::DeviceBuffer::view(b.data, b.data ? b.bytes : 0); }
+
+template <typename Args>
+const Args& given(const Args* args) {
+    if (args == nullptr) throw std::invalid_argument("the argument block is missing");
+    return *args;
+}
 
 std::uint32_t ld64(std::uint64_t columns) { return static_cast<std::uint32_t>((columns + 63) & ~63ull); }
 
@@ -417,6 +424,94 @@ dav2_status DAV2_CALL dav2_ops_gelu(dav2_ops* ops, dav2_device_buffer output, da
     return guard(ops, [&](dav2::HipOperators& o) {
         auto out = v(output);
         o.gelu(out, v(input), count);
+    });
+}
+
+dav2_status DAV2_CALL dav2_ops_rotary_frequencies(double* frequencies, uint32_t rotary_dim, double base,
+                                                  const dav2_rotary_scaling* scaling) {
+    const dav2_rotary_scaling none{};
+    const dav2_rotary_scaling& c = scaling ? *scaling : none;
+    auto refuse = [](const char* why) {
+        ops_error = why;
+        return DAV2_STATUS_INVALID_ARGUMENT;
+    };
+    // written so that a NaN is refused
+    if (frequencies == nullptr || rotary_dim < 2 || rotary_dim % 2 || !(base > 1.0) || !std::isfinite(base))
+        return refuse("invalid rotary frequencies");
+    if (c.kind > DAV2_ROTARY_SCALING_WAVELENGTH) return refuse("unknown rotary scaling");
+    if (c.kind != DAV2_ROTARY_SCALING_NONE && (!(c.factor >= 1.0) || !std::isfinite(c.factor)))
+        return refuse("invalid rotary scaling factor");
+    if (c.kind == DAV2_ROTARY_SCALING_BASE) {
+        if (rotary_dim < 4) return refuse("rotary base scaling needs two pairs");
+        base *= std::pow(c.factor, rotary_dim / (rotary_dim - 2.0));
+    }
+    if (c.kind == DAV2_ROTARY_SCALING_WAVELENGTH &&
+        (!(c.original_length > 0.0) || !(c.low_turns >= 0.0) || !(c.high_turns > c.low_turns)))
+        return refuse("invalid rotary wavelength scaling");
+    for (uint32_t i = 0; i < rotary_dim / 2; ++i) {
+        double f = std::pow(base, -2.0 * i / rotary_dim);
+        if (c.kind == DAV2_ROTARY_SCALING_LINEAR) f /= c.factor;
+        if (c.kind == DAV2_ROTARY_SCALING_WAVELENGTH) {
+            const double turns = c.original_length * f * 0.15915494309189533577;
+            const double kept = std::min(1.0, std::max(0.0, (turns - c.low_turns) / (c.high_turns - c.low_turns)));
+            f *= kept + (1.0 - kept) / c.factor;
+        }
+        frequencies[i] = f;
+    }
+    return DAV2_STATUS_OK;
+}
+
+dav2_status DAV2_CALL dav2_ops_rotary(dav2_ops* ops, dav2_device_buffer output, dav2_device_buffer input,
+                                      dav2_device_buffer positions, dav2_device_buffer frequencies,
+                                      const dav2_rotary_args* sizes) {
+    return guard(ops, [&](dav2::HipOperators& o) {
+        auto out = v(output);
+        o.rotary(out, v(input), v(positions), v(frequencies), given(sizes));
+    });
+}
+
+dav2_status DAV2_CALL dav2_ops_qk_norm_rotary(dav2_ops* ops, dav2_device_buffer query_out, dav2_device_buffer key_out,
+                                              dav2_device_buffer query, dav2_device_buffer key,
+                                              dav2_device_buffer query_weight, dav2_device_buffer key_weight,
+                                              dav2_device_buffer positions, dav2_device_buffer frequencies,
+                                              const dav2_qk_norm_rotary_args* sizes) {
+    return guard(ops, [&](dav2::HipOperators& o) {
+        auto q = v(query_out), k = v(key_out);
+        o.qk_norm_rotary(q, k, v(query), v(key), v(query_weight), v(key_weight), v(positions), v(frequencies),
+                         given(sizes));
+    });
+}
+
+dav2_status DAV2_CALL dav2_ops_cache_store_int8(dav2_ops* ops, dav2_ops_cache_int8 cache, dav2_device_buffer keys,
+                                                dav2_device_buffer values, dav2_device_buffer page_table,
+                                                dav2_device_buffer starts, dav2_device_buffer lengths,
+                                                const dav2_cache_store_i8_args* sizes) {
+    return guard(ops, [&](dav2::HipOperators& o) {
+        const auto ck = v(cache.keys), cv = v(cache.values), ks = v(cache.key_scales), vs = v(cache.value_scales);
+        o.cache_store_int8({ck, cv, ks, vs}, v(keys), v(values), v(page_table), v(starts), v(lengths), given(sizes));
+    });
+}
+
+dav2_status DAV2_CALL dav2_ops_attention_cache_int8(dav2_ops* ops, dav2_device_buffer output,
+                                                    dav2_device_buffer query, dav2_ops_cache_int8 cache,
+                                                    dav2_device_buffer page_table, dav2_device_buffer starts,
+                                                    dav2_device_buffer lengths, dav2_device_buffer scratch,
+                                                    const dav2_attention_cache_i8_args* sizes) {
+    return guard(ops, [&](dav2::HipOperators& o) {
+        const auto ck = v(cache.keys), cv = v(cache.values), ks = v(cache.key_scales), vs = v(cache.value_scales);
+        auto out = v(output);
+        o.attention_cache_int8(out, v(query), {ck, cv, ks, vs}, v(page_table), v(starts), v(lengths), v(scratch),
+                               given(sizes));
+    });
+}
+
+dav2_status DAV2_CALL dav2_ops_cross_attention(dav2_ops* ops, dav2_device_buffer output, dav2_device_buffer query,
+                                               dav2_device_buffer keys, dav2_device_buffer values,
+                                               dav2_device_buffer key_lengths, dav2_device_buffer key_mask,
+                                               dav2_device_buffer scratch, const dav2_cross_attention_args* sizes) {
+    return guard(ops, [&](dav2::HipOperators& o) {
+        auto out = v(output);
+        o.cross_attention(out, v(query), v(keys), v(values), v(key_lengths), v(key_mask), v(scratch), given(sizes));
     });
 }
 

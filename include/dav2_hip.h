@@ -477,6 +477,163 @@ DAV2_API int dav2_hip_finish_tokens(float* tokens, const float* interpolated,
                                     uint32_t patch_width, uint32_t patch_height,
                                     uint32_t embedding, uint32_t batch, void* stream);
 
+/* ---- operators of a decoder behind the encoder (no reference counterpart) ----
+ *
+ * Element types of their activations; sums, norms and softmax statistics are
+ * fp32 whatever the type, and a result is rounded once. */
+enum { DAV2_DTYPE_F32 = 0, DAV2_DTYPE_F16 = 1, DAV2_DTYPE_BF16 = 2 };
+
+/* Which features of a head form a rotated pair: i and i + rotary_dim/2
+ * (HALVES), or 2i and 2i + 1 (PAIRS). */
+enum { DAV2_ROTARY_HALVES = 0, DAV2_ROTARY_PAIRS = 1 };
+
+/* Rotary positions: the first rotary_dim features of every head turned pair
+ * by pair, (a, b) -> amplitude * (a cos t - b sin t, b cos t + a sin t) with
+ * t = positions[token] * frequencies[i]; the others are copied. t is formed
+ * and reduced to a turn in 64 bits, so far positions keep their angle.
+ * Tokens are *_stride elements apart (at least heads * head_dim), heads
+ * head_dim. output may be input with the same stride; it must not overlap it
+ * otherwise. head_dim <= 1024; rotary_dim even, 2 .. head_dim. frequencies is
+ * device memory: dav2_ops_rotary_frequencies() fills a host table. */
+typedef struct dav2_rotary_args {
+    const void* input;           /* [tokens][heads][head_dim]                      */
+    void* output;
+    uint64_t input_stride, output_stride;
+    const int32_t* positions;    /* [tokens], any sign                             */
+    const double* frequencies;   /* [rotary_dim / 2] radians per position          */
+    uint32_t tokens, heads, head_dim, rotary_dim;
+    uint32_t layout;             /* DAV2_ROTARY_*                                  */
+    uint32_t dtype;              /* DAV2_DTYPE_* of input and output               */
+    float amplitude;             /* 1 for a plain rotation                         */
+} dav2_rotary_args;
+DAV2_API int dav2_hip_rotary(const dav2_rotary_args* args, void* stream);
+
+/* Norm of a head: x / sqrt(mean(x^2) + epsilon) * weight (RMS), or
+ * (x - mean) / sqrt(variance + epsilon) * weight (LAYER). */
+enum { DAV2_QK_NORM_RMS = 0, DAV2_QK_NORM_LAYER = 1 };
+
+/* The norm of every query head and every key head over its head_dim
+ * features, then the rotation of dav2_hip_rotary, in one pass over both.
+ * weight [head_dim] fp32, NULL = ones. rotary_dim 0: the norm alone
+ * (positions and frequencies unused). Query and key may be parts of one
+ * packed row; an output may be its input with the same stride, and must not
+ * overlap any input otherwise. query_heads or key_heads may be 0. */
+typedef struct dav2_qk_norm_rotary_args {
+    const void* query;           /* [tokens][query_heads][head_dim]                */
+    const void* key;             /* [tokens][key_heads][head_dim]                  */
+    void* query_out;
+    void* key_out;
+    uint64_t query_stride, key_stride, query_out_stride, key_out_stride;
+    const float* query_weight;
+    const float* key_weight;
+    const int32_t* positions;
+    const double* frequencies;
+    uint32_t tokens, query_heads, key_heads, head_dim, rotary_dim;
+    uint32_t layout, dtype;
+    uint32_t norm;               /* DAV2_QK_NORM_*                                 */
+    float epsilon;               /* > 0                                            */
+    float amplitude;
+} dav2_qk_norm_rotary_args;
+DAV2_API int dav2_hip_qk_norm_rotary(const dav2_qk_norm_rotary_args* args, void* stream);
+
+/* A key/value cache in 8 bits: pages of page_size tokens, and in each page one
+ * scale per head for its keys and one for its values; a code c stands for
+ * c * scale. Values are held feature-major, so that the keys of one feature
+ * are contiguous. page_size a multiple of 16 up to 256, head_dim a multiple
+ * of 16 up to 128; keys and values 16-byte aligned. Sequence s owns the pages
+ * page_table[s][0], [1], ...: token t is slot t % page_size of page
+ * page_table[s][t / page_size]. A table entry outside [0, pages) is no page:
+ * nothing is stored there and its tokens are not seen. Pages need no
+ * clearing before their first use. */
+typedef struct dav2_cache_i8 {
+    int8_t* keys;                /* [pages][kv_heads][page_size][head_dim]         */
+    int8_t* values;              /* [pages][kv_heads][head_dim][page_size]         */
+    float* key_scales;           /* [pages][kv_heads]                              */
+    float* value_scales;         /* [pages][kv_heads]                              */
+    uint32_t pages, kv_heads, page_size, head_dim;
+} dav2_cache_i8;
+
+/* Stores new tokens. Rows starts[s] .. starts[s+1] of keys and values become
+ * the last tokens of sequence s, which holds lengths[s] tokens after the call.
+ * A page's scale is the larger of what it was (if older tokens are in the
+ * page) and max(absmax of its new rows / 127, 1e-8), codes are x / scale
+ * rounded half to even, and where a scale grows the page's older codes are
+ * rounded again: value = code * old scale in fp32, code = rint(value / scale).
+ * Storing the same rows at the same lengths again changes nothing. A NaN or
+ * infinity makes the scale of its page NaN or infinite, and with it the
+ * page's values, until the page is begun anew. starts must not decrease; rows
+ * outside [0, tokens) and positions outside the table are not stored. Pages
+ * that get tokens must belong to one sequence only. Other bytes of the cache
+ * are left as they were. */
+typedef struct dav2_cache_store_i8_args {
+    dav2_cache_i8 cache;
+    const void* keys;            /* [tokens][kv_heads][head_dim]                   */
+    const void* values;
+    uint64_t key_stride, value_stride;  /* elements between tokens                 */
+    const int32_t* page_table;   /* [sequences][table_pages]                       */
+    const int32_t* starts;       /* [sequences + 1]                                */
+    const int32_t* lengths;      /* [sequences]                                    */
+    uint32_t sequences, table_pages, tokens;
+    uint32_t max_new;            /* most new tokens of a sequence: sizes the launch */
+    uint32_t dtype;
+} dav2_cache_store_i8_args;
+DAV2_API int dav2_hip_cache_store_i8(const dav2_cache_store_i8_args* args, void* stream);
+
+/* softmax(scale * q k^T) v over a cache: query rows starts[s] .. starts[s+1]
+ * are the last tokens of sequence s, of lengths[s] tokens in all. causal: row
+ * i of n sees the first lengths[s] - n + 1 + i tokens; otherwise all. heads is
+ * a multiple of kv_heads; head h reads head h / (heads / kv_heads) of the
+ * cache. A row that sees nothing gives zeros; output rows of no sequence are
+ * left as they were. Strides (elements between tokens) are multiples of 8,
+ * query and output 16-byte aligned. max_query and max_length, the most new
+ * and the most tokens of a sequence, size the launch and the scratch; a
+ * sequence beyond them is still computed. scratch: dav2_hip_attention_cache_i8_
+ * scratch_bytes() bytes (0: none), 16-byte aligned, in use until the call's
+ * work is done. That number depends on the sizes, never on the pointers. */
+typedef struct dav2_attention_cache_i8_args {
+    dav2_cache_i8 cache;
+    const void* query;           /* [tokens][heads][head_dim]                      */
+    void* output;
+    uint64_t query_stride, output_stride;
+    const int32_t* page_table;   /* [sequences][table_pages]                       */
+    const int32_t* starts;       /* [sequences + 1]                                */
+    const int32_t* lengths;      /* [sequences]                                    */
+    uint32_t sequences, table_pages, tokens, heads;
+    uint32_t max_query, max_length;
+    uint32_t causal, dtype;
+    float scale;
+    void* scratch;
+    uint64_t scratch_bytes;
+} dav2_attention_cache_i8_args;
+DAV2_API uint64_t dav2_hip_attention_cache_i8_scratch_bytes(const dav2_attention_cache_i8_args* args);
+DAV2_API int dav2_hip_attention_cache_i8(const dav2_attention_cache_i8_args* args, void* stream);
+
+/* softmax(scale * q k^T) v of queries against keys and values of another
+ * length (an encoder's tokens), batch by batch. Key j of batch b is seen if
+ * j < key_lengths[b] (NULL: key_tokens) and key_mask[b][j] != 0 (NULL: all);
+ * what is not seen may hold anything, NaN included. A batch that sees nothing
+ * gives zeros. heads is a multiple of kv_heads; head h reads key head
+ * h / (heads / kv_heads). head_dim a multiple of 16 up to 128; strides in
+ * elements, multiples of 8; the four tensors 16-byte aligned. scratch as for
+ * dav2_hip_attention_cache_i8. */
+typedef struct dav2_cross_attention_args {
+    const void* query;           /* [batch][query_tokens][heads][head_dim]         */
+    const void* keys;            /* [batch][key_tokens][kv_heads][head_dim]        */
+    const void* values;          /* like keys                                      */
+    void* output;                /* like query                                     */
+    uint64_t query_stride, key_stride, value_stride, output_stride;  /* between tokens */
+    uint64_t query_batch_stride, key_batch_stride, value_batch_stride, output_batch_stride;
+    const int32_t* key_lengths;  /* [batch] or NULL                                */
+    const uint8_t* key_mask;     /* [batch][key_tokens] or NULL                    */
+    uint32_t batch, query_tokens, key_tokens, heads, kv_heads, head_dim;
+    uint32_t dtype;
+    float scale;
+    void* scratch;
+    uint64_t scratch_bytes;
+} dav2_cross_attention_args;
+DAV2_API uint64_t dav2_hip_cross_attention_scratch_bytes(const dav2_cross_attention_args* args);
+DAV2_API int dav2_hip_cross_attention(const dav2_cross_attention_args* args, void* stream);
+
 DAV2_API const char* dav2_hip_error_string(int error);
 
 #ifdef __cplusplus

@@ -19,6 +19,7 @@
 #ifndef DAV2_OPS_H
 #define DAV2_OPS_H
 
+#include "dav2_hip.h"
 #include "depth_anything_v2.h"
 
 #ifdef __cplusplus
@@ -162,6 +163,79 @@ DAV2_API dav2_status DAV2_CALL dav2_ops_add(dav2_ops* ops, dav2_device_buffer ou
                                             dav2_device_buffer right, uint32_t count);
 DAV2_API dav2_status DAV2_CALL dav2_ops_gelu(dav2_ops* ops, dav2_device_buffer output, dav2_device_buffer input,
                                              uint32_t count);
+
+/* Operators of a decoder behind the encoder (no counterpart in the
+ * reference): the kernels of dav2_hip.h on the instance's stream, with its
+ * rules, and with every buffer checked against the sizes. Sizes, strides,
+ * types and factors come in the kernel's own argument block; the pointers in
+ * that block are not read, the buffers take their place. Zero sizes and what
+ * the kernel rejects -> DAV2_STATUS_INVALID_ARGUMENT. An optional buffer is
+ * left out with data == NULL. */
+
+/* Host helper: the frequencies of dav2_hip_rotary, frequency i of
+ * rotary_dim / 2 being base^(-2 i / rotary_dim), changed for contexts longer
+ * than the trained one:
+ *   NONE        as they are;
+ *   LINEAR      all divided by factor;
+ *   BASE        base * factor^(rotary_dim / (rotary_dim - 2)), so that the
+ *               slowest pair is slowed by factor and the fastest not at all;
+ *   WAVELENGTH  by the turns r a pair makes in original_length tokens: as it
+ *               is for r >= high_turns, divided by factor for r <= low_turns,
+ *               blended linearly in r between.
+ * scaling NULL is NONE. base > 1, rotary_dim even and at least 2 (BASE: at
+ * least 4), factor >= 1, original_length > 0, high_turns > low_turns >= 0. */
+enum {
+    DAV2_ROTARY_SCALING_NONE = 0,
+    DAV2_ROTARY_SCALING_LINEAR = 1,
+    DAV2_ROTARY_SCALING_BASE = 2,
+    DAV2_ROTARY_SCALING_WAVELENGTH = 3
+};
+typedef struct dav2_rotary_scaling {
+    uint32_t kind;
+    double factor, original_length, low_turns, high_turns;
+} dav2_rotary_scaling;
+DAV2_API dav2_status DAV2_CALL dav2_ops_rotary_frequencies(double* frequencies, uint32_t rotary_dim, double base,
+                                                           const dav2_rotary_scaling* scaling);
+
+/* positions: tokens int32, frequencies: rotary_dim / 2 doubles. */
+DAV2_API dav2_status DAV2_CALL dav2_ops_rotary(dav2_ops* ops, dav2_device_buffer output, dav2_device_buffer input,
+                                               dav2_device_buffer positions, dav2_device_buffer frequencies,
+                                               const dav2_rotary_args* sizes);
+/* The weights may be left out; positions and frequencies with rotary_dim 0. */
+DAV2_API dav2_status DAV2_CALL dav2_ops_qk_norm_rotary(dav2_ops* ops, dav2_device_buffer query_out,
+                                                       dav2_device_buffer key_out, dav2_device_buffer query,
+                                                       dav2_device_buffer key, dav2_device_buffer query_weight,
+                                                       dav2_device_buffer key_weight, dav2_device_buffer positions,
+                                                       dav2_device_buffer frequencies,
+                                                       const dav2_qk_norm_rotary_args* sizes);
+
+typedef struct dav2_ops_cache_int8 {
+    dav2_device_buffer keys, values, key_scales, value_scales;
+} dav2_ops_cache_int8;
+/* page_table: sequences x table_pages int32, starts: sequences + 1 int32,
+ * lengths: sequences int32. */
+DAV2_API dav2_status DAV2_CALL dav2_ops_cache_store_int8(dav2_ops* ops, dav2_ops_cache_int8 cache,
+                                                         dav2_device_buffer keys, dav2_device_buffer values,
+                                                         dav2_device_buffer page_table, dav2_device_buffer starts,
+                                                         dav2_device_buffer lengths,
+                                                         const dav2_cache_store_i8_args* sizes);
+/* scratch left out: the instance's own, grown when a call needs more. A call
+ * under graph capture that needs scratch has to bring it (a graph would hold
+ * an address that a later call may free): dav2_hip_attention_cache_i8_
+ * scratch_bytes(sizes) bytes, one buffer for each graph that may run beside
+ * another. */
+DAV2_API dav2_status DAV2_CALL dav2_ops_attention_cache_int8(dav2_ops* ops, dav2_device_buffer output,
+                                                             dav2_device_buffer query, dav2_ops_cache_int8 cache,
+                                                             dav2_device_buffer page_table, dav2_device_buffer starts,
+                                                             dav2_device_buffer lengths, dav2_device_buffer scratch,
+                                                             const dav2_attention_cache_i8_args* sizes);
+/* key_lengths (batch int32) and key_mask (batch x key_tokens bytes) may be
+ * left out; scratch as above, dav2_hip_cross_attention_scratch_bytes(). */
+DAV2_API dav2_status DAV2_CALL dav2_ops_cross_attention(dav2_ops* ops, dav2_device_buffer output,
+                                                        dav2_device_buffer query, dav2_device_buffer keys,
+                                                        dav2_device_buffer values, dav2_device_buffer key_lengths,
+                                                        dav2_device_buffer key_mask, dav2_device_buffer scratch,
+                                                        const dav2_cross_attention_args* sizes);
 
 /* Whole-graph variant of dav2_infer_tensor_f32_device that also returns the
  * depth logits before the final ReLU (batch 1); for parity checks where
