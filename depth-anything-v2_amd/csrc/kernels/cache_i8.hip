@@ -3,6 +3,9 @@
 // One scale per page and head, s = max over the page of |x| / 127, so a page's
 // codes are bounded by its largest value and a scale is read once per page.
 
+#include <algorithm>
+#include <type_traits>
+
 #include "decoder.h"
 
 using namespace dav2k;
@@ -70,69 +73,366 @@ __global__ __launch_bounds__(256) void cache_store_kernel(dav2_cache_store_i8_ar
     }
 }
 
-// One wave per query row and head, 64 keys at a time: lane l scores key l,
-// then takes features l and l + 64 of the values.
-template <typename E>
-__global__ __launch_bounds__(64) void cache_attention_kernel(dav2_attention_cache_i8_args a) {
-    __shared__ float qs[128], w[64];
-    const uint32_t h = blockIdx.y, s = blockIdx.z, lane = threadIdx.x;
-    const uint32_t d = a.cache.head_dim, page_size = a.cache.page_size;
-    const uint32_t kvh = h / (a.heads / a.cache.kv_heads);
+// ---------------------------------------------------------------------------
+// Attention over the cache.
+//
+// Codes are exact in binary16, so both products run on the binary16 MFMA with
+// fp32 sums. A query row is multiplied by the power of two that puts its
+// largest value into [2^14, 2^15) and rounded to binary16: exact for binary16
+// and bfloat16 queries down to 2^-28 of the largest; an fp32 row is kept as
+// two such parts (22 bits).
+//
+// A value's scale sv goes with the weight of its key: with sv = 2^e f,
+// 1 <= f < 2, and t = s log2(e) + e for a score s,
+//   w = exp2(t - max t),  O = sum (w f) c,  L = sum w 2^-e,  o = O / L.
+// The maximum is that of what reaches the output, so w f rounded to binary16
+// (two parts in the fp32 mode) keeps its precision whatever the pages' scales
+// are; L is summed in fp32 from the unrounded w.
+
+constexpr float kLog2e = 1.44269504f;
+
+// Page and slot of a 16-token chunk; magic = ceil(2^32 / chunks per page),
+// which divides every chunk below 2^28 exactly (chunks per page <= 16).
+struct Pages {
+    const int32_t* table;  // of one sequence
+    uint32_t table_pages, pages, per_page, magic;
+    // the chunk's page, or -1 if there is none; its slot in the page
+    DAV2_DEV int32_t find(uint32_t chunk, uint32_t& slot) const {
+        const uint32_t index = per_page == 1 ? chunk : __umulhi(chunk, magic);
+        slot = (chunk - index * per_page) * 16u;
+        const int32_t page = table[min(index, table_pages - 1u)];
+        return index < table_pages && static_cast<uint32_t>(page) < pages ? page : -1;
+    }
+};
+
+DAV2_DEV Pages pages_of(const dav2_attention_cache_i8_args& a, uint32_t s) {
+    const uint32_t per_page = a.cache.page_size / 16u;
+    return {a.page_table + static_cast<uint64_t>(s) * a.table_pages, a.table_pages, a.cache.pages, per_page,
+            static_cast<uint32_t>(((1ull << 32) + per_page - 1u) / per_page)};
+}
+
+// Eight codes as binary16: the byte c + 128 below the exponent of 1024 is the
+// number 1152 + c.
+DAV2_DEV h8 widen(uint32_t lo, uint32_t hi) {
+    const uint32_t x = lo ^ 0x80808080u, y = hi ^ 0x80808080u;
+    const h2 shift = {static_cast<_Float16>(1152.0f), static_cast<_Float16>(1152.0f)};
+    const h2 a = __builtin_bit_cast(h2, __builtin_amdgcn_perm(0x64646464u, x, 0x04010400u)) - shift;
+    const h2 b = __builtin_bit_cast(h2, __builtin_amdgcn_perm(0x64646464u, x, 0x04030402u)) - shift;
+    const h2 c = __builtin_bit_cast(h2, __builtin_amdgcn_perm(0x64646464u, y, 0x04010400u)) - shift;
+    const h2 d = __builtin_bit_cast(h2, __builtin_amdgcn_perm(0x64646464u, y, 0x04030402u)) - shift;
+    return h8{a.x, a.y, b.x, b.y, c.x, c.y, d.x, d.y};
+}
+
+// A page's value scale as 2^e f. Below 2^-100 (a page of zeros with a scale of
+// 0) 2^-100 stands in: w 2^-e stays finite. Infinity and NaN make f NaN.
+DAV2_DEV void split_scale(float scale, float& exponent, float& fraction, float& inverse) {
+    const uint32_t bits = max(__float_as_uint(scale) & 0x7fffffffu, 27u << 23);
+    const int e = static_cast<int>(bits >> 23) - 127;
+    exponent = static_cast<float>(e);
+    fraction = bits >= 0x7f800000u ? __uint_as_float(0x7fc00000u)
+                                   : __uint_as_float((bits & 0x007fffffu) | 0x3f800000u);
+    inverse = ldexpf(1.0f, -e);
+}
+
+// What splits of the keys leave for the join: per row (token * heads + head)
+// and split, the output's sums and {maximum, L}.
+struct Parts {
+    float* sums;   // [rows][splits][head_dim]
+    float2* stats; // [rows][splits]
+};
+DAV2_DEV Parts parts_of(const dav2_attention_cache_i8_args& a, uint32_t splits) {
+    const uint64_t rows = static_cast<uint64_t>(a.tokens) * a.heads * splits;
+    float2* stats = static_cast<float2*>(a.scratch);
+    return {reinterpret_cast<float*>(stats + ((rows + 1u) & ~uint64_t(1))), stats};
+}
+
+// Few query rows for a cache head (single tokens, drafts): bound by reading
+// the cache. A workgroup has 16 rows (token-major: row r is token r / group,
+// query head r % group) of one sequence and cache head and a run of 64-key
+// blocks, which its four waves take in turn; each wave goes through its blocks
+// alone, and their sums are joined through LDS at the end.
+//
+// S^T = K Q^T and O^T = V^T P^T on v_mfma_f32_16x16x32_f16. The cache's layout
+// is such that both left operands are 16-byte pieces of global memory, taken
+// straight into registers: lane l has 16 features 64 kc + 16 (l / 16) .. of a
+// key, and the 16 keys of chunk l / 16 of one feature. Row i of score tile a
+// is key 16 (i / 4) + 4 a + i % 4 of the block; a lane then holds the scores of
+// chunk l / 16 in order, which is the right operand of the second product as
+// it stands, and the scales it needs are those of one page.
+template <typename E, int HEAD>
+__global__ __launch_bounds__(256, 2) void cache_rows_kernel(dav2_attention_cache_i8_args a, uint32_t splits,
+                                                            uint32_t tiles) {
+    constexpr bool kFloat = std::is_same_v<E, float>;
+    constexpr int KC = HEAD / 64, FT = HEAD / 16, NP = kFloat ? 2 : 1;
+    constexpr int kPad = 17;  // row length of the joining waves' sums in LDS
+    __shared__ float joined[4][HEAD * kPad];
+    __shared__ float shared_max[4][16], shared_sum[4][16];
+    const uint32_t lane = threadIdx.x & 63u, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const uint32_t col = lane & 15u, g = lane >> 4;
+    const uint32_t split = blockIdx.x % splits, h = blockIdx.y, s = blockIdx.z;
+    const uint32_t d = a.cache.head_dim, page_size = a.cache.page_size, kv_heads = a.cache.kv_heads;
+    const uint32_t group = a.heads / kv_heads;
     const Sequence q = sequence_of(a.starts, a.lengths, s, a.tokens);
+    const uint32_t n = static_cast<uint32_t>(q.end - q.begin);
+    const uint64_t rows = static_cast<uint64_t>(n) * group;
     const int64_t span = static_cast<int64_t>(a.table_pages) * page_size;
-    for (int32_t row = q.begin + static_cast<int32_t>(blockIdx.x); row < q.end; row += gridDim.x) {
-        int64_t seen = q.length;
-        if (a.causal) seen = static_cast<int64_t>(q.length) - q.end + 1 + row;
-        seen = max(min(seen, span), int64_t(0));
-        const E* x = static_cast<const E*>(a.query) + static_cast<uint64_t>(row) * a.query_stride + uint64_t(h) * d;
-        __syncthreads();
-        for (uint32_t f = lane; f < d; f += 64u) qs[f] = static_cast<float>(x[f]) * a.scale;
-        __syncthreads();
-        float most = -INFINITY, sum = 0.0f, o0 = 0.0f, o1 = 0.0f;
-        for (int64_t j0 = 0; j0 < seen; j0 += 64) {
-            const int64_t j = j0 + lane;
-            auto page_of = [&](int64_t t) {
-                return a.page_table[static_cast<uint64_t>(s) * a.table_pages + static_cast<uint64_t>(t / page_size)];
-            };
-            float score = -INFINITY;
-            if (j < seen) {
-                const int32_t page = page_of(j);
-                if (page >= 0 && static_cast<uint32_t>(page) < a.cache.pages) {
-                    const uint64_t plane = static_cast<uint64_t>(page) * a.cache.kv_heads + kvh;
-                    const int8_t* k = a.cache.keys + (plane * page_size + static_cast<uint64_t>(j % page_size)) * d;
-                    float dot = 0.0f;
-                    for (uint32_t f = 0; f < d; ++f) dot = fmaf(qs[f], static_cast<float>(k[f]), dot);
-                    score = dot * a.cache.key_scales[plane];
+    const Pages pages = pages_of(a, s);
+    const Parts parts = parts_of(a, splits);
+
+    for (uint64_t tile = blockIdx.x / splits; tile * 16u < rows; tile += tiles) {
+        const uint64_t row = tile * 16u + col;
+        const uint32_t token = static_cast<uint32_t>(min(row, rows - 1u) / group);
+        const uint32_t head = h * group + static_cast<uint32_t>(min(row, rows - 1u) % group);
+        // keys that this lane's row sees, and the most that a row of the tile does
+        auto seen = [&](uint32_t i) {
+            int64_t t = q.length;
+            if (a.causal) t += 1 + static_cast<int64_t>(i) - n;
+            return static_cast<uint32_t>(max(min(t, span), int64_t(0)));
+        };
+        const uint32_t limit = row < rows ? seen(token) : 0u;
+        const uint32_t most = seen(static_cast<uint32_t>(min(tile * 16u + 15u, rows - 1u) / group));
+        const uint32_t least = seen(static_cast<uint32_t>(tile * 16u / group));
+        const uint32_t blocks = (most + 63u) / 64u, per = (blocks + splits - 1u) / splits;
+        const uint32_t first = split * per, last = min(first + per, blocks);
+
+        // the right operand of the scores
+        h8 qf[NP][KC][2];
+        float factor;  // score = sum * factor, in units of log2
+        {
+            const E* x = static_cast<const E*>(a.query) + static_cast<uint64_t>(q.begin + token) * a.query_stride +
+                         static_cast<uint64_t>(head) * d;
+            float v[KC][16];
+            float largest = 0.0f;
+#pragma unroll
+            for (int kc = 0; kc < KC; ++kc)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) {
+                    v[kc][i] = 64u * kc + 16u * g < d ? static_cast<float>(x[64 * kc + 16 * g + i]) : 0.0f;
+                    largest = fmaxf(largest, fabsf(v[kc][i]));
+                }
+            largest = over_groups(largest, Larger());
+            // up is a power of two; rows of zeros, NaN and infinities stay as they are
+            const int e = largest > 0.0f && largest < INFINITY ? 14 - ilogbf(largest) : 0;
+            const float sign = a.scale < 0.0f ? -1.0f : 1.0f;
+            factor = ldexpf(fabsf(a.scale) * kLog2e, -e);
+#pragma unroll
+            for (int kc = 0; kc < KC; ++kc)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) {
+                    const float y = ldexpf(v[kc][i], e) * sign;
+                    const _Float16 hi = static_cast<_Float16>(y);
+                    qf[0][kc][i >> 3][i & 7] = hi;
+                    if constexpr (kFloat)
+                        qf[1][kc][i >> 3][i & 7] = static_cast<_Float16>(y - static_cast<float>(hi));
+                }
+        }
+
+        v4f o[FT];
+#pragma unroll
+        for (int f = 0; f < FT; ++f) o[f] = v4f{0.f, 0.f, 0.f, 0.f};
+        float maximum = kNoScore, sum = 0.0f;  // sum: this lane's keys only
+
+        uint4 kraw[4][KC];
+        uint32_t slot_v = 0, slot_k = 0;
+        int32_t page_v = -1, page_k = -1;
+        auto find = [&](uint32_t block) {
+            page_k = pages.find(block * 4u + col / 4u, slot_k);
+            page_v = pages.find(block * 4u + g, slot_v);
+        };
+        auto load_keys = [&] {
+            const int8_t* k = a.cache.keys +
+                              ((static_cast<uint64_t>(max(page_k, 0)) * kv_heads + h) * page_size + slot_k + col % 4u) * d +
+                              16u * g;
+#pragma unroll
+            for (int t = 0; t < 4; ++t)
+#pragma unroll
+                for (int kc = 0; kc < KC; ++kc) {
+                    kraw[t][kc] = make_uint4(0, 0, 0, 0);
+                    if (64u * kc + 16u * g < d) kraw[t][kc] = *reinterpret_cast<const uint4*>(k + 4u * t * d + 64 * kc);
+                }
+        };
+        uint32_t block = first + wave;
+        if (block < last) {
+            find(block);
+            load_keys();
+        }
+        for (; block < last; block += 4u) {
+            const bool exists = page_v >= 0;
+            const uint64_t plane = static_cast<uint64_t>(max(page_v, 0)) * kv_heads + h;
+            const float key_scale = a.cache.key_scales[plane], value_scale = a.cache.value_scales[plane];
+            uint4 vraw[FT];
+            const int8_t* v = a.cache.values + (plane * d + col) * page_size + slot_v;
+#pragma unroll
+            for (int f = 0; f < FT; ++f)
+                if (16u * f < d) vraw[f] = *reinterpret_cast<const uint4*>(v + static_cast<uint64_t>(16u * f) * page_size);
+            v4f sc[4];
+#pragma unroll
+            for (int t = 0; t < 4; ++t) {
+                sc[t] = v4f{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int kc = 0; kc < KC; ++kc) {
+                    const h8 k0 = widen(kraw[t][kc].x, kraw[t][kc].y), k1 = widen(kraw[t][kc].z, kraw[t][kc].w);
+#pragma unroll
+                    for (int p = 0; p < NP; ++p) {
+                        sc[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k0, qf[p][kc][0], sc[t], 0, 0, 0);
+                        sc[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k1, qf[p][kc][1], sc[t], 0, 0, 0);
+                    }
                 }
             }
-            const bool any = __ballot(score != -INFINITY) != 0;
-            if (!any) continue;
-            const float grown = fmaxf(most, wave_max(score));
-            const float keep = most == -INFINITY ? 0.0f : expf(most - grown);
-            const float weight = score == -INFINITY ? 0.0f : expf(score - grown);
-            most = grown;
-            sum = fmaf(sum, keep, wave_sum_tree(weight));
-            o0 *= keep;
-            o1 *= keep;
-            __syncthreads();
-            w[lane] = weight;
-            __syncthreads();
-            const uint32_t n = static_cast<uint32_t>(min(seen - j0, int64_t(64)));
-            for (uint32_t i = 0; i < n; ++i) {
-                const int32_t page = page_of(j0 + i);
-                if (page < 0 || static_cast<uint32_t>(page) >= a.cache.pages) continue;
-                const uint64_t plane = static_cast<uint64_t>(page) * a.cache.kv_heads + kvh;
-                const int8_t* v = a.cache.values + plane * page_size * d + static_cast<uint64_t>((j0 + i) % page_size);
-                const float ws = w[i] * a.cache.value_scales[plane];
-                if (lane < d) o0 = fmaf(ws, static_cast<float>(v[lane * page_size]), o0);
-                if (lane + 64u < d) o1 = fmaf(ws, static_cast<float>(v[(lane + 64u) * page_size]), o1);
+            if (block + 4u < last) {
+                find(block + 4u);
+                load_keys();
+            }
+            float exponent, fraction, inverse;
+            const uint32_t key0 = block * 64u + 16u * g;  // of this lane's first score
+            // a chunk that the row does not see may have any scale, NaN included
+            split_scale(exists && key0 < limit ? value_scale : 1.0f, exponent, fraction, inverse);
+            const float c = key_scale * factor;
+            const bool whole = (block + 1u) * 64u <= least && __all(exists);
+            float largest = kNoScore;
+#pragma unroll
+            for (int t = 0; t < 4; ++t)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    float x = fmaf(sc[t][r], c, exponent);
+                    if (!whole && (!exists || key0 + 4 * t + r >= limit)) x = -INFINITY;
+                    sc[t][r] = x;
+                    largest = fmaxf(largest, x);
+                }
+            largest = over_groups(largest, Larger());
+            if (__any(largest > maximum)) {
+                const float grown = fmaxf(maximum, largest);
+                const float keep = __builtin_amdgcn_exp2f(maximum - grown);
+                maximum = grown;
+                sum *= keep;
+#pragma unroll
+                for (int f = 0; f < FT; ++f) o[f] *= keep;
+            }
+            h8 pf[NP][2];
+            float part = 0.0f;
+#pragma unroll
+            for (int t = 0; t < 4; ++t)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    const float w = __builtin_amdgcn_exp2f(sc[t][r] - maximum);
+                    part += w;
+                    const float y = w * fraction;
+                    const _Float16 hi = static_cast<_Float16>(y);
+                    pf[0][t >> 1][4 * (t & 1) + r] = hi;
+                    if constexpr (kFloat)
+                        pf[1][t >> 1][4 * (t & 1) + r] = static_cast<_Float16>(y - static_cast<float>(hi));
+                }
+            sum = fmaf(part, inverse, sum);
+#pragma unroll
+            for (int f = 0; f < FT; ++f) {
+                if (16u * f >= d) continue;
+                const h8 v0 = widen(vraw[f].x, vraw[f].y), v1 = widen(vraw[f].z, vraw[f].w);
+#pragma unroll
+                for (int p = 0; p < NP; ++p) {
+                    o[f] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v0, pf[p][0], o[f], 0, 0, 0);
+                    o[f] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v1, pf[p][1], o[f], 0, 0, 0);
+                }
             }
         }
-        E* y = static_cast<E*>(a.output) + static_cast<uint64_t>(row) * a.output_stride + uint64_t(h) * d;
-        const float inverse = sum == 0.0f ? 0.0f : 1.0f / sum;
-        if (lane < d) y[lane] = static_cast<E>(o0 * inverse);
-        if (lane + 64u < d) y[lane + 64u] = static_cast<E>(o1 * inverse);
+        sum = over_groups(sum, Plus());
+
+        // join the four waves: lane (col, g), register r of o[f]: feature 16 f + 4 g + r of row col
+        __syncthreads();  // the tile before has been read
+        if (g == 0) {
+            shared_max[wave][col] = maximum;
+            shared_sum[wave][col] = sum;
+        }
+        __syncthreads();
+        float top = kNoScore;
+#pragma unroll
+        for (int w = 0; w < 4; ++w) top = fmaxf(top, shared_max[w][col]);
+        const float mine = __builtin_amdgcn_exp2f(maximum - top);
+#pragma unroll
+        for (int f = 0; f < FT; ++f)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) joined[wave][(16 * f + 4 * g + r) * kPad + col] = o[f][r] * mine;
+        __syncthreads();
+        // 16 threads for each of the 16 rows
+        const uint32_t out_col = threadIdx.x >> 4, lane16 = threadIdx.x & 15u;
+        const uint64_t out_row = tile * 16u + out_col;
+        if (out_row < rows) {
+            float all = kNoScore, total = 0.0f;
+#pragma unroll
+            for (int w = 0; w < 4; ++w) all = fmaxf(all, shared_max[w][out_col]);
+#pragma unroll
+            for (int w = 0; w < 4; ++w)
+                total = fmaf(shared_sum[w][out_col], __builtin_amdgcn_exp2f(shared_max[w][out_col] - all), total);
+            const uint64_t at = static_cast<uint64_t>(q.begin) + out_row / group;
+            const uint32_t out_head = h * group + static_cast<uint32_t>(out_row % group);
+            const float scale = splits > 1 ? 1.0f : total == 0.0f ? 0.0f : 1.0f / total;
+            E* y = static_cast<E*>(a.output) + at * a.output_stride + static_cast<uint64_t>(out_head) * d;
+            const uint64_t slot = (at * a.heads + out_head) * splits + split;
+            for (uint32_t f = lane16; f < d; f += 16u) {
+                float v = 0.0f;
+#pragma unroll
+                for (int w = 0; w < 4; ++w) v += joined[w][f * kPad + out_col];
+                if (splits > 1) parts.sums[slot * d + f] = v;
+                else y[f] = static_cast<E>(v * scale);
+            }
+            if (splits > 1 && lane16 == 0) parts.stats[slot] = make_float2(all, total);
+        }
     }
+}
+
+// The splits of a row joined: one wave per row.
+template <typename E>
+__global__ __launch_bounds__(256) void cache_join_kernel(dav2_attention_cache_i8_args a, uint32_t splits) {
+    const uint32_t lane = threadIdx.x & 63u, d = a.cache.head_dim;
+    const Sequence q = sequence_of(a.starts, a.lengths, blockIdx.y, a.tokens);
+    const uint64_t rows = static_cast<uint64_t>(q.end - q.begin) * a.heads;
+    const Parts parts = parts_of(a, splits);
+    for (uint64_t r = static_cast<uint64_t>(blockIdx.x) * 4u + (threadIdx.x >> 6); r < rows; r += gridDim.x * 4ull) {
+        const uint64_t token = static_cast<uint64_t>(q.begin) + r / a.heads, head = r % a.heads;
+        const uint64_t slot = (token * a.heads + head) * splits;
+        float top = kNoScore;
+        for (uint32_t i = 0; i < splits; ++i) top = fmaxf(top, parts.stats[slot + i].x);
+        float total = 0.0f, o0 = 0.0f, o1 = 0.0f;
+        for (uint32_t i = 0; i < splits; ++i) {
+            const float2 stat = parts.stats[slot + i];
+            const float share = __builtin_amdgcn_exp2f(stat.x - top);
+            total = fmaf(stat.y, share, total);
+            const float* sums = parts.sums + (slot + i) * d;
+            if (lane < d) o0 = fmaf(sums[lane], share, o0);
+            if (lane + 64u < d) o1 = fmaf(sums[lane + 64u], share, o1);
+        }
+        E* y = static_cast<E*>(a.output) + token * a.output_stride + head * d;
+        const float scale = total == 0.0f ? 0.0f : 1.0f / total;
+        if (lane < d) y[lane] = static_cast<E>(o0 * scale);
+        if (lane + 64u < d) y[lane + 64u] = static_cast<E>(o1 * scale);
+    }
+}
+
+bool valid(const dav2_attention_cache_i8_args& a) {
+    const uint64_t row = static_cast<uint64_t>(a.heads) * a.cache.head_dim;
+    return valid_cache(a.cache) && a.query && a.output && aligned16(a.query) && aligned16(a.output) && a.page_table &&
+           a.starts && a.lengths && a.dtype <= DAV2_DTYPE_BF16 && a.sequences <= 65535u && a.tokens <= 0x7fffffffu &&
+           a.table_pages > 0 && a.table_pages <= 0x7fffffffu && a.heads > 0 && a.heads <= 65535u &&
+           a.heads % a.cache.kv_heads == 0 && a.query_stride % 8 == 0 && a.output_stride % 8 == 0 &&
+           (a.tokens == 1 || (a.query_stride >= row && a.output_stride >= row));
+}
+
+// How a call is dealt out: row tiles, and splits of the keys so that the chip
+// is full where sequences, heads and tiles are few.
+struct RowsPlan {
+    uint32_t tiles, splits;
+};
+RowsPlan plan_rows(const dav2_attention_cache_i8_args& a) {
+    constexpr uint64_t kWorkgroups = 1024;  // wanted: two for each of 256 CUs at a time, twice over
+    constexpr uint32_t kLeastKeys = 256;    // of a split: a block for each wave
+    RowsPlan p{1, 1};
+    if (a.cache.kv_heads == 0 || a.heads < a.cache.kv_heads || a.sequences == 0 || a.max_query == 0) return p;
+    const uint64_t query = std::min(a.max_query, a.tokens);
+    const uint64_t rows = query * (a.heads / a.cache.kv_heads);
+    p.tiles = static_cast<uint32_t>(std::min<uint64_t>((rows + 15) / 16, 4096));
+    const uint64_t have = static_cast<uint64_t>(p.tiles) * a.cache.kv_heads * a.sequences;
+    const uint64_t most = std::max<uint64_t>(1, a.max_length / kLeastKeys);
+    p.splits = static_cast<uint32_t>(std::clamp<uint64_t>(kWorkgroups / std::max<uint64_t>(have, 1), 1, std::min<uint64_t>(most, 64)));
+    return p;
 }
 
 }  // namespace
@@ -159,27 +459,36 @@ int dav2_hip_cache_store_i8(const dav2_cache_store_i8_args* args, void* stream) 
     return hipGetLastError();
 }
 
-uint64_t dav2_hip_attention_cache_i8_scratch_bytes(const dav2_attention_cache_i8_args*) { return 0; }
+uint64_t dav2_hip_attention_cache_i8_scratch_bytes(const dav2_attention_cache_i8_args* args) {
+    if (!args) return 0;
+    const dav2_attention_cache_i8_args& a = *args;
+    const RowsPlan p = plan_rows(a);
+    if (p.splits == 1) return 0;
+    const uint64_t parts = static_cast<uint64_t>(a.tokens) * a.heads * p.splits;
+    return ((parts + 1) & ~1ull) * sizeof(float2) + parts * a.cache.head_dim * sizeof(float);
+}
 
 int dav2_hip_attention_cache_i8(const dav2_attention_cache_i8_args* args, void* stream) {
     if (!args) return hipErrorInvalidValue;
     const dav2_attention_cache_i8_args& a = *args;
     if (a.sequences == 0 || a.tokens == 0 || a.max_query == 0) return hipSuccess;
-    const uint64_t row = static_cast<uint64_t>(a.heads) * a.cache.head_dim;
-    if (!valid_cache(a.cache) || !a.query || !a.output || !aligned16(a.query) || !aligned16(a.output) ||
-        !a.page_table || !a.starts || !a.lengths || a.dtype > DAV2_DTYPE_BF16 || a.sequences > 65535u ||
-        a.tokens > 0x7fffffffu || a.table_pages == 0 || a.table_pages > 0x7fffffffu || a.heads == 0 ||
-        a.heads > 65535u || a.heads % a.cache.kv_heads || a.query_stride % 8 || a.output_stride % 8 ||
-        (a.tokens > 1 && (a.query_stride < row || a.output_stride < row)))
-        return hipErrorInvalidValue;
+    if (!valid(a)) return hipErrorInvalidValue;
     const uint64_t need = dav2_hip_attention_cache_i8_scratch_bytes(args);
     if (need && (!a.scratch || !aligned16(a.scratch) || a.scratch_bytes < need)) return hipErrorInvalidValue;
-    const dim3 grid(a.max_query < a.tokens ? a.max_query : a.tokens, a.heads, a.sequences);
-    with_dtype(a.dtype, [&](auto* e) {
-        dispatch(cache_attention_kernel<std::remove_pointer_t<decltype(e)>>, grid, dim3(64), 0,
-                 static_cast<hipStream_t>(stream), a);
+    const hipStream_t s = static_cast<hipStream_t>(stream);
+    const RowsPlan p = plan_rows(a);
+    const dim3 grid(p.tiles * p.splits, a.cache.kv_heads, a.sequences);
+    return with_dtype(a.dtype, [&](auto* e) -> int {
+        typedef std::remove_pointer_t<decltype(e)> E;
+        if (a.cache.head_dim <= 64) dispatch(cache_rows_kernel<E, 64>, grid, dim3(256), 0, s, a, p.splits, p.tiles);
+        else dispatch(cache_rows_kernel<E, 128>, grid, dim3(256), 0, s, a, p.splits, p.tiles);
+        if (p.splits > 1) {
+            const uint64_t rows = static_cast<uint64_t>(std::min(a.max_query, a.tokens)) * a.heads;
+            const dim3 join(static_cast<uint32_t>(std::min<uint64_t>((rows + 3) / 4, 4096)), a.sequences);
+            dispatch(cache_join_kernel<E>, join, dim3(256), 0, s, a, p.splits);
+        }
+        return hipGetLastError();
     });
-    return hipGetLastError();
 }
 
 }  // extern "C"

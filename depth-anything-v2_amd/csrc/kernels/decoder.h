@@ -60,4 +60,34 @@ DAV2_DEV Sequence sequence_of(const int32_t* starts, const int32_t* lengths, uin
     return q;
 }
 
+typedef _Float16 h4 __attribute__((ext_vector_type(4)));
+typedef _Float16 h8 __attribute__((ext_vector_type(8)));
+typedef __bf16 b8 __attribute__((ext_vector_type(8)));
+typedef float v16f __attribute__((ext_vector_type(16)));
+
+// The running maximum of a softmax before its first score. Finite, so that
+// exp2(maximum - larger maximum) is 0 and never the difference of infinities.
+constexpr float kNoScore = -3.0e38f;
+
+// op over the four lanes l, l ^ 16, l ^ 32, l ^ 48, received by all of them.
+template <typename Op>
+DAV2_DEV float over_groups(float v, Op op) {
+    const auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    v = op(__uint_as_float(a[0]), __uint_as_float(a[1]));
+    const auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return op(__uint_as_float(b[0]), __uint_as_float(b[1]));
+}
+// ... over the two lanes l, l ^ 32.
+template <typename Op>
+DAV2_DEV float over_halves(float v, Op op) {
+    const auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return op(__uint_as_float(b[0]), __uint_as_float(b[1]));
+}
+struct Larger {
+    DAV2_DEV float operator()(float a, float b) const { return fmaxf(a, b); }
+};
+struct Plus {
+    DAV2_DEV float operator()(float a, float b) const { return a + b; }
+};
+
 }  // namespace dav2k
