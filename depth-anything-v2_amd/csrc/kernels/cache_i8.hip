@@ -96,13 +96,23 @@ constexpr float kLog2e = 1.44269504f;
 struct Pages {
     const int32_t* table;  // of one sequence
     uint32_t table_pages, pages, per_page, magic;
-    // the chunk's page, or -1 if there is none; its slot in the page
-    DAV2_DEV int32_t find(uint32_t chunk, uint32_t& slot) const {
-        const uint32_t index = per_page == 1 ? chunk : __umulhi(chunk, magic);
-        slot = (chunk - index * per_page) * 16u;
-        const int32_t page = table[min(index, table_pages - 1u)];
-        return index < table_pages && static_cast<uint32_t>(page) < pages ? page : -1;
+    struct Place {
+        uint32_t index, slot;  // of the page in the table, of the chunk in the page
+        int32_t entry;
+    };
+    // A chunk's place; the entry's load is not waited for here.
+    DAV2_DEV Place find(uint32_t chunk) const {
+        Place p;
+        p.index = per_page == 1 ? chunk : __umulhi(chunk, magic);
+        p.slot = (chunk - p.index * per_page) * 16u;
+        p.entry = table[min(p.index, table_pages - 1u)];
+        return p;
     }
+    DAV2_DEV bool exists(const Place& p) const {
+        return p.index < table_pages && static_cast<uint32_t>(p.entry) < pages;
+    }
+    // the page, or one that may be read in its place
+    DAV2_DEV uint32_t page(const Place& p) const { return exists(p) ? static_cast<uint32_t>(p.entry) : 0u; }
 };
 
 DAV2_DEV Pages pages_of(const dav2_attention_cache_i8_args& a, uint32_t s) {
@@ -146,6 +156,24 @@ DAV2_DEV Parts parts_of(const dav2_attention_cache_i8_args& a, uint32_t splits) 
     return {reinterpret_cast<float*>(stats + ((rows + 1u) & ~uint64_t(1))), stats};
 }
 
+// Token and head of the rows of a tile of 16: row r is token r / group, head
+// r % group. One division for the tile; within it (t < group + 16) a compare,
+// or for small groups a product with 2^16 / group that is exact there.
+struct RowsOf16 {
+    uint32_t token, head, group, magic, most;
+    DAV2_DEV RowsOf16(uint32_t tile, uint32_t group_, uint32_t rows)
+        : token(tile * 16u / group_), group(group_), magic(65536u / group_ + 1u), most(min(rows - tile * 16u, 16u) - 1u) {
+        head = tile * 16u - token * group;
+    }
+    // row i < 16 of the tile; past the last row that one
+    DAV2_DEV void find(uint32_t i, uint32_t& t, uint32_t& h) const {
+        const uint32_t at = head + min(i, most);
+        const uint32_t more = group >= 16u ? (at >= group ? 1u : 0u) : (at * magic) >> 16;
+        t = token + more;
+        h = at - more * group;
+    }
+};
+
 // Few query rows for a cache head (single tokens, drafts): bound by reading
 // the cache. A workgroup has 16 rows (token-major: row r is token r / group,
 // query head r % group) of one sequence and cache head and a run of 64-key
@@ -174,15 +202,17 @@ __global__ __launch_bounds__(256, 2) void cache_rows_kernel(dav2_attention_cache
     const uint32_t group = a.heads / kv_heads;
     const Sequence q = sequence_of(a.starts, a.lengths, s, a.tokens);
     const uint32_t n = static_cast<uint32_t>(q.end - q.begin);
-    const uint64_t rows = static_cast<uint64_t>(n) * group;
+    const uint32_t rows = n * group;  // tokens * heads is below 2^32
     const int64_t span = static_cast<int64_t>(a.table_pages) * page_size;
     const Pages pages = pages_of(a, s);
     const Parts parts = parts_of(a, splits);
 
-    for (uint64_t tile = blockIdx.x / splits; tile * 16u < rows; tile += tiles) {
-        const uint64_t row = tile * 16u + col;
-        const uint32_t token = static_cast<uint32_t>(min(row, rows - 1u) / group);
-        const uint32_t head = h * group + static_cast<uint32_t>(min(row, rows - 1u) % group);
+    for (uint32_t tile = blockIdx.x / splits; tile < (rows + 15u) / 16u; tile += tiles) {
+        const RowsOf16 of(tile, group, rows);
+        const uint32_t row = tile * 16u + col;
+        uint32_t token, head;
+        of.find(col, token, head);
+        head += h * group;
         // keys that this lane's row sees, and the most that a row of the tile does
         auto seen = [&](uint32_t i) {
             int64_t t = q.length;
@@ -190,10 +220,56 @@ __global__ __launch_bounds__(256, 2) void cache_rows_kernel(dav2_attention_cache
             return static_cast<uint32_t>(max(min(t, span), int64_t(0)));
         };
         const uint32_t limit = row < rows ? seen(token) : 0u;
-        const uint32_t most = seen(static_cast<uint32_t>(min(tile * 16u + 15u, rows - 1u) / group));
-        const uint32_t least = seen(static_cast<uint32_t>(tile * 16u / group));
+        uint32_t last_token, last_head;
+        of.find(15u, last_token, last_head);
+        const uint32_t most = seen(last_token), least = seen(of.token);
         const uint32_t blocks = (most + 63u) / 64u, per = (blocks + splits - 1u) / splits;
         const uint32_t first = split * per, last = min(first + per, blocks);
+
+        v4f o[FT];
+#pragma unroll
+        for (int f = 0; f < FT; ++f) o[f] = v4f{0.f, 0.f, 0.f, 0.f};
+        float maximum = kNoScore, sum = 0.0f;  // sum: this lane's keys only
+
+        // A block's keys are loaded when the scores of the block before are
+        // done, its values and scales behind that block's values, its places
+        // in the table a block before those.
+        uint4 kraw[4][KC], vraw[FT];
+        Pages::Place of_key{}, of_value{};  // chunk col / 4 for the keys, chunk g for the values and the scales
+        bool exists = false;
+        float key_scale = 0.0f, value_scale = 1.0f;
+        auto find = [&](uint32_t block) {
+            of_key = pages.find(block * 4u + col / 4u);
+            of_value = pages.find(block * 4u + g);
+        };
+        auto load_keys = [&] {
+            const int8_t* k = a.cache.keys + ((static_cast<uint64_t>(pages.page(of_key)) * kv_heads + h) * page_size +
+                                              of_key.slot + col % 4u) * d + 16u * g;
+#pragma unroll
+            for (int t = 0; t < 4; ++t)
+#pragma unroll
+                for (int kc = 0; kc < KC; ++kc) {
+                    kraw[t][kc] = make_uint4(0, 0, 0, 0);
+                    if (64u * kc + 16u * g < d) kraw[t][kc] = *reinterpret_cast<const uint4*>(k + 4u * t * d + 64 * kc);
+                }
+        };
+        auto load_values = [&] {
+            exists = pages.exists(of_value);
+            const uint64_t plane = static_cast<uint64_t>(pages.page(of_value)) * kv_heads + h;
+            key_scale = a.cache.key_scales[plane];
+            value_scale = a.cache.value_scales[plane];
+            const int8_t* v = a.cache.values + (plane * d + col) * page_size + of_value.slot;
+#pragma unroll
+            for (int f = 0; f < FT; ++f)
+                if (16u * f < d) vraw[f] = *reinterpret_cast<const uint4*>(v + static_cast<uint64_t>(16u * f) * page_size);
+        };
+        uint32_t block = first + wave;
+        if (block < last) {
+            find(block);
+            load_keys();
+            load_values();
+            if (block + 4u < last) find(block + 4u);
+        }
 
         // the right operand of the scores
         h8 qf[NP][KC][2];
@@ -201,14 +277,21 @@ __global__ __launch_bounds__(256, 2) void cache_rows_kernel(dav2_attention_cache
         {
             const E* x = static_cast<const E*>(a.query) + static_cast<uint64_t>(q.begin + token) * a.query_stride +
                          static_cast<uint64_t>(head) * d;
+            typedef E V __attribute__((ext_vector_type(16 / sizeof(E))));
+            constexpr int kVec = 16 / sizeof(E);
             float v[KC][16];
             float largest = 0.0f;
 #pragma unroll
             for (int kc = 0; kc < KC; ++kc)
 #pragma unroll
-                for (int i = 0; i < 16; ++i) {
-                    v[kc][i] = 64u * kc + 16u * g < d ? static_cast<float>(x[64 * kc + 16 * g + i]) : 0.0f;
-                    largest = fmaxf(largest, fabsf(v[kc][i]));
+                for (int j = 0; j < 16 / kVec; ++j) {
+                    V piece{};
+                    if (64u * kc + 16u * g < d) piece = *reinterpret_cast<const V*>(x + 64 * kc + 16 * g + kVec * j);
+#pragma unroll
+                    for (int i = 0; i < kVec; ++i) {
+                        v[kc][kVec * j + i] = static_cast<float>(piece[i]);
+                        largest = fmaxf(largest, fabsf(v[kc][kVec * j + i]));
+                    }
                 }
             largest = over_groups(largest, Larger());
             // up is a power of two; rows of zeros, NaN and infinities stay as they are
@@ -227,44 +310,8 @@ __global__ __launch_bounds__(256, 2) void cache_rows_kernel(dav2_attention_cache
                 }
         }
 
-        v4f o[FT];
-#pragma unroll
-        for (int f = 0; f < FT; ++f) o[f] = v4f{0.f, 0.f, 0.f, 0.f};
-        float maximum = kNoScore, sum = 0.0f;  // sum: this lane's keys only
-
-        uint4 kraw[4][KC];
-        uint32_t slot_v = 0, slot_k = 0;
-        int32_t page_v = -1, page_k = -1;
-        auto find = [&](uint32_t block) {
-            page_k = pages.find(block * 4u + col / 4u, slot_k);
-            page_v = pages.find(block * 4u + g, slot_v);
-        };
-        auto load_keys = [&] {
-            const int8_t* k = a.cache.keys +
-                              ((static_cast<uint64_t>(max(page_k, 0)) * kv_heads + h) * page_size + slot_k + col % 4u) * d +
-                              16u * g;
-#pragma unroll
-            for (int t = 0; t < 4; ++t)
-#pragma unroll
-                for (int kc = 0; kc < KC; ++kc) {
-                    kraw[t][kc] = make_uint4(0, 0, 0, 0);
-                    if (64u * kc + 16u * g < d) kraw[t][kc] = *reinterpret_cast<const uint4*>(k + 4u * t * d + 64 * kc);
-                }
-        };
-        uint32_t block = first + wave;
-        if (block < last) {
-            find(block);
-            load_keys();
-        }
         for (; block < last; block += 4u) {
-            const bool exists = page_v >= 0;
-            const uint64_t plane = static_cast<uint64_t>(max(page_v, 0)) * kv_heads + h;
-            const float key_scale = a.cache.key_scales[plane], value_scale = a.cache.value_scales[plane];
-            uint4 vraw[FT];
-            const int8_t* v = a.cache.values + (plane * d + col) * page_size + slot_v;
-#pragma unroll
-            for (int f = 0; f < FT; ++f)
-                if (16u * f < d) vraw[f] = *reinterpret_cast<const uint4*>(v + static_cast<uint64_t>(16u * f) * page_size);
+            const bool more = block + 4u < last;
             v4f sc[4];
 #pragma unroll
             for (int t = 0; t < 4; ++t) {
@@ -279,10 +326,7 @@ __global__ __launch_bounds__(256, 2) void cache_rows_kernel(dav2_attention_cache
                     }
                 }
             }
-            if (block + 4u < last) {
-                find(block + 4u);
-                load_keys();
-            }
+            if (more) load_keys();
             float exponent, fraction, inverse;
             const uint32_t key0 = block * 64u + 16u * g;  // of this lane's first score
             // a chunk that the row does not see may have any scale, NaN included
@@ -333,6 +377,10 @@ __global__ __launch_bounds__(256, 2) void cache_rows_kernel(dav2_attention_cache
                     o[f] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v1, pf[p][1], o[f], 0, 0, 0);
                 }
             }
+            if (more) {
+                load_values();
+                if (block + 8u < last) find(block + 8u);
+            }
         }
         sum = over_groups(sum, Plus());
 
@@ -354,16 +402,17 @@ __global__ __launch_bounds__(256, 2) void cache_rows_kernel(dav2_attention_cache
         __syncthreads();
         // 16 threads for each of the 16 rows
         const uint32_t out_col = threadIdx.x >> 4, lane16 = threadIdx.x & 15u;
-        const uint64_t out_row = tile * 16u + out_col;
-        if (out_row < rows) {
+        if (tile * 16u + out_col < rows) {
             float all = kNoScore, total = 0.0f;
 #pragma unroll
             for (int w = 0; w < 4; ++w) all = fmaxf(all, shared_max[w][out_col]);
 #pragma unroll
             for (int w = 0; w < 4; ++w)
                 total = fmaf(shared_sum[w][out_col], __builtin_amdgcn_exp2f(shared_max[w][out_col] - all), total);
-            const uint64_t at = static_cast<uint64_t>(q.begin) + out_row / group;
-            const uint32_t out_head = h * group + static_cast<uint32_t>(out_row % group);
+            uint32_t out_token, out_head;
+            of.find(out_col, out_token, out_head);
+            out_head += h * group;
+            const uint64_t at = static_cast<uint64_t>(q.begin) + out_token;
             const float scale = splits > 1 ? 1.0f : total == 0.0f ? 0.0f : 1.0f / total;
             E* y = static_cast<E*>(a.output) + at * a.output_stride + static_cast<uint64_t>(out_head) * d;
             const uint64_t slot = (at * a.heads + out_head) * splits + split;
@@ -379,31 +428,51 @@ __global__ __launch_bounds__(256, 2) void cache_rows_kernel(dav2_attention_cache
     }
 }
 
-// The splits of a row joined: one wave per row.
+// The splits of a row joined: one workgroup per row, thread (i, f) for the
+// four features 4 f .. of splits i, i + 8, ..., so that few loads follow one
+// another (a wave per row that walked over 64 splits took 60 us).
+constexpr uint32_t kMostSplits = 64;
 template <typename E>
 __global__ __launch_bounds__(256) void cache_join_kernel(dav2_attention_cache_i8_args a, uint32_t splits) {
+    __shared__ float share[kMostSplits];
+    __shared__ __attribute__((aligned(16))) v4f partial[8][32];
     const uint32_t lane = threadIdx.x & 63u, d = a.cache.head_dim;
+    const uint32_t f4 = threadIdx.x & 31u, from = threadIdx.x >> 5;
     const Sequence q = sequence_of(a.starts, a.lengths, blockIdx.y, a.tokens);
     const uint64_t rows = static_cast<uint64_t>(q.end - q.begin) * a.heads;
     const Parts parts = parts_of(a, splits);
-    for (uint64_t r = static_cast<uint64_t>(blockIdx.x) * 4u + (threadIdx.x >> 6); r < rows; r += gridDim.x * 4ull) {
+    for (uint64_t r = blockIdx.x; r < rows; r += gridDim.x) {
         const uint64_t token = static_cast<uint64_t>(q.begin) + r / a.heads, head = r % a.heads;
         const uint64_t slot = (token * a.heads + head) * splits;
-        float top = kNoScore;
-        for (uint32_t i = 0; i < splits; ++i) top = fmaxf(top, parts.stats[slot + i].x);
-        float total = 0.0f, o0 = 0.0f, o1 = 0.0f;
-        for (uint32_t i = 0; i < splits; ++i) {
-            const float2 stat = parts.stats[slot + i];
-            const float share = __builtin_amdgcn_exp2f(stat.x - top);
-            total = fmaf(stat.y, share, total);
-            const float* sums = parts.sums + (slot + i) * d;
-            if (lane < d) o0 = fmaf(sums[lane], share, o0);
-            if (lane + 64u < d) o1 = fmaf(sums[lane + 64u], share, o1);
+        const float2 stat = lane < splits ? parts.stats[slot + lane] : make_float2(kNoScore, 0.0f);
+        v4f mine[kMostSplits / 8];
+#pragma unroll
+        for (uint32_t i = 0; i < kMostSplits / 8; ++i) {
+            mine[i] = v4f{0.f, 0.f, 0.f, 0.f};
+            if (from + 8 * i < splits && 4 * f4 < d)
+                mine[i] = *reinterpret_cast<const v4f*>(parts.sums + (slot + from + 8 * i) * d + 4 * f4);
         }
-        E* y = static_cast<E*>(a.output) + token * a.output_stride + head * d;
-        const float scale = total == 0.0f ? 0.0f : 1.0f / total;
-        if (lane < d) y[lane] = static_cast<E>(o0 * scale);
-        if (lane + 64u < d) y[lane + 64u] = static_cast<E>(o1 * scale);
+        const float top = wave_max(stat.x);
+        const float weight = __builtin_amdgcn_exp2f(stat.x - top);  // 1 for splits that saw nothing, if all did not
+        const float total = wave_sum_tree(stat.y * weight);
+        __syncthreads();  // the row before has been read
+        if (threadIdx.x < kMostSplits) share[lane] = weight;
+        __syncthreads();
+        v4f sum = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (uint32_t i = 0; i < kMostSplits / 8; ++i)
+            if (from + 8 * i < splits) sum += mine[i] * share[from + 8 * i];
+        partial[from][f4] = sum;
+        __syncthreads();
+        if (threadIdx.x < 32 && 4 * f4 < d) {
+            sum = partial[0][f4];
+#pragma unroll
+            for (int i = 1; i < 8; ++i) sum += partial[i][f4];
+            E* y = static_cast<E*>(a.output) + token * a.output_stride + head * d + 4 * f4;
+            const float scale = total == 0.0f ? 0.0f : 1.0f / total;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) y[i] = static_cast<E>(sum[i] * scale);
+        }
     }
 }
 
@@ -412,26 +481,31 @@ bool valid(const dav2_attention_cache_i8_args& a) {
     return valid_cache(a.cache) && a.query && a.output && aligned16(a.query) && aligned16(a.output) && a.page_table &&
            a.starts && a.lengths && a.dtype <= DAV2_DTYPE_BF16 && a.sequences <= 65535u && a.tokens <= 0x7fffffffu &&
            a.table_pages > 0 && a.table_pages <= 0x7fffffffu && a.heads > 0 && a.heads <= 65535u &&
-           a.heads % a.cache.kv_heads == 0 && a.query_stride % 8 == 0 && a.output_stride % 8 == 0 &&
+           a.heads % a.cache.kv_heads == 0 && static_cast<uint64_t>(a.tokens) * a.heads <= 0xfffffff0ull &&
+           a.query_stride % 8 == 0 && a.output_stride % 8 == 0 &&
            (a.tokens == 1 || (a.query_stride >= row && a.output_stride >= row));
 }
 
-// How a call is dealt out: row tiles, and splits of the keys so that the chip
-// is full where sequences, heads and tiles are few.
+// How a call is dealt out: row tiles, and splits of the keys. Two workgroups
+// share a CU, so up to 512 all run at once: split as far as that goes, down to
+// 128 keys (two waves' blocks) each. Beyond it a further split only evens out
+// sequences of different lengths and pays for long ones: up to 2048 workgroups
+// of at least 2048 keys. Heads 32 of 8, 128 features, us: 40 sequences of 300
+// keys 13.2 whole, 19.6 in two (640 workgroups); 8 of 4096 19.5 in 8 (512
+// workgroups), 24.0 in 16; 32 of up to 32768 257 in 2 (512), 244 in 4, 242 in
+// 8; one token over 1370 keys, 16 heads of 64, 11.9 in 2, 10.4 in 5, 9.2 in 10.
 struct RowsPlan {
     uint32_t tiles, splits;
 };
 RowsPlan plan_rows(const dav2_attention_cache_i8_args& a) {
-    constexpr uint64_t kWorkgroups = 1024;  // wanted: two for each of 256 CUs at a time, twice over
-    constexpr uint32_t kLeastKeys = 256;    // of a split: a block for each wave
     RowsPlan p{1, 1};
     if (a.cache.kv_heads == 0 || a.heads < a.cache.kv_heads || a.sequences == 0 || a.max_query == 0) return p;
-    const uint64_t query = std::min(a.max_query, a.tokens);
-    const uint64_t rows = query * (a.heads / a.cache.kv_heads);
+    const uint64_t rows = static_cast<uint64_t>(std::min(a.max_query, a.tokens)) * (a.heads / a.cache.kv_heads);
     p.tiles = static_cast<uint32_t>(std::min<uint64_t>((rows + 15) / 16, 4096));
-    const uint64_t have = static_cast<uint64_t>(p.tiles) * a.cache.kv_heads * a.sequences;
-    const uint64_t most = std::max<uint64_t>(1, a.max_length / kLeastKeys);
-    p.splits = static_cast<uint32_t>(std::clamp<uint64_t>(kWorkgroups / std::max<uint64_t>(have, 1), 1, std::min<uint64_t>(most, 64)));
+    const uint64_t have = std::max<uint64_t>(1, static_cast<uint64_t>(p.tiles) * a.cache.kv_heads * a.sequences);
+    const uint64_t resident = std::min<uint64_t>(512 / have, a.max_length / 128);
+    const uint64_t even = std::min<uint64_t>(2048 / have, a.max_length / 2048);
+    p.splits = static_cast<uint32_t>(std::clamp<uint64_t>(std::max(resident, even), 1, kMostSplits));
     return p;
 }
 
@@ -484,7 +558,7 @@ int dav2_hip_attention_cache_i8(const dav2_attention_cache_i8_args* args, void* 
         else dispatch(cache_rows_kernel<E, 128>, grid, dim3(256), 0, s, a, p.splits, p.tiles);
         if (p.splits > 1) {
             const uint64_t rows = static_cast<uint64_t>(std::min(a.max_query, a.tokens)) * a.heads;
-            const dim3 join(static_cast<uint32_t>(std::min<uint64_t>((rows + 3) / 4, 4096)), a.sequences);
+            const dim3 join(static_cast<uint32_t>(std::min<uint64_t>(rows, 4096)), a.sequences);
             dispatch(cache_join_kernel<E>, join, dim3(256), 0, s, a, p.splits);
         }
         return hipGetLastError();
