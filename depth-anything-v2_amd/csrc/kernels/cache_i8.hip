@@ -156,19 +156,20 @@ DAV2_DEV Parts parts_of(const dav2_attention_cache_i8_args& a, uint32_t splits) 
     return {reinterpret_cast<float*>(stats + ((rows + 1u) & ~uint64_t(1))), stats};
 }
 
-// Token and head of the rows of a tile of 16: row r is token r / group, head
-// r % group. One division for the tile; within it (t < group + 16) a compare,
-// or for small groups a product with 2^16 / group that is exact there.
-struct RowsOf16 {
+// Token and head of N rows from row `first` on: row r is token r / group, head
+// r % group. One division for all; behind it (t < group + N) a compare, or for
+// groups below N <= 128 a product with 2^16 / group that is exact there.
+template <uint32_t N>
+struct Rows {
     uint32_t token, head, group, magic, most;
-    DAV2_DEV RowsOf16(uint32_t tile, uint32_t group_, uint32_t rows)
-        : token(tile * 16u / group_), group(group_), magic(65536u / group_ + 1u), most(min(rows - tile * 16u, 16u) - 1u) {
-        head = tile * 16u - token * group;
+    DAV2_DEV Rows(uint32_t first, uint32_t group_, uint32_t rows)
+        : token(first / group_), group(group_), magic(65536u / group_ + 1u), most(min(rows - first, N) - 1u) {
+        head = first - token * group;
     }
-    // row i < 16 of the tile; past the last row that one
+    // row first + i, i < N; past the last row that one
     DAV2_DEV void find(uint32_t i, uint32_t& t, uint32_t& h) const {
         const uint32_t at = head + min(i, most);
-        const uint32_t more = group >= 16u ? (at >= group ? 1u : 0u) : (at * magic) >> 16;
+        const uint32_t more = group >= N ? (at >= group ? 1u : 0u) : (at * magic) >> 16;
         t = token + more;
         h = at - more * group;
     }
@@ -208,7 +209,7 @@ __global__ __launch_bounds__(256, 2) void cache_rows_kernel(dav2_attention_cache
     const Parts parts = parts_of(a, splits);
 
     for (uint32_t tile = blockIdx.x / splits; tile < (rows + 15u) / 16u; tile += tiles) {
-        const RowsOf16 of(tile, group, rows);
+        const Rows<16> of(tile * 16u, group, rows);
         const uint32_t row = tile * 16u + col;
         uint32_t token, head;
         of.find(col, token, head);
@@ -302,7 +303,7 @@ __global__ __launch_bounds__(256, 2) void cache_rows_kernel(dav2_attention_cache
             for (int kc = 0; kc < KC; ++kc)
 #pragma unroll
                 for (int i = 0; i < 16; ++i) {
-                    const float y = ldexpf(v[kc][i], e) * sign;
+                    const float y = keep_fp32(ldexpf(v[kc][i], e) * sign);
                     const _Float16 hi = static_cast<_Float16>(y);
                     qf[0][kc][i >> 3][i & 7] = hi;
                     if constexpr (kFloat)
@@ -360,7 +361,7 @@ __global__ __launch_bounds__(256, 2) void cache_rows_kernel(dav2_attention_cache
                 for (int r = 0; r < 4; ++r) {
                     const float w = __builtin_amdgcn_exp2f(sc[t][r] - maximum);
                     part += w;
-                    const float y = w * fraction;
+                    const float y = kFloat ? keep_fp32(w * fraction) : w * fraction;  // hi and lo of one rounded product
                     const _Float16 hi = static_cast<_Float16>(y);
                     pf[0][t >> 1][4 * (t & 1) + r] = hi;
                     if constexpr (kFloat)
@@ -428,6 +429,319 @@ __global__ __launch_bounds__(256, 2) void cache_rows_kernel(dav2_attention_cache
     }
 }
 
+// Many query rows for a cache head (prompts): bound by the matrix cores, the
+// exponentials and LDS. A workgroup has 128 rows of one sequence and cache head,
+// 32 for each of four waves, and goes through the keys 64 at a time: codes are
+// widened to binary16 once for all waves on their way into LDS (two buffers,
+// one barrier for a tile; the next tile's codes are in registers meanwhile, its
+// places in the table a tile before).
+//
+// S^T = K Q^T and O^T = V^T P^T on v_mfma_f32_32x32x16_f16. Lane l holds, for
+// query l % 32, the scores of keys 8 (r / 4) + 4 (l / 32) + r % 4 of a 32-key
+// block in registers r; registers 8 t .. 8 t + 7 are the right operand of the
+// second product's step t if V^T holds its keys in that order, which their
+// place in LDS gives them: keys 0-3, 8-11 of a chunk, then 4-7, 12-15. Eight
+// registers are one 16-token chunk, so scales are uniform for them.
+template <typename E, int HEAD>
+__global__ __launch_bounds__(256, 2) void cache_tiles_kernel(dav2_attention_cache_i8_args a, uint32_t splits,
+                                                             uint32_t tiles) {
+    constexpr bool kFloat = std::is_same_v<E, float>;
+    constexpr int KS = HEAD / 16, FB = HEAD / 32, NP = kFloat ? 2 : 1;
+    constexpr int kPieces = HEAD / 64;   // of 16 codes, for each thread and tile: keys, and values
+    constexpr int kRow = HEAD * 2;       // bytes of a key row in LDS
+    // rescale when a score passes the running maximum by this: weights stay
+    // below 2^6, far inside binary16, and most tiles leave the sums alone
+    constexpr float kSlack = 6.0f;
+    __shared__ __attribute__((aligned(16))) int8_t lds_keys[2][64 * kRow];
+    __shared__ __attribute__((aligned(16))) int8_t lds_values[2][HEAD * 128];
+    __shared__ __attribute__((aligned(16))) v4f lds_scales[2][4];  // of a chunk: key scale, log2 / exponent, inverse, fraction
+    const uint32_t lane = threadIdx.x & 63u, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const uint32_t col = lane & 31u, hf = lane >> 5;
+    const uint32_t kv_heads = a.cache.kv_heads, d = a.cache.head_dim, page_size = a.cache.page_size;
+    const uint32_t s = blockIdx.x / kv_heads, h = blockIdx.x - s * kv_heads, group = a.heads / kv_heads;
+    const uint32_t split = blockIdx.y % splits;
+    const Sequence q = sequence_of(a.starts, a.lengths, s, a.tokens);
+    const uint32_t n = static_cast<uint32_t>(q.end - q.begin), rows = n * group;
+    const int64_t span = static_cast<int64_t>(a.table_pages) * page_size;
+    const Pages pages = pages_of(a, s);
+    const Parts parts = parts_of(a, splits);
+    const uint32_t row_tiles = (rows + 127u) / 128u;
+    auto seen = [&](uint32_t i) {
+        int64_t t = q.length;
+        if (a.causal) t += 1 + static_cast<int64_t>(i) - n;
+        return static_cast<uint32_t>(max(min(t, span), int64_t(0)));
+    };
+
+    // the last rows first: under a causal mask they see the most keys
+    for (uint32_t turn = blockIdx.y / splits; turn < row_tiles; turn += tiles) {
+        const uint32_t tile = row_tiles - 1u - turn;
+        const uint32_t row0 = tile * 128u + wave * 32u;  // of this wave
+        const bool any_row = row0 < rows;
+        const Rows<32> of(any_row ? row0 : tile * 128u, group, rows);
+        uint32_t token, head, last_token, last_head;
+        of.find(col, token, head);
+        of.find(31u, last_token, last_head);
+        head += h * group;
+        const uint32_t limit = row0 + col < rows ? seen(token) : 0u;
+        const uint32_t wave_most = any_row ? seen(last_token) : 0u, wave_least = seen(of.token);
+        const uint32_t most = seen((min(tile * 128u + 128u, rows) - 1u) / group);
+        const uint32_t blocks = (most + 63u) / 64u, per = (blocks + splits - 1u) / splits;
+        const uint32_t first = split * per, last = min(first + per, blocks);
+
+        // staging
+        uint4 key_codes[kPieces], value_codes[kPieces];
+        Pages::Place of_key[kPieces]{}, of_value{};
+        float key_scale = 0.0f, value_scale = 1.0f;
+        bool exists = false;
+        const uint32_t key_chunk = threadIdx.x % (HEAD / 16), key_row = threadIdx.x / (HEAD / 16);
+        const uint32_t value_chunk = threadIdx.x & 3u, value_row = threadIdx.x >> 2;
+        constexpr uint32_t kKeyStep = 256u / (HEAD / 16);
+        auto find = [&](uint32_t block) {
+#pragma unroll
+            for (int i = 0; i < kPieces; ++i) of_key[i] = pages.find(block * 4u + (key_row + kKeyStep * i) / 16u);
+            of_value = pages.find(block * 4u + value_chunk);
+        };
+        auto load = [&] {
+#pragma unroll
+            for (int i = 0; i < kPieces; ++i) {
+                const uint64_t plane = static_cast<uint64_t>(pages.page(of_key[i])) * kv_heads + h;
+                const int8_t* k = a.cache.keys +
+                                  (plane * page_size + of_key[i].slot + (key_row + kKeyStep * i) % 16u) * d + 16u * key_chunk;
+                if (16u * key_chunk < d) key_codes[i] = *reinterpret_cast<const uint4*>(k);
+            }
+            exists = pages.exists(of_value);
+            const uint64_t plane = static_cast<uint64_t>(pages.page(of_value)) * kv_heads + h;
+#pragma unroll
+            for (int i = 0; i < kPieces; ++i) {
+                const uint32_t f = value_row + 64u * i;
+                if (f < d)
+                    value_codes[i] = *reinterpret_cast<const uint4*>(a.cache.values + (plane * d + f) * page_size + of_value.slot);
+            }
+            if (threadIdx.x < 4) {
+                key_scale = a.cache.key_scales[plane];
+                value_scale = a.cache.value_scales[plane];
+            }
+        };
+        auto store = [&](uint32_t buffer) {
+#pragma unroll
+            for (int i = 0; i < kPieces; ++i) {
+                const uint4 k = key_codes[i], v = value_codes[i];
+                const uint32_t r = key_row + kKeyStep * i, f = value_row + 64u * i;
+                if (16u * key_chunk < d) {
+                    *reinterpret_cast<h8*>(lds_keys[buffer] + swz<kRow>(r, 2u * key_chunk)) = widen(k.x, k.y);
+                    *reinterpret_cast<h8*>(lds_keys[buffer] + swz<kRow>(r, 2u * key_chunk + 1u)) = widen(k.z, k.w);
+                }
+                if (f < d) {
+                    *reinterpret_cast<h8*>(lds_values[buffer] + swz<128>(f, 2u * value_chunk)) = widen(v.x, v.z);
+                    *reinterpret_cast<h8*>(lds_values[buffer] + swz<128>(f, 2u * value_chunk + 1u)) = widen(v.y, v.w);
+                }
+            }
+            if (threadIdx.x < 4) {
+                float exponent, fraction, inverse;
+                split_scale(value_scale, exponent, fraction, inverse);
+                v4f c = {key_scale, exponent, inverse, fraction};
+                if constexpr (!kFloat) {
+                    // the weights take the whole scale: exact to 2^-22 of them
+                    c[1] = exponent + __builtin_amdgcn_logf(fraction);
+                    c[2] = inverse / fraction;
+                }
+                if (!exists) c = v4f{0.f, 0.f, 0.f, 0.f};
+                c[3] = exists ? fraction : 0.0f;
+                lds_scales[buffer][threadIdx.x] = c;
+            }
+        };
+        // places of the table that a tile past the last may not be asked for
+        __syncthreads();  // the row tile before has been read
+        if (first < last) {
+            find(first);
+            load();
+        }
+
+        // the right operand of the scores
+        h8 qf[NP][KS];
+        float factor;
+        {
+            const E* x = static_cast<const E*>(a.query) + static_cast<uint64_t>(q.begin + token) * a.query_stride +
+                         static_cast<uint64_t>(head) * d + 8u * hf;
+            typedef E V __attribute__((ext_vector_type(16 / sizeof(E))));
+            constexpr int kVec = 16 / sizeof(E);
+            V raw[KS][8 / kVec];
+            float largest = 0.0f;
+#pragma unroll
+            for (int k = 0; k < KS; ++k)
+#pragma unroll
+                for (int j = 0; j < 8 / kVec; ++j) {
+                    raw[k][j] = V{};
+                    if (16u * k < d) raw[k][j] = *reinterpret_cast<const V*>(x + 16 * k + kVec * j);
+#pragma unroll
+                    for (int i = 0; i < kVec; ++i) largest = fmaxf(largest, fabsf(static_cast<float>(raw[k][j][i])));
+                }
+            largest = over_halves(largest, Larger());
+            const int e = largest > 0.0f && largest < INFINITY ? 14 - ilogbf(largest) : 0;
+            const float sign = a.scale < 0.0f ? -1.0f : 1.0f;
+            factor = ldexpf(fabsf(a.scale) * kLog2e, -e);
+#pragma unroll
+            for (int k = 0; k < KS; ++k)
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    const float y = keep_fp32(ldexpf(static_cast<float>(raw[k][i / kVec][i % kVec]), e) * sign);
+                    const _Float16 hi = static_cast<_Float16>(y);
+                    qf[0][k][i] = hi;
+                    if constexpr (kFloat) qf[1][k][i] = static_cast<_Float16>(y - static_cast<float>(hi));
+                }
+        }
+
+        v16f o[FB];
+#pragma unroll
+        for (int f = 0; f < FB; ++f)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) o[f][r] = 0.0f;
+        float maximum = kNoScore, sum = 0.0f;  // sum: this lane's keys only
+
+        if (first < last) {
+            store(0);
+            if (first + 1u < last) {
+                find(first + 1u);
+                load();
+                if (first + 2u < last) find(first + 2u);
+            }
+        }
+        __syncthreads();
+        for (uint32_t block = first; block < last; ++block) {
+            const uint32_t buffer = (block - first) & 1u;
+            if (block + 1u < last) {
+                store(buffer ^ 1u);
+                if (block + 2u < last) {
+                    load();
+                    if (block + 3u < last) find(block + 3u);
+                }
+            }
+            const uint32_t k0 = block * 64u;
+            if (k0 < wave_most) {
+                v16f sc[2];
+#pragma unroll
+                for (int b = 0; b < 2; ++b) {
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) sc[b][r] = 0.0f;
+#pragma unroll
+                    for (int k = 0; k < KS; ++k) {
+                        if (16u * k >= d) continue;
+                        const h8 kf = *reinterpret_cast<const h8*>(lds_keys[buffer] + swz<kRow>(32u * b + col, 2u * k + hf));
+#pragma unroll
+                        for (int p = 0; p < NP; ++p)
+                            sc[b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf, qf[p][k], sc[b], 0, 0, 0);
+                    }
+                }
+                // chunk t of the tile: registers 8 (t % 2) .. of block t / 2
+                float c[4], shift[4], inverse[4], fraction[4];
+                bool whole = k0 + 64u <= wave_least;
+#pragma unroll
+                for (int t = 0; t < 4; ++t) {
+                    const v4f of_chunk = lds_scales[buffer][t];
+                    c[t] = of_chunk[0] * factor;
+                    shift[t] = of_chunk[1];
+                    inverse[t] = of_chunk[2];
+                    fraction[t] = of_chunk[3];
+                    whole = whole && of_chunk[3] != 0.0f;  // else the page does not exist
+                }
+                if (!__all(whole)) {
+#pragma unroll
+                    for (int t = 0; t < 4; ++t) {
+                        const bool here = fraction[t] != 0.0f;
+#pragma unroll
+                        for (int r = 0; r < 8; ++r) {
+                            const float x = fmaf(sc[t >> 1][8 * (t & 1) + r], c[t], shift[t]);
+                            const uint32_t key = k0 + 16u * t + 8u * (r >> 2) + 4u * hf + (r & 3);
+                            sc[t >> 1][8 * (t & 1) + r] = here && key < limit ? x : -INFINITY;
+                        }
+                        c[t] = 1.0f;
+                        shift[t] = 0.0f;
+                        // a chunk that the row does not see may have any scale, NaN included
+                        if (!here || k0 + 16u * t >= limit) inverse[t] = fraction[t] = 1.0f;
+                    }
+                }
+                float largest = kNoScore;
+#pragma unroll
+                for (int t = 0; t < 4; ++t) {
+                    float m = sc[t >> 1][8 * (t & 1)];
+#pragma unroll
+                    for (int r = 1; r < 8; ++r) m = fmaxf(m, sc[t >> 1][8 * (t & 1) + r]);
+                    largest = fmaxf(largest, fmaf(m, c[t], shift[t]));
+                }
+                largest = over_halves(largest, Larger());
+                if (__any(largest > maximum + kSlack)) {
+                    const float grown = fmaxf(maximum, largest);
+                    const float keep = __builtin_amdgcn_exp2f(maximum - grown);
+                    maximum = grown;
+                    sum *= keep;
+#pragma unroll
+                    for (int f = 0; f < FB; ++f)
+#pragma unroll
+                        for (int r = 0; r < 16; ++r) o[f][r] *= keep;
+                }
+                h8 pf[NP][4];
+#pragma unroll
+                for (int t = 0; t < 4; ++t) {
+                    float part = 0.0f;
+                    const float less = shift[t] - maximum;
+#pragma unroll
+                    for (int r = 0; r < 8; ++r) {
+                        const float w = __builtin_amdgcn_exp2f(fmaf(sc[t >> 1][8 * (t & 1) + r], c[t], less));
+                        part += w;
+                        if constexpr (kFloat) {
+                            const float y = keep_fp32(w * fraction[t]);  // hi and lo of one rounded product
+                            const _Float16 hi = static_cast<_Float16>(y);
+                            pf[0][t][r] = hi;
+                            pf[1][t][r] = static_cast<_Float16>(y - static_cast<float>(hi));
+                        } else {
+                            pf[0][t][r] = static_cast<_Float16>(w);
+                        }
+                    }
+                    sum = fmaf(part, inverse[t], sum);
+                }
+#pragma unroll
+                for (int f = 0; f < FB; ++f) {
+                    if (32u * f >= d) continue;
+#pragma unroll
+                    for (int t = 0; t < 4; ++t) {
+                        const h8 vf = *reinterpret_cast<const h8*>(lds_values[buffer] + swz<128>(32u * f + col, 2u * t + hf));
+#pragma unroll
+                        for (int p = 0; p < NP; ++p)
+                            o[f] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf, pf[p][t], o[f], 0, 0, 0);
+                    }
+                }
+            }
+            __syncthreads();
+        }
+        sum = over_halves(sum, Plus());
+        // register r of o[f]: feature 32 f + 8 (r / 4) + 4 hf + r % 4 of row col
+        if (row0 + col < rows) {
+            const uint64_t at = static_cast<uint64_t>(q.begin) + token;
+            const uint64_t slot = (at * a.heads + head) * splits + split;
+            const float scale = sum == 0.0f ? 0.0f : 1.0f / sum;
+            typedef E V4 __attribute__((ext_vector_type(4)));
+            E* y = static_cast<E*>(a.output) + at * a.output_stride + static_cast<uint64_t>(head) * d;
+#pragma unroll
+            for (int f = 0; f < FB; ++f)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    const uint32_t feature = 32u * f + 8u * r + 4u * hf;
+                    if (feature >= d) continue;
+                    if (splits > 1) {
+                        *reinterpret_cast<v4f*>(parts.sums + slot * d + feature) =
+                            v4f{o[f][4 * r], o[f][4 * r + 1], o[f][4 * r + 2], o[f][4 * r + 3]};
+                    } else {
+                        V4 out;
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) out[i] = static_cast<E>(o[f][4 * r + i] * scale);
+                        *reinterpret_cast<V4*>(y + feature) = out;
+                    }
+                }
+            if (splits > 1 && hf == 0) parts.stats[slot] = make_float2(maximum, sum);
+        }
+    }
+}
+
 // The splits of a row joined: one workgroup per row, thread (i, f) for the
 // four features 4 f .. of splits i, i + 8, ..., so that few loads follow one
 // another (a wave per row that walked over 64 splits took 60 us).
@@ -481,7 +795,8 @@ bool valid(const dav2_attention_cache_i8_args& a) {
     return valid_cache(a.cache) && a.query && a.output && aligned16(a.query) && aligned16(a.output) && a.page_table &&
            a.starts && a.lengths && a.dtype <= DAV2_DTYPE_BF16 && a.sequences <= 65535u && a.tokens <= 0x7fffffffu &&
            a.table_pages > 0 && a.table_pages <= 0x7fffffffu && a.heads > 0 && a.heads <= 65535u &&
-           a.heads % a.cache.kv_heads == 0 && static_cast<uint64_t>(a.tokens) * a.heads <= 0xfffffff0ull &&
+           a.heads % a.cache.kv_heads == 0 && static_cast<uint64_t>(a.tokens) * a.heads <= 0xffffff00ull &&
+           static_cast<uint64_t>(a.sequences) * a.cache.kv_heads <= 0x7fffffull &&
            a.query_stride % 8 == 0 && a.output_stride % 8 == 0 &&
            (a.tokens == 1 || (a.query_stride >= row && a.output_stride >= row));
 }
@@ -494,17 +809,20 @@ bool valid(const dav2_attention_cache_i8_args& a) {
 // keys 13.2 whole, 19.6 in two (640 workgroups); 8 of 4096 19.5 in 8 (512
 // workgroups), 24.0 in 16; 32 of up to 32768 257 in 2 (512), 244 in 4, 242 in
 // 8; one token over 1370 keys, 16 heads of 64, 11.9 in 2, 10.4 in 5, 9.2 in 10.
-struct RowsPlan {
+struct Plan {
+    bool tiled;  // cache_tiles_kernel, otherwise cache_rows_kernel
     uint32_t tiles, splits;
 };
-RowsPlan plan_rows(const dav2_attention_cache_i8_args& a) {
-    RowsPlan p{1, 1};
+Plan plan_of(const dav2_attention_cache_i8_args& a) {
+    Plan p{false, 1, 1};
     if (a.cache.kv_heads == 0 || a.heads < a.cache.kv_heads || a.sequences == 0 || a.max_query == 0) return p;
     const uint64_t rows = static_cast<uint64_t>(std::min(a.max_query, a.tokens)) * (a.heads / a.cache.kv_heads);
-    p.tiles = static_cast<uint32_t>(std::min<uint64_t>((rows + 15) / 16, 4096));
+    p.tiled = rows > 32;
+    const uint32_t tile = p.tiled ? 128 : 16;
+    p.tiles = static_cast<uint32_t>(std::min<uint64_t>((rows + tile - 1) / tile, p.tiled ? 512 : 4096));
     const uint64_t have = std::max<uint64_t>(1, static_cast<uint64_t>(p.tiles) * a.cache.kv_heads * a.sequences);
     const uint64_t resident = std::min<uint64_t>(512 / have, a.max_length / 128);
-    const uint64_t even = std::min<uint64_t>(2048 / have, a.max_length / 2048);
+    const uint64_t even = p.tiled ? 1 : std::min<uint64_t>(2048 / have, a.max_length / 2048);
     p.splits = static_cast<uint32_t>(std::clamp<uint64_t>(std::max(resident, even), 1, kMostSplits));
     return p;
 }
@@ -536,7 +854,7 @@ int dav2_hip_cache_store_i8(const dav2_cache_store_i8_args* args, void* stream) 
 uint64_t dav2_hip_attention_cache_i8_scratch_bytes(const dav2_attention_cache_i8_args* args) {
     if (!args) return 0;
     const dav2_attention_cache_i8_args& a = *args;
-    const RowsPlan p = plan_rows(a);
+    const Plan p = plan_of(a);
     if (p.splits == 1) return 0;
     const uint64_t parts = static_cast<uint64_t>(a.tokens) * a.heads * p.splits;
     return ((parts + 1) & ~1ull) * sizeof(float2) + parts * a.cache.head_dim * sizeof(float);
@@ -550,11 +868,15 @@ int dav2_hip_attention_cache_i8(const dav2_attention_cache_i8_args* args, void* 
     const uint64_t need = dav2_hip_attention_cache_i8_scratch_bytes(args);
     if (need && (!a.scratch || !aligned16(a.scratch) || a.scratch_bytes < need)) return hipErrorInvalidValue;
     const hipStream_t s = static_cast<hipStream_t>(stream);
-    const RowsPlan p = plan_rows(a);
-    const dim3 grid(p.tiles * p.splits, a.cache.kv_heads, a.sequences);
+    const Plan p = plan_of(a);
+    const dim3 grid = p.tiled ? dim3(a.cache.kv_heads * a.sequences, p.tiles * p.splits)
+                              : dim3(p.tiles * p.splits, a.cache.kv_heads, a.sequences);
     return with_dtype(a.dtype, [&](auto* e) -> int {
         typedef std::remove_pointer_t<decltype(e)> E;
-        if (a.cache.head_dim <= 64) dispatch(cache_rows_kernel<E, 64>, grid, dim3(256), 0, s, a, p.splits, p.tiles);
+        if (p.tiled) {
+            if (a.cache.head_dim <= 64) dispatch(cache_tiles_kernel<E, 64>, grid, dim3(256), 0, s, a, p.splits, p.tiles);
+            else dispatch(cache_tiles_kernel<E, 128>, grid, dim3(256), 0, s, a, p.splits, p.tiles);
+        } else if (a.cache.head_dim <= 64) dispatch(cache_rows_kernel<E, 64>, grid, dim3(256), 0, s, a, p.splits, p.tiles);
         else dispatch(cache_rows_kernel<E, 128>, grid, dim3(256), 0, s, a, p.splits, p.tiles);
         if (p.splits > 1) {
             const uint64_t rows = static_cast<uint64_t>(std::min(a.max_query, a.tokens)) * a.heads;

@@ -415,6 +415,29 @@ def test_cache_attention_not_finite(gpu, pkg, lib, queries, dtype):
     assert out[:queries].isnan().all() and out[queries:].isfinite().all()
 
 
+@pytest.mark.parametrize("queries", [3, 60])
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_cache_attention_not_finite_ahead(gpu, pkg, lib, queries, dtype):
+    # a page that only the later rows of a tile see is not finite: the earlier rows are untouched
+    torch = gpu
+    cache = random_cache(torch, 3, 8, 2, 16, 64)
+    table = ints(torch, [[0, 1, 2, 3, 4, 5]])
+    total, last = 80, 64  # the page of tokens 64 .. 79
+    cache[2][4, 0], cache[3][4, 1] = math.nan, math.inf
+    q = rand(torch, 8, queries, 4, 64, dtype=dtype)
+    out = torch.zeros_like(q)
+    total = last + 2  # the last two rows see into it
+    starts, lengths = ints(torch, [0, queries]), ints(torch, [total])
+    a, keep = attend_args(torch, pkg, lib, cache, q, out, table, starts, lengths, True, dtype, 0.125)
+    launch(torch, lib, "dav2_hip_attention_cache_i8", a)
+    torch.cuda.synchronize()
+    assert out[-2:].isnan().all() and out[:-2].isfinite().all()
+    fine = [t.clone() for t in cache]
+    fine[2][4], fine[3][4] = 0.01, 0.01
+    want, bound = ref.attend(q, fine, table, starts, lengths, True, 0.125, dtype)
+    ref.assert_within(out[:-2], want[:-2], bound[:-2])
+
+
 # ---- cross attention -------------------------------------------------------------------------
 
 
