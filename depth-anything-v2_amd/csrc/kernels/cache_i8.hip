@@ -89,8 +89,6 @@ __global__ __launch_bounds__(256) void cache_store_kernel(dav2_cache_store_i8_ar
 // (two parts in the fp32 mode) keeps its precision whatever the pages' scales
 // are; L is summed in fp32 from the unrounded w.
 
-constexpr float kLog2e = 1.44269504f;
-
 // Page and slot of a 16-token chunk; magic = ceil(2^32 / chunks per page),
 // which divides every chunk below 2^28 exactly (chunks per page <= 16).
 struct Pages {
@@ -144,36 +142,9 @@ DAV2_DEV void split_scale(float scale, float& exponent, float& fraction, float& 
     inverse = ldexpf(1.0f, -e);
 }
 
-// What splits of the keys leave for the join: per row (token * heads + head)
-// and split, the output's sums and {maximum, L}.
-struct Parts {
-    float* sums;   // [rows][splits][head_dim]
-    float2* stats; // [rows][splits]
-};
 DAV2_DEV Parts parts_of(const dav2_attention_cache_i8_args& a, uint32_t splits) {
-    const uint64_t rows = static_cast<uint64_t>(a.tokens) * a.heads * splits;
-    float2* stats = static_cast<float2*>(a.scratch);
-    return {reinterpret_cast<float*>(stats + ((rows + 1u) & ~uint64_t(1))), stats};
+    return parts_at(a.scratch, static_cast<uint64_t>(a.tokens) * a.heads * splits);
 }
-
-// Token and head of N rows from row `first` on: row r is token r / group, head
-// r % group. One division for all; behind it (t < group + N) a compare, or for
-// groups below N <= 128 a product with 2^16 / group that is exact there.
-template <uint32_t N>
-struct Rows {
-    uint32_t token, head, group, magic, most;
-    DAV2_DEV Rows(uint32_t first, uint32_t group_, uint32_t rows)
-        : token(first / group_), group(group_), magic(65536u / group_ + 1u), most(min(rows - first, N) - 1u) {
-        head = first - token * group;
-    }
-    // row first + i, i < N; past the last row that one
-    DAV2_DEV void find(uint32_t i, uint32_t& t, uint32_t& h) const {
-        const uint32_t at = head + min(i, most);
-        const uint32_t more = group >= N ? (at >= group ? 1u : 0u) : (at * magic) >> 16;
-        t = token + more;
-        h = at - more * group;
-    }
-};
 
 // Few query rows for a cache head (single tokens, drafts): bound by reading
 // the cache. A workgroup has 16 rows (token-major: row r is token r / group,
@@ -742,51 +713,16 @@ __global__ __launch_bounds__(256, 2) void cache_tiles_kernel(dav2_attention_cach
     }
 }
 
-// The splits of a row joined: one workgroup per row, thread (i, f) for the
-// four features 4 f .. of splits i, i + 8, ..., so that few loads follow one
-// another (a wave per row that walked over 64 splits took 60 us).
-constexpr uint32_t kMostSplits = 64;
+// The splits of the sequences' rows joined: one workgroup per row.
 template <typename E>
 __global__ __launch_bounds__(256) void cache_join_kernel(dav2_attention_cache_i8_args a, uint32_t splits) {
-    __shared__ float share[kMostSplits];
-    __shared__ __attribute__((aligned(16))) v4f partial[8][32];
-    const uint32_t lane = threadIdx.x & 63u, d = a.cache.head_dim;
-    const uint32_t f4 = threadIdx.x & 31u, from = threadIdx.x >> 5;
     const Sequence q = sequence_of(a.starts, a.lengths, blockIdx.y, a.tokens);
     const uint64_t rows = static_cast<uint64_t>(q.end - q.begin) * a.heads;
     const Parts parts = parts_of(a, splits);
     for (uint64_t r = blockIdx.x; r < rows; r += gridDim.x) {
         const uint64_t token = static_cast<uint64_t>(q.begin) + r / a.heads, head = r % a.heads;
-        const uint64_t slot = (token * a.heads + head) * splits;
-        const float2 stat = lane < splits ? parts.stats[slot + lane] : make_float2(kNoScore, 0.0f);
-        v4f mine[kMostSplits / 8];
-#pragma unroll
-        for (uint32_t i = 0; i < kMostSplits / 8; ++i) {
-            mine[i] = v4f{0.f, 0.f, 0.f, 0.f};
-            if (from + 8 * i < splits && 4 * f4 < d)
-                mine[i] = *reinterpret_cast<const v4f*>(parts.sums + (slot + from + 8 * i) * d + 4 * f4);
-        }
-        const float top = wave_max(stat.x);
-        const float weight = __builtin_amdgcn_exp2f(stat.x - top);  // 1 for splits that saw nothing, if all did not
-        const float total = wave_sum_tree(stat.y * weight);
-        __syncthreads();  // the row before has been read
-        if (threadIdx.x < kMostSplits) share[lane] = weight;
-        __syncthreads();
-        v4f sum = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-        for (uint32_t i = 0; i < kMostSplits / 8; ++i)
-            if (from + 8 * i < splits) sum += mine[i] * share[from + 8 * i];
-        partial[from][f4] = sum;
-        __syncthreads();
-        if (threadIdx.x < 32 && 4 * f4 < d) {
-            sum = partial[0][f4];
-#pragma unroll
-            for (int i = 1; i < 8; ++i) sum += partial[i][f4];
-            E* y = static_cast<E*>(a.output) + token * a.output_stride + head * d + 4 * f4;
-            const float scale = total == 0.0f ? 0.0f : 1.0f / total;
-#pragma unroll
-            for (int i = 0; i < 4; ++i) y[i] = static_cast<E>(sum[i] * scale);
-        }
+        join_row(parts, (token * a.heads + head) * splits, splits, a.cache.head_dim,
+                 static_cast<E*>(a.output) + token * a.output_stride + head * a.cache.head_dim);
     }
 }
 
@@ -856,8 +792,7 @@ uint64_t dav2_hip_attention_cache_i8_scratch_bytes(const dav2_attention_cache_i8
     const dav2_attention_cache_i8_args& a = *args;
     const Plan p = plan_of(a);
     if (p.splits == 1) return 0;
-    const uint64_t parts = static_cast<uint64_t>(a.tokens) * a.heads * p.splits;
-    return ((parts + 1) & ~1ull) * sizeof(float2) + parts * a.cache.head_dim * sizeof(float);
+    return parts_bytes(static_cast<uint64_t>(a.tokens) * a.heads * p.splits, a.cache.head_dim);
 }
 
 int dav2_hip_attention_cache_i8(const dav2_attention_cache_i8_args* args, void* stream) {

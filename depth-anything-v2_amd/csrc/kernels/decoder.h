@@ -90,4 +90,79 @@ struct Plus {
     DAV2_DEV float operator()(float a, float b) const { return a + b; }
 };
 
+constexpr float kLog2e = 1.44269504f;
+
+// Token and head of N rows from row `first` on: row r is token r / group, head
+// r % group. One division for all; behind it (t < group + N) a compare, or for
+// groups below N <= 128 a product with 2^16 / group that is exact there.
+template <uint32_t N>
+struct Rows {
+    uint32_t token, head, group, magic, most;
+    DAV2_DEV Rows(uint32_t first, uint32_t group_, uint32_t rows)
+        : token(first / group_), group(group_), magic(65536u / group_ + 1u), most(min(rows - first, N) - 1u) {
+        head = first - token * group;
+    }
+    // row first + i, i < N; past the last row that one
+    DAV2_DEV void find(uint32_t i, uint32_t& t, uint32_t& h) const {
+        const uint32_t at = head + min(i, most);
+        const uint32_t more = group >= N ? (at >= group ? 1u : 0u) : (at * magic) >> 16;
+        t = token + more;
+        h = at - more * group;
+    }
+};
+
+// What splits of the keys leave for the join: for each row and split the
+// output's sums and {maximum in units of log2, sum of weights}.
+constexpr uint32_t kMostSplits = 64;
+struct Parts {
+    float* sums;    // [rows * splits][head_dim]
+    float2* stats;  // [rows * splits]
+};
+DAV2_DEV Parts parts_at(void* scratch, uint64_t count) {
+    float2* stats = static_cast<float2*>(scratch);
+    return {reinterpret_cast<float*>(stats + ((count + 1u) & ~uint64_t(1))), stats};
+}
+inline uint64_t parts_bytes(uint64_t count, uint32_t head_dim) {
+    return ((count + 1u) & ~uint64_t(1)) * sizeof(float2) + count * head_dim * sizeof(float);
+}
+
+// One row's splits, parts slot .. slot + splits - 1, joined by a workgroup of
+// 256: thread (i, f) has the four features 4 f .. of splits i, i + 8, ..., so
+// that few loads follow one another (a wave per row that walked over 64 splits
+// took 60 us). A split that saw nothing has a sum of 0 and drops out.
+template <typename E>
+DAV2_DEV void join_row(const Parts& parts, uint64_t slot, uint32_t splits, uint32_t d, E* y) {
+    __shared__ float share[kMostSplits];
+    __shared__ __attribute__((aligned(16))) v4f partial[8][32];
+    const uint32_t lane = threadIdx.x & 63u, f4 = threadIdx.x & 31u, from = threadIdx.x >> 5;
+    const float2 stat = lane < splits ? parts.stats[slot + lane] : make_float2(kNoScore, 0.0f);
+    v4f mine[kMostSplits / 8];
+#pragma unroll
+    for (uint32_t i = 0; i < kMostSplits / 8; ++i) {
+        mine[i] = v4f{0.f, 0.f, 0.f, 0.f};
+        if (from + 8 * i < splits && 4 * f4 < d)
+            mine[i] = *reinterpret_cast<const v4f*>(parts.sums + (slot + from + 8 * i) * d + 4 * f4);
+    }
+    const float top = wave_max(stat.x);
+    const float weight = __builtin_amdgcn_exp2f(stat.x - top);  // 1 for all, if no split saw anything
+    const float total = wave_sum_tree(stat.y * weight);
+    __syncthreads();  // the row before has been read
+    if (threadIdx.x < kMostSplits) share[lane] = weight;
+    __syncthreads();
+    v4f sum = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (uint32_t i = 0; i < kMostSplits / 8; ++i)
+        if (from + 8 * i < splits) sum += mine[i] * share[from + 8 * i];
+    partial[from][f4] = sum;
+    __syncthreads();
+    if (threadIdx.x < 32 && 4 * f4 < d) {
+        sum = partial[0][f4];
+#pragma unroll
+        for (int i = 1; i < 8; ++i) sum += partial[i][f4];
+        const float scale = total == 0.0f ? 0.0f : 1.0f / total;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) y[4 * f4 + i] = static_cast<E>(sum[i] * scale);
+    }
+}
+
 }  // namespace dav2k
