@@ -24,16 +24,39 @@ DAV2_DEV uint32_t workgroup_max_bits(uint32_t v, uint32_t* shared) {
     return v;
 }
 
-// A workgroup per (touched page, head, sequence).
-template <typename E>
+// A code at another scale (see dav2_cache_store_i8_args).
+DAV2_DEV int requantize(int code, float old, float now, float inverse) {
+    return quantize_div(static_cast<float>(code) * old, now, inverse);
+}
+
+DAV2_DEV uint32_t byte_of(uint32_t word, uint32_t i, int code) {
+    return (word & ~(0xffu << (8u * i))) | ((static_cast<uint32_t>(code) & 0xffu) << (8u * i));
+}
+
+// A workgroup per (touched page, head and side, sequence); side 0 keys, 1
+// values. The new rows are read once for their largest value and again for
+// their codes, which keys keep in registers (up to kKept pieces of 16 features
+// a thread) and values take from the caches: their pages are feature-major, so
+// a thread needs 16 tokens of one 4-byte piece of features. Codes are written
+// 16 at a time; a value chunk that also holds older or later tokens is read,
+// changed and written back. Bound by memory: 8 prompts of up to 2048 tokens, 8
+// heads of 128, f16 %PROMPTS%.
+template <typename E, bool ALIGNED>
 __global__ __launch_bounds__(256) void cache_store_kernel(dav2_cache_store_i8_args a) {
+    constexpr int kKept = 2;
+    constexpr int kWords = sizeof(E);  // 16-byte words of 16 elements
     __shared__ uint32_t shared[4];
-    const uint32_t h = blockIdx.y, s = blockIdx.z, page_size = a.cache.page_size, d = a.cache.head_dim;
+    typedef E V __attribute__((ext_vector_type(16 / sizeof(E))));
+    constexpr int N = 16 / sizeof(E);
+    const uint32_t h = blockIdx.y >> 1, side = blockIdx.y & 1u, s = blockIdx.z;
+    const uint32_t page_size = a.cache.page_size, d = a.cache.head_dim, pieces = d / 16u;
     const Sequence q = sequence_of(a.starts, a.lengths, s, a.tokens);
     // positions [first, last) are new; in 64 bits, as a length may be anything
     const int64_t origin = static_cast<int64_t>(q.length) - (q.end - q.begin);  // row r has position origin + r - begin
     const int64_t first = max(origin, int64_t(0));
     const int64_t last = min(static_cast<int64_t>(q.length), static_cast<int64_t>(a.table_pages) * page_size);
+    const uint64_t stride = side ? a.value_stride : a.key_stride;
+    const E* x = static_cast<const E*>(side ? a.values : a.keys) + static_cast<uint64_t>(h) * d;
     for (int64_t p = first / page_size + blockIdx.x; p * page_size < last; p += gridDim.x) {
         const int32_t page = a.page_table[static_cast<uint64_t>(s) * a.table_pages + p];
         if (page < 0 || static_cast<uint32_t>(page) >= a.cache.pages) continue;  // the same for the whole workgroup
@@ -41,34 +64,112 @@ __global__ __launch_bounds__(256) void cache_store_kernel(dav2_cache_store_i8_ar
         const uint32_t from = static_cast<uint32_t>(max(first - base, int64_t(0)));
         const uint32_t to = static_cast<uint32_t>(min(last - base, static_cast<int64_t>(page_size)));
         const uint64_t plane = static_cast<uint64_t>(page) * a.cache.kv_heads + h;
-        for (int side = 0; side < 2; ++side) {
-            const E* x = static_cast<const E*>(side ? a.values : a.keys) + static_cast<uint64_t>(h) * d;
-            const uint64_t stride = side ? a.value_stride : a.key_stride;
-            int8_t* codes = (side ? a.cache.values : a.cache.keys) + plane * page_size * d;
-            float* scale = (side ? a.cache.value_scales : a.cache.key_scales) + plane;
-            auto row = [&](uint32_t slot) { return x + static_cast<uint64_t>(q.begin + (base + slot - origin)) * stride; };
-            auto place = [&](uint32_t slot, uint32_t f) { return side ? f * page_size + slot : slot * d + f; };
-            uint32_t most = 0;
-            for (uint32_t i = threadIdx.x; i < (to - from) * d; i += 256u)
-                most = max(most, __float_as_uint(fabsf(static_cast<float>(row(from + i / d)[i % d]))));
-            most = workgroup_max_bits(most, shared);
-            const float old = from ? *scale : 0.0f;
-            // fmaxf would drop a NaN: compare bits again
-            uint32_t bits = max(__float_as_uint(div_rn(__uint_as_float(most), 127.0f)), __float_as_uint(1.0e-8f));
-            bits = max(bits, __float_as_uint(old) & 0x7fffffffu);
-            const float now = __uint_as_float(bits);
-            __syncthreads();  // every thread has read the old scale
-            if (threadIdx.x == 0) *scale = now;
-            if (from && now != old)
-                for (uint32_t i = threadIdx.x; i < from * d; i += 256u) {
-                    int8_t* c = codes + place(i / d, i % d);
-                    *c = static_cast<int8_t>(quantize_rne(div_rn(static_cast<float>(*c) * old, now)));
+        int8_t* codes = (side ? a.cache.values : a.cache.keys) + plane * page_size * d;
+        float* scale = (side ? a.cache.value_scales : a.cache.key_scales) + plane;
+        const E* slot0 = x + (q.begin + (base - origin)) * static_cast<int64_t>(stride);  // of slot 0, new or not
+        auto load = [&](uint32_t item, E (&v)[16]) {
+            const E* in = slot0 + (from + item / pieces) * stride + 16u * (item % pieces);
+            if constexpr (ALIGNED) {
+#pragma unroll
+                for (int w = 0; w < kWords; ++w) {
+                    const V word = *reinterpret_cast<const V*>(in + N * w);
+#pragma unroll
+                    for (int i = 0; i < N; ++i) v[N * w + i] = word[i];
                 }
-            for (uint32_t i = threadIdx.x; i < (to - from) * d; i += 256u) {
-                const uint32_t slot = from + i / d, f = i % d;
-                codes[place(slot, f)] =
-                    static_cast<int8_t>(quantize_rne(div_rn(static_cast<float>(row(slot)[f]), now)));
+            } else {
+#pragma unroll
+                for (int i = 0; i < 16; ++i) v[i] = in[i];
             }
+        };
+        const float old = from ? *scale : 0.0f;
+        const uint32_t items = (to - from) * pieces;
+        E kept[kKept][16];
+        uint32_t most = 0;
+#pragma unroll
+        for (int k = 0; k < kKept; ++k) {
+            if (threadIdx.x + 256u * k >= items) continue;
+            load(threadIdx.x + 256u * k, kept[k]);
+#pragma unroll
+            for (int i = 0; i < 16; ++i) most = max(most, __float_as_uint(fabsf(static_cast<float>(kept[k][i]))));
+        }
+        for (uint32_t item = threadIdx.x + 256u * kKept; item < items; item += 256u) {
+            E v[16];
+            load(item, v);
+#pragma unroll
+            for (int i = 0; i < 16; ++i) most = max(most, __float_as_uint(fabsf(static_cast<float>(v[i]))));
+        }
+        most = workgroup_max_bits(most, shared);
+        // fmaxf would drop a NaN: compare bits again
+        uint32_t bits = max(__float_as_uint(div_rn(__uint_as_float(most), 127.0f)), __float_as_uint(1.0e-8f));
+        bits = max(bits, __float_as_uint(old) & 0x7fffffffu);
+        const float now = __uint_as_float(bits), inverse = div_rn(1.0f, now);
+        __syncthreads();  // every thread has read the old scale
+        if (threadIdx.x == 0) *scale = now;
+        const bool again = from && now != old;  // the older codes change
+        if (side == 0) {
+            auto put = [&](uint32_t item, const E (&v)[16]) {
+                uint32_t w[4];
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    w[i] = pack4(quantize_div(static_cast<float>(v[4 * i]), now, inverse),
+                                 quantize_div(static_cast<float>(v[4 * i + 1]), now, inverse),
+                                 quantize_div(static_cast<float>(v[4 * i + 2]), now, inverse),
+                                 quantize_div(static_cast<float>(v[4 * i + 3]), now, inverse));
+                *reinterpret_cast<uint4*>(codes + from * d + 16u * item) = make_uint4(w[0], w[1], w[2], w[3]);
+            };
+#pragma unroll
+            for (int k = 0; k < kKept; ++k)
+                if (threadIdx.x + 256u * k < items) put(threadIdx.x + 256u * k, kept[k]);
+            for (uint32_t item = threadIdx.x + 256u * kKept; item < items; item += 256u) {
+                E v[16];
+                load(item, v);
+                put(item, v);
+            }
+            if (again)
+                for (uint32_t i = threadIdx.x; i < from * d / 4u; i += 256u) {
+                    uint32_t* word = reinterpret_cast<uint32_t*>(codes) + i;
+                    const uint32_t w = *word;
+                    *word = pack4(requantize(static_cast<int8_t>(w), old, now, inverse),
+                                  requantize(static_cast<int8_t>(w >> 8), old, now, inverse),
+                                  requantize(static_cast<int8_t>(w >> 16), old, now, inverse),
+                                  requantize(static_cast<int8_t>(w >> 24), old, now, inverse));
+                }
+            continue;
+        }
+        constexpr uint32_t F = ALIGNED ? 4 / sizeof(E) : 1;  // features of an item
+        typedef E Piece __attribute__((ext_vector_type(F)));
+        const uint32_t features = d / F, chunk0 = again ? 0u : from / 16u, chunks = (to + 15u) / 16u - chunk0;
+        for (uint32_t item = threadIdx.x; item < features * chunks; item += 256u) {
+            const uint32_t chunk = chunk0 + item / features, f = item % features * F, s0 = chunk * 16u;
+            uint4* out[F];
+            uint32_t w[F][4] = {};
+#pragma unroll
+            for (uint32_t j = 0; j < F; ++j) out[j] = reinterpret_cast<uint4*>(codes + (f + j) * page_size + s0);
+            const bool whole = s0 >= from && s0 + 16u <= to;
+            if (!whole) {
+#pragma unroll
+                for (uint32_t j = 0; j < F; ++j) {
+                    const uint4 o = *out[j];
+                    w[j][0] = o.x, w[j][1] = o.y, w[j][2] = o.z, w[j][3] = o.w;
+                }
+            }
+#pragma unroll
+            for (uint32_t i = 0; i < 16; ++i) {
+                const uint32_t slot = s0 + i;
+                if (slot >= from && slot < to) {
+                    const Piece piece = *reinterpret_cast<const Piece*>(slot0 + slot * stride + f);
+#pragma unroll
+                    for (uint32_t j = 0; j < F; ++j)
+                        w[j][i / 4] = byte_of(w[j][i / 4], i % 4, quantize_div(static_cast<float>(piece[j]), now, inverse));
+                } else if (again && slot < from) {
+#pragma unroll
+                    for (uint32_t j = 0; j < F; ++j)
+                        w[j][i / 4] = byte_of(w[j][i / 4], i % 4,
+                                              requantize(static_cast<int8_t>(w[j][i / 4] >> (8 * (i % 4))), old, now, inverse));
+                }
+            }
+#pragma unroll
+            for (uint32_t j = 0; j < F; ++j) *out[j] = make_uint4(w[j][0], w[j][1], w[j][2], w[j][3]);
         }
     }
 }
@@ -779,9 +880,13 @@ int dav2_hip_cache_store_i8(const dav2_cache_store_i8_args* args, void* stream) 
     const uint64_t new_most = a.max_new < a.tokens ? a.max_new : a.tokens;
     uint64_t touched = (new_most + a.cache.page_size - 2) / a.cache.page_size + 1;
     if (touched > a.table_pages) touched = a.table_pages;
-    const dim3 grid(static_cast<uint32_t>(touched), a.cache.kv_heads, a.sequences);
+    const dim3 grid(static_cast<uint32_t>(touched), 2 * a.cache.kv_heads, a.sequences);
+    const uint64_t size = dtype_bytes(a.dtype);
+    const bool aligned = aligned16(a.keys) && aligned16(a.values) && a.key_stride * size % 16 == 0 &&
+                         a.value_stride * size % 16 == 0;
     with_dtype(a.dtype, [&](auto* e) {
-        dispatch(cache_store_kernel<std::remove_pointer_t<decltype(e)>>, grid, dim3(256), 0,
+        typedef std::remove_pointer_t<decltype(e)> E;
+        dispatch(aligned ? cache_store_kernel<E, true> : cache_store_kernel<E, false>, grid, dim3(256), 0,
                  static_cast<hipStream_t>(stream), a);
     });
     return hipGetLastError();

@@ -40,7 +40,7 @@ auto with_dtype(uint32_t dtype, F&& f) {
 
 inline bool valid_cache(const dav2_cache_i8& c) {
     return c.keys && c.values && c.key_scales && c.value_scales && aligned16(c.keys) && aligned16(c.values) &&
-           c.pages > 0 && c.pages <= 0x7fffffffu && c.kv_heads > 0 && c.kv_heads <= 65535u && c.page_size >= 16 &&
+           c.pages > 0 && c.pages <= 0x7fffffffu && c.kv_heads > 0 && c.kv_heads <= 32767u && c.page_size >= 16 &&
            c.page_size <= 256 && c.page_size % 16 == 0 && c.head_dim >= 16 && c.head_dim <= 128 &&
            c.head_dim % 16 == 0;
 }
