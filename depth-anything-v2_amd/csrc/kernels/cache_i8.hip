@@ -42,8 +42,8 @@ DAV2_DEV uint32_t byte_of(uint32_t word, uint32_t i, int code) {
 // changed and written back. Bound by memory: 8 prompts of up to 2048 tokens, 8
 // heads of 128, f16 %PROMPTS%.
 template <typename E, bool ALIGNED>
-__global__ __launch_bounds__(256) void cache_store_kernel(dav2_cache_store_i8_args a) {
-    constexpr int kKept = 2;
+__global__ __launch_bounds__(256, 8) void cache_store_kernel(dav2_cache_store_i8_args a) {
+    constexpr int kKept = 1;
     constexpr int kWords = sizeof(E);  // 16-byte words of 16 elements
     __shared__ uint32_t shared[4];
     typedef E V __attribute__((ext_vector_type(16 / sizeof(E))));
@@ -260,18 +260,19 @@ DAV2_DEV Parts parts_of(const dav2_attention_cache_i8_args& a, uint32_t splits) 
 // is key 16 (i / 4) + 4 a + i % 4 of the block; a lane then holds the scores of
 // chunk l / 16 in order, which is the right operand of the second product as
 // it stands, and the scales it needs are those of one page.
-template <typename E, int HEAD>
+template <typename E, int D>
 __global__ __launch_bounds__(256, 2) void cache_rows_kernel(dav2_attention_cache_i8_args a, uint32_t splits,
                                                             uint32_t tiles) {
     constexpr bool kFloat = std::is_same_v<E, float>;
-    constexpr int KC = HEAD / 64, FT = HEAD / 16, NP = kFloat ? 2 : 1;
+    constexpr int KC = (D + 63) / 64, FT = D / 16, NP = kFloat ? 2 : 1;
+    constexpr uint32_t d = D;
     constexpr int kPad = 17;  // row length of the joining waves' sums in LDS
-    __shared__ float joined[4][HEAD * kPad];
+    __shared__ float joined[4][D * kPad];
     __shared__ float shared_max[4][16], shared_sum[4][16];
     const uint32_t lane = threadIdx.x & 63u, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const uint32_t col = lane & 15u, g = lane >> 4;
     const uint32_t split = blockIdx.x % splits, h = blockIdx.y, s = blockIdx.z;
-    const uint32_t d = a.cache.head_dim, page_size = a.cache.page_size, kv_heads = a.cache.kv_heads;
+    const uint32_t page_size = a.cache.page_size, kv_heads = a.cache.kv_heads;
     const uint32_t group = a.heads / kv_heads;
     const Sequence q = sequence_of(a.starts, a.lengths, s, a.tokens);
     const uint32_t n = static_cast<uint32_t>(q.end - q.begin);
@@ -334,7 +335,7 @@ __global__ __launch_bounds__(256, 2) void cache_rows_kernel(dav2_attention_cache
             const int8_t* v = a.cache.values + (plane * d + col) * page_size + of_value.slot;
 #pragma unroll
             for (int f = 0; f < FT; ++f)
-                if (16u * f < d) vraw[f] = *reinterpret_cast<const uint4*>(v + static_cast<uint64_t>(16u * f) * page_size);
+                vraw[f] = *reinterpret_cast<const uint4*>(v + static_cast<uint64_t>(16u * f) * page_size);
         };
         uint32_t block = first + wave;
         if (block < last) {
@@ -442,7 +443,6 @@ __global__ __launch_bounds__(256, 2) void cache_rows_kernel(dav2_attention_cache
             sum = fmaf(part, inverse, sum);
 #pragma unroll
             for (int f = 0; f < FT; ++f) {
-                if (16u * f >= d) continue;
                 const h8 v0 = widen(vraw[f].x, vraw[f].y), v1 = widen(vraw[f].z, vraw[f].w);
 #pragma unroll
                 for (int p = 0; p < NP; ++p) {
@@ -514,11 +514,13 @@ __global__ __launch_bounds__(256, 2) void cache_rows_kernel(dav2_attention_cache
 // second product's step t if V^T holds its keys in that order, which their
 // place in LDS gives them: keys 0-3, 8-11 of a chunk, then 4-7, 12-15. Eight
 // registers are one 16-token chunk, so scales are uniform for them.
-template <typename E, int HEAD>
+template <typename E, int D>
 __global__ __launch_bounds__(256, 2) void cache_tiles_kernel(dav2_attention_cache_i8_args a, uint32_t splits,
                                                              uint32_t tiles) {
     constexpr bool kFloat = std::is_same_v<E, float>;
-    constexpr int KS = HEAD / 16, FB = HEAD / 32, NP = kFloat ? 2 : 1;
+    constexpr int HEAD = D <= 64 ? 64 : 128;  // features of a row in LDS
+    constexpr int KS = D / 16, FB = (D + 31) / 32, NP = kFloat ? 2 : 1;
+    constexpr uint32_t d = D;
     constexpr int kPieces = HEAD / 64;   // of 16 codes, for each thread and tile: keys, and values
     constexpr int kRow = HEAD * 2;       // bytes of a key row in LDS
     // rescale when a score passes the running maximum by this: weights stay
@@ -529,7 +531,7 @@ __global__ __launch_bounds__(256, 2) void cache_tiles_kernel(dav2_attention_cach
     __shared__ __attribute__((aligned(16))) v4f lds_scales[2][4];  // of a chunk: key scale, log2 / exponent, inverse, fraction
     const uint32_t lane = threadIdx.x & 63u, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const uint32_t col = lane & 31u, hf = lane >> 5;
-    const uint32_t kv_heads = a.cache.kv_heads, d = a.cache.head_dim, page_size = a.cache.page_size;
+    const uint32_t kv_heads = a.cache.kv_heads, page_size = a.cache.page_size;
     const uint32_t s = blockIdx.x / kv_heads, h = blockIdx.x - s * kv_heads, group = a.heads / kv_heads;
     const uint32_t split = blockIdx.y % splits;
     const Sequence q = sequence_of(a.starts, a.lengths, s, a.tokens);
@@ -643,8 +645,7 @@ __global__ __launch_bounds__(256, 2) void cache_tiles_kernel(dav2_attention_cach
             for (int k = 0; k < KS; ++k)
 #pragma unroll
                 for (int j = 0; j < 8 / kVec; ++j) {
-                    raw[k][j] = V{};
-                    if (16u * k < d) raw[k][j] = *reinterpret_cast<const V*>(x + 16 * k + kVec * j);
+                    raw[k][j] = *reinterpret_cast<const V*>(x + 16 * k + kVec * j);
 #pragma unroll
                     for (int i = 0; i < kVec; ++i) largest = fmaxf(largest, fabsf(static_cast<float>(raw[k][j][i])));
                 }
@@ -697,7 +698,6 @@ __global__ __launch_bounds__(256, 2) void cache_tiles_kernel(dav2_attention_cach
                     for (int r = 0; r < 16; ++r) sc[b][r] = 0.0f;
 #pragma unroll
                     for (int k = 0; k < KS; ++k) {
-                        if (16u * k >= d) continue;
                         const h8 kf = *reinterpret_cast<const h8*>(lds_keys[buffer] + swz<kRow>(32u * b + col, 2u * k + hf));
 #pragma unroll
                         for (int p = 0; p < NP; ++p)
@@ -773,7 +773,6 @@ __global__ __launch_bounds__(256, 2) void cache_tiles_kernel(dav2_attention_cach
                 }
 #pragma unroll
                 for (int f = 0; f < FB; ++f) {
-                    if (32u * f >= d) continue;
 #pragma unroll
                     for (int t = 0; t < 4; ++t) {
                         const h8 vf = *reinterpret_cast<const h8*>(lds_values[buffer] + swz<128>(32u * f + col, 2u * t + hf));
@@ -913,11 +912,11 @@ int dav2_hip_attention_cache_i8(const dav2_attention_cache_i8_args* args, void* 
                               : dim3(p.tiles * p.splits, a.cache.kv_heads, a.sequences);
     return with_dtype(a.dtype, [&](auto* e) -> int {
         typedef std::remove_pointer_t<decltype(e)> E;
-        if (p.tiled) {
-            if (a.cache.head_dim <= 64) dispatch(cache_tiles_kernel<E, 64>, grid, dim3(256), 0, s, a, p.splits, p.tiles);
-            else dispatch(cache_tiles_kernel<E, 128>, grid, dim3(256), 0, s, a, p.splits, p.tiles);
-        } else if (a.cache.head_dim <= 64) dispatch(cache_rows_kernel<E, 64>, grid, dim3(256), 0, s, a, p.splits, p.tiles);
-        else dispatch(cache_rows_kernel<E, 128>, grid, dim3(256), 0, s, a, p.splits, p.tiles);
+        with_head_dim(a.cache.head_dim, [&](auto dim) {
+            constexpr int D = decltype(dim)::value;
+            if (p.tiled) dispatch(cache_tiles_kernel<E, D>, grid, dim3(256), 0, s, a, p.splits, p.tiles);
+            else dispatch(cache_rows_kernel<E, D>, grid, dim3(256), 0, s, a, p.splits, p.tiles);
+        });
         if (p.splits > 1) {
             const uint64_t rows = static_cast<uint64_t>(std::min(a.max_query, a.tokens)) * a.heads;
             const dim3 join(static_cast<uint32_t>(std::min<uint64_t>(rows, 4096)), a.sequences);

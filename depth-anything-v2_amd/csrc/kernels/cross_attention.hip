@@ -97,13 +97,15 @@ DAV2_DEV v16f multiply(v4f a, v4f b, v16f c) {
 // right operand of the second product as it stands, if the left one takes its
 // keys in that order. In 16 bits that is two transposing LDS reads of four
 // keys by 16 features each; in fp32 four plain ones.
-template <typename E, int HEAD>
+template <typename E, int D>
 __global__ __launch_bounds__(256, 2) void cross_tiles_kernel(dav2_cross_attention_args a, Lists lists, uint32_t splits,
                                                              uint32_t tiles) {
     constexpr bool kFloat = std::is_same_v<E, float>;
     constexpr int kTile = kFloat ? 32 : 64, kBlocks = kTile / 32;
     constexpr int N = 16 / sizeof(E);                  // values of a piece
-    constexpr int KS = HEAD / (2 * N), FB = HEAD / 32;  // steps over the features, blocks of 32 features
+    constexpr int HEAD = D <= 64 ? 64 : 128;           // features of a row in LDS
+    constexpr int KS = D / (2 * N), FB = (D + 31) / 32;  // steps over the features, blocks of 32 features
+    constexpr uint32_t d = D;
     constexpr uint32_t kRow = HEAD * sizeof(E);        // bytes of a key in LDS
     constexpr uint32_t kChunks = kRow / 16, kRowsPerCopy = 64 / kChunks;
     constexpr int kCopies = kTile * kRow / 4096;       // of each wave, for the keys and again for the values
@@ -112,7 +114,7 @@ __global__ __launch_bounds__(256, 2) void cross_tiles_kernel(dav2_cross_attentio
     __shared__ __attribute__((aligned(16))) int8_t lds[2][2][kTile * kRow];  // [buffer][keys, values]
     const uint32_t lane = threadIdx.x & 63u, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const uint32_t col = lane & 31u, hf = lane >> 5;
-    const uint32_t d = a.head_dim, group = a.heads / a.kv_heads;
+    const uint32_t group = a.heads / a.kv_heads;
     const uint32_t b = blockIdx.x / a.kv_heads, h = blockIdx.x - b * a.kv_heads;
     const uint32_t split = blockIdx.y % splits;
     const uint32_t rows = a.query_tokens * group;  // batch * query_tokens * heads is below 2^32
@@ -178,8 +180,7 @@ __global__ __launch_bounds__(256, 2) void cross_tiles_kernel(dav2_cross_attentio
                          static_cast<uint64_t>(head) * d + N * hf;
 #pragma unroll
             for (int k = 0; k < KS; ++k) {
-                qf[k] = V{};
-                if (2u * N * k < d) qf[k] = *reinterpret_cast<const V*>(x + 2 * N * k);
+                qf[k] = *reinterpret_cast<const V*>(x + 2 * N * k);
                 if (a.scale < 0.0f) qf[k] = -qf[k];
             }
         }
@@ -206,10 +207,8 @@ __global__ __launch_bounds__(256, 2) void cross_tiles_kernel(dav2_cross_attentio
 #pragma unroll
                     for (int r = 0; r < 16; ++r) sc[i][r] = 0.0f;
 #pragma unroll
-                    for (int k = 0; k < KS; ++k) {
-                        if (2u * N * k >= d) continue;
+                    for (int k = 0; k < KS; ++k)
                         sc[i] = multiply(key_piece(buffer, 32u * i + col, 2u * k + hf), qf[k], sc[i]);
-                    }
                 }
                 if ((block + 1u) * kTile > count) {
 #pragma unroll
@@ -247,7 +246,6 @@ __global__ __launch_bounds__(256, 2) void cross_tiles_kernel(dav2_cross_attentio
                     }
 #pragma unroll
                 for (int f = 0; f < FB; ++f) {
-                    if (32u * f >= d) continue;
 #pragma unroll
                     for (int t = 0; t < kTile / (2 * N); ++t) {
                         V vf;
@@ -376,8 +374,9 @@ int dav2_hip_cross_attention(const dav2_cross_attention_args* args, void* stream
     const dim3 grid(a.batch * a.kv_heads, p.tiles * p.splits);
     return with_dtype(a.dtype, [&](auto* e) -> int {
         typedef std::remove_pointer_t<decltype(e)> E;
-        if (a.head_dim <= 64) dispatch(cross_tiles_kernel<E, 64>, grid, dim3(256), 0, s, a, lists, p.splits, p.tiles);
-        else dispatch(cross_tiles_kernel<E, 128>, grid, dim3(256), 0, s, a, lists, p.splits, p.tiles);
+        with_head_dim(a.head_dim, [&](auto dim) {
+            dispatch(cross_tiles_kernel<E, decltype(dim)::value>, grid, dim3(256), 0, s, a, lists, p.splits, p.tiles);
+        });
         if (p.splits > 1) {
             const uint64_t all = static_cast<uint64_t>(a.batch) * a.query_tokens * a.heads;
             dispatch(cross_join_kernel<E>, dim3(static_cast<uint32_t>(std::min<uint64_t>(all, 65536))), dim3(256), 0, s, a,

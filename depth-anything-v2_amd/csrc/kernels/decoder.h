@@ -2,6 +2,8 @@
 // cross_attention.hip): element types and their checks.
 #pragma once
 
+#include <type_traits>
+
 #include "common.h"
 #include "dav2_hip.h"
 
@@ -35,6 +37,24 @@ auto with_dtype(uint32_t dtype, F&& f) {
         case DAV2_DTYPE_F16: return f(static_cast<_Float16*>(nullptr));
         case DAV2_DTYPE_BF16: return f(static_cast<__bf16*>(nullptr));
         default: return f(static_cast<float*>(nullptr));
+    }
+}
+
+// Calls f with a valid head_dim as a constant: the attention kernels are made
+// for each, as a branch around a matrix instruction keeps the compiler from
+// overlapping it with anything (4 x 2048 queries of 128 features against 5477
+// keys: 873 us with, 6xx without).
+template <typename F>
+auto with_head_dim(uint32_t d, F&& f) {
+    switch (d / 16) {
+        case 1: return f(std::integral_constant<int, 16>{});
+        case 2: return f(std::integral_constant<int, 32>{});
+        case 3: return f(std::integral_constant<int, 48>{});
+        case 4: return f(std::integral_constant<int, 64>{});
+        case 5: return f(std::integral_constant<int, 80>{});
+        case 6: return f(std::integral_constant<int, 96>{});
+        case 7: return f(std::integral_constant<int, 112>{});
+        default: return f(std::integral_constant<int, 128>{});
     }
 }
 
