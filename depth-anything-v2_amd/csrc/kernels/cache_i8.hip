@@ -717,6 +717,7 @@ __global__ __launch_bounds__(256, 2) void cache_tiles_kernel(dav2_attention_cach
                     whole = whole && of_chunk[3] != 0.0f;  // else the page does not exist
                 }
                 if (!__all(whole)) {
+                    stay_in_branch();
 #pragma unroll
                     for (int t = 0; t < 4; ++t) {
                         const bool here = fraction[t] != 0.0f;
@@ -742,6 +743,7 @@ __global__ __launch_bounds__(256, 2) void cache_tiles_kernel(dav2_attention_cach
                 }
                 largest = over_halves(largest, Larger());
                 if (__any(largest > maximum + kSlack)) {
+                    stay_in_branch();
                     const float grown = fmaxf(maximum, largest);
                     const float keep = __builtin_amdgcn_exp2f(maximum - grown);
                     maximum = grown;
@@ -815,15 +817,22 @@ __global__ __launch_bounds__(256, 2) void cache_tiles_kernel(dav2_attention_cach
 
 // The splits of the sequences' rows joined: one workgroup per row.
 template <typename E>
-__global__ __launch_bounds__(256) void cache_join_kernel(dav2_attention_cache_i8_args a, uint32_t splits) {
+__global__ __launch_bounds__(256) void cache_join_kernel(dav2_attention_cache_i8_args a, uint32_t splits,
+                                                         bool by_lanes) {
     const Sequence q = sequence_of(a.starts, a.lengths, blockIdx.y, a.tokens);
     const uint64_t rows = static_cast<uint64_t>(q.end - q.begin) * a.heads;
     const Parts parts = parts_of(a, splits);
-    for (uint64_t r = blockIdx.x; r < rows; r += gridDim.x) {
-        const uint64_t token = static_cast<uint64_t>(q.begin) + r / a.heads, head = r % a.heads;
-        join_row(parts, (token * a.heads + head) * splits, splits, a.cache.head_dim,
-                 static_cast<E*>(a.output) + token * a.output_stride + head * a.cache.head_dim);
+    const uint32_t d = a.cache.head_dim, heads = a.heads;
+    auto token = [&](uint64_t r) { return q.begin + static_cast<uint64_t>(static_cast<uint32_t>(r) / heads); };
+    auto head = [&](uint64_t r) { return static_cast<uint64_t>(static_cast<uint32_t>(r) % heads); };
+    auto output = [&](uint64_t r) { return static_cast<E*>(a.output) + token(r) * a.output_stride + head(r) * d; };
+    auto slot = [&](uint64_t r) { return (token(r) * heads + head(r)) * splits; };
+    if (by_lanes) {
+        for (uint64_t r = blockIdx.x * 8ull + threadIdx.x / 32u; r < rows; r += gridDim.x * 8ull)
+            join_few(parts, slot(r), splits, d, output(r));
+        return;
     }
+    for (uint64_t r = blockIdx.x; r < rows; r += gridDim.x) join_row(parts, slot(r), splits, d, output(r));
 }
 
 bool valid(const dav2_attention_cache_i8_args& a) {
@@ -919,8 +928,9 @@ int dav2_hip_attention_cache_i8(const dav2_attention_cache_i8_args* args, void* 
         });
         if (p.splits > 1) {
             const uint64_t rows = static_cast<uint64_t>(std::min(a.max_query, a.tokens)) * a.heads;
-            const dim3 join(static_cast<uint32_t>(std::min<uint64_t>(rows, 4096)), a.sequences);
-            dispatch(cache_join_kernel<E>, join, dim3(256), 0, s, a, p.splits);
+            const bool by_lanes = join_by_lanes(rows * a.sequences, p.splits);
+            const dim3 join(static_cast<uint32_t>(std::min<uint64_t>(by_lanes ? (rows + 7) / 8 : rows, 4096)), a.sequences);
+            dispatch(cache_join_kernel<E>, join, dim3(256), 0, s, a, p.splits, by_lanes);
         }
         return hipGetLastError();
     });

@@ -120,7 +120,8 @@ __global__ __launch_bounds__(256, 2) void cross_tiles_kernel(dav2_cross_attentio
     const uint32_t rows = a.query_tokens * group;  // batch * query_tokens * heads is below 2^32
     const uint32_t row_tiles = (rows + 127u) / 128u;
     const uint32_t* list = lists.keys ? lists.keys + static_cast<uint64_t>(b) * a.key_tokens : nullptr;
-    const uint32_t count = lists.keys ? lists.counts[b] : length_of(a, b);
+    // in a scalar register: the loop and the branch for its last tile are the same for all lanes
+    const uint32_t count = __builtin_amdgcn_readfirstlane(lists.keys ? lists.counts[b] : length_of(a, b));
     const uint32_t blocks = (count + kTile - 1u) / kTile, per = (blocks + splits - 1u) / splits;
     const uint32_t first = split * per, last = min(first + per, blocks);
     const E* keys = static_cast<const E*>(a.keys) + b * a.key_batch_stride + static_cast<uint64_t>(h) * d;
@@ -203,14 +204,24 @@ __global__ __launch_bounds__(256, 2) void cross_tiles_kernel(dav2_cross_attentio
             if (any_row) {
                 v16f sc[kBlocks];
 #pragma unroll
-                for (int i = 0; i < kBlocks; ++i) {
+                for (int i = 0; i < kBlocks; ++i)
 #pragma unroll
                     for (int r = 0; r < 16; ++r) sc[i][r] = 0.0f;
 #pragma unroll
-                    for (int k = 0; k < KS; ++k)
+                for (int k = 0; k < KS; ++k)
+#pragma unroll
+                    for (int i = 0; i < kBlocks; ++i)
                         sc[i] = multiply(key_piece(buffer, 32u * i + col, 2u * k + hf), qf[k], sc[i]);
+                // reads kAhead pieces ahead of their products
+                constexpr int kAhead = KS * kBlocks < 8 ? KS * kBlocks : 8, kEach = kFloat ? 4 : 1;
+                DAV2_ORDER(kLdsReads, kAhead);
+#pragma unroll
+                for (int i = 0; i < KS * kBlocks; ++i) {
+                    DAV2_ORDER(kProducts, kEach);
+                    if (i + kAhead < KS * kBlocks) DAV2_ORDER(kLdsReads, 1);
                 }
                 if ((block + 1u) * kTile > count) {
+                    stay_in_branch();
 #pragma unroll
                     for (int i = 0; i < kBlocks; ++i)
 #pragma unroll
@@ -226,6 +237,7 @@ __global__ __launch_bounds__(256, 2) void cross_tiles_kernel(dav2_cross_attentio
                     for (int r = 0; r < 16; ++r) largest = fmaxf(largest, sc[i][r]);
                 largest = over_halves(fmaxf(kNoScore, largest * c), Larger());
                 if (__any(largest > maximum + kSlack)) {
+                    stay_in_branch();
                     const float grown = fmaxf(maximum, largest);
                     const float keep = __builtin_amdgcn_exp2f(maximum - grown);
                     maximum = grown;
@@ -235,19 +247,27 @@ __global__ __launch_bounds__(256, 2) void cross_tiles_kernel(dav2_cross_attentio
 #pragma unroll
                         for (int r = 0; r < 16; ++r) o[f][r] *= keep;
                 }
-                V pf[kTile / (2 * N)];  // step t: keys 2 N t ..
+                // step t: keys 2 N t ..; its weights are formed among the products of the step before
+                constexpr int T = kTile / (2 * N);
+                V pf[T];
+                float parts_of_sum[T];
 #pragma unroll
-                for (int i = 0; i < kBlocks; ++i)
+                for (int t = 0; t < T; ++t) {
+                    parts_of_sum[t] = 0.0f;
 #pragma unroll
-                    for (int r = 0; r < 16; ++r) {
-                        const float w = __builtin_amdgcn_exp2f(fmaf(sc[i][r], c, -maximum));
-                        sum += w;
-                        pf[(16 * i + r) / N][r % N] = static_cast<E>(w);
+                    for (int r = 0; r < N; ++r) {
+                        const int at = N * t + r;
+                        const float w = __builtin_amdgcn_exp2f(fmaf(sc[at >> 4][at & 15], c, -maximum));
+                        parts_of_sum[t] += w;
+                        pf[t][r] = static_cast<E>(w);
                     }
+                }
 #pragma unroll
-                for (int f = 0; f < FB; ++f) {
+                for (int t = 0; t < T; ++t) sum += parts_of_sum[t];
 #pragma unroll
-                    for (int t = 0; t < kTile / (2 * N); ++t) {
+                for (int t = 0; t < T; ++t)
+#pragma unroll
+                    for (int f = 0; f < FB; ++f) {
                         V vf;
                         if constexpr (kFloat) {
 #pragma unroll
@@ -273,7 +293,22 @@ __global__ __launch_bounds__(256, 2) void cross_tiles_kernel(dav2_cross_attentio
                         }
                         o[f] = multiply(vf, pf[t], o[f]);
                     }
-                }
+                // a step's values are read, and its weights formed, among the products of the step before
+                constexpr int kReads = kFloat ? 4 : 2;
+                DAV2_ORDER(kLdsReads, FB * kReads);
+                DAV2_ORDER(kVector, 3 * N);
+                DAV2_ORDER(kExponentials, N);
+#pragma unroll
+                for (int t = 0; t < T; ++t)
+#pragma unroll
+                    for (int f = 0; f < FB; ++f) {
+                        DAV2_ORDER(kProducts, kEach);
+                        if (t + 1 < T) {
+                            DAV2_ORDER(kLdsReads, kReads);
+                            DAV2_ORDER(kVector, (3 * N + FB - 1) / FB);
+                            DAV2_ORDER(kExponentials, (N + FB - 1) / FB);
+                        }
+                    }
             }
             DAV2_WAIT_VMCNT(0);
             __syncthreads();
@@ -308,14 +343,21 @@ __global__ __launch_bounds__(256, 2) void cross_tiles_kernel(dav2_cross_attentio
 }
 
 template <typename E>
-__global__ __launch_bounds__(256) void cross_join_kernel(dav2_cross_attention_args a, uint32_t splits) {
+__global__ __launch_bounds__(256) void cross_join_kernel(dav2_cross_attention_args a, uint32_t splits,
+                                                         bool by_lanes) {
     const uint64_t per_batch = static_cast<uint64_t>(a.query_tokens) * a.heads, rows = a.batch * per_batch;
     const Parts parts = parts_at(a.scratch, rows * splits);
-    for (uint64_t r = blockIdx.x; r < rows; r += gridDim.x) {
-        const uint64_t b = r / per_batch, in = r - b * per_batch, token = in / a.heads, head = in - token * a.heads;
-        join_row(parts, r * splits, splits, a.head_dim,
-                 static_cast<E*>(a.output) + b * a.output_batch_stride + token * a.output_stride + head * a.head_dim);
+    auto output = [&](uint64_t r) {
+        const uint32_t row = static_cast<uint32_t>(r), each = static_cast<uint32_t>(per_batch);  // below 2^32
+        const uint32_t b = row / each, in = row - b * each, token = in / a.heads, head = in - token * a.heads;
+        return static_cast<E*>(a.output) + b * a.output_batch_stride + token * a.output_stride + head * a.head_dim;
+    };
+    if (by_lanes) {
+        for (uint64_t r = blockIdx.x * 8ull + threadIdx.x / 32u; r < rows; r += gridDim.x * 8ull)
+            join_few(parts, r * splits, splits, a.head_dim, output(r));
+        return;
     }
+    for (uint64_t r = blockIdx.x; r < rows; r += gridDim.x) join_row(parts, r * splits, splits, a.head_dim, output(r));
 }
 
 struct Plan {
@@ -378,9 +420,11 @@ int dav2_hip_cross_attention(const dav2_cross_attention_args* args, void* stream
             dispatch(cross_tiles_kernel<E, decltype(dim)::value>, grid, dim3(256), 0, s, a, lists, p.splits, p.tiles);
         });
         if (p.splits > 1) {
-            const uint64_t all = static_cast<uint64_t>(a.batch) * a.query_tokens * a.heads;
+            const uint64_t rows = static_cast<uint64_t>(a.batch) * a.query_tokens * a.heads;
+            const bool by_lanes = join_by_lanes(rows, p.splits);
+            const uint64_t all = by_lanes ? (rows + 7) / 8 : rows;
             dispatch(cross_join_kernel<E>, dim3(static_cast<uint32_t>(std::min<uint64_t>(all, 65536))), dim3(256), 0, s, a,
-                     p.splits);
+                     p.splits, by_lanes);
         }
         return hipGetLastError();
     });

@@ -43,7 +43,7 @@ auto with_dtype(uint32_t dtype, F&& f) {
 // Calls f with a valid head_dim as a constant: the attention kernels are made
 // for each, as a branch around a matrix instruction keeps the compiler from
 // overlapping it with anything (4 x 2048 queries of 128 features against 5477
-// keys: 873 us with, 6xx without).
+// keys: 873 us with, 575 without).
 template <typename F>
 auto with_head_dim(uint32_t d, F&& f) {
     switch (d / 16) {
@@ -57,6 +57,15 @@ auto with_head_dim(uint32_t d, F&& f) {
         default: return f(std::integral_constant<int, 128>{});
     }
 }
+
+// The order of instructions wanted from the scheduler: the next n of a kind.
+// Left alone it puts LDS reads right before the products that wait for them.
+enum Kind { kVector = 0x2, kProducts = 0x8, kLdsReads = 0x100, kExponentials = 0x400 };
+#define DAV2_ORDER(kind, n) __builtin_amdgcn_sched_group_barrier(kind, n, 0)
+
+// Inside a branch: keeps the compiler from doing the branch's work always and
+// selecting its results afterwards.
+DAV2_DEV void stay_in_branch() { asm volatile(""); }
 
 inline bool valid_cache(const dav2_cache_i8& c) {
     return c.keys && c.values && c.key_scales && c.value_scales && aligned16(c.keys) && aligned16(c.values) &&
@@ -74,9 +83,10 @@ struct Sequence {
 DAV2_DEV Sequence sequence_of(const int32_t* starts, const int32_t* lengths, uint32_t s, uint32_t tokens) {
     Sequence q;
     const int32_t most = static_cast<int32_t>(tokens);
-    q.begin = min(max(starts[s], 0), most);
-    q.end = min(max(starts[s + 1], q.begin), most);
-    q.length = max(lengths[s], 0);
+    // in scalar registers: what is formed from them is the same for all lanes
+    q.begin = __builtin_amdgcn_readfirstlane(min(max(starts[s], 0), most));
+    q.end = __builtin_amdgcn_readfirstlane(min(max(starts[s + 1], q.begin), most));
+    q.length = __builtin_amdgcn_readfirstlane(max(lengths[s], 0));
     return q;
 }
 
@@ -146,10 +156,45 @@ inline uint64_t parts_bytes(uint64_t count, uint32_t head_dim) {
     return ((count + 1u) & ~uint64_t(1)) * sizeof(float2) + count * head_dim * sizeof(float);
 }
 
-// One row's splits, parts slot .. slot + splits - 1, joined by a workgroup of
-// 256: thread (i, f) has the four features 4 f .. of splits i, i + 8, ..., so
-// that few loads follow one another (a wave per row that walked over 64 splits
-// took 60 us). A split that saw nothing has a sum of 0 and drops out.
+// Which of the two joins below: 32 lanes per row where there are rows enough
+// to fill the chip (18464 rows of three splits: 70 us less than a workgroup
+// per row), a workgroup per row else (64 rows of eight splits: 3 us less).
+inline bool join_by_lanes(uint64_t rows, uint32_t splits) { return splits <= 8 && rows > 2048; }
+
+// Up to 8 splits of a row joined by 32 lanes, the four features 4 f .. each,
+// all loads at once. A split that saw nothing has a sum of 0 and drops out.
+template <typename E>
+DAV2_DEV void join_few(const Parts& parts, uint64_t slot, uint32_t splits, uint32_t d, E* y) {
+    const uint32_t f4 = threadIdx.x & 31u;
+    float2 stats[8];
+    v4f sums[8];
+    float top = kNoScore;
+#pragma unroll
+    for (uint32_t i = 0; i < 8; ++i) {
+        stats[i] = i < splits ? parts.stats[slot + i] : make_float2(kNoScore, 0.0f);
+        sums[i] = v4f{0.f, 0.f, 0.f, 0.f};
+        if (i < splits && 4 * f4 < d) sums[i] = *reinterpret_cast<const v4f*>(parts.sums + (slot + i) * d + 4 * f4);
+        top = fmaxf(top, stats[i].x);
+    }
+    v4f sum = {0.f, 0.f, 0.f, 0.f};
+    float total = 0.0f;
+#pragma unroll
+    for (uint32_t i = 0; i < 8; ++i) {
+        if (i >= splits) break;
+        const float weight = __builtin_amdgcn_exp2f(stats[i].x - top);
+        total = fmaf(stats[i].y, weight, total);
+        sum += sums[i] * weight;
+    }
+    if (4 * f4 >= d) return;
+    const float scale = total == 0.0f ? 0.0f : 1.0f / total;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) y[4 * f4 + i] = static_cast<E>(sum[i] * scale);
+}
+
+// More splits of a row, parts slot .. slot + splits - 1, joined by a workgroup
+// of 256: thread (i, f) has the four features 4 f .. of splits i, i + 8, ...,
+// so that few loads follow one another (a wave per row that walked over 64
+// splits took 60 us).
 template <typename E>
 DAV2_DEV void join_row(const Parts& parts, uint64_t slot, uint32_t splits, uint32_t d, E* y) {
     __shared__ float share[kMostSplits];
