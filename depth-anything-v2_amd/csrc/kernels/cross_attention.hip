@@ -87,258 +87,344 @@ DAV2_DEV v16f multiply(v4f a, v4f b, v16f c) {
     return c;
 }
 
-// A workgroup has 128 rows (row r: token r / group, query head r % group) of
-// one batch and key head, 32 for each of four waves, and goes through the keys
-// kTile at a time, copied straight into LDS (two buffers, one barrier for a
-// tile, the next tile's copies under way during a tile's products).
+// A workgroup has 32 rows (row r: token r / group, query head r % group) of one
+// batch and key head for each of its waves, and goes through the keys kTile at
+// a time.
 //
 // S^T = K Q^T and O^T = V^T P^T. Lane l holds, for query l % 32, the scores of
 // keys 8 (r / 4) + 4 (l / 32) + r % 4 of a 32-key block in registers r: the
 // right operand of the second product as it stands, if the left one takes its
 // keys in that order. In 16 bits that is two transposing LDS reads of four
 // keys by 16 features each; in fp32 four plain ones.
-template <typename E, int D>
-__global__ __launch_bounds__(256, 2) void cross_tiles_kernel(dav2_cross_attention_args a, Lists lists, uint32_t splits,
-                                                             uint32_t tiles) {
-    constexpr bool kFloat = std::is_same_v<E, float>;
-    constexpr int kTile = kFloat ? 32 : 64, kBlocks = kTile / 32;
-    constexpr int N = 16 / sizeof(E);                  // values of a piece
-    constexpr int HEAD = D <= 64 ? 64 : 128;           // features of a row in LDS
-    constexpr int KS = D / (2 * N), FB = (D + 31) / 32;  // steps over the features, blocks of 32 features
-    constexpr uint32_t d = D;
-    constexpr uint32_t kRow = HEAD * sizeof(E);        // bytes of a key in LDS
-    constexpr uint32_t kChunks = kRow / 16, kRowsPerCopy = 64 / kChunks;
-    constexpr int kCopies = kTile * kRow / 4096;       // of each wave, for the keys and again for the values
-    constexpr float kSlack = 6.0f;                     // as in cache_tiles_kernel: weights below 2^6
+template <typename E_, int D_, bool LISTED>
+struct Tiles {
+    typedef E_ E;
+    static constexpr int D = D_;
+    static constexpr bool kFloat = std::is_same_v<E, float>;
+    static constexpr int kTile = kFloat ? 32 : 64, kBlocks = kTile / 32;
+    static constexpr int N = 16 / sizeof(E);                  // values of a piece
+    static constexpr int HEAD = D <= 64 ? 64 : 128;           // features of a row in LDS
+    static constexpr int KS = D / (2 * N), FB = (D + 31) / 32;  // steps over the features, blocks of 32 features
+    static constexpr int T = kTile / (2 * N);                 // steps over the keys; step t: keys 2 N t ..
+    static constexpr uint32_t kRow = HEAD * sizeof(E);        // bytes of a key in LDS
+    static constexpr uint32_t kChunks = kRow / 16, kRowsPerCopy = 64 / kChunks;
+    static constexpr int kCopies = kTile * kRow / 4096;  // of each wave, for the keys and again for the values
+    // rescale when a score passes the running maximum by this: weights stay
+    // below 2^6 and most tiles leave the sums alone
+    static constexpr float kSlack = 6.0f;
     typedef E V __attribute__((ext_vector_type(N)));
-    __shared__ __attribute__((aligned(16))) int8_t lds[2][2][kTile * kRow];  // [buffer][keys, values]
-    const uint32_t lane = threadIdx.x & 63u, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const uint32_t col = lane & 31u, hf = lane >> 5;
-    const uint32_t group = a.heads / a.kv_heads;
-    const uint32_t b = blockIdx.x / a.kv_heads, h = blockIdx.x - b * a.kv_heads;
-    const uint32_t split = blockIdx.y % splits;
-    const uint32_t rows = a.query_tokens * group;  // batch * query_tokens * heads is below 2^32
-    const uint32_t row_tiles = (rows + 127u) / 128u;
-    const uint32_t* list = lists.keys ? lists.keys + static_cast<uint64_t>(b) * a.key_tokens : nullptr;
-    // in a scalar register: the loop and the branch for its last tile are the same for all lanes
-    const uint32_t count = __builtin_amdgcn_readfirstlane(lists.keys ? lists.counts[b] : length_of(a, b));
-    const uint32_t blocks = (count + kTile - 1u) / kTile, per = (blocks + splits - 1u) / splits;
-    const uint32_t first = split * per, last = min(first + per, blocks);
-    const E* keys = static_cast<const E*>(a.keys) + b * a.key_batch_stride + static_cast<uint64_t>(h) * d;
-    const E* values = static_cast<const E*>(a.values) + b * a.value_batch_stride + static_cast<uint64_t>(h) * d;
-    const Parts parts = parts_at(a.scratch, static_cast<uint64_t>(a.batch) * a.query_tokens * a.heads * splits);
+
+    // of the workgroup
+    const dav2_cross_attention_args& a;
+    uint32_t b, h, group, rows, count, lane, col, hf, wave;
+    const uint32_t* list;
+    const E *keys, *values;
+    // of the wave's rows
+    uint32_t token, head;
+    float c;
+    V qf[KS];       // the right operand of the scores
+    v16f o[FB];     // register r of o[f]: feature 32 f + 8 (r / 4) + 4 hf + r % 4 of row col
+    float maximum, sum;  // sum: this lane's keys only
+    V pf[T];
+
+    DAV2_DEV Tiles(const dav2_cross_attention_args& args, const Lists& lists, uint32_t plane) : a(args) {
+        lane = threadIdx.x & 63u;
+        wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+        col = lane & 31u;
+        hf = lane >> 5;
+        group = a.heads / a.kv_heads;
+        b = plane / a.kv_heads;
+        h = plane - b * a.kv_heads;
+        rows = a.query_tokens * group;  // batch * query_tokens * heads is below 2^32
+        if (LISTED) list = lists.keys + static_cast<uint64_t>(b) * a.key_tokens;
+        // in a scalar register: the loop and the branch for its last tile are the same for all lanes
+        count = __builtin_amdgcn_readfirstlane(LISTED ? lists.counts[b] : length_of(a, b));
+        keys = static_cast<const E*>(a.keys) + b * a.key_batch_stride + static_cast<uint64_t>(h) * D;
+        values = static_cast<const E*>(a.values) + b * a.value_batch_stride + static_cast<uint64_t>(h) * D;
+        // not 0, for -infinity times it has to stay what it is
+        c = a.scale == 0.0f ? 1.0e-37f : fabsf(a.scale) * kLog2e;
+    }
 
     // Copies: this wave's copy i brings rows kRowsPerCopy (kCopies wave + i) ..;
     // lane l row + l / kChunks, place l % kChunks of it. A row's chunks are
     // permuted so that what one LDS read takes from several rows lies in
     // different banks: for the keys, 16 rows at one chunk; for the values in 16
     // bits, four neighbouring rows at 32 (two times 32) bytes.
-    uint32_t place[kCopies];  // key of the copy's row in the next tile to be copied
-    auto find = [&](uint32_t block) {
+    DAV2_DEV static uint32_t key_chunk(uint32_t r, uint32_t c) { return kRow >= 256u ? c ^ (r & 15u) : c ^ ((r >> 1) & 7u); }
+    DAV2_DEV static uint32_t value_chunk(uint32_t r, uint32_t c) {
+        return kFloat ? c : kRow >= 256u ? c ^ ((r & 3u) << 2) : c ^ (((r >> 1) & 1u) << 2);
+    }
+    // The keys of this lane's rows in tile `block`; past the last key that one.
+    // Called without a condition: registers that are loaded in one branch only
+    // are waited for where the branches meet.
+    DAV2_DEV void find(uint32_t block, uint32_t (&place)[kCopies]) const {
 #pragma unroll
         for (int i = 0; i < kCopies; ++i) {
             const uint32_t r = kRowsPerCopy * (kCopies * wave + i) + lane / kChunks;
-            const uint32_t at = min(block * kTile + r, count - 1u);  // past the last key that one
-            place[i] = list ? list[at] : at;
+            const uint32_t at = min(block * kTile + r, count - 1u);
+            place[i] = LISTED ? list[at] : at;
         }
-    };
-    auto copy = [&](uint32_t buffer) {
+    }
+    // where this lane's piece of copy i is, in memory
+    DAV2_DEV const E* key_at(int i, uint32_t place) const {
+        const uint32_t r = kRowsPerCopy * (kCopies * wave + i) + lane / kChunks;
+        const uint32_t chunk = key_chunk(r, lane % kChunks);
+        // a head may end inside the row; what is behind it is not used
+        return keys + place * a.key_stride + (chunk * N >= D ? 0 : chunk * N);
+    }
+    DAV2_DEV const E* value_at(int i, uint32_t place) const {
+        const uint32_t r = kRowsPerCopy * (kCopies * wave + i) + lane / kChunks;
+        const uint32_t chunk = value_chunk(r, lane % kChunks);
+        return values + place * a.value_stride + (chunk * N >= D ? 0 : chunk * N);
+    }
+    // The tile at `place` into LDS; then place is that of tile `next`. Its loads
+    // are started before the copies, so that who uses it waits for them without
+    // the copies, and straight into its registers, which nobody has to move.
+    DAV2_DEV void copy(int8_t* to_keys, int8_t* to_values, uint32_t (&place)[kCopies], uint32_t next) const {
+        const E *from_keys[kCopies], *from_values[kCopies];
 #pragma unroll
         for (int i = 0; i < kCopies; ++i) {
-            const uint32_t r = kRowsPerCopy * (kCopies * wave + i) + lane / kChunks, c = lane % kChunks;
-            uint32_t kc = kRow >= 256u ? c ^ (r & 15u) : c ^ ((r >> 1) & 7u);
-            uint32_t vc = kFloat ? c : kRow >= 256u ? c ^ ((r & 3u) << 2) : c ^ (((r >> 1) & 1u) << 2);
-            // a head may end inside the row; what is behind it is not used
-            if (kc * N >= d) kc = 0;
-            if (vc * N >= d) vc = 0;
-            const uint32_t to = (kCopies * wave + i) * 1024u;
-            copy16_to_lds(keys + place[i] * a.key_stride + kc * N, &lds[buffer][0][to]);
-            copy16_to_lds(values + place[i] * a.value_stride + vc * N, &lds[buffer][1][to]);
+            from_keys[i] = key_at(i, place[i]);
+            from_values[i] = value_at(i, place[i]);
         }
-    };
-    auto key_piece = [&](uint32_t buffer, uint32_t r, uint32_t c) {
-        const uint32_t at = kRow >= 256u ? c ^ (r & 15u) : c ^ ((r >> 1) & 7u);
-        return *reinterpret_cast<const V*>(&lds[buffer][0][r * kRow + at * 16u]);
-    };
+        find(next, place);
+#pragma unroll
+        for (int i = 0; i < kCopies; ++i) {
+            copy16_to_lds(from_keys[i], to_keys + (kCopies * wave + i) * 1024u);
+            copy16_to_lds(from_values[i], to_values + (kCopies * wave + i) * 1024u);
+        }
+    }
 
-    for (uint32_t tile = blockIdx.y / splits; tile < row_tiles; tile += tiles) {
-        const uint32_t row0 = tile * 128u + wave * 32u;
-        const bool any_row = row0 < rows;
-        const Rows<32> of(any_row ? row0 : tile * 128u, group, rows);
-        uint32_t token, head;
+    // Rows row0 .. row0 + 31 (row0 < rows): the query, and nothing seen yet.
+    DAV2_DEV void begin(uint32_t row0) {
+        const Rows<32> of(row0, group, rows);
         of.find(col, token, head);
         head += h * group;
-        __syncthreads();  // the row tile before has been read
-        if (first < last) {
-            find(first);
-            copy(0);
-            if (first + 1u < last) find(first + 1u);
-        }
-        // the right operand of the scores; a negative scale turns its sign
-        V qf[KS];
-        {
-            const E* x = static_cast<const E*>(a.query) + b * a.query_batch_stride + token * a.query_stride +
-                         static_cast<uint64_t>(head) * d + N * hf;
+        const E* x = static_cast<const E*>(a.query) + b * a.query_batch_stride + token * a.query_stride +
+                     static_cast<uint64_t>(head) * D + N * hf;
 #pragma unroll
-            for (int k = 0; k < KS; ++k) {
-                qf[k] = *reinterpret_cast<const V*>(x + 2 * N * k);
-                if (a.scale < 0.0f) qf[k] = -qf[k];
-            }
+        for (int k = 0; k < KS; ++k) {
+            qf[k] = *reinterpret_cast<const V*>(x + 2 * N * k);
+            if (a.scale < 0.0f) qf[k] = -qf[k];
         }
-        // not 0, for -infinity times it has to stay what it is
-        const float c = a.scale == 0.0f ? 1.0e-37f : fabsf(a.scale) * kLog2e;
-        v16f o[FB];
 #pragma unroll
         for (int f = 0; f < FB; ++f)
 #pragma unroll
             for (int r = 0; r < 16; ++r) o[f][r] = 0.0f;
-        float maximum = kNoScore, sum = 0.0f;  // sum: this lane's keys only
+        maximum = kNoScore;
+        sum = 0.0f;
+    }
+
+    // A step's pieces are read before the products of the step before, which run
+    // while the read waits.
+    DAV2_DEV void multiply_keys(const int8_t* from, v16f (&sc)[kBlocks]) const {
+#pragma unroll
+        for (int i = 0; i < kBlocks; ++i)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) sc[i][r] = 0.0f;
+        // one block of reads for two steps; rows 32 apart have their chunks at the same places
+        constexpr int S = (KS + 1) / 2;
+        v4i_t in[2][4];
+        const uint32_t base = lds_address(from) + col * kRow;
+        auto at = [&](int k) { return base + key_chunk(col, 2u * k + hf) * 16u; };
+        auto read = [&](int s, v4i_t (&v)[4]) {
+            if constexpr (kBlocks == 2) {
+                if (2 * s + 1 < KS) {
+                    lds_read4<32 * kRow>(at(2 * s), at(2 * s + 1), v);
+                } else {
+                    v4i_t w[2];
+                    lds_read2<32 * kRow>(at(2 * s), w);
+                    v[0] = w[0];
+                    v[1] = w[1];
+                }
+            }
+        };
+        if constexpr (kBlocks == 2) {
+            read(0, in[0]);
+#pragma unroll
+            for (int s = 0; s < S; ++s) {
+                if (s + 1 < S) read(s + 1, in[(s + 1) & 1]);
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+                    if (2 * s + j / 2 < KS)
+                        sc[j & 1] = multiply(__builtin_bit_cast(V, in[s & 1][j]), qf[2 * s + j / 2], sc[j & 1]);
+            }
+        } else {
+            // KS is even: fp32 steps are 8 features
+            lds_read_pair(at(0), at(1), in[0][0], in[0][1]);
+#pragma unroll
+            for (int s = 0; s < S; ++s) {
+                if (s + 1 < S) lds_read_pair(at(2 * s + 2), at(2 * s + 3), in[(s + 1) & 1][0], in[(s + 1) & 1][1]);
+#pragma unroll
+                for (int j = 0; j < 2; ++j)
+                    sc[0] = multiply(__builtin_bit_cast(V, in[s & 1][j]), qf[2 * s + j], sc[0]);
+            }
+        }
+    }
+
+    // The scores of tile `block` as weights: the running maximum, the sums so
+    // far brought to it, pf and the sum of the weights.
+    DAV2_DEV void weigh(uint32_t block, v16f (&sc)[kBlocks]) {
+        if ((block + 1u) * kTile > count) {
+            stay_in_branch();
+#pragma unroll
+            for (int i = 0; i < kBlocks; ++i)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) {
+                    const uint32_t key = block * kTile + 32u * i + 8u * (r >> 2) + 4u * hf + (r & 3);
+                    if (key >= count) sc[i][r] = -INFINITY;
+                }
+        }
+        float largest = sc[0][0];
+#pragma unroll
+        for (int i = 0; i < kBlocks; ++i)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) largest = fmaxf(largest, sc[i][r]);
+        largest = over_halves(fmaxf(kNoScore, largest * c), Larger());
+        if (__any(largest > maximum + kSlack)) {
+            stay_in_branch();
+            const float grown = fmaxf(maximum, largest);
+            const float keep = __builtin_amdgcn_exp2f(maximum - grown);
+            maximum = grown;
+            sum *= keep;
+#pragma unroll
+            for (int f = 0; f < FB; ++f)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) o[f][r] *= keep;
+        }
+        float of_step[T];
+#pragma unroll
+        for (int t = 0; t < T; ++t) {
+            of_step[t] = 0.0f;
+#pragma unroll
+            for (int r = 0; r < N; ++r) {
+                const int at = N * t + r;
+                const float w = __builtin_amdgcn_exp2f(fmaf(sc[at >> 4][at & 15], c, -maximum));
+                of_step[t] += w;
+                pf[t][r] = static_cast<E>(w);
+            }
+        }
+#pragma unroll
+        for (int t = 0; t < T; ++t) sum += of_step[t];
+    }
+
+    // The values of step t, left operands of FB products. In 16 bits by
+    // transposing reads: lane j of 16 points at row j / 4, features 4 (j % 4) ..,
+    // and gets feature j of the four rows.
+    DAV2_DEV void read_values(const int8_t* from, const int t, V (&v)[FB]) const {
+        if constexpr (kFloat) {
+            const uint32_t base = lds_address(from) + (8u * t + 4u * hf) * kRow + col * 4u;
+#pragma unroll
+            for (int f = 0; f < FB; ++f) v[f] = lds_read_column<kRow>(base + 128u * f);
+        } else {
+            const uint32_t j = lane & 15u, half16 = (lane >> 4) & 1u, turn = kRow >= 256u ? j >> 2 : j >> 3;
+            const uint32_t base = lds_address(from) + (16u * t + 4u * hf + (j >> 2)) * kRow +
+                                  ((half16 << 1 | (j & 3u) >> 1) << 4) + 8u * (j & 1u);
+            s4_t p[2 * FB];
+            uint32_t at[FB];
+#pragma unroll
+            for (int f = 0; f < FB; ++f) at[f] = base + ((static_cast<uint32_t>(f) ^ turn) << 6);
+            lds_read_transposed<8 * kRow>(at, p);
+#pragma unroll
+            for (int f = 0; f < FB; ++f) {
+                union {
+                    s4_t part[2];
+                    V all;
+                } both;
+                both.part[0] = p[2 * f];
+                both.part[1] = p[2 * f + 1];
+                v[f] = both.all;
+            }
+        }
+    }
+    // A step's values are read before the products of the step before, which
+    // run while the read waits.
+    DAV2_DEV void multiply_values(const int8_t* from) {
+        V v[2][FB];
+        read_values(from, 0, v[0]);
+#pragma unroll
+        for (int t = 0; t < T; ++t) {
+            if (t + 1 < T) read_values(from, t + 1, v[(t + 1) & 1]);
+#pragma unroll
+            for (int f = 0; f < FB; ++f) o[f] = multiply(v[t & 1][f], pf[t], o[f]);
+        }
+    }
+
+    DAV2_DEV void end(uint32_t row0, uint32_t split, uint32_t splits) {
+        sum = over_halves(sum, Plus());
+        if (row0 + col >= rows) return;
+        const uint64_t slot = ((static_cast<uint64_t>(b) * a.query_tokens + token) * a.heads + head) * splits + split;
+        const Parts parts = parts_at(a.scratch, static_cast<uint64_t>(a.batch) * a.query_tokens * a.heads * splits);
+        const float scale = sum == 0.0f ? 0.0f : 1.0f / sum;
+        typedef E V4 __attribute__((ext_vector_type(4)));
+        E* y = static_cast<E*>(a.output) + b * a.output_batch_stride + token * a.output_stride +
+               static_cast<uint64_t>(head) * D;
+#pragma unroll
+        for (int f = 0; f < FB; ++f)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                const uint32_t feature = 32u * f + 8u * r + 4u * hf;
+                if (feature >= D) continue;
+                if (splits > 1) {
+                    *reinterpret_cast<v4f*>(parts.sums + slot * D + feature) =
+                        v4f{o[f][4 * r], o[f][4 * r + 1], o[f][4 * r + 2], o[f][4 * r + 3]};
+                } else {
+                    V4 out;
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) out[i] = static_cast<E>(o[f][4 * r + i] * scale);
+                    *reinterpret_cast<V4*>(y + feature) = out;
+                }
+            }
+        if (splits > 1 && hf == 0) parts.stats[slot] = make_float2(maximum, sum);
+    }
+};
+
+// Four waves, 128 rows, two buffers and one barrier for a tile, whose copies go
+// straight into LDS during the products of the tile before.
+//
+// Bound by the matrix cores and, as long again in 16 bits, the exponentials of
+// the vector units beside them: 8 x 2048 queries of 32 heads of 128 on 4096
+// keys of 8, bf16, 1.16 ms, 950 TFLOP/s, where a large library product runs at
+// 1190; heads of 64 750. fp32: 72 TFLOP/s of 152 at 2 x 577 queries, 16 heads of
+// 64, 1370 keys and fewer, where 160 workgroups are split in three. Tried and
+// not kept: eight waves in two groups that multiply and weigh in turns
+// (barriers between; 952 TFLOP/s, no difference), a tile's scores one tile
+// ahead among the exponentials (spills), tiles through registers (575 -> 610 us
+// at the masked case above).
+template <typename E, int D, bool LISTED>
+__global__ __launch_bounds__(256, 2) void cross_tiles_kernel(dav2_cross_attention_args a, Lists lists, uint32_t splits,
+                                                             uint32_t tiles) {
+    typedef Tiles<E, D, LISTED> K;
+    __shared__ __attribute__((aligned(16))) int8_t lds[2][2][K::kTile * K::kRow];  // [buffer][keys, values]
+    K k(a, lists, blockIdx.x);
+    const uint32_t split = blockIdx.y % splits, row_tiles = (k.rows + 127u) / 128u;
+    const uint32_t blocks = (k.count + K::kTile - 1u) / K::kTile, per = (blocks + splits - 1u) / splits;
+    const uint32_t first = split * per, last = min(first + per, blocks);
+    for (uint32_t tile = blockIdx.y / splits; tile < row_tiles; tile += tiles) {
+        const uint32_t row0 = tile * 128u + k.wave * 32u;
+        const bool any_row = row0 < k.rows;
+        uint32_t place[K::kCopies];  // of the tile that is copied next
+        __syncthreads();             // the row tile before has been read
+        if (first < last) {
+            k.find(first, place);
+            k.copy(lds[0][0], lds[0][1], place, first + 1u);
+        }
+        k.begin(any_row ? row0 : tile * 128u);
         DAV2_WAIT_VMCNT(0);
         __syncthreads();
         for (uint32_t block = first; block < last; ++block) {
             const uint32_t buffer = (block - first) & 1u;
-            if (block + 1u < last) {
-                copy(buffer ^ 1u);
-                if (block + 2u < last) find(block + 2u);
-            }
+            k.copy(lds[buffer ^ 1u][0], lds[buffer ^ 1u][1], place, block + 2u);  // behind the last tile its last key, unread
             if (any_row) {
-                v16f sc[kBlocks];
-#pragma unroll
-                for (int i = 0; i < kBlocks; ++i)
-#pragma unroll
-                    for (int r = 0; r < 16; ++r) sc[i][r] = 0.0f;
-#pragma unroll
-                for (int k = 0; k < KS; ++k)
-#pragma unroll
-                    for (int i = 0; i < kBlocks; ++i)
-                        sc[i] = multiply(key_piece(buffer, 32u * i + col, 2u * k + hf), qf[k], sc[i]);
-                // reads kAhead pieces ahead of their products
-                constexpr int kAhead = KS * kBlocks < 8 ? KS * kBlocks : 8, kEach = kFloat ? 4 : 1;
-                DAV2_ORDER(kLdsReads, kAhead);
-#pragma unroll
-                for (int i = 0; i < KS * kBlocks; ++i) {
-                    DAV2_ORDER(kProducts, kEach);
-                    if (i + kAhead < KS * kBlocks) DAV2_ORDER(kLdsReads, 1);
-                }
-                if ((block + 1u) * kTile > count) {
-                    stay_in_branch();
-#pragma unroll
-                    for (int i = 0; i < kBlocks; ++i)
-#pragma unroll
-                        for (int r = 0; r < 16; ++r) {
-                            const uint32_t key = block * kTile + 32u * i + 8u * (r >> 2) + 4u * hf + (r & 3);
-                            if (key >= count) sc[i][r] = -INFINITY;
-                        }
-                }
-                float largest = sc[0][0];
-#pragma unroll
-                for (int i = 0; i < kBlocks; ++i)
-#pragma unroll
-                    for (int r = 0; r < 16; ++r) largest = fmaxf(largest, sc[i][r]);
-                largest = over_halves(fmaxf(kNoScore, largest * c), Larger());
-                if (__any(largest > maximum + kSlack)) {
-                    stay_in_branch();
-                    const float grown = fmaxf(maximum, largest);
-                    const float keep = __builtin_amdgcn_exp2f(maximum - grown);
-                    maximum = grown;
-                    sum *= keep;
-#pragma unroll
-                    for (int f = 0; f < FB; ++f)
-#pragma unroll
-                        for (int r = 0; r < 16; ++r) o[f][r] *= keep;
-                }
-                // step t: keys 2 N t ..; its weights are formed among the products of the step before
-                constexpr int T = kTile / (2 * N);
-                V pf[T];
-                float parts_of_sum[T];
-#pragma unroll
-                for (int t = 0; t < T; ++t) {
-                    parts_of_sum[t] = 0.0f;
-#pragma unroll
-                    for (int r = 0; r < N; ++r) {
-                        const int at = N * t + r;
-                        const float w = __builtin_amdgcn_exp2f(fmaf(sc[at >> 4][at & 15], c, -maximum));
-                        parts_of_sum[t] += w;
-                        pf[t][r] = static_cast<E>(w);
-                    }
-                }
-#pragma unroll
-                for (int t = 0; t < T; ++t) sum += parts_of_sum[t];
-#pragma unroll
-                for (int t = 0; t < T; ++t)
-#pragma unroll
-                    for (int f = 0; f < FB; ++f) {
-                        V vf;
-                        if constexpr (kFloat) {
-#pragma unroll
-                            for (int e = 0; e < 4; ++e)
-                                vf[e] = *reinterpret_cast<const float*>(
-                                    &lds[buffer][1][(8u * t + 4u * hf + e) * kRow + (32u * f + col) * 4u]);
-                        } else {
-                            // lane j of 16 points at row j / 4, features 4 (j % 4) ..; it gets feature j of the four rows
-                            const uint32_t j = lane & 15u, half16 = (lane >> 4) & 1u;
-                            const uint32_t turn = kRow >= 256u ? j >> 2 : j >> 3;
-                            const uint32_t at = (((static_cast<uint32_t>(f) ^ turn) << 2 | half16 << 1 | (j & 3u) >> 1) << 4) +
-                                                8u * (j & 1u);
-                            typedef short s4 __attribute__((ext_vector_type(4)));
-                            typedef __attribute__((address_space(3))) s4* lds_s4;
-                            int8_t* row = &lds[buffer][1][(16u * t + 4u * hf + (j >> 2)) * kRow + at];
-                            union {
-                                s4 part[2];
-                                V all;
-                            } both;
-                            both.part[0] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4)row);
-                            both.part[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4)(row + 8u * kRow));
-                            vf = both.all;
-                        }
-                        o[f] = multiply(vf, pf[t], o[f]);
-                    }
-                // a step's values are read, and its weights formed, among the products of the step before
-                constexpr int kReads = kFloat ? 4 : 2;
-                DAV2_ORDER(kLdsReads, FB * kReads);
-                DAV2_ORDER(kVector, 3 * N);
-                DAV2_ORDER(kExponentials, N);
-#pragma unroll
-                for (int t = 0; t < T; ++t)
-#pragma unroll
-                    for (int f = 0; f < FB; ++f) {
-                        DAV2_ORDER(kProducts, kEach);
-                        if (t + 1 < T) {
-                            DAV2_ORDER(kLdsReads, kReads);
-                            DAV2_ORDER(kVector, (3 * N + FB - 1) / FB);
-                            DAV2_ORDER(kExponentials, (N + FB - 1) / FB);
-                        }
-                    }
+                v16f sc[K::kBlocks];
+                k.multiply_keys(lds[buffer][0], sc);
+                k.weigh(block, sc);
+                k.multiply_values(lds[buffer][1]);
             }
             DAV2_WAIT_VMCNT(0);
-            __syncthreads();
+            lds_turn();
         }
-        sum = over_halves(sum, Plus());
-        // register r of o[f]: feature 32 f + 8 (r / 4) + 4 hf + r % 4 of row col
-        if (row0 + col < rows) {
-            const uint64_t slot = ((static_cast<uint64_t>(b) * a.query_tokens + token) * a.heads + head) * splits + split;
-            const float scale = sum == 0.0f ? 0.0f : 1.0f / sum;
-            typedef E V4 __attribute__((ext_vector_type(4)));
-            E* y = static_cast<E*>(a.output) + b * a.output_batch_stride + token * a.output_stride +
-                   static_cast<uint64_t>(head) * d;
-#pragma unroll
-            for (int f = 0; f < FB; ++f)
-#pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    const uint32_t feature = 32u * f + 8u * r + 4u * hf;
-                    if (feature >= d) continue;
-                    if (splits > 1) {
-                        *reinterpret_cast<v4f*>(parts.sums + slot * d + feature) =
-                            v4f{o[f][4 * r], o[f][4 * r + 1], o[f][4 * r + 2], o[f][4 * r + 3]};
-                    } else {
-                        V4 out;
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) out[i] = static_cast<E>(o[f][4 * r + i] * scale);
-                        *reinterpret_cast<V4*>(y + feature) = out;
-                    }
-                }
-            if (splits > 1 && hf == 0) parts.stats[slot] = make_float2(maximum, sum);
-        }
+        k.end(row0, split, splits);
     }
 }
 
@@ -417,7 +503,9 @@ int dav2_hip_cross_attention(const dav2_cross_attention_args* args, void* stream
     return with_dtype(a.dtype, [&](auto* e) -> int {
         typedef std::remove_pointer_t<decltype(e)> E;
         with_head_dim(a.head_dim, [&](auto dim) {
-            dispatch(cross_tiles_kernel<E, decltype(dim)::value>, grid, dim3(256), 0, s, a, lists, p.splits, p.tiles);
+            constexpr int D = decltype(dim)::value;
+            dispatch(lists.keys ? cross_tiles_kernel<E, D, true> : cross_tiles_kernel<E, D, false>, grid, dim3(256), 0, s, a,
+                     lists, p.splits, p.tiles);
         });
         if (p.splits > 1) {
             const uint64_t rows = static_cast<uint64_t>(a.batch) * a.query_tokens * a.heads;

@@ -58,10 +58,69 @@ auto with_head_dim(uint32_t d, F&& f) {
     }
 }
 
-// The order of instructions wanted from the scheduler: the next n of a kind.
-// Left alone it puts LDS reads right before the products that wait for them.
-enum Kind { kVector = 0x2, kProducts = 0x8, kLdsReads = 0x100, kExponentials = 0x400 };
-#define DAV2_ORDER(kind, n) __builtin_amdgcn_sched_group_barrier(kind, n, 0)
+// LDS reads beside copies into LDS that are under way. The compiler would have
+// a read wait for every such copy, so these are written out, each block with
+// its own wait: nothing of it is in flight behind it. What was copied is
+// visible after DAV2_WAIT_VMCNT and lds_turn.
+typedef int v4i_t __attribute__((ext_vector_type(4)));
+typedef short s4_t __attribute__((ext_vector_type(4)));
+DAV2_DEV uint32_t lds_address(const void* p) { return static_cast<uint32_t>(reinterpret_cast<uintptr_t>((lds_ptr_t)p)); }
+
+// 16 bytes each at a and a + STEP (and b and b + STEP)
+template <uint32_t STEP>
+DAV2_DEV void lds_read2(uint32_t a, v4i_t (&v)[2]) {
+    asm volatile("ds_read_b128 %0, %2\n\tds_read_b128 %1, %2 offset:%3\n\ts_waitcnt lgkmcnt(0)"
+                 : "=&v"(v[0]), "=&v"(v[1]) : "v"(a), "n"(STEP) : "memory");
+}
+template <uint32_t STEP>
+DAV2_DEV void lds_read4(uint32_t a, uint32_t b, v4i_t (&v)[4]) {
+    asm volatile("ds_read_b128 %0, %4\n\tds_read_b128 %1, %4 offset:%6\n\t"
+                 "ds_read_b128 %2, %5\n\tds_read_b128 %3, %5 offset:%6\n\ts_waitcnt lgkmcnt(0)"
+                 : "=&v"(v[0]), "=&v"(v[1]), "=&v"(v[2]), "=&v"(v[3]) : "v"(a), "v"(b), "n"(STEP) : "memory");
+}
+DAV2_DEV void lds_read_pair(uint32_t a, uint32_t b, v4i_t& v, v4i_t& w) {
+    asm volatile("ds_read_b128 %0, %2\n\tds_read_b128 %1, %3\n\ts_waitcnt lgkmcnt(0)"
+                 : "=&v"(v), "=&v"(w) : "v"(a), "v"(b) : "memory");
+}
+// transposing reads: four rows by 16 columns of 16 bits for each 16 lanes, at
+// a[i] and a[i] + STEP
+template <uint32_t STEP, int N>
+DAV2_DEV void lds_read_transposed(const uint32_t (&a)[N], s4_t (&v)[2 * N]) {
+    static_assert(N >= 1 && N <= 4);
+    if constexpr (N == 1)
+        asm volatile("ds_read_b64_tr_b16 %0, %2\n\tds_read_b64_tr_b16 %1, %2 offset:%3\n\ts_waitcnt lgkmcnt(0)"
+                     : "=&v"(v[0]), "=&v"(v[1]) : "v"(a[0]), "n"(STEP) : "memory");
+    else if constexpr (N == 2)
+        asm volatile("ds_read_b64_tr_b16 %0, %4\n\tds_read_b64_tr_b16 %1, %4 offset:%6\n\t"
+                     "ds_read_b64_tr_b16 %2, %5\n\tds_read_b64_tr_b16 %3, %5 offset:%6\n\ts_waitcnt lgkmcnt(0)"
+                     : "=&v"(v[0]), "=&v"(v[1]), "=&v"(v[2]), "=&v"(v[3]) : "v"(a[0]), "v"(a[1]), "n"(STEP) : "memory");
+    else if constexpr (N == 3)
+        asm volatile("ds_read_b64_tr_b16 %0, %6\n\tds_read_b64_tr_b16 %1, %6 offset:%9\n\t"
+                     "ds_read_b64_tr_b16 %2, %7\n\tds_read_b64_tr_b16 %3, %7 offset:%9\n\t"
+                     "ds_read_b64_tr_b16 %4, %8\n\tds_read_b64_tr_b16 %5, %8 offset:%9\n\ts_waitcnt lgkmcnt(0)"
+                     : "=&v"(v[0]), "=&v"(v[1]), "=&v"(v[2]), "=&v"(v[3]), "=&v"(v[4]), "=&v"(v[5])
+                     : "v"(a[0]), "v"(a[1]), "v"(a[2]), "n"(STEP) : "memory");
+    else
+        asm volatile("ds_read_b64_tr_b16 %0, %8\n\tds_read_b64_tr_b16 %1, %8 offset:%12\n\t"
+                     "ds_read_b64_tr_b16 %2, %9\n\tds_read_b64_tr_b16 %3, %9 offset:%12\n\t"
+                     "ds_read_b64_tr_b16 %4, %10\n\tds_read_b64_tr_b16 %5, %10 offset:%12\n\t"
+                     "ds_read_b64_tr_b16 %6, %11\n\tds_read_b64_tr_b16 %7, %11 offset:%12\n\ts_waitcnt lgkmcnt(0)"
+                     : "=&v"(v[0]), "=&v"(v[1]), "=&v"(v[2]), "=&v"(v[3]), "=&v"(v[4]), "=&v"(v[5]), "=&v"(v[6]),
+                       "=&v"(v[7])
+                     : "v"(a[0]), "v"(a[1]), "v"(a[2]), "v"(a[3]), "n"(STEP) : "memory");
+}
+// one float each at a, a + ROW, a + 2 ROW, a + 3 ROW
+template <uint32_t ROW>
+DAV2_DEV v4f lds_read_column(uint32_t a) {
+    float x, y, z, w;
+    asm volatile("ds_read_b32 %0, %4\n\tds_read_b32 %1, %4 offset:%5\n\tds_read_b32 %2, %4 offset:%6\n\t"
+                 "ds_read_b32 %3, %4 offset:%7\n\ts_waitcnt lgkmcnt(0)"
+                 : "=&v"(x), "=&v"(y), "=&v"(z), "=&v"(w) : "v"(a), "n"(ROW), "n"(2 * ROW), "n"(3 * ROW) : "memory");
+    return v4f{x, y, z, w};
+}
+
+// A barrier that waits for this wave's LDS accesses and for nothing else.
+DAV2_DEV void lds_turn() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
 
 // Inside a branch: keeps the compiler from doing the branch's work always and
 // selecting its results afterwards.
