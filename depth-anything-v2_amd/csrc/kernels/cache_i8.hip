@@ -514,14 +514,15 @@ __global__ __launch_bounds__(256, 2) void cache_rows_kernel(dav2_attention_cache
 // second product's step t if V^T holds its keys in that order, which their
 // place in LDS gives them: keys 0-3, 8-11 of a chunk, then 4-7, 12-15. Eight
 // registers are one 16-token chunk, so scales are uniform for them.
-template <typename E, int D>
-__global__ __launch_bounds__(256, 2) void cache_tiles_kernel(dav2_attention_cache_i8_args a, uint32_t splits,
+template <typename E, int D, int WAVES>
+__global__ __launch_bounds__(64 * WAVES, 2) void cache_tiles_kernel(dav2_attention_cache_i8_args a, uint32_t splits,
                                                              uint32_t tiles) {
     constexpr bool kFloat = std::is_same_v<E, float>;
     constexpr int HEAD = D <= 64 ? 64 : 128;  // features of a row in LDS
     constexpr int KS = D / 16, FB = (D + 31) / 32, NP = kFloat ? 2 : 1;
     constexpr uint32_t d = D;
-    constexpr int kPieces = HEAD / 64;   // of 16 codes, for each thread and tile: keys, and values
+    constexpr uint32_t kThreads = 64 * WAVES, kTileRows = 32 * WAVES;
+    constexpr int kPieces = HEAD * 4 > kThreads ? HEAD * 4 / kThreads : 1;  // of 16 codes, for each thread and tile: keys, and values
     constexpr int kRow = HEAD * 2;       // bytes of a key row in LDS
     // rescale when a score passes the running maximum by this: weights stay
     // below 2^6, far inside binary16, and most tiles leave the sums alone
@@ -539,7 +540,7 @@ __global__ __launch_bounds__(256, 2) void cache_tiles_kernel(dav2_attention_cach
     const int64_t span = static_cast<int64_t>(a.table_pages) * page_size;
     const Pages pages = pages_of(a, s);
     const Parts parts = parts_of(a, splits);
-    const uint32_t row_tiles = (rows + 127u) / 128u;
+    const uint32_t row_tiles = (rows + kTileRows - 1u) / kTileRows;
     auto seen = [&](uint32_t i) {
         int64_t t = q.length;
         if (a.causal) t += 1 + static_cast<int64_t>(i) - n;
@@ -549,16 +550,16 @@ __global__ __launch_bounds__(256, 2) void cache_tiles_kernel(dav2_attention_cach
     // the last rows first: under a causal mask they see the most keys
     for (uint32_t turn = blockIdx.y / splits; turn < row_tiles; turn += tiles) {
         const uint32_t tile = row_tiles - 1u - turn;
-        const uint32_t row0 = tile * 128u + wave * 32u;  // of this wave
+        const uint32_t row0 = tile * kTileRows + wave * 32u;  // of this wave
         const bool any_row = row0 < rows;
-        const Rows<32> of(any_row ? row0 : tile * 128u, group, rows);
+        const Rows<32> of(any_row ? row0 : tile * kTileRows, group, rows);
         uint32_t token, head, last_token, last_head;
         of.find(col, token, head);
         of.find(31u, last_token, last_head);
         head += h * group;
         const uint32_t limit = row0 + col < rows ? seen(token) : 0u;
         const uint32_t wave_most = any_row ? seen(last_token) : 0u, wave_least = seen(of.token);
-        const uint32_t most = seen((min(tile * 128u + 128u, rows) - 1u) / group);
+        const uint32_t most = seen((min(tile * kTileRows + kTileRows, rows) - 1u) / group);
         const uint32_t blocks = (most + 63u) / 64u, per = (blocks + splits - 1u) / splits;
         const uint32_t first = split * per, last = min(first + per, blocks);
 
@@ -569,39 +570,41 @@ __global__ __launch_bounds__(256, 2) void cache_tiles_kernel(dav2_attention_cach
         bool exists = false;
         const uint32_t key_chunk = threadIdx.x % (HEAD / 16), key_row = threadIdx.x / (HEAD / 16);
         const uint32_t value_chunk = threadIdx.x & 3u, value_row = threadIdx.x >> 2;
-        constexpr uint32_t kKeyStep = 256u / (HEAD / 16);
+        constexpr uint32_t kKeyStep = kThreads / (HEAD / 16), kValueStep = kThreads / 4;
+        // rows of keys and values that this thread brings (heads of 64 leave half of eight waves without)
+        const bool has_key = 16u * key_chunk < d && key_row < 64u;
+        // Called without a condition, and never past the last block: registers
+        // that are loaded in one branch only are waited for where the branches
+        // meet.
         auto find = [&](uint32_t block) {
+            block = min(block, last - 1u);
 #pragma unroll
-            for (int i = 0; i < kPieces; ++i) of_key[i] = pages.find(block * 4u + (key_row + kKeyStep * i) / 16u);
+            for (int i = 0; i < kPieces; ++i) of_key[i] = pages.find(block * 4u + min((key_row + kKeyStep * i) / 16u, 3u));
             of_value = pages.find(block * 4u + value_chunk);
         };
         auto load = [&] {
 #pragma unroll
             for (int i = 0; i < kPieces; ++i) {
                 const uint64_t plane = static_cast<uint64_t>(pages.page(of_key[i])) * kv_heads + h;
-                const int8_t* k = a.cache.keys +
-                                  (plane * page_size + of_key[i].slot + (key_row + kKeyStep * i) % 16u) * d + 16u * key_chunk;
-                if (16u * key_chunk < d) key_codes[i] = *reinterpret_cast<const uint4*>(k);
+                key_codes[i] = *reinterpret_cast<const uint4*>(
+                    a.cache.keys + (plane * page_size + of_key[i].slot + (key_row + kKeyStep * i) % 16u) * d +
+                    (has_key ? 16u * key_chunk : 0u));
             }
             exists = pages.exists(of_value);
             const uint64_t plane = static_cast<uint64_t>(pages.page(of_value)) * kv_heads + h;
 #pragma unroll
-            for (int i = 0; i < kPieces; ++i) {
-                const uint32_t f = value_row + 64u * i;
-                if (f < d)
-                    value_codes[i] = *reinterpret_cast<const uint4*>(a.cache.values + (plane * d + f) * page_size + of_value.slot);
-            }
-            if (threadIdx.x < 4) {
-                key_scale = a.cache.key_scales[plane];
-                value_scale = a.cache.value_scales[plane];
-            }
+            for (int i = 0; i < kPieces; ++i)
+                value_codes[i] = *reinterpret_cast<const uint4*>(
+                    a.cache.values + (plane * d + min(value_row + kValueStep * i, d - 1u)) * page_size + of_value.slot);
+            key_scale = a.cache.key_scales[plane];
+            value_scale = a.cache.value_scales[plane];
         };
         auto store = [&](uint32_t buffer) {
 #pragma unroll
             for (int i = 0; i < kPieces; ++i) {
                 const uint4 k = key_codes[i], v = value_codes[i];
-                const uint32_t r = key_row + kKeyStep * i, f = value_row + 64u * i;
-                if (16u * key_chunk < d) {
+                const uint32_t r = key_row + kKeyStep * i, f = value_row + kValueStep * i;
+                if (has_key) {
                     *reinterpret_cast<h8*>(lds_keys[buffer] + swz<kRow>(r, 2u * key_chunk)) = widen(k.x, k.y);
                     *reinterpret_cast<h8*>(lds_keys[buffer] + swz<kRow>(r, 2u * key_chunk + 1u)) = widen(k.z, k.w);
                 }
@@ -620,11 +623,9 @@ __global__ __launch_bounds__(256, 2) void cache_tiles_kernel(dav2_attention_cach
                     c[2] = inverse / fraction;
                 }
                 if (!exists) c = v4f{0.f, 0.f, 0.f, 0.f};
-                c[3] = exists ? fraction : 0.0f;
                 lds_scales[buffer][threadIdx.x] = c;
             }
         };
-        // places of the table that a tile past the last may not be asked for
         __syncthreads();  // the row tile before has been read
         if (first < last) {
             find(first);
@@ -673,35 +674,51 @@ __global__ __launch_bounds__(256, 2) void cache_tiles_kernel(dav2_attention_cach
 
         if (first < last) {
             store(0);
-            if (first + 1u < last) {
-                find(first + 1u);
-                load();
-                if (first + 2u < last) find(first + 2u);
-            }
+            find(first + 1u);
+            load();
+            find(first + 2u);
         }
         __syncthreads();
         for (uint32_t block = first; block < last; ++block) {
             const uint32_t buffer = (block - first) & 1u;
-            if (block + 1u < last) {
-                store(buffer ^ 1u);
-                if (block + 2u < last) {
-                    load();
-                    if (block + 3u < last) find(block + 3u);
-                }
-            }
+            store(buffer ^ 1u);  // behind the last tile that one again, unread
+            load();
+            find(block + 3u);
             const uint32_t k0 = block * 64u;
             if (k0 < wave_most) {
                 v16f sc[2];
 #pragma unroll
-                for (int b = 0; b < 2; ++b) {
+                for (int b = 0; b < 2; ++b)
 #pragma unroll
                     for (int r = 0; r < 16; ++r) sc[b][r] = 0.0f;
+                // A step's pieces are read before the products of the step
+                // before, which run while the read waits.
+                {
+                    constexpr int S = (KS + 1) / 2;  // of two steps over the features and both blocks
+                    v4i_t in[2][4];
+                    const uint32_t base = lds_address(lds_keys[buffer]);
+                    auto read = [&](int i, v4i_t (&v)[4]) {
+                        const uint32_t at = base + swz<kRow>(col, 4u * i + hf);
+                        if (2 * i + 1 < KS) {
+                            lds_read4<32 * kRow>(at, base + swz<kRow>(col, 4u * i + 2u + hf), v);
+                        } else {
+                            v4i_t w[2];
+                            lds_read2<32 * kRow>(at, w);
+                            v[0] = w[0];
+                            v[1] = w[1];
+                        }
+                    };
+                    read(0, in[0]);
 #pragma unroll
-                    for (int k = 0; k < KS; ++k) {
-                        const h8 kf = *reinterpret_cast<const h8*>(lds_keys[buffer] + swz<kRow>(32u * b + col, 2u * k + hf));
+                    for (int i = 0; i < S; ++i) {
+                        if (i + 1 < S) read(i + 1, in[(i + 1) & 1]);
 #pragma unroll
-                        for (int p = 0; p < NP; ++p)
-                            sc[b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf, qf[p][k], sc[b], 0, 0, 0);
+                        for (int j = 0; j < 4; ++j)
+                            if (2 * i + j / 2 < KS)
+#pragma unroll
+                                for (int p = 0; p < NP; ++p)
+                                    sc[j & 1] = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(h8, in[i & 1][j]),
+                                                                                       qf[p][2 * i + j / 2], sc[j & 1], 0, 0, 0);
                     }
                 }
                 // chunk t of the tile: registers 8 (t % 2) .. of block t / 2
@@ -773,18 +790,23 @@ __global__ __launch_bounds__(256, 2) void cache_tiles_kernel(dav2_attention_cach
                     }
                     sum = fmaf(part, inverse[t], sum);
                 }
-#pragma unroll
-                for (int f = 0; f < FB; ++f) {
+                {
+                    v4i_t in[2][FB];  // of rows 32 f + col, whose chunks are at the same places
+                    const uint32_t base = lds_address(lds_values[buffer]);
+                    lds_read_rows<32 * 128>(base + swz<128>(col, hf), in[0]);
 #pragma unroll
                     for (int t = 0; t < 4; ++t) {
-                        const h8 vf = *reinterpret_cast<const h8*>(lds_values[buffer] + swz<128>(32u * f + col, 2u * t + hf));
+                        if (t < 3) lds_read_rows<32 * 128>(base + swz<128>(col, 2u * t + 2u + hf), in[(t + 1) & 1]);
 #pragma unroll
-                        for (int p = 0; p < NP; ++p)
-                            o[f] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf, pf[p][t], o[f], 0, 0, 0);
+                        for (int f = 0; f < FB; ++f)
+#pragma unroll
+                            for (int p = 0; p < NP; ++p)
+                                o[f] = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(h8, in[t & 1][f]), pf[p][t],
+                                                                              o[f], 0, 0, 0);
                     }
                 }
             }
-            __syncthreads();
+            lds_turn();
         }
         sum = over_halves(sum, Plus());
         // register r of o[f]: feature 32 f + 8 (r / 4) + 4 hf + r % 4 of row col
@@ -840,7 +862,7 @@ bool valid(const dav2_attention_cache_i8_args& a) {
     return valid_cache(a.cache) && a.query && a.output && aligned16(a.query) && aligned16(a.output) && a.page_table &&
            a.starts && a.lengths && a.dtype <= DAV2_DTYPE_BF16 && a.sequences <= 65535u && a.tokens <= 0x7fffffffu &&
            a.table_pages > 0 && a.table_pages <= 0x7fffffffu && a.heads > 0 && a.heads <= 65535u &&
-           a.heads % a.cache.kv_heads == 0 && static_cast<uint64_t>(a.tokens) * a.heads <= 0xffffff00ull &&
+           a.heads % a.cache.kv_heads == 0 && static_cast<uint64_t>(a.tokens) * a.heads <= 0xfffffe00ull &&
            static_cast<uint64_t>(a.sequences) * a.cache.kv_heads <= 0x7fffffull &&
            a.query_stride % 8 == 0 && a.output_stride % 8 == 0 &&
            (a.tokens == 1 || (a.query_stride >= row && a.output_stride >= row));
@@ -855,19 +877,18 @@ bool valid(const dav2_attention_cache_i8_args& a) {
 // workgroups), 24.0 in 16; 32 of up to 32768 257 in 2 (512), 244 in 4, 242 in
 // 8; one token over 1370 keys, 16 heads of 64, 11.9 in 2, 10.4 in 5, 9.2 in 10.
 struct Plan {
-    bool tiled;  // cache_tiles_kernel, otherwise cache_rows_kernel
+    uint32_t tile;  // rows: 16 of cache_rows_kernel, 128 or 256 of cache_tiles_kernel
     uint32_t tiles, splits;
 };
 Plan plan_of(const dav2_attention_cache_i8_args& a) {
-    Plan p{false, 1, 1};
+    Plan p{16, 1, 1};
     if (a.cache.kv_heads == 0 || a.heads < a.cache.kv_heads || a.sequences == 0 || a.max_query == 0) return p;
     const uint64_t rows = static_cast<uint64_t>(std::min(a.max_query, a.tokens)) * (a.heads / a.cache.kv_heads);
-    p.tiled = rows > 32;
-    const uint32_t tile = p.tiled ? 128 : 16;
-    p.tiles = static_cast<uint32_t>(std::min<uint64_t>((rows + tile - 1) / tile, p.tiled ? 512 : 4096));
+    p.tile = rows > 32 ? (rows >= 1024 ? 256 : 128) : 16;
+    p.tiles = static_cast<uint32_t>(std::min<uint64_t>((rows + p.tile - 1) / p.tile, p.tile > 16 ? 512 : 4096));
     const uint64_t have = std::max<uint64_t>(1, static_cast<uint64_t>(p.tiles) * a.cache.kv_heads * a.sequences);
-    const uint64_t resident = std::min<uint64_t>(512 / have, a.max_length / 128);
-    const uint64_t even = p.tiled ? 1 : std::min<uint64_t>(2048 / have, a.max_length / 2048);
+    const uint64_t resident = std::min<uint64_t>((p.tile == 256 ? 256 : 512) / have, a.max_length / 128);
+    const uint64_t even = p.tile > 16 ? 1 : std::min<uint64_t>(2048 / have, a.max_length / 2048);
     p.splits = static_cast<uint32_t>(std::clamp<uint64_t>(std::max(resident, even), 1, kMostSplits));
     return p;
 }
@@ -917,13 +938,14 @@ int dav2_hip_attention_cache_i8(const dav2_attention_cache_i8_args* args, void* 
     if (need && (!a.scratch || !aligned16(a.scratch) || a.scratch_bytes < need)) return hipErrorInvalidValue;
     const hipStream_t s = static_cast<hipStream_t>(stream);
     const Plan p = plan_of(a);
-    const dim3 grid = p.tiled ? dim3(a.cache.kv_heads * a.sequences, p.tiles * p.splits)
+    const dim3 grid = p.tile > 16 ? dim3(a.cache.kv_heads * a.sequences, p.tiles * p.splits)
                               : dim3(p.tiles * p.splits, a.cache.kv_heads, a.sequences);
     return with_dtype(a.dtype, [&](auto* e) -> int {
         typedef std::remove_pointer_t<decltype(e)> E;
         with_head_dim(a.cache.head_dim, [&](auto dim) {
             constexpr int D = decltype(dim)::value;
-            if (p.tiled) dispatch(cache_tiles_kernel<E, D>, grid, dim3(256), 0, s, a, p.splits, p.tiles);
+            if (p.tile == 256) dispatch(cache_tiles_kernel<E, D, 8>, grid, dim3(512), 0, s, a, p.splits, p.tiles);
+            else if (p.tile == 128) dispatch(cache_tiles_kernel<E, D, 4>, grid, dim3(256), 0, s, a, p.splits, p.tiles);
             else dispatch(cache_rows_kernel<E, D>, grid, dim3(256), 0, s, a, p.splits, p.tiles);
         });
         if (p.splits > 1) {

@@ -78,6 +78,25 @@ DAV2_DEV void lds_read4(uint32_t a, uint32_t b, v4i_t (&v)[4]) {
                  "ds_read_b128 %2, %5\n\tds_read_b128 %3, %5 offset:%6\n\ts_waitcnt lgkmcnt(0)"
                  : "=&v"(v[0]), "=&v"(v[1]), "=&v"(v[2]), "=&v"(v[3]) : "v"(a), "v"(b), "n"(STEP) : "memory");
 }
+// ... at a, a + STEP, .. of N rows
+template <uint32_t STEP, int N>
+DAV2_DEV void lds_read_rows(uint32_t a, v4i_t (&v)[N]) {
+    static_assert(N >= 1 && N <= 4);
+    if constexpr (N == 1)
+        asm volatile("ds_read_b128 %0, %1\n\ts_waitcnt lgkmcnt(0)" : "=&v"(v[0]) : "v"(a) : "memory");
+    else if constexpr (N == 2)
+        asm volatile("ds_read_b128 %0, %2\n\tds_read_b128 %1, %2 offset:%3\n\ts_waitcnt lgkmcnt(0)"
+                     : "=&v"(v[0]), "=&v"(v[1]) : "v"(a), "n"(STEP) : "memory");
+    else if constexpr (N == 3)
+        asm volatile("ds_read_b128 %0, %3\n\tds_read_b128 %1, %3 offset:%4\n\tds_read_b128 %2, %3 offset:%5\n\t"
+                     "s_waitcnt lgkmcnt(0)"
+                     : "=&v"(v[0]), "=&v"(v[1]), "=&v"(v[2]) : "v"(a), "n"(STEP), "n"(2 * STEP) : "memory");
+    else
+        asm volatile("ds_read_b128 %0, %4\n\tds_read_b128 %1, %4 offset:%5\n\tds_read_b128 %2, %4 offset:%6\n\t"
+                     "ds_read_b128 %3, %4 offset:%7\n\ts_waitcnt lgkmcnt(0)"
+                     : "=&v"(v[0]), "=&v"(v[1]), "=&v"(v[2]), "=&v"(v[3])
+                     : "v"(a), "n"(STEP), "n"(2 * STEP), "n"(3 * STEP) : "memory");
+}
 DAV2_DEV void lds_read_pair(uint32_t a, uint32_t b, v4i_t& v, v4i_t& w) {
     asm volatile("ds_read_b128 %0, %2\n\tds_read_b128 %1, %3\n\ts_waitcnt lgkmcnt(0)"
                  : "=&v"(v), "=&v"(w) : "v"(a), "v"(b) : "memory");

@@ -584,7 +584,7 @@ DAV2_API int dav2_hip_cache_store_i8(const dav2_cache_store_i8_args* args, void*
  * i of n sees the first lengths[s] - n + 1 + i tokens; otherwise all. heads is
  * a multiple of kv_heads; head h reads head h / (heads / kv_heads) of the
  * cache. A row that sees nothing gives zeros; output rows of no sequence are
- * left as they were. tokens * heads stays below 2^32 - 256, sequences *
+ * left as they were. tokens * heads stays below 2^32 - 512, sequences *
  * kv_heads below 2^23. Strides (elements
  * between tokens) are multiples of 8, query and output 16-byte aligned. max_query and max_length, the most new
  * and the most tokens of a sequence, size the launch and the scratch; a
