@@ -191,10 +191,11 @@ __global__ __launch_bounds__(256, 8) void cache_store_kernel(dav2_cache_store_i8
 // are; L is summed in fp32 from the unrounded w.
 
 // Page and slot of a 16-token chunk; magic = ceil(2^32 / chunks per page),
-// which divides every chunk below 2^28 exactly (chunks per page <= 16).
+// which divides every chunk below 2^28 exactly (2 to 16 chunks per page). For
+// one chunk per page that is 0 in 32 bits, and alone adds the chunk itself.
 struct Pages {
     const int32_t* table;  // of one sequence
-    uint32_t table_pages, pages, per_page, magic;
+    uint32_t table_pages, pages, per_page, magic, alone;
     struct Place {
         uint32_t index, slot;  // of the page in the table, of the chunk in the page
         int32_t entry;
@@ -202,7 +203,7 @@ struct Pages {
     // A chunk's place; the entry's load is not waited for here.
     DAV2_DEV Place find(uint32_t chunk) const {
         Place p;
-        p.index = per_page == 1 ? chunk : __umulhi(chunk, magic);
+        p.index = __umulhi(chunk, magic) + (chunk & alone);
         p.slot = (chunk - p.index * per_page) * 16u;
         p.entry = table[min(p.index, table_pages - 1u)];
         return p;
@@ -217,7 +218,7 @@ struct Pages {
 DAV2_DEV Pages pages_of(const dav2_attention_cache_i8_args& a, uint32_t s) {
     const uint32_t per_page = a.cache.page_size / 16u;
     return {a.page_table + static_cast<uint64_t>(s) * a.table_pages, a.table_pages, a.cache.pages, per_page,
-            static_cast<uint32_t>(((1ull << 32) + per_page - 1u) / per_page)};
+            static_cast<uint32_t>(((1ull << 32) + per_page - 1u) / per_page), per_page == 1 ? ~0u : 0u};
 }
 
 // Eight codes as binary16: the byte c + 128 below the exponent of 1024 is the
@@ -571,8 +572,11 @@ __global__ __launch_bounds__(64 * WAVES, 2) void cache_tiles_kernel(dav2_attenti
         const uint32_t key_chunk = threadIdx.x % (HEAD / 16), key_row = threadIdx.x / (HEAD / 16);
         const uint32_t value_chunk = threadIdx.x & 3u, value_row = threadIdx.x >> 2;
         constexpr uint32_t kKeyStep = kThreads / (HEAD / 16), kValueStep = kThreads / 4;
-        // rows of keys and values that this thread brings (heads of 64 leave half of eight waves without)
-        const bool has_key = 16u * key_chunk < d && key_row < 64u;
+        // heads of 64 leave half of eight waves without a piece
+        const bool brings = HEAD * 4 >= kThreads || wave < HEAD / 16;
+        // features that the head does not have: others in their place, whose
+        // copies in LDS meet no query feature and reach no output
+        const uint32_t key_feature = 16u * key_chunk < d ? 16u * key_chunk : 0u;
         // Called without a condition, and never past the last block: registers
         // that are loaded in one branch only are waited for where the branches
         // meet.
@@ -582,14 +586,15 @@ __global__ __launch_bounds__(64 * WAVES, 2) void cache_tiles_kernel(dav2_attenti
             for (int i = 0; i < kPieces; ++i) of_key[i] = pages.find(block * 4u + min((key_row + kKeyStep * i) / 16u, 3u));
             of_value = pages.find(block * 4u + value_chunk);
         };
-        auto load = [&] {
+        auto load_keys = [&] {
 #pragma unroll
             for (int i = 0; i < kPieces; ++i) {
                 const uint64_t plane = static_cast<uint64_t>(pages.page(of_key[i])) * kv_heads + h;
                 key_codes[i] = *reinterpret_cast<const uint4*>(
-                    a.cache.keys + (plane * page_size + of_key[i].slot + (key_row + kKeyStep * i) % 16u) * d +
-                    (has_key ? 16u * key_chunk : 0u));
+                    a.cache.keys + (plane * page_size + of_key[i].slot + (key_row + kKeyStep * i) % 16u) * d + key_feature);
             }
+        };
+        auto load_values = [&] {
             exists = pages.exists(of_value);
             const uint64_t plane = static_cast<uint64_t>(pages.page(of_value)) * kv_heads + h;
 #pragma unroll
@@ -599,20 +604,7 @@ __global__ __launch_bounds__(64 * WAVES, 2) void cache_tiles_kernel(dav2_attenti
             key_scale = a.cache.key_scales[plane];
             value_scale = a.cache.value_scales[plane];
         };
-        auto store = [&](uint32_t buffer) {
-#pragma unroll
-            for (int i = 0; i < kPieces; ++i) {
-                const uint4 k = key_codes[i], v = value_codes[i];
-                const uint32_t r = key_row + kKeyStep * i, f = value_row + kValueStep * i;
-                if (has_key) {
-                    *reinterpret_cast<h8*>(lds_keys[buffer] + swz<kRow>(r, 2u * key_chunk)) = widen(k.x, k.y);
-                    *reinterpret_cast<h8*>(lds_keys[buffer] + swz<kRow>(r, 2u * key_chunk + 1u)) = widen(k.z, k.w);
-                }
-                if (f < d) {
-                    *reinterpret_cast<h8*>(lds_values[buffer] + swz<128>(f, 2u * value_chunk)) = widen(v.x, v.z);
-                    *reinterpret_cast<h8*>(lds_values[buffer] + swz<128>(f, 2u * value_chunk + 1u)) = widen(v.y, v.w);
-                }
-            }
+        auto store_scales = [&](uint32_t buffer) {
             if (threadIdx.x < 4) {
                 float exponent, fraction, inverse;
                 split_scale(value_scale, exponent, fraction, inverse);
@@ -626,10 +618,44 @@ __global__ __launch_bounds__(64 * WAVES, 2) void cache_tiles_kernel(dav2_attenti
                 lds_scales[buffer][threadIdx.x] = c;
             }
         };
+        // Bringing a tile in small steps that fit between matrix instructions:
+        // the codes loaded before go to LDS, the next ones are loaded, and the
+        // places of those after them are looked up.
+        constexpr int kStages = 4 * kPieces + 3;
+        auto stage = [&](int n, uint32_t buffer, uint32_t block) {
+            if (n < 4 * kPieces) {
+                const int i = n / 4, half = n & 1;
+                if (brings) {
+                    if (n & 2) {
+                        const uint4 v = value_codes[i];
+                        *reinterpret_cast<h8*>(lds_values[buffer] +
+                                               swz<128>(value_row + kValueStep * i, 2u * value_chunk + half)) =
+                            half ? widen(v.y, v.w) : widen(v.x, v.z);
+                    } else {
+                        const uint4 k = key_codes[i];
+                        *reinterpret_cast<h8*>(lds_keys[buffer] + swz<kRow>(key_row + kKeyStep * i, 2u * key_chunk + half)) =
+                            half ? widen(k.z, k.w) : widen(k.x, k.y);
+                    }
+                }
+            } else if (n == 4 * kPieces) {
+                load_keys();
+            } else if (n == 4 * kPieces + 1) {
+                load_values();
+            } else if (n == 4 * kPieces + 2) {
+                find(block);
+            }
+        };
+        auto stage_rest = [&](int n, uint32_t buffer, uint32_t block) {
+#pragma unroll
+            for (int i = 0; i < kStages; ++i)
+                if (i >= n) stage(i, buffer, block);
+        };
         __syncthreads();  // the row tile before has been read
         if (first < last) {
             find(first);
-            load();
+            load_keys();
+            load_values();
+            find(first + 1u);
         }
 
         // the right operand of the scores
@@ -673,54 +699,55 @@ __global__ __launch_bounds__(64 * WAVES, 2) void cache_tiles_kernel(dav2_attenti
         float maximum = kNoScore, sum = 0.0f;  // sum: this lane's keys only
 
         if (first < last) {
-            store(0);
-            find(first + 1u);
-            load();
-            find(first + 2u);
+            store_scales(0);
+            stage_rest(0, 0, first + 2u);
         }
         __syncthreads();
         for (uint32_t block = first; block < last; ++block) {
             const uint32_t buffer = (block - first) & 1u;
-            store(buffer ^ 1u);  // behind the last tile that one again, unread
-            load();
-            find(block + 3u);
             const uint32_t k0 = block * 64u;
-            if (k0 < wave_most) {
+            // behind the last tile that one is brought again, unread
+            store_scales(buffer ^ 1u);
+            if (k0 >= wave_most) {
+                stage_rest(0, buffer ^ 1u, block + 3u);
+            } else {
+                // A matrix instruction leaves the wave some seven others for
+                // free: the order is written out and held.
                 v16f sc[2];
 #pragma unroll
                 for (int b = 0; b < 2; ++b)
 #pragma unroll
                     for (int r = 0; r < 16; ++r) sc[b][r] = 0.0f;
-                // A step's pieces are read before the products of the step
-                // before, which run while the read waits.
                 {
-                    constexpr int S = (KS + 1) / 2;  // of two steps over the features and both blocks
-                    v4i_t in[2][4];
-                    const uint32_t base = lds_address(lds_keys[buffer]);
-                    auto read = [&](int i, v4i_t (&v)[4]) {
-                        const uint32_t at = base + swz<kRow>(col, 4u * i + hf);
-                        if (2 * i + 1 < KS) {
-                            lds_read4<32 * kRow>(at, base + swz<kRow>(col, 4u * i + 2u + hf), v);
-                        } else {
-                            v4i_t w[2];
-                            lds_read2<32 * kRow>(at, w);
-                            v[0] = w[0];
-                            v[1] = w[1];
-                        }
+                    h8 in[2][2];
+                    auto read = [&](int k, h8 (&v)[2]) {
+                        v[0] = *reinterpret_cast<const h8*>(lds_keys[buffer] + swz<kRow>(col, 2u * k + hf));
+                        v[1] = *reinterpret_cast<const h8*>(lds_keys[buffer] + swz<kRow>(col + 32u, 2u * k + hf));
                     };
                     read(0, in[0]);
+                    __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-                    for (int i = 0; i < S; ++i) {
-                        if (i + 1 < S) read(i + 1, in[(i + 1) & 1]);
+                    for (int k = 0; k < KS; ++k) {
+                        if (k + 1 < KS) read(k + 1, in[(k + 1) & 1]);
 #pragma unroll
-                        for (int j = 0; j < 4; ++j)
-                            if (2 * i + j / 2 < KS)
+                        for (int b = 0; b < 2; ++b) {
 #pragma unroll
-                                for (int p = 0; p < NP; ++p)
-                                    sc[j & 1] = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(h8, in[i & 1][j]),
-                                                                                       qf[p][2 * i + j / 2], sc[j & 1], 0, 0, 0);
+                            for (int p = 0; p < NP; ++p)
+                                sc[b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(in[k & 1][b], qf[p][k], sc[b], 0, 0, 0);
+                            stage(2 * k + b, buffer ^ 1u, block + 3u);
+                            __builtin_amdgcn_sched_barrier(0);
+                        }
                     }
+                    stage_rest(2 * KS, buffer ^ 1u, block + 3u);
                 }
+                h8 vf[2][FB];
+                auto read_values = [&](int t, h8 (&v)[FB]) {
+#pragma unroll
+                    for (int f = 0; f < FB; ++f)
+                        v[f] = *reinterpret_cast<const h8*>(lds_values[buffer] + swz<128>(32u * f + col, 2u * t + hf));
+                };
+                read_values(0, vf[0]);
+                __builtin_amdgcn_sched_barrier(0);
                 // chunk t of the tile: registers 8 (t % 2) .. of block t / 2
                 float c[4], shift[4], inverse[4], fraction[4];
                 bool whole = k0 + 64u <= wave_least;
@@ -770,39 +797,37 @@ __global__ __launch_bounds__(64 * WAVES, 2) void cache_tiles_kernel(dav2_attenti
 #pragma unroll
                         for (int r = 0; r < 16; ++r) o[f][r] *= keep;
                 }
-                h8 pf[NP][4];
+                // weights of chunk t + 1 between the products of chunk t
+                h8 pf[2][NP];
+                float part = 0.0f;
+                auto weigh = [&](int t, int r) {
+                    const float w = __builtin_amdgcn_exp2f(fmaf(sc[t >> 1][8 * (t & 1) + r], c[t], shift[t] - maximum));
+                    part = r ? part + w : w;
+                    if constexpr (kFloat) {
+                        const float y = keep_fp32(w * fraction[t]);  // hi and lo of one rounded product
+                        const _Float16 hi = static_cast<_Float16>(y);
+                        pf[t & 1][0][r] = hi;
+                        pf[t & 1][1][r] = static_cast<_Float16>(y - static_cast<float>(hi));
+                    } else {
+                        pf[t & 1][0][r] = static_cast<_Float16>(w);
+                    }
+                    if (r == 7) sum = fmaf(part, inverse[t], sum);
+                };
+#pragma unroll
+                for (int r = 0; r < 8; ++r) weigh(0, r);
 #pragma unroll
                 for (int t = 0; t < 4; ++t) {
-                    float part = 0.0f;
-                    const float less = shift[t] - maximum;
+                    __builtin_amdgcn_sched_barrier(0);
+                    if (t < 3) read_values(t + 1, vf[(t + 1) & 1]);
 #pragma unroll
-                    for (int r = 0; r < 8; ++r) {
-                        const float w = __builtin_amdgcn_exp2f(fmaf(sc[t >> 1][8 * (t & 1) + r], c[t], less));
-                        part += w;
-                        if constexpr (kFloat) {
-                            const float y = keep_fp32(w * fraction[t]);  // hi and lo of one rounded product
-                            const _Float16 hi = static_cast<_Float16>(y);
-                            pf[0][t][r] = hi;
-                            pf[1][t][r] = static_cast<_Float16>(y - static_cast<float>(hi));
-                        } else {
-                            pf[0][t][r] = static_cast<_Float16>(w);
-                        }
-                    }
-                    sum = fmaf(part, inverse[t], sum);
-                }
-                {
-                    v4i_t in[2][FB];  // of rows 32 f + col, whose chunks are at the same places
-                    const uint32_t base = lds_address(lds_values[buffer]);
-                    lds_read_rows<32 * 128>(base + swz<128>(col, hf), in[0]);
+                    for (int f = 0; f < FB; ++f) {
 #pragma unroll
-                    for (int t = 0; t < 4; ++t) {
-                        if (t < 3) lds_read_rows<32 * 128>(base + swz<128>(col, 2u * t + 2u + hf), in[(t + 1) & 1]);
+                        for (int p = 0; p < NP; ++p)
+                            o[f] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf[t & 1][f], pf[t & 1][p], o[f], 0, 0, 0);
+                        if (t < 3)
 #pragma unroll
-                        for (int f = 0; f < FB; ++f)
-#pragma unroll
-                            for (int p = 0; p < NP; ++p)
-                                o[f] = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(h8, in[t & 1][f]), pf[p][t],
-                                                                              o[f], 0, 0, 0);
+                            for (int r = 8 * f / FB; r < 8 * (f + 1) / FB; ++r) weigh(t + 1, r);
+                        __builtin_amdgcn_sched_barrier(0);
                     }
                 }
             }
