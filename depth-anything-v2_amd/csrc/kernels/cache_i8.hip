@@ -862,10 +862,9 @@ __global__ __launch_bounds__(64 * WAVES, 2) void cache_tiles_kernel(dav2_attenti
     }
 }
 
-// The splits of the sequences' rows joined: one workgroup per row.
-template <typename E>
-__global__ __launch_bounds__(256) void cache_join_kernel(dav2_attention_cache_i8_args a, uint32_t splits,
-                                                         bool by_lanes) {
+// The splits of the sequences' rows joined.
+template <typename E, int FEW>
+__global__ __launch_bounds__(256) void cache_join_kernel(dav2_attention_cache_i8_args a, uint32_t splits) {
     const Sequence q = sequence_of(a.starts, a.lengths, blockIdx.y, a.tokens);
     const uint64_t rows = static_cast<uint64_t>(q.end - q.begin) * a.heads;
     const Parts parts = parts_of(a, splits);
@@ -874,12 +873,14 @@ __global__ __launch_bounds__(256) void cache_join_kernel(dav2_attention_cache_i8
     auto head = [&](uint64_t r) { return static_cast<uint64_t>(static_cast<uint32_t>(r) % heads); };
     auto output = [&](uint64_t r) { return static_cast<E*>(a.output) + token(r) * a.output_stride + head(r) * d; };
     auto slot = [&](uint64_t r) { return (token(r) * heads + head(r)) * splits; };
-    if (by_lanes) {
-        for (uint64_t r = blockIdx.x * 8ull + threadIdx.x / 32u; r < rows; r += gridDim.x * 8ull)
-            join_few(parts, slot(r), splits, d, output(r));
-        return;
+    if constexpr (FEW > 0) {
+        const uint32_t lanes = join_lanes_log2(d), each = 256u >> lanes, f4 = threadIdx.x & ((1u << lanes) - 1u);
+        for (uint64_t r = static_cast<uint64_t>(blockIdx.x) * each + (threadIdx.x >> lanes); r < rows;
+             r += static_cast<uint64_t>(gridDim.x) * each)
+            join_few<FEW>(parts, slot(r), splits, d, f4, output(r));
+    } else {
+        for (uint64_t r = blockIdx.x; r < rows; r += gridDim.x) join_row(parts, slot(r), splits, d, output(r));
     }
-    for (uint64_t r = blockIdx.x; r < rows; r += gridDim.x) join_row(parts, slot(r), splits, d, output(r));
 }
 
 bool valid(const dav2_attention_cache_i8_args& a) {
@@ -975,9 +976,13 @@ int dav2_hip_attention_cache_i8(const dav2_attention_cache_i8_args* args, void* 
         });
         if (p.splits > 1) {
             const uint64_t rows = static_cast<uint64_t>(std::min(a.max_query, a.tokens)) * a.heads;
-            const bool by_lanes = join_by_lanes(rows * a.sequences, p.splits);
-            const dim3 join(static_cast<uint32_t>(std::min<uint64_t>(by_lanes ? (rows + 7) / 8 : rows, 4096)), a.sequences);
-            dispatch(cache_join_kernel<E>, join, dim3(256), 0, s, a, p.splits, by_lanes);
+            const int few = join_kind(rows * a.sequences, p.splits);
+            const uint64_t each = few ? join_rows(a.cache.head_dim) : 1;
+            const dim3 join(static_cast<uint32_t>(std::min<uint64_t>((rows + each - 1) / each, 4096)), a.sequences);
+            dispatch(few == 4   ? cache_join_kernel<E, 4>
+                     : few == 8 ? cache_join_kernel<E, 8>
+                                : cache_join_kernel<E, 0>,
+                     join, dim3(256), 0, s, a, p.splits);
         }
         return hipGetLastError();
     });

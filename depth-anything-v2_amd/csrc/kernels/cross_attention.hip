@@ -428,9 +428,8 @@ __global__ __launch_bounds__(256, 2) void cross_tiles_kernel(dav2_cross_attentio
     }
 }
 
-template <typename E>
-__global__ __launch_bounds__(256) void cross_join_kernel(dav2_cross_attention_args a, uint32_t splits,
-                                                         bool by_lanes) {
+template <typename E, int FEW>
+__global__ __launch_bounds__(256) void cross_join_kernel(dav2_cross_attention_args a, uint32_t splits) {
     const uint64_t per_batch = static_cast<uint64_t>(a.query_tokens) * a.heads, rows = a.batch * per_batch;
     const Parts parts = parts_at(a.scratch, rows * splits);
     auto output = [&](uint64_t r) {
@@ -438,12 +437,14 @@ __global__ __launch_bounds__(256) void cross_join_kernel(dav2_cross_attention_ar
         const uint32_t b = row / each, in = row - b * each, token = in / a.heads, head = in - token * a.heads;
         return static_cast<E*>(a.output) + b * a.output_batch_stride + token * a.output_stride + head * a.head_dim;
     };
-    if (by_lanes) {
-        for (uint64_t r = blockIdx.x * 8ull + threadIdx.x / 32u; r < rows; r += gridDim.x * 8ull)
-            join_few(parts, r * splits, splits, a.head_dim, output(r));
-        return;
+    if constexpr (FEW > 0) {
+        const uint32_t lanes = join_lanes_log2(a.head_dim), each = 256u >> lanes, f4 = threadIdx.x & ((1u << lanes) - 1u);
+        for (uint64_t r = static_cast<uint64_t>(blockIdx.x) * each + (threadIdx.x >> lanes); r < rows;
+             r += static_cast<uint64_t>(gridDim.x) * each)
+            join_few<FEW>(parts, r * splits, splits, a.head_dim, f4, output(r));
+    } else {
+        for (uint64_t r = blockIdx.x; r < rows; r += gridDim.x) join_row(parts, r * splits, splits, a.head_dim, output(r));
     }
-    for (uint64_t r = blockIdx.x; r < rows; r += gridDim.x) join_row(parts, r * splits, splits, a.head_dim, output(r));
 }
 
 struct Plan {
@@ -509,10 +510,13 @@ int dav2_hip_cross_attention(const dav2_cross_attention_args* args, void* stream
         });
         if (p.splits > 1) {
             const uint64_t rows = static_cast<uint64_t>(a.batch) * a.query_tokens * a.heads;
-            const bool by_lanes = join_by_lanes(rows, p.splits);
-            const uint64_t all = by_lanes ? (rows + 7) / 8 : rows;
-            dispatch(cross_join_kernel<E>, dim3(static_cast<uint32_t>(std::min<uint64_t>(all, 65536))), dim3(256), 0, s, a,
-                     p.splits, by_lanes);
+            const int few = join_kind(rows, p.splits);
+            const uint64_t each = few ? join_rows(a.head_dim) : 1;
+            const dim3 join(static_cast<uint32_t>(std::min<uint64_t>((rows + each - 1) / each, 65536)));
+            dispatch(few == 4   ? cross_join_kernel<E, 4>
+                     : few == 8 ? cross_join_kernel<E, 8>
+                                : cross_join_kernel<E, 0>,
+                     join, dim3(256), 0, s, a, p.splits);
         }
         return hipGetLastError();
     });

@@ -234,39 +234,52 @@ inline uint64_t parts_bytes(uint64_t count, uint32_t head_dim) {
     return ((count + 1u) & ~uint64_t(1)) * sizeof(float2) + count * head_dim * sizeof(float);
 }
 
-// Which of the two joins below: 32 lanes per row where there are rows enough
-// to fill the chip (18464 rows of three splits: 70 us less than a workgroup
-// per row), a workgroup per row else (64 rows of eight splits: 3 us less).
-inline bool join_by_lanes(uint64_t rows, uint32_t splits) { return splits <= 8 && rows > 2048; }
+// Which of the two joins below: lanes, up to FEW = 4 or 8 splits of a row, where
+// there are rows enough to fill the chip, a workgroup per row (FEW = 0) else
+// (64 rows of eight splits: 3 us less).
+inline int join_kind(uint64_t rows, uint32_t splits) { return rows <= 2048 || splits > 8 ? 0 : splits <= 4 ? 4 : 8; }
 
-// Up to 8 splits of a row joined by 32 lanes, the four features 4 f .. each,
-// all loads at once. A split that saw nothing has a sum of 0 and drops out.
-template <typename E>
-DAV2_DEV void join_few(const Parts& parts, uint64_t slot, uint32_t splits, uint32_t d, E* y) {
-    const uint32_t f4 = threadIdx.x & 31u;
-    float2 stats[8];
-    v4f sums[8];
+// The lanes that have a row, as a power of two: of 4 features each.
+DAV2_DEV uint32_t join_lanes_log2(uint32_t d) { return 32u - __clz(d / 4u - 1u); }
+inline uint32_t join_rows(uint32_t d) {  // of a workgroup of 256
+    uint32_t lanes = 4;
+    while (4 * lanes < d) lanes *= 2;
+    return 256 / lanes;
+}
+
+// Up to FEW splits of a row joined by its lanes, the features 4 f4 .. each, all
+// loads at once and none under a condition (18464 rows of three splits of 64
+// features %JOIN%). A split that saw nothing has a sum of 0 and drops out.
+template <int FEW, typename E>
+DAV2_DEV void join_few(const Parts& parts, uint64_t slot, uint32_t splits, uint32_t d, uint32_t f4, E* y) {
+    typedef E V4 __attribute__((ext_vector_type(4)));
+    const uint32_t f = min(4u * f4, d - 4u);
+    float2 stats[FEW];
+    v4f sums[FEW];
+#pragma unroll
+    for (uint32_t i = 0; i < FEW; ++i) {
+        const uint64_t at = slot + min(i, splits - 1u);
+        stats[i] = parts.stats[at];
+        sums[i] = *reinterpret_cast<const v4f*>(parts.sums + at * d + f);
+    }
     float top = kNoScore;
 #pragma unroll
-    for (uint32_t i = 0; i < 8; ++i) {
-        stats[i] = i < splits ? parts.stats[slot + i] : make_float2(kNoScore, 0.0f);
-        sums[i] = v4f{0.f, 0.f, 0.f, 0.f};
-        if (i < splits && 4 * f4 < d) sums[i] = *reinterpret_cast<const v4f*>(parts.sums + (slot + i) * d + 4 * f4);
-        top = fmaxf(top, stats[i].x);
-    }
+    for (uint32_t i = 0; i < FEW; ++i) top = fmaxf(top, stats[i].x);
     v4f sum = {0.f, 0.f, 0.f, 0.f};
     float total = 0.0f;
 #pragma unroll
-    for (uint32_t i = 0; i < 8; ++i) {
+    for (uint32_t i = 0; i < FEW; ++i) {
         if (i >= splits) break;
         const float weight = __builtin_amdgcn_exp2f(stats[i].x - top);
         total = fmaf(stats[i].y, weight, total);
         sum += sums[i] * weight;
     }
-    if (4 * f4 >= d) return;
+    if (4u * f4 >= d) return;
     const float scale = total == 0.0f ? 0.0f : 1.0f / total;
+    V4 out;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) y[4 * f4 + i] = static_cast<E>(sum[i] * scale);
+    for (int i = 0; i < 4; ++i) out[i] = static_cast<E>(sum[i] * scale);
+    *reinterpret_cast<V4*>(y + f) = out;
 }
 
 // More splits of a row, parts slot .. slot + splits - 1, joined by a workgroup
