@@ -40,7 +40,7 @@ DAV2_DEV uint32_t byte_of(uint32_t word, uint32_t i, int code) {
 // a thread needs 16 tokens of one 4-byte piece of features. Codes are written
 // 16 at a time; a value chunk that also holds older or later tokens is read,
 // changed and written back. Bound by memory: 8 prompts of up to 2048 tokens, 8
-// heads of 128, f16 %PROMPTS%.
+// heads of 128, f16 (55 MB): 32 us, 1.7 TB/s.
 template <typename E, bool ALIGNED>
 __global__ __launch_bounds__(256, 8) void cache_store_kernel(dav2_cache_store_i8_args a) {
     constexpr int kKept = 1;
@@ -343,7 +343,7 @@ __global__ __launch_bounds__(256, 2) void cache_rows_kernel(dav2_attention_cache
             find(block);
             load_keys();
             load_values();
-            if (block + 4u < last) find(block + 4u);
+            find(min(block + 4u, last - 1u));
         }
 
         // the right operand of the scores
@@ -385,8 +385,11 @@ __global__ __launch_bounds__(256, 2) void cache_rows_kernel(dav2_attention_cache
                 }
         }
 
-        for (; block < last; block += 4u) {
-            const bool more = block + 4u < last;
+        // A wave's last block is apart: registers that are loaded in one branch
+        // only are waited for where the branches meet (64 sequences of up to
+        // 2048 keys, 16 heads of 64: 44 us with the branch, 38 without).
+        auto step = [&](auto more) {
+            constexpr bool kMore = decltype(more)::value;
             v4f sc[4];
 #pragma unroll
             for (int t = 0; t < 4; ++t) {
@@ -401,7 +404,7 @@ __global__ __launch_bounds__(256, 2) void cache_rows_kernel(dav2_attention_cache
                     }
                 }
             }
-            if (more) load_keys();
+            if constexpr (kMore) load_keys();
             float exponent, fraction, inverse;
             const uint32_t key0 = block * 64u + 16u * g;  // of this lane's first score
             // a chunk that the row does not see may have any scale, NaN included
@@ -451,11 +454,13 @@ __global__ __launch_bounds__(256, 2) void cache_rows_kernel(dav2_attention_cache
                     o[f] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v1, pf[p][1], o[f], 0, 0, 0);
                 }
             }
-            if (more) {
+            if constexpr (kMore) {
                 load_values();
-                if (block + 8u < last) find(block + 8u);
+                find(min(block + 8u, last - 1u));
             }
-        }
+        };
+        for (; block + 4u < last; block += 4u) step(std::true_type());
+        if (block < last) step(std::false_type());
         sum = over_groups(sum, Plus());
 
         // join the four waves: lane (col, g), register r of o[f]: feature 16 f + 4 g + r of row col
@@ -503,11 +508,16 @@ __global__ __launch_bounds__(256, 2) void cache_rows_kernel(dav2_attention_cache
 }
 
 // Many query rows for a cache head (prompts): bound by the matrix cores, the
-// exponentials and LDS. A workgroup has 128 rows of one sequence and cache head,
-// 32 for each of four waves, and goes through the keys 64 at a time: codes are
-// widened to binary16 once for all waves on their way into LDS (two buffers,
-// one barrier for a tile; the next tile's codes are in registers meanwhile, its
-// places in the table a tile before).
+// vector units and LDS, each busy for some 40 % of the time. A workgroup has
+// 128 or 256 rows of one sequence and cache head, 32 for each of its waves, and
+// goes through the keys 64 at a time: codes are widened to binary16 once for
+// all waves on their way into LDS (two buffers, one barrier for a tile; the
+// next tile's codes are in registers meanwhile, its places in the table a tile
+// before). Two prompts' last 2048 of up to 8192 tokens, 32 heads of 8, 128
+// features, f16: 441 us, 717 TFLOP/s; 8 times 512 of 4096 770 TFLOP/s; every
+// row all keys 820. A tile shared by eight waves instead of four is worth 10 %
+// there, the staging and the exponentials written between the matrix
+// instructions 8 %.
 //
 // S^T = K Q^T and O^T = V^T P^T on v_mfma_f32_32x32x16_f16. Lane l holds, for
 // query l % 32, the scores of keys 8 (r / 4) + 4 (l / 32) + r % 4 of a 32-key
@@ -517,13 +527,14 @@ __global__ __launch_bounds__(256, 2) void cache_rows_kernel(dav2_attention_cache
 // registers are one 16-token chunk, so scales are uniform for them.
 template <typename E, int D, int WAVES>
 __global__ __launch_bounds__(64 * WAVES, 2) void cache_tiles_kernel(dav2_attention_cache_i8_args a, uint32_t splits,
-                                                             uint32_t tiles) {
+                                                                    uint32_t tiles) {
     constexpr bool kFloat = std::is_same_v<E, float>;
     constexpr int HEAD = D <= 64 ? 64 : 128;  // features of a row in LDS
     constexpr int KS = D / 16, FB = (D + 31) / 32, NP = kFloat ? 2 : 1;
     constexpr uint32_t d = D;
     constexpr uint32_t kThreads = 64 * WAVES, kTileRows = 32 * WAVES;
-    constexpr int kPieces = HEAD * 4 > kThreads ? HEAD * 4 / kThreads : 1;  // of 16 codes, for each thread and tile: keys, and values
+    // of 16 codes, for each thread and tile: keys, and values
+    constexpr int kPieces = HEAD * 4 > kThreads ? HEAD * 4 / kThreads : 1;
     constexpr int kRow = HEAD * 2;       // bytes of a key row in LDS
     // rescale when a score passes the running maximum by this: weights stay
     // below 2^6, far inside binary16, and most tiles leave the sums alone
@@ -894,14 +905,33 @@ bool valid(const dav2_attention_cache_i8_args& a) {
            (a.tokens == 1 || (a.query_stride >= row && a.output_stride >= row));
 }
 
-// How a call is dealt out: row tiles, and splits of the keys. Two workgroups
-// share a CU, so up to 512 all run at once: split as far as that goes, down to
-// 128 keys (two waves' blocks) each. Beyond it a further split only evens out
-// sequences of different lengths and pays for long ones: up to 2048 workgroups
-// of at least 2048 keys. Heads 32 of 8, 128 features, us: 40 sequences of 300
-// keys 13.2 whole, 19.6 in two (640 workgroups); 8 of 4096 19.5 in 8 (512
-// workgroups), 24.0 in 16; 32 of up to 32768 257 in 2 (512), 244 in 4, 242 in
-// 8; one token over 1370 keys, 16 heads of 64, 11.9 in 2, 10.4 in 5, 9.2 in 10.
+// How a call is dealt out. cache_rows_kernel for up to 32 rows of a cache head,
+// or little work: the tiles of cache_tiles_kernel have four times its latency,
+// but do the same work in less than two thirds of the time where they fill the
+// chip. us, rows against tiles (32 or 16 heads): 32 rows, 8 sequences of 2048
+// keys 26 / 29; 64 rows, 8 of 4096 (2^26) 23 / 27; 128 rows, 2 of 8192 (2^26)
+// 19 / 25; 72 rows, 32 of 1500 (2^27) 36 / 31; 100 rows, 8 of 4096 (2^28) 52 / 39.
+//
+// cache_rows_kernel: two workgroups share a CU, so up to 512 all run at once:
+// split the keys as far as that goes, down to 128 keys (two waves' blocks) each.
+// Beyond it a further split only evens out sequences of different lengths and
+// pays for long ones: up to 2048 workgroups of at least 2048 keys. Heads 32 of
+// 8, 128 features, us: 40 sequences of 300 keys 13.2 whole, 19.6 in two (640
+// workgroups); 8 of 4096 19.5 in 8 (512 workgroups), 24.0 in 16; 32 of up to
+// 32768 257 in 2 (512), 244 in 4, 242 in 8; one token over 1370 keys, 16 heads
+// of 64, 11.9 in 2, 10.4 in 5, 9.2 in 10.
+//
+// cache_tiles_kernel: splitting n keys s times costs n / s tiles one after the
+// other and s parts to join, so s grows with sqrt(n), as sqrt(n / 32) (128 rows
+// of 8 heads, 32768 keys, us: 46; sqrt(n / 64) 56, sqrt(n / 16) 53), and to
+// one workgroup of 256 rows or two of 128 a CU. Tiles of 256 rows read and
+// widen the keys once for twice the rows (441 us against 493 above, 36 against
+// 40 for 8 times 64 tokens), if the head is wide enough that three waves of the
+// smaller ones do not fit a SIMD instead (heads of 64, 16 times 1500 tokens:
+// 166 against 151), if they add no rows that do not exist (2 times 577 tokens
+// 60 against 45), and if there are enough of them: one for each CU, and two
+// where a causal mask makes them unequal (4 prompts of 1024 tokens, 16 heads:
+// 43 against 38).
 struct Plan {
     uint32_t tile;  // rows: 16 of cache_rows_kernel, 128 or 256 of cache_tiles_kernel
     uint32_t tiles, splits;
@@ -910,11 +940,23 @@ Plan plan_of(const dav2_attention_cache_i8_args& a) {
     Plan p{16, 1, 1};
     if (a.cache.kv_heads == 0 || a.heads < a.cache.kv_heads || a.sequences == 0 || a.max_query == 0) return p;
     const uint64_t rows = static_cast<uint64_t>(std::min(a.max_query, a.tokens)) * (a.heads / a.cache.kv_heads);
-    p.tile = rows > 32 ? (rows >= 1024 ? 256 : 128) : 16;
-    p.tiles = static_cast<uint32_t>(std::min<uint64_t>((rows + p.tile - 1) / p.tile, p.tile > 16 ? 512 : 4096));
-    const uint64_t have = std::max<uint64_t>(1, static_cast<uint64_t>(p.tiles) * a.cache.kv_heads * a.sequences);
-    const uint64_t resident = std::min<uint64_t>((p.tile == 256 ? 256 : 512) / have, a.max_length / 128);
-    const uint64_t even = p.tile > 16 ? 1 : std::min<uint64_t>(2048 / have, a.max_length / 2048);
+    const uint64_t planes = static_cast<uint64_t>(a.cache.kv_heads) * a.sequences;
+    const double work = static_cast<double>((rows + 15) / 16 * planes) * a.max_length * a.cache.head_dim;
+    if (rows > 32 && work > 67108864.0) {
+        uint64_t most = 1;  // splits
+        while (most < kMostSplits && (most + 1) * (most + 1) * 32 <= a.max_length) ++most;
+        const uint64_t wide = (rows + 255) / 256 * planes;
+        const bool unequal = a.causal && a.max_query > a.max_length / 2 && wide < 512;
+        p.tile = a.cache.head_dim > 64 && (rows + 127) / 128 % 2 == 0 && wide * most >= 256 && !unequal ? 256 : 128;
+        p.tiles = static_cast<uint32_t>(std::min<uint64_t>((rows + p.tile - 1) / p.tile, 512));
+        p.splits = static_cast<uint32_t>(
+            std::clamp<uint64_t>((p.tile == 256 ? 256 : 512) / std::max<uint64_t>(1, p.tiles * planes), 1, most));
+        return p;
+    }
+    p.tiles = static_cast<uint32_t>(std::min<uint64_t>((rows + 15) / 16, 4096));
+    const uint64_t have = std::max<uint64_t>(1, p.tiles * planes);
+    const uint64_t resident = std::min<uint64_t>(512 / have, a.max_length / 128);
+    const uint64_t even = std::min<uint64_t>(2048 / have, a.max_length / 2048);
     p.splits = static_cast<uint32_t>(std::clamp<uint64_t>(std::max(resident, even), 1, kMostSplits));
     return p;
 }

@@ -385,11 +385,13 @@ struct Tiles {
 // Bound by the matrix cores and, as long again in 16 bits, the exponentials of
 // the vector units beside them: 8 x 2048 queries of 32 heads of 128 on 4096
 // keys of 8, bf16, 1.16 ms, 950 TFLOP/s, where a large library product runs at
-// 1190; heads of 64 750. fp32: 72 TFLOP/s of 152 at 2 x 577 queries, 16 heads of
-// 64, 1370 keys and fewer, where 160 workgroups are split in three. Tried and
+// 1190; heads of 64 750. fp32: 129 TFLOP/s of 152 at 8 x 1024 queries, 16 heads
+// of 64, 4096 keys; 82 at 2 x 577 queries and 1370 keys, where 160 workgroups
+// are split in three. Tried and
 // not kept: eight waves in two groups that multiply and weigh in turns
 // (barriers between; 952 TFLOP/s, no difference), a tile's scores one tile
-// ahead among the exponentials (spills), tiles through registers (575 -> 610 us
+// ahead among the exponentials (spills), a step's exponentials between the
+// products of the step before (556 -> 563 us at the masked case), tiles through registers (575 -> 610 us
 // at the masked case above).
 template <typename E, int D, bool LISTED>
 __global__ __launch_bounds__(256, 2) void cross_tiles_kernel(dav2_cross_attention_args a, Lists lists, uint32_t splits,
@@ -447,6 +449,12 @@ __global__ __launch_bounds__(256) void cross_join_kernel(dav2_cross_attention_ar
     }
 }
 
+// How a call is dealt out: 128 rows a workgroup, and the keys split while all
+// workgroups run at once, two on a CU, down to two tiles each (fp32: 128 queries,
+// 12 heads of 64, 1024 keys, 20.0 us in 16, 21.9 in 8). us: 64 workgroups of one
+// query each and 1370 keys, f16, 11.9 in 4, 10.1 in 8, 10.7 in 10; 160 of 577
+// queries, 25.6 whole, 22.5 in 3, fp32 102 whole, 110 in 2, 75 in 3; 80 of 300
+// queries, 32 heads of 8 of 128, 4096 keys, bf16, 40.8 in 3, 39.5 in 6.
 struct Plan {
     uint32_t tiles, splits;
 };
@@ -457,7 +465,7 @@ Plan plan_of(const dav2_cross_attention_args& a) {
     p.tiles = static_cast<uint32_t>(std::min<uint64_t>((rows + 127) / 128, 512));
     const uint64_t have = static_cast<uint64_t>(p.tiles) * a.kv_heads * a.batch;
     p.splits = static_cast<uint32_t>(
-        std::clamp<uint64_t>(std::min<uint64_t>(512 / have, a.key_tokens / 128), 1, kMostSplits));
+        std::clamp<uint64_t>(std::min<uint64_t>(512 / have, a.key_tokens / (a.dtype == DAV2_DTYPE_F32 ? 64 : 128)), 1, kMostSplits));
     return p;
 }
 uint64_t split_bytes(const dav2_cross_attention_args& a, const Plan& p) {

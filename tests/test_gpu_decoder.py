@@ -577,7 +577,6 @@ def ops_cache(pkg, cache):
     return pkg.OpsCacheInt8(*[db(pkg, t) for t in cache])
 
 
-NONE = None
 
 
 class Step:
