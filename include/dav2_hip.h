@@ -540,7 +540,7 @@ DAV2_API int dav2_hip_qk_norm_rotary(const dav2_qk_norm_rotary_args* args, void*
  * scale per head for its keys and one for its values; a code c stands for
  * c * scale. Values are held feature-major, so that the keys of one feature
  * are contiguous. page_size a multiple of 16 up to 256, head_dim a multiple
- * of 16 up to 128; keys and values 16-byte aligned. Sequence s owns the pages
+ * of 16 up to 128, kv_heads up to 32767; keys and values 16-byte aligned. Sequence s owns the pages
  * page_table[s][0], [1], ...: token t is slot t % page_size of page
  * page_table[s][t / page_size]. A table entry outside [0, pages) is no page:
  * nothing is stored there and its tokens are not seen. Pages need no
@@ -564,7 +564,7 @@ typedef struct dav2_cache_i8 {
  * page's values, until the page is begun anew. starts must not decrease; rows
  * outside [0, tokens) and positions outside the table are not stored. Pages
  * that get tokens must belong to one sequence only. Other bytes of the cache
- * are left as they were. */
+ * are left as they were. sequences stays below 2^16. */
 typedef struct dav2_cache_store_i8_args {
     dav2_cache_i8 cache;
     const void* keys;            /* [tokens][kv_heads][head_dim]                   */
@@ -584,13 +584,15 @@ DAV2_API int dav2_hip_cache_store_i8(const dav2_cache_store_i8_args* args, void*
  * i of n sees the first lengths[s] - n + 1 + i tokens; otherwise all. heads is
  * a multiple of kv_heads; head h reads head h / (heads / kv_heads) of the
  * cache. A row that sees nothing gives zeros; output rows of no sequence are
- * left as they were. tokens * heads stays below 2^32 - 512, sequences *
- * kv_heads below 2^23. Strides (elements
- * between tokens) are multiples of 8, query and output 16-byte aligned. max_query and max_length, the most new
- * and the most tokens of a sequence, size the launch and the scratch; a
- * sequence beyond them is still computed. scratch: dav2_hip_attention_cache_i8_
- * scratch_bytes() bytes (0: none), 16-byte aligned, in use until the call's
- * work is done. That number depends on the sizes, never on the pointers. */
+ * left as they were. Scales of pages are not negative. tokens * heads stays
+ * below 2^32 - 512, sequences * kv_heads below 2^23, sequences below 2^16.
+ * Strides (elements between tokens) are multiples of 8, query and output
+ * 16-byte aligned; output overlaps no input. max_query and max_length, the
+ * most new and the most tokens of a sequence, size the launch and the scratch;
+ * a sequence beyond them is still computed. scratch:
+ * dav2_hip_attention_cache_i8_scratch_bytes() bytes (0: none), 16-byte
+ * aligned, in use until the call's work is done. That number depends on the
+ * sizes, never on the pointers. */
 typedef struct dav2_attention_cache_i8_args {
     dav2_cache_i8 cache;
     const void* query;           /* [tokens][heads][head_dim]                      */
@@ -615,7 +617,9 @@ DAV2_API int dav2_hip_attention_cache_i8(const dav2_attention_cache_i8_args* arg
  * what is not seen may hold anything, NaN included. A batch that sees nothing
  * gives zeros. heads is a multiple of kv_heads; head h reads key head
  * h / (heads / kv_heads). head_dim a multiple of 16 up to 128; strides in
- * elements, multiples of 8; the four tensors 16-byte aligned. scratch as for
+ * elements, multiples of 8; the four tensors 16-byte aligned; output overlaps
+ * no input. batch stays below 2^16, batch * query_tokens * heads below
+ * 2^32 - 256, batch * kv_heads below 2^23. scratch as for
  * dav2_hip_attention_cache_i8. */
 typedef struct dav2_cross_attention_args {
     const void* query;           /* [batch][query_tokens][heads][head_dim]         */

@@ -218,6 +218,19 @@ def test_cache_store(gpu, pkg, lib, dtype, page_size, heads, head_dim):
     check_store(torch, pkg, lib, cache, k, v, table, starts, ints(torch, total), max(new), dtype)
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("offset,more", [(1, 0), (0, 1), (3, 5)])
+def test_cache_store_alignment(gpu, pkg, lib, dtype, offset, more):
+    torch = gpu
+    tokens, heads, d, page_size = 45, 3, 48, 32
+    stride = heads * d + more
+    k, v = (rand(torch, i, offset + tokens * stride, dtype=dtype).as_strided((tokens, heads, d), (stride, d, 1), offset)
+            for i in (1, 2))
+    cache = random_cache(torch, 3, 8, heads, page_size, d)
+    table = shuffled_table(torch, 4, 2, 4, 8)
+    check_store(torch, pkg, lib, cache, k, v, table, ints(torch, [0, 5, 45]), ints(torch, [37, 100]), 40, dtype)
+
+
 def test_cache_store_one_by_one(gpu, pkg, lib):
     # growing values: every token of a page makes its scale larger and its older codes smaller
     torch = gpu
@@ -279,16 +292,20 @@ def attend_args(torch, pkg, lib, cache, q, out, table, starts, lengths, causal, 
     return a, scratch
 
 
+LONG = 2 ** 22  # as max_length: many rows take the way of a long cache, whatever the lengths are
+
+
 def check_attend(torch, pkg, lib, cache, q, table, starts, lengths, causal, dtype, scale=None, **hints):
     scale = scale or 1 / math.sqrt(q.shape[2])
-    out = torch.full(q.shape, 3.0, dtype=q.dtype, device="cuda")
-    a, keep = attend_args(torch, pkg, lib, cache, q, out, table, starts, lengths, causal, dtype, scale, **hints)
-    launch(torch, lib, "dav2_hip_attention_cache_i8", a)
     want, bound = ref.attend(q, cache, table, starts, lengths, causal, scale, dtype)
-    torch.cuda.synchronize()
     nobody = want.isnan()
-    assert (out[nobody] == 3.0).all()  # rows of no sequence are left alone
-    ref.assert_within(torch.where(nobody, want, out.double()), want, bound)
+    for hint in (hints, dict(max_length=LONG)) if "max_length" not in hints else (hints,):
+        out = torch.full(q.shape, 3.0, dtype=q.dtype, device="cuda")
+        a, keep = attend_args(torch, pkg, lib, cache, q, out, table, starts, lengths, causal, dtype, scale, **hint)
+        launch(torch, lib, "dav2_hip_attention_cache_i8", a)
+        torch.cuda.synchronize()
+        assert (out[nobody] == 3.0).all()  # rows of no sequence are left alone
+        ref.assert_within(torch.where(nobody, want, out.double()), want, bound, str(hint))
     return out
 
 
@@ -333,6 +350,102 @@ def test_cache_attention_long(gpu, pkg, lib):
     for dtype in DTYPES:
         q = rand(torch, 8, 3, 8, 128, dtype=dtype)
         check_attend(torch, pkg, lib, cache, q, table, ints(torch, [0, 1, 2, 3]), ints(torch, lengths), True, dtype)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("sequences,queries,heads,kv,head_dim,page_size", [(64, 20, 16, 8, 64, 16), (8, 256, 32, 32, 80, 32),
+                                                                           (8, 250, 32, 32, 128, 16)])
+def test_cache_attention_whole(gpu, pkg, lib, dtype, sequences, queries, heads, kv, head_dim, page_size):
+    # tiles enough to fill the chip: the keys are not split
+    torch = gpu
+    total = [queries - 1 + 37 * (i % 5) for i in range(sequences)]
+    most = -(-max(total) // page_size)
+    cache = random_cache(torch, 5 + heads, 200, kv, page_size, head_dim)
+    table = torch.randint(0, 200, (sequences, most), dtype=torch.int32, device="cuda")  # pages that several have
+    q = rand(torch, 6, sequences * queries, heads, head_dim, dtype=dtype)
+    starts = ints(torch, [queries * i for i in range(sequences + 1)])
+    check_attend(torch, pkg, lib, cache, q, table, starts, ints(torch, total), True, dtype)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_cache_attention_more_tiles_than_said(gpu, pkg, lib, dtype):
+    # max_query 1 with 40 heads of one cache head: a workgroup goes through all tiles of rows
+    torch = gpu
+    cache = random_cache(torch, 5, 40, 1, 16, 128)
+    table = shuffled_table(torch, 6, 2, 20, 40)
+    q = rand(torch, 6, 71, 40, 128, dtype=dtype)
+    check_attend(torch, pkg, lib, cache, q, table, ints(torch, [0, 40, 71]), ints(torch, [300, 31]), True, dtype,
+                 max_query=1, max_length=LONG)
+
+
+@pytest.mark.parametrize("queries", [1, 40])
+def test_far_pages(gpu, pkg, lib, queries):
+    # pages past 2^32 bytes of a cache: stored and read as in a small one
+    torch = gpu
+    heads, page_size, d, count = 2, 256, 128, 3
+    pages = 2 ** 32 // (heads * page_size * d) + 4
+    near = random_cache(torch, 1, count, heads, page_size, d)
+    far = [torch.empty((pages, *t.shape[1:]), dtype=t.dtype, device="cuda") for t in near]
+    for a, b in zip(near, far):
+        b[-count:].copy_(a)
+    order = ints(torch, [[2, 0, 1]])
+    k, v = rand(torch, 2, queries, heads, d), rand(torch, 3, queries, heads, d)
+    q = rand(torch, 4, queries, 2 * heads, d)
+    starts, lengths = ints(torch, [0, queries]), ints(torch, [530])
+    outs = []
+    for cache, table in ((near, order), (far, order + pages - count)):
+        launch(torch, lib, "dav2_hip_cache_store_i8", store_args(pkg, cache, k, v, table, starts, lengths, queries, "f32"))
+        for hint in (None, LONG):
+            out = torch.full_like(q, math.nan)
+            a, keep = attend_args(torch, pkg, lib, cache, q, out, table, starts, lengths, True, "f32", 0.1, max_length=hint)
+            launch(torch, lib, "dav2_hip_attention_cache_i8", a)
+            outs.append(out)
+            torch.cuda.synchronize()
+    for a, b in zip(near, far):
+        assert torch.equal(a, b[-count:])
+    assert torch.equal(outs[0], outs[2]) and torch.equal(outs[1], outs[3]) and outs[0].isfinite().all()
+
+
+@pytest.mark.parametrize("dtype", ["f16", "f32"])
+def test_far_strides(gpu, pkg, lib, dtype):
+    # rows and batches past 2^32 bytes of their tensor
+    torch = gpu
+    apart, d, heads = 2 ** 31 + 64, 64, 2
+    store = torch.empty(apart + 512 * heads * d, dtype=ref.DTYPES[dtype], device="cuda")
+
+    def far(x, stride):  # x with its first axis apart
+        y = store.as_strided(x.shape, (apart, *stride[1:]), 0)
+        y.copy_(x)
+        return y
+
+    q, k, v = (rand(torch, i, 2, n, heads, d, dtype=dtype) for i, n in ((1, 5), (2, 200), (3, 200)))
+    mask = torch.ones((2, 200), dtype=torch.uint8, device="cuda")
+    mask[:, ::3] = 0
+    outs = []
+    for tensors in ((q, k, v), (far(q, q.stride()), k, v), (q, far(k, k.stride()), v), (q, k, far(v, v.stride()))):
+        for m in (None, mask):
+            out = torch.full_like(q, math.nan)
+            # the buffer holds one of them at a time: written here, read before the next is written
+            if tensors[0] is not q:
+                tensors[0].copy_(q)
+            if tensors[1] is not k:
+                tensors[1].copy_(k)
+            if tensors[2] is not v:
+                tensors[2].copy_(v)
+            a, keep = cross_args(torch, pkg, lib, *tensors, out, None, m, dtype, 0.125)
+            launch(torch, lib, "dav2_hip_cross_attention", a)
+            torch.cuda.synchronize()
+            outs.append(out)
+    for i in range(2, len(outs)):
+        assert torch.equal(outs[i], outs[i % 2])
+    assert outs[0].isfinite().all()
+    x = rand(torch, 5, 2, heads, d, dtype=dtype)
+    positions, freq = ints(torch, [3, 70000]), ref.frequencies(d)
+    y, z = torch.empty_like(x), far(x, x.stride())
+    launch(torch, lib, "dav2_hip_rotary", rotary_args(pkg, x, y, positions, freq, d, "halves", dtype))
+    launch(torch, lib, "dav2_hip_rotary", rotary_args(pkg, z, z, positions, freq, d, "halves", dtype))
+    torch.cuda.synchronize()
+    assert torch.equal(y, z)
 
 
 @pytest.mark.parametrize("queries", [1, 40])
@@ -388,7 +501,8 @@ def test_cache_attention_range_of_queries(gpu, pkg, lib, queries):
 
 @pytest.mark.parametrize("queries", [1, 40])
 @pytest.mark.parametrize("dtype", DTYPES)
-def test_cache_attention_not_finite(gpu, pkg, lib, queries, dtype):
+@pytest.mark.parametrize("most", [None, LONG])
+def test_cache_attention_not_finite(gpu, pkg, lib, queries, dtype, most):
     # NaN and infinity in a query, NaN pages behind the last token and in pages of nobody stay where they are
     torch = gpu
     cache = random_cache(torch, 3, 8, 2, 32, 64)
@@ -400,7 +514,7 @@ def test_cache_attention_not_finite(gpu, pkg, lib, queries, dtype):
     q[0, 1, 3] = math.nan
     q[0, 2, 7] = math.inf
     out = torch.zeros_like(q)
-    a, keep = attend_args(torch, pkg, lib, cache, q, out, table, starts, lengths, True, dtype, 0.125)
+    a, keep = attend_args(torch, pkg, lib, cache, q, out, table, starts, lengths, True, dtype, 0.125, max_length=most)
     launch(torch, lib, "dav2_hip_attention_cache_i8", a)
     torch.cuda.synchronize()
     assert out[0, 1].isnan().all() and out[0, 2].isnan().any()
@@ -409,7 +523,7 @@ def test_cache_attention_not_finite(gpu, pkg, lib, queries, dtype):
     out.zero_()
     q = rand(torch, 8, 2 * queries, 4, 64, dtype=dtype)
     a, keep = attend_args(torch, pkg, lib, cache, q, out, table, starts, ints(torch, [65 + queries, 64]), False, dtype,
-                          0.125)
+                          0.125, max_length=most)
     launch(torch, lib, "dav2_hip_attention_cache_i8", a)
     torch.cuda.synchronize()
     assert out[:queries].isnan().all() and out[queries:].isfinite().all()
@@ -417,7 +531,8 @@ def test_cache_attention_not_finite(gpu, pkg, lib, queries, dtype):
 
 @pytest.mark.parametrize("queries", [3, 60])
 @pytest.mark.parametrize("dtype", DTYPES)
-def test_cache_attention_not_finite_ahead(gpu, pkg, lib, queries, dtype):
+@pytest.mark.parametrize("most", [None, LONG])
+def test_cache_attention_not_finite_ahead(gpu, pkg, lib, queries, dtype, most):
     # a page that only the later rows of a tile see is not finite: the earlier rows are untouched
     torch = gpu
     cache = random_cache(torch, 3, 8, 2, 16, 64)
@@ -428,7 +543,7 @@ def test_cache_attention_not_finite_ahead(gpu, pkg, lib, queries, dtype):
     out = torch.zeros_like(q)
     total = last + 2  # the last two rows see into it
     starts, lengths = ints(torch, [0, queries]), ints(torch, [total])
-    a, keep = attend_args(torch, pkg, lib, cache, q, out, table, starts, lengths, True, dtype, 0.125)
+    a, keep = attend_args(torch, pkg, lib, cache, q, out, table, starts, lengths, True, dtype, 0.125, max_length=most)
     launch(torch, lib, "dav2_hip_attention_cache_i8", a)
     torch.cuda.synchronize()
     assert out[-2:].isnan().all() and out[:-2].isfinite().all()
@@ -681,6 +796,26 @@ def test_decoder_step(gpu, pkg, lib, ops, dtype, sequences, queries, older):
     other.by_surface(lib, ops)
     for a, b in zip(by_launchers, other.outputs()):
         assert torch.equal(a, b)  # the same kernels
+
+
+def test_decoder_step_on_another_stream(gpu, pkg, lib):
+    # behind work of that stream that the default stream knows nothing of
+    torch = gpu
+    side = torch.cuda.Stream()
+    step = Step(torch, pkg, "f16", 3, 11, 50, seed=9)
+    blocks, keep = step.blocks(lib)
+    rows = step.rows.clone()
+    step.rows.zero_()
+    torch.cuda.synchronize()
+    with torch.cuda.stream(side):
+        burn = torch.randn(4096, 4096, device="cuda")
+        for _ in range(4):
+            burn = burn @ burn
+        step.rows.copy_(rows)
+        for entry, args in blocks:
+            launch(torch, lib, entry, args)
+    side.synchronize()
+    step.check()
 
 
 def test_decoder_step_captured(gpu, pkg, lib):
