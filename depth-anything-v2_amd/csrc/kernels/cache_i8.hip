@@ -517,7 +517,8 @@ __global__ __launch_bounds__(256, 2) void cache_rows_kernel(dav2_attention_cache
 // features, f16: 441 us, 717 TFLOP/s; 8 times 512 of 4096 770 TFLOP/s; every
 // row all keys 820. A tile shared by eight waves instead of four is worth 10 %
 // there, the staging and the exponentials written between the matrix
-// instructions 8 %.
+// instructions 8 %. Heads of 64 are held to registers for three waves a SIMD:
+// 16 prompts' last 300 of up to 2048 tokens 74 us, 83 with four registers more.
 //
 // S^T = K Q^T and O^T = V^T P^T on v_mfma_f32_32x32x16_f16. Lane l holds, for
 // query l % 32, the scores of keys 8 (r / 4) + 4 (l / 32) + r % 4 of a 32-key
@@ -526,15 +527,14 @@ __global__ __launch_bounds__(256, 2) void cache_rows_kernel(dav2_attention_cache
 // place in LDS gives them: keys 0-3, 8-11 of a chunk, then 4-7, 12-15. Eight
 // registers are one 16-token chunk, so scales are uniform for them.
 template <typename E, int D, int WAVES>
-__global__ __launch_bounds__(64 * WAVES, 2) void cache_tiles_kernel(dav2_attention_cache_i8_args a, uint32_t splits,
-                                                                    uint32_t tiles) {
+__global__ __launch_bounds__(64 * WAVES, D <= 64 && sizeof(E) == 2 ? 3 : 2)
+void cache_tiles_kernel(dav2_attention_cache_i8_args a, uint32_t splits, uint32_t tiles) {
     constexpr bool kFloat = std::is_same_v<E, float>;
     constexpr int HEAD = D <= 64 ? 64 : 128;  // features of a row in LDS
     constexpr int KS = D / 16, FB = (D + 31) / 32, NP = kFloat ? 2 : 1;
     constexpr uint32_t d = D;
     constexpr uint32_t kThreads = 64 * WAVES, kTileRows = 32 * WAVES;
-    // of 16 codes, for each thread and tile: keys, and values
-    constexpr int kPieces = HEAD * 4 > kThreads ? HEAD * 4 / kThreads : 1;
+    constexpr int kPieces = HEAD * 4 / kThreads;  // of 16 codes, for each thread and tile: keys, and values
     constexpr int kRow = HEAD * 2;       // bytes of a key row in LDS
     // rescale when a score passes the running maximum by this: weights stay
     // below 2^6, far inside binary16, and most tiles leave the sums alone
@@ -583,8 +583,6 @@ __global__ __launch_bounds__(64 * WAVES, 2) void cache_tiles_kernel(dav2_attenti
         const uint32_t key_chunk = threadIdx.x % (HEAD / 16), key_row = threadIdx.x / (HEAD / 16);
         const uint32_t value_chunk = threadIdx.x & 3u, value_row = threadIdx.x >> 2;
         constexpr uint32_t kKeyStep = kThreads / (HEAD / 16), kValueStep = kThreads / 4;
-        // heads of 64 leave half of eight waves without a piece
-        const bool brings = HEAD * 4 >= kThreads || wave < HEAD / 16;
         // features that the head does not have: others in their place, whose
         // copies in LDS meet no query feature and reach no output
         const uint32_t key_feature = 16u * key_chunk < d ? 16u * key_chunk : 0u;
@@ -594,7 +592,7 @@ __global__ __launch_bounds__(64 * WAVES, 2) void cache_tiles_kernel(dav2_attenti
         auto find = [&](uint32_t block) {
             block = min(block, last - 1u);
 #pragma unroll
-            for (int i = 0; i < kPieces; ++i) of_key[i] = pages.find(block * 4u + min((key_row + kKeyStep * i) / 16u, 3u));
+            for (int i = 0; i < kPieces; ++i) of_key[i] = pages.find(block * 4u + (key_row + kKeyStep * i) / 16u);
             of_value = pages.find(block * 4u + value_chunk);
         };
         auto load_keys = [&] {
@@ -636,17 +634,15 @@ __global__ __launch_bounds__(64 * WAVES, 2) void cache_tiles_kernel(dav2_attenti
         auto stage = [&](int n, uint32_t buffer, uint32_t block) {
             if (n < 4 * kPieces) {
                 const int i = n / 4, half = n & 1;
-                if (brings) {
-                    if (n & 2) {
-                        const uint4 v = value_codes[i];
-                        *reinterpret_cast<h8*>(lds_values[buffer] +
-                                               swz<128>(value_row + kValueStep * i, 2u * value_chunk + half)) =
-                            half ? widen(v.y, v.w) : widen(v.x, v.z);
-                    } else {
-                        const uint4 k = key_codes[i];
-                        *reinterpret_cast<h8*>(lds_keys[buffer] + swz<kRow>(key_row + kKeyStep * i, 2u * key_chunk + half)) =
-                            half ? widen(k.z, k.w) : widen(k.x, k.y);
-                    }
+                if (n & 2) {
+                    const uint4 v = value_codes[i];
+                    *reinterpret_cast<h8*>(lds_values[buffer] +
+                                           swz<128>(value_row + kValueStep * i, 2u * value_chunk + half)) =
+                        half ? widen(v.y, v.w) : widen(v.x, v.z);
+                } else {
+                    const uint4 k = key_codes[i];
+                    *reinterpret_cast<h8*>(lds_keys[buffer] + swz<kRow>(key_row + kKeyStep * i, 2u * key_chunk + half)) =
+                        half ? widen(k.z, k.w) : widen(k.x, k.y);
                 }
             } else if (n == 4 * kPieces) {
                 load_keys();
@@ -928,7 +924,7 @@ bool valid(const dav2_attention_cache_i8_args& a) {
 // widen the keys once for twice the rows (441 us against 493 above, 36 against
 // 40 for 8 times 64 tokens), if the head is wide enough that three waves of the
 // smaller ones do not fit a SIMD instead (heads of 64, 16 times 1500 tokens:
-// 166 against 151), if they add no rows that do not exist (2 times 577 tokens
+// 166 against 141), if they add no rows that do not exist (2 times 577 tokens
 // 60 against 45), and if there are enough of them: one for each CU, and two
 // where a causal mask makes them unequal (4 prompts of 1024 tokens, 16 heads:
 // 43 against 38).
@@ -1012,8 +1008,10 @@ int dav2_hip_attention_cache_i8(const dav2_attention_cache_i8_args* args, void* 
         typedef std::remove_pointer_t<decltype(e)> E;
         with_head_dim(a.cache.head_dim, [&](auto dim) {
             constexpr int D = decltype(dim)::value;
-            if (p.tile == 256) dispatch(cache_tiles_kernel<E, D, 8>, grid, dim3(512), 0, s, a, p.splits, p.tiles);
-            else if (p.tile == 128) dispatch(cache_tiles_kernel<E, D, 4>, grid, dim3(256), 0, s, a, p.splits, p.tiles);
+            if constexpr (D > 64) {
+                if (p.tile == 256) return dispatch(cache_tiles_kernel<E, D, 8>, grid, dim3(512), 0, s, a, p.splits, p.tiles);
+            }
+            if (p.tile == 128) dispatch(cache_tiles_kernel<E, D, 4>, grid, dim3(256), 0, s, a, p.splits, p.tiles);
             else dispatch(cache_rows_kernel<E, D>, grid, dim3(256), 0, s, a, p.splits, p.tiles);
         });
         if (p.splits > 1) {

@@ -465,7 +465,8 @@ Plan plan_of(const dav2_cross_attention_args& a) {
     p.tiles = static_cast<uint32_t>(std::min<uint64_t>((rows + 127) / 128, 512));
     const uint64_t have = static_cast<uint64_t>(p.tiles) * a.kv_heads * a.batch;
     p.splits = static_cast<uint32_t>(
-        std::clamp<uint64_t>(std::min<uint64_t>(512 / have, a.key_tokens / (a.dtype == DAV2_DTYPE_F32 ? 64 : 128)), 1, kMostSplits));
+        std::clamp<uint64_t>(std::min<uint64_t>(512 / have, a.key_tokens / (a.dtype == DAV2_DTYPE_F32 ? 64 : 128)), 1,
+                             kMostSplits));
     return p;
 }
 uint64_t split_bytes(const dav2_cross_attention_args& a, const Plan& p) {
