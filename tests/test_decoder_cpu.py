@@ -62,19 +62,20 @@ QK = [dict(query=None), dict(key=None), dict(query_out=None), dict(key_out=None)
 CACHE = [dict(keys=None), dict(values=None), dict(key_scales=None), dict(value_scales=None), dict(keys=P + 8),
          dict(values=P + 1), dict(pages=0), dict(pages=1 << 31), dict(kv_heads=0), dict(page_size=0),
          dict(page_size=8), dict(page_size=24), dict(page_size=272), dict(head_dim=0), dict(head_dim=8),
-         dict(head_dim=72), dict(head_dim=144)]
+         dict(head_dim=72), dict(head_dim=144), dict(kv_heads=32768)]
 STORE = [dict(keys=None), dict(values=None), dict(page_table=None), dict(starts=None), dict(lengths=None),
          dict(table_pages=0), dict(dtype=3), dict(sequences=65536), dict(tokens=1 << 31), dict(key_stride=127),
          dict(value_stride=0)]
 ATTEND = [dict(query=None), dict(output=None), dict(query=P + 8), dict(output=P + 2), dict(page_table=None),
           dict(starts=None), dict(lengths=None), dict(table_pages=0), dict(dtype=3), dict(heads=0), dict(heads=3),
           dict(query_stride=255), dict(query_stride=248), dict(output_stride=260), dict(sequences=65536),
-          dict(tokens=1 << 31)]
+          dict(tokens=1 << 31), dict(tokens=1 << 20, heads=1 << 12, query_stride=1 << 19, output_stride=1 << 19)]
 CROSS = [dict(query=None), dict(keys=None), dict(values=None), dict(output=None), dict(query=P + 4), dict(keys=P + 8),
          dict(values=P + 2), dict(output=P + 1), dict(heads=0), dict(heads=3), dict(kv_heads=0), dict(head_dim=0),
          dict(head_dim=72), dict(head_dim=8), dict(head_dim=144), dict(dtype=3), dict(query_stride=248),
          dict(key_stride=120), dict(value_stride=132), dict(output_stride=0), dict(query_batch_stride=2561),
-         dict(key_batch_stride=4), dict(batch=65536), dict(query_tokens=1 << 31), dict(key_tokens=1 << 31)]
+         dict(key_batch_stride=4), dict(batch=65536), dict(query_tokens=1 << 31), dict(key_tokens=1 << 31),
+         dict(batch=60000, query_tokens=1 << 16)]
 
 
 @pytest.mark.parametrize("bad", ROTARY)
