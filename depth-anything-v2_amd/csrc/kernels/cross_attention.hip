@@ -96,7 +96,7 @@ DAV2_DEV v16f multiply(v4f a, v4f b, v16f c) {
 // right operand of the second product as it stands, if the left one takes its
 // keys in that order. In 16 bits that is two transposing LDS reads of four
 // keys by 16 features each; in fp32 four plain ones.
-template <typename E_, int D_, bool LISTED>
+template <typename E_, int D_, bool LISTED, int WAVES>
 struct Tiles {
     typedef E_ E;
     static constexpr int D = D_;
@@ -108,7 +108,7 @@ struct Tiles {
     static constexpr int T = kTile / (2 * N);                 // steps over the keys; step t: keys 2 N t ..
     static constexpr uint32_t kRow = HEAD * sizeof(E);        // bytes of a key in LDS
     static constexpr uint32_t kChunks = kRow / 16, kRowsPerCopy = 64 / kChunks;
-    static constexpr int kCopies = kTile * kRow / 4096;  // of each wave, for the keys and again for the values
+    static constexpr int kCopies = kTile * kRow / (1024 * WAVES);  // of each wave, for the keys and again for the values
     // rescale when a score passes the running maximum by this: weights stay
     // below 2^6 and most tiles leave the sums alone
     static constexpr float kSlack = 6.0f;
@@ -379,31 +379,31 @@ struct Tiles {
     }
 };
 
-// Four waves, 128 rows, two buffers and one barrier for a tile, whose copies go
-// straight into LDS during the products of the tile before.
+// Four or eight waves, 128 or 256 rows, two buffers and one barrier for a tile,
+// whose copies go straight into LDS during the products of the tile before.
 //
 // Bound by the matrix cores and, as long again in 16 bits, the exponentials of
 // the vector units beside them: 8 x 2048 queries of 32 heads of 128 on 4096
-// keys of 8, bf16, 1.16 ms, 950 TFLOP/s, where a large library product runs at
-// 1190; heads of 64 750. fp32: 129 TFLOP/s of 152 at 8 x 1024 queries, 16 heads
-// of 64, 4096 keys; 82 at 2 x 577 queries and 1370 keys, where 160 workgroups
-// are split in three. Tried and
-// not kept: eight waves in two groups that multiply and weigh in turns
-// (barriers between; 952 TFLOP/s, no difference), a tile's scores one tile
-// ahead among the exponentials (spills), a step's exponentials between the
-// products of the step before (556 -> 563 us at the masked case), tiles through registers (575 -> 610 us
-// at the masked case above).
-template <typename E, int D, bool LISTED>
-__global__ __launch_bounds__(256, 2) void cross_tiles_kernel(dav2_cross_attention_args a, Lists lists, uint32_t splits,
-                                                             uint32_t tiles) {
-    typedef Tiles<E, D, LISTED> K;
+// keys of 8, bf16, 1.15 ms, 956 TFLOP/s, where a large library product runs at
+// 1190 (four waves 1.20 ms); heads of 64 750. fp32: 129 TFLOP/s of 152 at 8 x
+// 1024 queries, 16 heads of 64, 4096 keys; 82 at 2 x 577 queries and 1370 keys,
+// where 160 workgroups are split in three. Tried and not kept: eight waves in
+// two groups that multiply and weigh in turns (barriers between; no
+// difference), a tile's scores one tile ahead among the exponentials (spills),
+// a step's exponentials between the products of the step before (556 -> 563 us
+// at a masked case of 8 prompts), tiles through registers (575 -> 610 us).
+template <typename E, int D, bool LISTED, int WAVES>
+__global__ __launch_bounds__(64 * WAVES, 2)
+void cross_tiles_kernel(dav2_cross_attention_args a, Lists lists, uint32_t splits, uint32_t tiles) {
+    constexpr uint32_t kTileRows = 32 * WAVES;
+    typedef Tiles<E, D, LISTED, WAVES> K;
     __shared__ __attribute__((aligned(16))) int8_t lds[2][2][K::kTile * K::kRow];  // [buffer][keys, values]
     K k(a, lists, blockIdx.x);
-    const uint32_t split = blockIdx.y % splits, row_tiles = (k.rows + 127u) / 128u;
+    const uint32_t split = blockIdx.y % splits, row_tiles = (k.rows + kTileRows - 1u) / kTileRows;
     const uint32_t blocks = (k.count + K::kTile - 1u) / K::kTile, per = (blocks + splits - 1u) / splits;
     const uint32_t first = split * per, last = min(first + per, blocks);
     for (uint32_t tile = blockIdx.y / splits; tile < row_tiles; tile += tiles) {
-        const uint32_t row0 = tile * 128u + k.wave * 32u;
+        const uint32_t row0 = tile * kTileRows + k.wave * 32u;
         const bool any_row = row0 < k.rows;
         uint32_t place[K::kCopies];  // of the tile that is copied next
         __syncthreads();             // the row tile before has been read
@@ -411,7 +411,7 @@ __global__ __launch_bounds__(256, 2) void cross_tiles_kernel(dav2_cross_attentio
             k.find(first, place);
             k.copy(lds[0][0], lds[0][1], place, first + 1u);
         }
-        k.begin(any_row ? row0 : tile * 128u);
+        k.begin(any_row ? row0 : tile * kTileRows);
         DAV2_WAIT_VMCNT(0);
         __syncthreads();
         for (uint32_t block = first; block < last; ++block) {
@@ -449,24 +449,31 @@ __global__ __launch_bounds__(256) void cross_join_kernel(dav2_cross_attention_ar
     }
 }
 
-// How a call is dealt out: 128 rows a workgroup, and the keys split while all
-// workgroups run at once, two on a CU, down to two tiles each (fp32: 128 queries,
-// 12 heads of 64, 1024 keys, 20.0 us in 16, 21.9 in 8). us: 64 workgroups of one
-// query each and 1370 keys, f16, 11.9 in 4, 10.1 in 8, 10.7 in 10; 160 of 577
-// queries, 25.6 whole, 22.5 in 3, fp32 102 whole, 110 in 2, 75 in 3; 80 of 300
-// queries, 32 heads of 8 of 128, 4096 keys, bf16, 40.8 in 3, 39.5 in 6.
+// How a call is dealt out: 128 rows a workgroup, two on a CU, or 256 and one,
+// where wide heads of 16 bits leave no room for a third and the larger tiles
+// add no rows that do not exist and fill the chip (us, 256 against 128: 8 x 2048
+// queries, 4096 keys 1150 / 1200; 16 x 100 queries, 577 keys 29.2 / 30.5; 2 x 1024
+// queries and keys 38.6 / 38.9). The keys are split while all workgroups run at
+// once, down to two tiles each (fp32: 128 queries, 12 heads of 64, 1024 keys,
+// 20.0 us in 16, 21.9 in 8). us: 64 workgroups of one query each and 1370 keys,
+// f16, 11.9 in 4, 10.1 in 8, 10.7 in 10; 160 of 577 queries, 25.6 whole, 22.5 in
+// 3, fp32 102 whole, 110 in 2, 75 in 3; 80 of 300 queries, 32 heads of 8 of 128,
+// 4096 keys, bf16, 40.8 in 3, 39.5 in 6.
 struct Plan {
+    uint32_t tile;  // rows of a workgroup: 128 or 256
     uint32_t tiles, splits;
 };
 Plan plan_of(const dav2_cross_attention_args& a) {
-    Plan p{1, 1};
+    Plan p{128, 1, 1};
     if (a.kv_heads == 0 || a.heads < a.kv_heads || a.batch == 0 || a.query_tokens == 0) return p;
     const uint64_t rows = static_cast<uint64_t>(a.query_tokens) * (a.heads / a.kv_heads);
-    p.tiles = static_cast<uint32_t>(std::min<uint64_t>((rows + 127) / 128, 512));
-    const uint64_t have = static_cast<uint64_t>(p.tiles) * a.kv_heads * a.batch;
-    p.splits = static_cast<uint32_t>(
-        std::clamp<uint64_t>(std::min<uint64_t>(512 / have, a.key_tokens / (a.dtype == DAV2_DTYPE_F32 ? 64 : 128)), 1,
-                             kMostSplits));
+    const uint64_t planes = static_cast<uint64_t>(a.kv_heads) * a.batch;
+    const uint64_t most = std::clamp<uint64_t>(a.key_tokens / (a.dtype == DAV2_DTYPE_F32 ? 64 : 128), 1, kMostSplits);
+    if (a.head_dim > 64 && a.dtype != DAV2_DTYPE_F32 && (rows + 127) / 128 % 2 == 0 &&
+        (rows + 255) / 256 * planes * most >= 256)
+        p.tile = 256;
+    p.tiles = static_cast<uint32_t>(std::min<uint64_t>((rows + p.tile - 1) / p.tile, 512));
+    p.splits = static_cast<uint32_t>(std::clamp<uint64_t>((p.tile == 256 ? 256 : 512) / (p.tiles * planes), 1, most));
     return p;
 }
 uint64_t split_bytes(const dav2_cross_attention_args& a, const Plan& p) {
@@ -514,8 +521,13 @@ int dav2_hip_cross_attention(const dav2_cross_attention_args* args, void* stream
         typedef std::remove_pointer_t<decltype(e)> E;
         with_head_dim(a.head_dim, [&](auto dim) {
             constexpr int D = decltype(dim)::value;
-            dispatch(lists.keys ? cross_tiles_kernel<E, D, true> : cross_tiles_kernel<E, D, false>, grid, dim3(256), 0, s, a,
-                     lists, p.splits, p.tiles);
+            if constexpr (D > 64 && sizeof(E) == 2) {
+                if (p.tile == 256)
+                    return dispatch(lists.keys ? cross_tiles_kernel<E, D, true, 8> : cross_tiles_kernel<E, D, false, 8>, grid,
+                                    dim3(512), 0, s, a, lists, p.splits, p.tiles);
+            }
+            dispatch(lists.keys ? cross_tiles_kernel<E, D, true, 4> : cross_tiles_kernel<E, D, false, 4>, grid, dim3(256), 0,
+                     s, a, lists, p.splits, p.tiles);
         });
         if (p.splits > 1) {
             const uint64_t rows = static_cast<uint64_t>(a.batch) * a.query_tokens * a.heads;
