@@ -594,6 +594,21 @@ def test_cross_attention(gpu, pkg, lib, dtype, heads, kv, head_dim, queries, key
     check_cross(torch, pkg, lib, q, k, v, None, None, dtype)
 
 
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("masked", [False, True])
+@pytest.mark.parametrize("batch,queries,keys,heads,kv,head_dim", [(2, 200, 1370, 16, 8, 128), (8, 250, 130, 16, 16, 80),
+                                                                  (2, 129, 999, 32, 16, 112), (9, 130, 64, 15, 15, 96)])
+def test_cross_attention_wide(gpu, pkg, lib, dtype, masked, batch, queries, keys, heads, kv, head_dim):
+    # tiles of 256 rows, with splits of the keys and without; a batch that sees one key, one that sees none
+    torch = gpu
+    q = rand(torch, 1, batch, queries, heads, head_dim, dtype=dtype)
+    k, v = (rand(torch, i, batch, keys, kv, head_dim, dtype=dtype) for i in (2, 3))
+    lengths = ints(torch, [keys - 7 * i for i in range(batch)])
+    lengths[1] = 0 if masked else 1
+    mask = (torch.rand((batch, keys), device="cuda") < 0.6).to(torch.uint8) if masked else None
+    check_cross(torch, pkg, lib, q, k, v, lengths, mask, dtype)
+
+
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("queries", [1, 21, 150])
 def test_cross_attention_lengths_and_masks(gpu, pkg, lib, dtype, queries):
