@@ -319,14 +319,13 @@ __global__ __launch_bounds__(256, 2) void cache_rows_kernel(dav2_attention_cache
         };
         auto load_keys = [&] {
             const int8_t* k = a.cache.keys + ((static_cast<uint64_t>(pages.page(of_key)) * kv_heads + h) * page_size +
-                                              of_key.slot + col % 4u) * d + 16u * g;
+                                              of_key.slot + col % 4u) * d;
+            // features that the head does not have: others in their place, which meet zeros of the query
 #pragma unroll
             for (int t = 0; t < 4; ++t)
 #pragma unroll
-                for (int kc = 0; kc < KC; ++kc) {
-                    kraw[t][kc] = make_uint4(0, 0, 0, 0);
-                    if (64u * kc + 16u * g < d) kraw[t][kc] = *reinterpret_cast<const uint4*>(k + 4u * t * d + 64 * kc);
-                }
+                for (int kc = 0; kc < KC; ++kc)
+                    kraw[t][kc] = *reinterpret_cast<const uint4*>(k + 4u * t * d + min(64u * kc + 16u * g, d - 16u));
         };
         auto load_values = [&] {
             exists = pages.exists(of_value);
