@@ -1,5 +1,6 @@
 // Shared by the decoder operators' kernels (rotary.hip, cache_i8.hip,
-// cross_attention.hip): element types and their checks.
+// cross_attention.hip): element types and head widths, sequences and rows, LDS
+// reads beside copies, and the join of what splits of the keys leave.
 #pragma once
 
 #include <type_traits>
@@ -8,23 +9,6 @@
 #include "dav2_hip.h"
 
 namespace dav2k {
-
-// An activation type: E as stored, widened to fp32 on load, rounded to
-// nearest even on store.
-template <uint32_t DTYPE>
-struct Activation;
-template <>
-struct Activation<DAV2_DTYPE_F32> {
-    typedef float E;
-};
-template <>
-struct Activation<DAV2_DTYPE_F16> {
-    typedef _Float16 E;
-};
-template <>
-struct Activation<DAV2_DTYPE_BF16> {
-    typedef __bf16 E;
-};
 
 inline uint32_t dtype_bytes(uint32_t dtype) { return dtype == DAV2_DTYPE_F32 ? 4u : 2u; }
 
@@ -77,25 +61,6 @@ DAV2_DEV void lds_read4(uint32_t a, uint32_t b, v4i_t (&v)[4]) {
     asm volatile("ds_read_b128 %0, %4\n\tds_read_b128 %1, %4 offset:%6\n\t"
                  "ds_read_b128 %2, %5\n\tds_read_b128 %3, %5 offset:%6\n\ts_waitcnt lgkmcnt(0)"
                  : "=&v"(v[0]), "=&v"(v[1]), "=&v"(v[2]), "=&v"(v[3]) : "v"(a), "v"(b), "n"(STEP) : "memory");
-}
-// ... at a, a + STEP, .. of N rows
-template <uint32_t STEP, int N>
-DAV2_DEV void lds_read_rows(uint32_t a, v4i_t (&v)[N]) {
-    static_assert(N >= 1 && N <= 4);
-    if constexpr (N == 1)
-        asm volatile("ds_read_b128 %0, %1\n\ts_waitcnt lgkmcnt(0)" : "=&v"(v[0]) : "v"(a) : "memory");
-    else if constexpr (N == 2)
-        asm volatile("ds_read_b128 %0, %2\n\tds_read_b128 %1, %2 offset:%3\n\ts_waitcnt lgkmcnt(0)"
-                     : "=&v"(v[0]), "=&v"(v[1]) : "v"(a), "n"(STEP) : "memory");
-    else if constexpr (N == 3)
-        asm volatile("ds_read_b128 %0, %3\n\tds_read_b128 %1, %3 offset:%4\n\tds_read_b128 %2, %3 offset:%5\n\t"
-                     "s_waitcnt lgkmcnt(0)"
-                     : "=&v"(v[0]), "=&v"(v[1]), "=&v"(v[2]) : "v"(a), "n"(STEP), "n"(2 * STEP) : "memory");
-    else
-        asm volatile("ds_read_b128 %0, %4\n\tds_read_b128 %1, %4 offset:%5\n\tds_read_b128 %2, %4 offset:%6\n\t"
-                     "ds_read_b128 %3, %4 offset:%7\n\ts_waitcnt lgkmcnt(0)"
-                     : "=&v"(v[0]), "=&v"(v[1]), "=&v"(v[2]), "=&v"(v[3])
-                     : "v"(a), "n"(STEP), "n"(2 * STEP), "n"(3 * STEP) : "memory");
 }
 DAV2_DEV void lds_read_pair(uint32_t a, uint32_t b, v4i_t& v, v4i_t& w) {
     asm volatile("ds_read_b128 %0, %2\n\tds_read_b128 %1, %3\n\ts_waitcnt lgkmcnt(0)"
@@ -168,7 +133,6 @@ DAV2_DEV Sequence sequence_of(const int32_t* starts, const int32_t* lengths, uin
     return q;
 }
 
-typedef _Float16 h4 __attribute__((ext_vector_type(4)));
 typedef _Float16 h8 __attribute__((ext_vector_type(8)));
 typedef __bf16 b8 __attribute__((ext_vector_type(8)));
 typedef float v16f __attribute__((ext_vector_type(16)));
