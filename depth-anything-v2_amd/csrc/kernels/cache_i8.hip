@@ -185,10 +185,22 @@ __global__ __launch_bounds__(256, 8) void cache_store_kernel(dav2_cache_store_i8
 //
 // A value's scale sv goes with the weight of its key: with sv = 2^e f,
 // 1 <= f < 2, and t = s log2(e) + e for a score s,
-//   w = exp2(t - max t),  O = sum (w f) c,  L = sum w 2^-e,  o = O / L.
-// The maximum is that of what reaches the output, so w f rounded to binary16
-// (two parts in the fp32 mode) keeps its precision whatever the pages' scales
-// are; L is summed in fp32 from the unrounded w.
+//   w = exp2(t - base),  O = sum (w f) c,  L = sum w 2^-e,  o = O / L.
+// L is summed in fp32 from the unrounded w. For the product w f is rounded to
+// binary16, whose smallest step is 2^-24: base lies kBias below the running
+// maximum of t, so that the largest weights are near 2^15 and small ones, of
+// which a long context has many, keep their bits. Against a weight of the
+// maximum, w f is good to half a step (2^-11) down to 2^-14 - kBias, and loses
+// at most 2^-25 - kBias below. The fp32 mode has a second part: the rest times
+// 2^11, whose product takes the codes times 2^-11 (exact in binary16), so that
+// it ends 2^11 later: 2^-23 of a weight down to 2^-14 - kBias, at most
+// 2^-36 - kBias below.
+//
+// A score past kFar is rounded to more than the exponentials' range has room
+// for, and kBias would be lost beside it: base is then the maximum itself.
+constexpr float kFar = 1048576.0f;
+constexpr float kSecond = 2048.0f;  // what the second part is multiplied by
+DAV2_DEV h8 for_second(h8 codes) { return codes * static_cast<_Float16>(1.0f / kSecond); }
 
 // Page and slot of a 16-token chunk; magic = ceil(2^32 / chunks per page),
 // which divides every chunk below 2^28 exactly (2 to 16 chunks per page). For
@@ -233,10 +245,11 @@ DAV2_DEV h8 widen(uint32_t lo, uint32_t hi) {
     return h8{a.x, a.y, b.x, b.y, c.x, c.y, d.x, d.y};
 }
 
-// A page's value scale as 2^e f. Below 2^-100 (a page of zeros with a scale of
-// 0) 2^-100 stands in: w 2^-e stays finite. Infinity and NaN make f NaN.
+// A page's value scale as 2^e f. Below 2^-80 (a page of zeros with a scale of
+// 0) 2^-80 stands in: the sum of w 2^-e, of up to 2^31 weights of 2^15, stays
+// finite. Infinity and NaN make f NaN.
 DAV2_DEV void split_scale(float scale, float& exponent, float& fraction, float& inverse) {
-    const uint32_t bits = max(__float_as_uint(scale) & 0x7fffffffu, 27u << 23);
+    const uint32_t bits = max(__float_as_uint(scale) & 0x7fffffffu, 47u << 23);
     const int e = static_cast<int>(bits >> 23) - 127;
     exponent = static_cast<float>(e);
     fraction = bits >= 0x7f800000u ? __uint_as_float(0x7fc00000u)
@@ -270,8 +283,9 @@ __global__ __launch_bounds__(256, 2) void cache_rows_kernel(dav2_attention_cache
     constexpr int KC = (D + 63) / 64, FT = D / 16, NP = kFloat ? 2 : 1;
     constexpr uint32_t d = D;
     constexpr int kPad = 17;  // row length of the joining waves' sums in LDS
+    constexpr float kBias = 14.0f;  // a weight times a fraction stays below 2^15
     __shared__ float joined[4][D * kPad];
-    __shared__ float shared_max[4][16], shared_sum[4][16];
+    __shared__ float shared_base[4][16], shared_sum[4][16];
     const uint32_t lane = threadIdx.x & 63u, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const uint32_t col = lane & 15u, g = lane >> 4;
     const uint32_t split = blockIdx.x % splits, h = blockIdx.y, s = blockIdx.z;
@@ -306,7 +320,7 @@ __global__ __launch_bounds__(256, 2) void cache_rows_kernel(dav2_attention_cache
         v4f o[FT];
 #pragma unroll
         for (int f = 0; f < FT; ++f) o[f] = v4f{0.f, 0.f, 0.f, 0.f};
-        float maximum = kNoScore, sum = 0.0f;  // sum: this lane's keys only
+        float maximum = kNoScore, base = kNoScore, sum = 0.0f;  // sum: this lane's keys only
 
         // A block's keys are loaded when the scores of the block before are
         // done, its values and scales behind that block's values, its places
@@ -424,9 +438,10 @@ __global__ __launch_bounds__(256, 2) void cache_rows_kernel(dav2_attention_cache
                 }
             largest = over_groups(largest, Larger());
             if (__any(largest > maximum)) {
-                const float grown = fmaxf(maximum, largest);
-                const float keep = __builtin_amdgcn_exp2f(maximum - grown);
-                maximum = grown;
+                maximum = fmaxf(maximum, largest);
+                const float moved = fabsf(maximum) < kFar ? maximum - kBias : maximum;
+                const float keep = __builtin_amdgcn_exp2f(base - moved);
+                base = moved;
                 sum *= keep;
 #pragma unroll
                 for (int f = 0; f < FT; ++f) o[f] *= keep;
@@ -437,22 +452,23 @@ __global__ __launch_bounds__(256, 2) void cache_rows_kernel(dav2_attention_cache
             for (int t = 0; t < 4; ++t)
 #pragma unroll
                 for (int r = 0; r < 4; ++r) {
-                    const float w = __builtin_amdgcn_exp2f(sc[t][r] - maximum);
+                    const float w = __builtin_amdgcn_exp2f(sc[t][r] - base);
                     part += w;
                     const float y = kFloat ? keep_fp32(w * fraction) : w * fraction;  // hi and lo of one rounded product
                     const _Float16 hi = static_cast<_Float16>(y);
                     pf[0][t >> 1][4 * (t & 1) + r] = hi;
                     if constexpr (kFloat)
-                        pf[1][t >> 1][4 * (t & 1) + r] = static_cast<_Float16>(y - static_cast<float>(hi));
+                        pf[1][t >> 1][4 * (t & 1) + r] = static_cast<_Float16>((y - static_cast<float>(hi)) * kSecond);
                 }
             sum = fmaf(part, inverse, sum);
 #pragma unroll
             for (int f = 0; f < FT; ++f) {
                 const h8 v0 = widen(vraw[f].x, vraw[f].y), v1 = widen(vraw[f].z, vraw[f].w);
-#pragma unroll
-                for (int p = 0; p < NP; ++p) {
-                    o[f] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v0, pf[p][0], o[f], 0, 0, 0);
-                    o[f] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v1, pf[p][1], o[f], 0, 0, 0);
+                o[f] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v0, pf[0][0], o[f], 0, 0, 0);
+                o[f] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v1, pf[0][1], o[f], 0, 0, 0);
+                if constexpr (kFloat) {
+                    o[f] = __builtin_amdgcn_mfma_f32_16x16x32_f16(for_second(v0), pf[1][0], o[f], 0, 0, 0);
+                    o[f] = __builtin_amdgcn_mfma_f32_16x16x32_f16(for_second(v1), pf[1][1], o[f], 0, 0, 0);
                 }
             }
             if constexpr (kMore) {
@@ -467,14 +483,14 @@ __global__ __launch_bounds__(256, 2) void cache_rows_kernel(dav2_attention_cache
         // join the four waves: lane (col, g), register r of o[f]: feature 16 f + 4 g + r of row col
         __syncthreads();  // the tile before has been read
         if (g == 0) {
-            shared_max[wave][col] = maximum;
+            shared_base[wave][col] = base;
             shared_sum[wave][col] = sum;
         }
         __syncthreads();
         float top = kNoScore;
 #pragma unroll
-        for (int w = 0; w < 4; ++w) top = fmaxf(top, shared_max[w][col]);
-        const float mine = __builtin_amdgcn_exp2f(maximum - top);
+        for (int w = 0; w < 4; ++w) top = fmaxf(top, shared_base[w][col]);
+        const float mine = __builtin_amdgcn_exp2f(base - top);
 #pragma unroll
         for (int f = 0; f < FT; ++f)
 #pragma unroll
@@ -485,10 +501,10 @@ __global__ __launch_bounds__(256, 2) void cache_rows_kernel(dav2_attention_cache
         if (tile * 16u + out_col < rows) {
             float all = kNoScore, total = 0.0f;
 #pragma unroll
-            for (int w = 0; w < 4; ++w) all = fmaxf(all, shared_max[w][out_col]);
+            for (int w = 0; w < 4; ++w) all = fmaxf(all, shared_base[w][out_col]);
 #pragma unroll
             for (int w = 0; w < 4; ++w)
-                total = fmaf(shared_sum[w][out_col], __builtin_amdgcn_exp2f(shared_max[w][out_col] - all), total);
+                total = fmaf(shared_sum[w][out_col], __builtin_amdgcn_exp2f(shared_base[w][out_col] - all), total);
             uint32_t out_token, out_head;
             of.find(out_col, out_token, out_head);
             out_head += h * group;
@@ -537,9 +553,10 @@ void cache_tiles_kernel(dav2_attention_cache_i8_args a, uint32_t splits, uint32_
     constexpr uint32_t kThreads = 64 * WAVES, kTileRows = 32 * WAVES;
     constexpr int kPieces = HEAD * 4 / kThreads;  // of 16 codes, for each thread and tile: keys, and values
     constexpr int kRow = HEAD * 2;       // bytes of a key row in LDS
-    // rescale when a score passes the running maximum by this: weights stay
-    // below 2^6, far inside binary16, and most tiles leave the sums alone
-    constexpr float kSlack = 6.0f;
+    // rescale when a score passes the running maximum by kSlack: most tiles
+    // leave the sums alone. Weights (times a fraction in the fp32 mode) stay
+    // below 2^15.
+    constexpr float kSlack = 2.0f, kBias = kFloat ? 14.0f - kSlack : 15.0f - kSlack;
     __shared__ __attribute__((aligned(16))) int8_t lds_keys[2][64 * kRow];
     __shared__ __attribute__((aligned(16))) int8_t lds_values[2][HEAD * 128];
     __shared__ __attribute__((aligned(16))) v4f lds_scales[2][4];  // of a chunk: key scale, log2 / exponent, inverse, fraction
@@ -620,7 +637,8 @@ void cache_tiles_kernel(dav2_attention_cache_i8_args a, uint32_t splits, uint32_
                 split_scale(value_scale, exponent, fraction, inverse);
                 v4f c = {key_scale, exponent, inverse, fraction};
                 if constexpr (!kFloat) {
-                    // the weights take the whole scale: exact to 2^-22 of them
+                    // the weights take the whole scale, off by half a step of its
+                    // logarithm: below 2^-20 of them for scales of 1e-8 and more
                     c[1] = exponent + __builtin_amdgcn_logf(fraction);
                     c[2] = inverse / fraction;
                 }
@@ -704,7 +722,8 @@ void cache_tiles_kernel(dav2_attention_cache_i8_args a, uint32_t splits, uint32_
         for (int f = 0; f < FB; ++f)
 #pragma unroll
             for (int r = 0; r < 16; ++r) o[f][r] = 0.0f;
-        float maximum = kNoScore, sum = 0.0f;  // sum: this lane's keys only
+        float base = kNoScore, sum = 0.0f;  // sum: this lane's keys only
+        bool far = false;                   // the same for all lanes
 
         if (first < last) {
             store_scales(0);
@@ -794,11 +813,13 @@ void cache_tiles_kernel(dav2_attention_cache_i8_args a, uint32_t splits, uint32_
                     largest = fmaxf(largest, fmaf(m, c[t], shift[t]));
                 }
                 largest = over_halves(largest, Larger());
-                if (__any(largest > maximum + kSlack)) {
+                if (__any(largest > base + (far ? 0.0f : kBias + kSlack))) {
                     stay_in_branch();
-                    const float grown = fmaxf(maximum, largest);
-                    const float keep = __builtin_amdgcn_exp2f(maximum - grown);
-                    maximum = grown;
+                    const float grown = fmaxf(base + (far ? 0.0f : kBias), largest);
+                    far = far || __any(fabsf(grown) >= kFar && grown != kNoScore);
+                    const float moved = grown - (far ? 0.0f : kBias);
+                    const float keep = __builtin_amdgcn_exp2f(base - moved);
+                    base = moved;
                     sum *= keep;
 #pragma unroll
                     for (int f = 0; f < FB; ++f)
@@ -809,13 +830,13 @@ void cache_tiles_kernel(dav2_attention_cache_i8_args a, uint32_t splits, uint32_
                 h8 pf[2][NP];
                 float part = 0.0f;
                 auto weigh = [&](int t, int r) {
-                    const float w = __builtin_amdgcn_exp2f(fmaf(sc[t >> 1][8 * (t & 1) + r], c[t], shift[t] - maximum));
+                    const float w = __builtin_amdgcn_exp2f(fmaf(sc[t >> 1][8 * (t & 1) + r], c[t], shift[t] - base));
                     part = r ? part + w : w;
                     if constexpr (kFloat) {
                         const float y = keep_fp32(w * fraction[t]);  // hi and lo of one rounded product
                         const _Float16 hi = static_cast<_Float16>(y);
                         pf[t & 1][0][r] = hi;
-                        pf[t & 1][1][r] = static_cast<_Float16>(y - static_cast<float>(hi));
+                        pf[t & 1][1][r] = static_cast<_Float16>((y - static_cast<float>(hi)) * kSecond);
                     } else {
                         pf[t & 1][0][r] = static_cast<_Float16>(w);
                     }
@@ -829,9 +850,10 @@ void cache_tiles_kernel(dav2_attention_cache_i8_args a, uint32_t splits, uint32_
                     if (t < 3) read_values(t + 1, vf[(t + 1) & 1]);
 #pragma unroll
                     for (int f = 0; f < FB; ++f) {
-#pragma unroll
-                        for (int p = 0; p < NP; ++p)
-                            o[f] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf[t & 1][f], pf[t & 1][p], o[f], 0, 0, 0);
+                        o[f] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf[t & 1][f], pf[t & 1][0], o[f], 0, 0, 0);
+                        if constexpr (kFloat)
+                            o[f] = __builtin_amdgcn_mfma_f32_32x32x16_f16(for_second(vf[t & 1][f]), pf[t & 1][1], o[f], 0,
+                                                                          0, 0);
                         if (t < 3)
 #pragma unroll
                             for (int r = 8 * f / FB; r < 8 * (f + 1) / FB; ++r) weigh(t + 1, r);
@@ -865,7 +887,7 @@ void cache_tiles_kernel(dav2_attention_cache_i8_args a, uint32_t splits, uint32_
                         *reinterpret_cast<V4*>(y + feature) = out;
                     }
                 }
-            if (splits > 1 && hf == 0) parts.stats[slot] = make_float2(maximum, sum);
+            if (splits > 1 && hf == 0) parts.stats[slot] = make_float2(base, sum);
         }
     }
 }

@@ -1,0 +1,120 @@
+"""Softmax weights of the decoder's attention over their whole range: keys far
+below the largest, whose sum is what the output holds. Against float64, with
+bounds that leave a small weight no more than its own rounding."""
+
+import math
+
+import pytest
+
+import decoder_ref as ref
+from test_gpu_decoder import attend_args, ints, launch, rand
+
+pytestmark = pytest.mark.gpu
+
+DTYPES = ["f32", "f16", "bf16"]
+
+
+def want_of(q, k, v, scale, dtype, step, floor, exponent=0.0):
+    """softmax(scale q k^T) v of float64 rows, and how far a kernel may be off.
+
+    A score is an fp32 sum of d products (d + 4 roundings of at most sum |q k|;
+    the kernels' other factors are exact or counted there), changed to units of
+    log2 and rounded beside the exponent of a value scale (`exponent` at most).
+    A weight is rounded by `step` of itself, or by `floor` of the largest one.
+    Sums over n keys are of blocks of 32 and more, one after the other: 64 +
+    n / 32 roundings."""
+    s = (q @ k.T) * scale
+    ds = (q.abs() @ k.abs().T) * abs(scale) * (q.shape[1] + 4) * ref.U + (s.abs() + exponent) * 4 * ref.U
+    p = torch_exp(s)
+    total = p.sum(-1, keepdim=True)
+    n = k.shape[0]
+    off = (p * (step + 2 * ds + (64 + n / 32) * ref.U) + floor) @ v.abs()
+    # the sum of the weights is of unrounded ones
+    want = (p @ v) / total
+    off = off / total + want.abs() * ((p * 2 * ds).sum(-1, keepdim=True) / total + (64 + n / 32) * ref.U)
+    return want, off + want.abs() * ref.half_step(dtype) + ref.floor_of(dtype)
+
+
+def torch_exp(s):
+    return (s - s.amax(-1, keepdim=True)).exp()
+
+
+def sink_cache(torch, n, gap, at, page_size, kv, d, seed):
+    """A cache of n tokens whose key `at` is ahead of all others by about `gap` for a query whose first feature is 1,
+    and has values of zero; the others' scores lie close together and their values are of one sign."""
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    pages = n // page_size
+    keys = torch.randint(-3, 4, (pages, kv, page_size, d), generator=g, dtype=torch.int8, device="cuda")
+    values = torch.randint(40, 128, (pages, kv, d, page_size), generator=g, dtype=torch.int8, device="cuda")
+    keys[..., 0] = 0
+    keys[at // page_size, :, at % page_size] = 0
+    keys[at // page_size, :, at % page_size, 0] = 127
+    values[at // page_size, :, :, at % page_size] = 0
+    ks = torch.full((pages, kv), gap / 127.0, device="cuda")
+    vs = 0.005 + 0.02 * torch.rand((pages, kv), generator=g, device="cuda")
+    return [keys, values, ks, vs]
+
+
+def sink_query(torch, tokens, heads, d, dtype, seed):
+    q = rand(torch, seed, tokens, heads, d, dtype=dtype, scale=0.2)
+    q[..., 0] = 1.0
+    return q
+
+
+# half a step of a weight, and what a small one may lose, of the largest
+CACHE_STEPS = {"f32": (2.0 ** -22, 2.0 ** -47), "f16": (2.0 ** -11 + 2.0 ** -19, 2.0 ** -37),
+               "bf16": (2.0 ** -11 + 2.0 ** -19, 2.0 ** -37)}
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("gap", [12, 16, 18])
+@pytest.mark.parametrize("queries,sequences,most", [(1, 1, 1), (1, 1, 16384), (40, 512, 127), (40, 1, 16384)])
+@pytest.mark.parametrize("at", [0, 9000])
+def test_cache_attention_dominant_key(gpu, pkg, lib, dtype, gap, queries, sequences, most, at):
+    # rows and tiles of the cache kernels, the keys whole and split; the sequences behind the first are empty
+    torch = gpu
+    n, page_size, kv, d, heads = 16384, 64, 1, 64, 8
+    cache = sink_cache(torch, n, gap, at, page_size, kv, d, 3)
+    q = sink_query(torch, queries, heads, d, dtype, 5)
+    table = torch.randperm(n // page_size, device="cuda").to(torch.int32)
+    table = table.expand(sequences, -1).contiguous()
+    # the sink stays at position `at`
+    where = (table[0] == at // page_size).nonzero()[0, 0]
+    table[:, where], table[:, at // page_size] = table[:, at // page_size].clone(), at // page_size
+    starts, lengths = ints(torch, [0] + [queries] * sequences), ints(torch, [n] + [0] * (sequences - 1))
+    out = torch.full(q.shape, math.nan, dtype=q.dtype, device="cuda")
+    a, keep = attend_args(torch, pkg, lib, cache, q, out, table, starts, lengths, False, dtype, 1.0, max_length=most)
+    launch(torch, lib, "dav2_hip_attention_cache_i8", a)
+    entry = table[0].long()
+    k = (cache[0][entry, 0].double() * cache[2][entry, 0].double()[:, None, None]).reshape(n, d)
+    v = (cache[1][entry, 0].double() * cache[3][entry, 0].double()[:, None, None]).transpose(1, 2).reshape(n, d)
+    torch.cuda.synchronize()
+    step, floor = CACHE_STEPS[dtype]
+    for h in range(heads):
+        want, bound = want_of(q[:, h].double(), k, v, 1.0, dtype, step, floor, exponent=8.0)
+        ref.assert_within(out[:, h], want, bound)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("queries,sequences,most", [(1, 1, 1), (1, 1, 16384), (40, 512, 127), (40, 1, 16384)])
+def test_cache_attention_pages_with_a_scale_of_zero(gpu, pkg, lib, dtype, queries, sequences, most):
+    # half of a long context in pages whose values are zeros by their scale: the sum of the weights stays finite
+    torch = gpu
+    n, page_size, d, heads = 16384, 64, 64, 8
+    cache = sink_cache(torch, n, 4, 100, page_size, 1, d, 3)
+    cache[3][:128] = 0.0
+    q = sink_query(torch, queries, heads, d, dtype, 5)
+    starts, lengths = ints(torch, [0] + [queries] * sequences), ints(torch, [n] + [0] * (sequences - 1))
+    for table in (torch.arange(256, device="cuda"), torch.arange(256, device="cuda").flip(0)):
+        table = table.to(torch.int32).expand(sequences, -1).contiguous()
+        out = torch.full(q.shape, math.nan, dtype=q.dtype, device="cuda")
+        a, keep = attend_args(torch, pkg, lib, cache, q, out, table, starts, lengths, False, dtype, 1.0, max_length=most)
+        launch(torch, lib, "dav2_hip_attention_cache_i8", a)
+        k = (cache[0][:, 0].double() * cache[2][:, 0].double()[:, None, None]).reshape(n, d)
+        v = (cache[1][:, 0].double() * cache[3][:, 0].double()[:, None, None]).transpose(1, 2).reshape(n, d)
+        torch.cuda.synchronize()
+        step, floor = CACHE_STEPS[dtype]
+        for h in range(heads):
+            # a scale of 2^-80, of 1e-24 of the others, stands for zero; its logarithm is rounded to 2^-18
+            want, bound = want_of(q[:, h].double(), k, v, 1.0, dtype, step + 2.0 ** -18, floor, exponent=80.0)
+            ref.assert_within(out[:, h], want, bound + 127 * 2.0 ** -80)
