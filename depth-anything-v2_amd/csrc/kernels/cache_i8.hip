@@ -826,6 +826,18 @@ void cache_tiles_kernel(dav2_attention_cache_i8_args a, uint32_t splits, uint32_
 #pragma unroll
                         for (int r = 0; r < 16; ++r) o[f][r] *= keep;
                 }
+                if (far) {
+                    // a fused score minus the base would keep bits that the base has lost
+                    stay_in_branch();
+#pragma unroll
+                    for (int t = 0; t < 4; ++t) {
+#pragma unroll
+                        for (int r = 0; r < 8; ++r)
+                            sc[t >> 1][8 * (t & 1) + r] = fmaf(sc[t >> 1][8 * (t & 1) + r], c[t], shift[t]);
+                        c[t] = 1.0f;
+                        shift[t] = 0.0f;
+                    }
+                }
                 // weights of chunk t + 1 between the products of chunk t
                 h8 pf[2][NP];
                 float part = 0.0f;

@@ -1,5 +1,6 @@
 """Softmax weights of the decoder's attention over their whole range: keys far
-below the largest, whose sum is what the output holds. Against float64, with
+below the largest, whose sum is what the output holds, and scores so large that
+their rounding is larger than the exponentials' range. Against float64, with
 bounds that leave a small weight no more than its own rounding."""
 
 import math
@@ -118,3 +119,42 @@ def test_cache_attention_pages_with_a_scale_of_zero(gpu, pkg, lib, dtype, querie
             # a scale of 2^-80, of 1e-24 of the others, stands for zero; its logarithm is rounded to 2^-18
             want, bound = want_of(q[:, h].double(), k, v, 1.0, dtype, step + 2.0 ** -18, floor, exponent=80.0)
             ref.assert_within(out[:, h], want, bound + 127 * 2.0 ** -80)
+
+
+def mean_of_largest(s, v):
+    """The values of the keys with the largest score, in equal parts: what is left where scores lie 10^3 and more apart."""
+    most = (s == s.amax(-1, keepdim=True)).double()
+    return (most / most.sum(-1, keepdim=True)) @ v
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("sign", [1, -1])
+@pytest.mark.parametrize("queries,sequences,most", [(1, 1, 1), (1, 1, 2 ** 22), (40, 512, 127), (40, 1, 2 ** 22)])
+def test_cache_attention_scores_past_2_to_30(gpu, pkg, lib, dtype, sign, queries, sequences, most):
+    # scores of one feature, multiples of 2^24 and more: their rounding in fp32 is larger than what an exponential
+    # bears; ties, which are exact as the pages share a scale, are halved
+    torch = gpu
+    n, page_size, d, heads = 640, 32, 64, 8
+    g = torch.Generator(device="cuda").manual_seed(3)
+    pages = n // page_size
+    keys = torch.zeros((pages, 1, page_size, d), dtype=torch.int8, device="cuda")
+    keys[..., 0] = sign * torch.randint(2, 127, (pages, 1, page_size), generator=g, device="cuda").to(torch.int8)
+    same = torch.tensor([3, 70, 300, 639], device="cuda")
+    keys.view(n, d)[same, 0] = 127 if sign > 0 else -1  # the largest, several times
+    values = torch.randint(-127, 128, (pages, 1, d, page_size), generator=g, dtype=torch.int8, device="cuda")
+    ks = torch.full((pages, 1), 0.7310585786 * 2.0 ** 12, device="cuda")
+    vs = torch.full((pages, 1), 0.0123, device="cuda")
+    q = torch.zeros((queries, heads, d), dtype=ref.DTYPES[dtype], device="cuda")
+    q[..., 0] = (2.0 ** 15 - 2.0 ** 7 * torch.arange(heads, device="cuda")).to(q.dtype)
+    table = torch.arange(pages, device="cuda", dtype=torch.int32).expand(sequences, -1).contiguous()
+    starts, lengths = ints(torch, [0] + [queries] * sequences), ints(torch, [n] + [0] * (sequences - 1))
+    out = torch.full(q.shape, math.nan, dtype=q.dtype, device="cuda")
+    a, keep = attend_args(torch, pkg, lib, [keys, values, ks, vs], q, out, table, starts, lengths, False, dtype, 1.0,
+                          max_length=most)
+    launch(torch, lib, "dav2_hip_attention_cache_i8", a)
+    k, v = keys.view(n, d).double(), values.transpose(2, 3).reshape(n, d).double() * vs[0].double()
+    torch.cuda.synchronize()
+    for h in range(heads):
+        want = mean_of_largest(q[:, h].double() @ k.T, v)
+        bound = want.abs() * (ref.half_step(dtype) + 2.0 ** -10) + v.abs().max() * 2.0 ** -20
+        ref.assert_within(out[:, h], want, bound)
