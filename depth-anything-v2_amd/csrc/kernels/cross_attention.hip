@@ -4,7 +4,10 @@
 // Products run on the matrix cores in the tensors' own type (binary16 and
 // bfloat16: exact products, fp32 sums; fp32: v_mfma_f32_32x32x2_f32). Weights
 // are rounded to that type for the second product (half a step, 2^-11 or 2^-8
-// of each); their sum is taken in fp32 from the unrounded ones.
+// of each); their sum is taken in fp32 from the unrounded ones. Binary16 ends at
+// 2^-24: its weights are formed kBias powers of two larger, which cancels in the
+// quotient, so that against the largest they keep 2^-11 down to 2^-27 and lose
+// at most 2^-38 below.
 //
 // A key mask becomes a list of the keys that a batch sees, made by a kernel
 // of its own before the attention: hidden keys are never loaded, so what they
@@ -109,9 +112,9 @@ struct Tiles {
     static constexpr uint32_t kRow = HEAD * sizeof(E);        // bytes of a key in LDS
     static constexpr uint32_t kChunks = kRow / 16, kRowsPerCopy = 64 / kChunks;
     static constexpr int kCopies = kTile * kRow / (1024 * WAVES);  // of each wave, for the keys and again for the values
-    // rescale when a score passes the running maximum by this: weights stay
-    // below 2^6 and most tiles leave the sums alone
-    static constexpr float kSlack = 6.0f;
+    // rescale when a score passes the running maximum by kSlack: most tiles
+    // leave the sums alone. Weights stay below 2^(kBias + kSlack).
+    static constexpr float kSlack = 2.0f, kBias = std::is_same_v<E, _Float16> ? 13.0f : 0.0f;
     typedef E V __attribute__((ext_vector_type(N)));
 
     // of the workgroup
@@ -124,7 +127,7 @@ struct Tiles {
     float c;
     V qf[KS];       // the right operand of the scores
     v16f o[FB];     // register r of o[f]: feature 32 f + 8 (r / 4) + 4 hf + r % 4 of row col
-    float maximum, sum;  // sum: this lane's keys only
+    float base, sum;  // the running maximum less kBias; sum: this lane's keys only
     V pf[T];
 
     DAV2_DEV Tiles(const dav2_cross_attention_args& args, const Lists& lists, uint32_t plane) : a(args) {
@@ -211,7 +214,7 @@ struct Tiles {
         for (int f = 0; f < FB; ++f)
 #pragma unroll
             for (int r = 0; r < 16; ++r) o[f][r] = 0.0f;
-        maximum = kNoScore;
+        base = kNoScore;
         sum = 0.0f;
     }
 
@@ -281,11 +284,11 @@ struct Tiles {
 #pragma unroll
             for (int r = 0; r < 16; ++r) largest = fmaxf(largest, sc[i][r]);
         largest = over_halves(fmaxf(kNoScore, largest * c), Larger());
-        if (__any(largest > maximum + kSlack)) {
+        if (__any(largest > base + (kBias + kSlack))) {
             stay_in_branch();
-            const float grown = fmaxf(maximum, largest);
-            const float keep = __builtin_amdgcn_exp2f(maximum - grown);
-            maximum = grown;
+            const float moved = fmaxf(base, largest - kBias);
+            const float keep = __builtin_amdgcn_exp2f(base - moved);
+            base = moved;
             sum *= keep;
 #pragma unroll
             for (int f = 0; f < FB; ++f)
@@ -299,7 +302,7 @@ struct Tiles {
 #pragma unroll
             for (int r = 0; r < N; ++r) {
                 const int at = N * t + r;
-                const float w = __builtin_amdgcn_exp2f(fmaf(sc[at >> 4][at & 15], c, -maximum));
+                const float w = __builtin_amdgcn_exp2f(fmaf(sc[at >> 4][at & 15], c, -base));
                 of_step[t] += w;
                 pf[t][r] = static_cast<E>(w);
             }
@@ -375,7 +378,7 @@ struct Tiles {
                     *reinterpret_cast<V4*>(y + feature) = out;
                 }
             }
-        if (splits > 1 && hf == 0) parts.stats[slot] = make_float2(maximum, sum);
+        if (splits > 1 && hf == 0) parts.stats[slot] = make_float2(base, sum);
     }
 };
 

@@ -8,7 +8,7 @@ import math
 import pytest
 
 import decoder_ref as ref
-from test_gpu_decoder import attend_args, ints, launch, rand
+from test_gpu_decoder import attend_args, cross_args, ints, launch, rand
 
 pytestmark = pytest.mark.gpu
 
@@ -158,3 +158,32 @@ def test_cache_attention_scores_past_2_to_30(gpu, pkg, lib, dtype, sign, queries
         want = mean_of_largest(q[:, h].double() @ k.T, v)
         bound = want.abs() * (ref.half_step(dtype) + 2.0 ** -10) + v.abs().max() * 2.0 ** -20
         ref.assert_within(out[:, h], want, bound)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("gap", [12, 16, 18])
+@pytest.mark.parametrize("batch,queries,kv", [(1, 1, 1), (1, 70, 1), (256, 70, 2)])
+@pytest.mark.parametrize("d", [64, 128])
+def test_cross_attention_dominant_key(gpu, pkg, lib, dtype, gap, batch, queries, kv, d):
+    # one batch's keys for all: 512 planes are not split
+    torch = gpu
+    n, heads, at = 16384, 2, 5000
+    q = sink_query(torch, batch * queries, heads, d, dtype, 5).view(batch, queries, heads, d)
+    k = rand(torch, 6, 1, n, kv, d, dtype=dtype, scale=0.2)
+    k[..., 0] = 0
+    k[:, at] = 0
+    k[:, at, :, 0] = gap
+    v = rand(torch, 7, 1, n, kv, d, dtype=dtype).abs() + 0.5
+    v[:, at] = 0
+    out = torch.full(q.shape, math.nan, dtype=q.dtype, device="cuda")
+    a, keep = cross_args(torch, pkg, lib, q, k.expand(batch, -1, -1, -1), v.expand(batch, -1, -1, -1), out, None, None,
+                         dtype, 1.0)
+    launch(torch, lib, "dav2_hip_cross_attention", a)
+    torch.cuda.synchronize()
+    step, floor = {"f32": (2.0 ** -24, 0.0), "f16": (2.0 ** -11, 2.0 ** -37), "bf16": (2.0 ** -8, 0.0)}[dtype]
+    for b in (0, batch - 1):
+        for h in range(heads):
+            head = h * kv // heads
+            want, bound = want_of(q[b, :, h].double(), k[0, :, head].double(), v[0, :, head].double(), 1.0, dtype, step,
+                                  floor)
+            ref.assert_within(out[b, :, h], want, bound)
