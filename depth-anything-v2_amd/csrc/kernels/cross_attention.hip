@@ -128,6 +128,11 @@ struct Tiles {
     V qf[KS];       // the right operand of the scores
     v16f o[FB];     // register r of o[f]: feature 32 f + 8 (r / 4) + 4 hf + r % 4 of row col
     float base, sum;  // the running maximum less kBias; sum: this lane's keys only
+    // The wave has met a maximum past kFar, where fp32 has too few bits for a
+    // bias and a fused score minus base would keep bits that base has lost,
+    // more of them than an exponential bears: base is the maximum itself then.
+    bool far;
+    static constexpr float kFar = 1048576.0f;
     V pf[T];
 
     DAV2_DEV Tiles(const dav2_cross_attention_args& args, const Lists& lists, uint32_t plane) : a(args) {
@@ -216,6 +221,7 @@ struct Tiles {
             for (int r = 0; r < 16; ++r) o[f][r] = 0.0f;
         base = kNoScore;
         sum = 0.0f;
+        far = false;
     }
 
     // A step's pieces are read before the products of the step before, which run
@@ -284,9 +290,11 @@ struct Tiles {
 #pragma unroll
             for (int r = 0; r < 16; ++r) largest = fmaxf(largest, sc[i][r]);
         largest = over_halves(fmaxf(kNoScore, largest * c), Larger());
-        if (__any(largest > base + (kBias + kSlack))) {
+        if (__any(largest > base + (far ? 0.0f : kBias + kSlack))) {
             stay_in_branch();
-            const float moved = fmaxf(base, largest - kBias);
+            const float grown = fmaxf(base + (far ? 0.0f : kBias), largest);
+            far = far || __any(fabsf(grown) >= kFar && grown != kNoScore);
+            const float moved = grown - (far ? 0.0f : kBias);
             const float keep = __builtin_amdgcn_exp2f(base - moved);
             base = moved;
             sum *= keep;
@@ -295,6 +303,15 @@ struct Tiles {
 #pragma unroll
                 for (int r = 0; r < 16; ++r) o[f][r] *= keep;
         }
+        float factor = c;
+        if (far) {
+            stay_in_branch();
+#pragma unroll
+            for (int i = 0; i < kBlocks; ++i)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) sc[i][r] *= c;
+            factor = 1.0f;
+        }
         float of_step[T];
 #pragma unroll
         for (int t = 0; t < T; ++t) {
@@ -302,7 +319,7 @@ struct Tiles {
 #pragma unroll
             for (int r = 0; r < N; ++r) {
                 const int at = N * t + r;
-                const float w = __builtin_amdgcn_exp2f(fmaf(sc[at >> 4][at & 15], c, -base));
+                const float w = __builtin_amdgcn_exp2f(fmaf(sc[at >> 4][at & 15], factor, -base));
                 of_step[t] += w;
                 pf[t][r] = static_cast<E>(w);
             }

@@ -187,3 +187,38 @@ def test_cross_attention_dominant_key(gpu, pkg, lib, dtype, gap, batch, queries,
             want, bound = want_of(q[b, :, h].double(), k[0, :, head].double(), v[0, :, head].double(), 1.0, dtype, step,
                                   floor)
             ref.assert_within(out[b, :, h], want, bound)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("sign", [1, -1])
+@pytest.mark.parametrize("batch,queries,masked", [(1, 1, False), (3, 70, False), (64, 70, False), (2, 300, True)])
+@pytest.mark.parametrize("d", [64, 128])
+def test_cross_attention_scores_past_2_to_30(gpu, pkg, lib, dtype, sign, batch, queries, masked, d):
+    # as over the cache: multiples of 2^30
+    torch = gpu
+    n, heads = 700, 8
+    g = torch.Generator(device="cuda").manual_seed(3)
+    k = torch.zeros((batch, n, heads, d), device="cuda")
+    k[..., 0] = sign * torch.randint(2, 127, (batch, n, heads), generator=g, device="cuda") * 2.0 ** 15 / 128
+    same = torch.tensor([3, 70, 300, 699], device="cuda")
+    k[:, same, :, 0] = (127 if sign > 0 else -1) * 2.0 ** 15 / 128  # the largest, several times
+    k = k.to(ref.DTYPES[dtype])
+    k[..., 1:4] = k[..., :1]
+    v = rand(torch, 7, batch, n, heads, d, dtype=dtype)
+    q = torch.zeros((batch, queries, heads, d), dtype=k.dtype, device="cuda")
+    q[..., :4] = (2.0 ** 15 - 2.0 ** 8 * torch.arange(heads, device="cuda"))[:, None].to(k.dtype)
+    mask = torch.ones((batch, n), dtype=torch.uint8, device="cuda") if masked else None
+    if masked:
+        mask[:, 70] = mask[:, 300:400] = 0
+    out = torch.full(q.shape, math.nan, dtype=q.dtype, device="cuda")
+    a, keep = cross_args(torch, pkg, lib, q, k, v, out, None, mask, dtype, 1.0)
+    launch(torch, lib, "dav2_hip_cross_attention", a)
+    torch.cuda.synchronize()
+    for b in range(batch):
+        for h in range(heads):
+            s = q[b, :, h].double() @ k[b, :, h].double().T
+            if masked:
+                s = s.masked_fill(mask[b] == 0, -math.inf)
+            want = mean_of_largest(s, v[b, :, h].double())
+            bound = want.abs() * (ref.half_step(dtype) + 2.0 ** -8) + v[b, :, h].abs().max().double() * 2.0 ** -20
+            ref.assert_within(out[b, :, h], want, bound)
