@@ -55,6 +55,8 @@ __global__ __launch_bounds__(256, 8) void cache_store_kernel(dav2_cache_store_i8
     const int64_t origin = static_cast<int64_t>(q.length) - (q.end - q.begin);  // row r has position origin + r - begin
     const int64_t first = max(origin, int64_t(0));
     const int64_t last = min(static_cast<int64_t>(q.length), static_cast<int64_t>(a.table_pages) * page_size);
+    // nothing new: the page that the next token goes to is left alone, it may be another sequence's by now
+    if (first >= last) return;
     const uint64_t stride = side ? a.value_stride : a.key_stride;
     const E* x = static_cast<const E*>(side ? a.values : a.keys) + static_cast<uint64_t>(h) * d;
     for (int64_t p = first / page_size + blockIdx.x; p * page_size < last; p += gridDim.x) {
