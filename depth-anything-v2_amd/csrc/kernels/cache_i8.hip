@@ -1008,9 +1008,10 @@ int dav2_hip_cache_store_i8(const dav2_cache_store_i8_args* args, void* stream) 
         a.table_pages > 0x7fffffffu || (a.tokens > 1 && (a.key_stride < row || a.value_stride < row)))
         return hipErrorInvalidValue;
     const uint64_t new_most = a.max_new < a.tokens ? a.max_new : a.tokens;
-    uint64_t touched = (new_most + a.cache.page_size - 2) / a.cache.page_size + 1;
-    if (touched > a.table_pages) touched = a.table_pages;
-    const dim3 grid(static_cast<uint32_t>(touched), 2 * a.cache.kv_heads, a.sequences);
+    const uint64_t touched = (new_most + a.cache.page_size - 2) / a.cache.page_size + 1;
+    constexpr uint64_t kMostPages = 1u << 22;  // workgroups along x: threads of a launch stay below 2^32
+    const dim3 grid(static_cast<uint32_t>(std::min<uint64_t>({touched, a.table_pages, kMostPages})), 2 * a.cache.kv_heads,
+                    a.sequences);
     const uint64_t size = dtype_bytes(a.dtype);
     const bool aligned = aligned16(a.keys) && aligned16(a.values) && a.key_stride * size % 16 == 0 &&
                          a.value_stride * size % 16 == 0;

@@ -56,3 +56,23 @@ def test_store_beside_idle_sequences(gpu, pkg, lib, dtype):
     torch.cuda.synchronize()
     for got, w in zip(cache, want):
         assert torch.equal(got.cpu(), w)
+
+
+def test_store_of_more_pages_than_a_launch_has(gpu, pkg, lib):
+    # room for 2^29 new tokens in pages of 16; five come, at the end of a table of 2^25 pages
+    torch = gpu
+    tokens, d = 1 << 29, 16
+    cache = random_cache(torch, 3, 4, 1, 16, d)
+    small = [t.clone() for t in cache]
+    rows = torch.empty((tokens, 1, d), dtype=torch.float16, device="cuda")
+    rows[:5] = rand(torch, 1, 5, 1, d, dtype="f16", scale=2.0)
+    table = torch.full((1, 1 << 25), 2, dtype=torch.int32, device="cuda")
+    table[0, -1] = 1
+    starts = ints(torch, [0, 5])
+    launch(torch, lib, "dav2_hip_cache_store_i8",
+           store_args(pkg, cache, rows, rows, table, starts, ints(torch, [tokens - 3]), tokens, "f16"))
+    launch(torch, lib, "dav2_hip_cache_store_i8",
+           store_args(pkg, small, rows[:5], rows[:5], ints(torch, [[2, 1]]), starts, ints(torch, [29]), 5, "f16"))
+    torch.cuda.synchronize()
+    for a, b in zip(cache, small):
+        assert torch.equal(a, b)
