@@ -28,7 +28,7 @@ struct Lists {
     uint32_t* counts;  // [batch]
 };
 uint64_t list_bytes(const dav2_cross_attention_args& a) {
-    if (!a.key_mask) return 0;
+    if (a.key_tokens == 0) return 0;
     return ((static_cast<uint64_t>(a.batch) * a.key_tokens + a.batch) * sizeof(uint32_t) + 15u) & ~uint64_t(15);
 }
 
@@ -505,6 +505,14 @@ uint64_t split_bytes(const dav2_cross_attention_args& a, const Plan& p) {
 
 }  // namespace
 
+// dav2_hip_cross_attention_scratch_bytes() goes by the sizes alone and always
+// has room for a mask's lists; this is whether a call touches it.
+namespace dav2k {
+bool cross_attention_uses_scratch(const dav2_cross_attention_args& a) {
+    return plan_of(a).splits > 1 || (a.key_mask && a.key_tokens);
+}
+}  // namespace dav2k
+
 extern "C" {
 
 uint64_t dav2_hip_cross_attention_scratch_bytes(const dav2_cross_attention_args* args) {
@@ -528,8 +536,9 @@ int dav2_hip_cross_attention(const dav2_cross_attention_args* args, void* stream
         (a.query_tokens > 1 && (a.query_stride < row || a.output_stride < row)) ||
         (a.key_tokens > 1 && (a.key_stride < key_row || a.value_stride < key_row)))
         return hipErrorInvalidValue;
-    const uint64_t need = dav2_hip_cross_attention_scratch_bytes(args);
-    if (need && (!a.scratch || !aligned16(a.scratch) || a.scratch_bytes < need)) return hipErrorInvalidValue;
+    if (cross_attention_uses_scratch(a) && (!a.scratch || !aligned16(a.scratch) ||
+                                            a.scratch_bytes < dav2_hip_cross_attention_scratch_bytes(args)))
+        return hipErrorInvalidValue;
     const hipStream_t s = static_cast<hipStream_t>(stream);
     const Plan p = plan_of(a);
     Lists lists{nullptr, nullptr};

@@ -8,6 +8,10 @@
 #include <stdexcept>
 #include <string>
 
+namespace dav2k {
+bool cross_attention_uses_scratch(const dav2_cross_attention_args& a);  // kernels/cross_attention.hip
+}
+
 namespace dav2 {
 namespace {
 
@@ -1196,7 +1200,8 @@ void HipOperators::cross_attention(DeviceBuffer& output, const DeviceBuffer& que
     a.values = values.data();
     a.key_lengths = key_lengths.as<std::int32_t>();
     a.key_mask = key_mask.as<std::uint8_t>();
-    a.scratch = attention_scratch(scratch, dav2_hip_cross_attention_scratch_bytes(&a), a.scratch_bytes);
+    const std::uint64_t need = dav2k::cross_attention_uses_scratch(a) ? dav2_hip_cross_attention_scratch_bytes(&a) : 0;
+    a.scratch = attention_scratch(scratch, need, a.scratch_bytes);
     ProfileScope prof(context_.profiler(), "cross_attention",
                       4.0 * row * a.query_tokens * double(a.batch) * a.key_tokens, "FLOP", stream());
     launch_check(dav2_hip_cross_attention(&a, stream()), "cross attention");

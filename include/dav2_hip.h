@@ -620,7 +620,9 @@ DAV2_API int dav2_hip_attention_cache_i8(const dav2_attention_cache_i8_args* arg
  * elements, multiples of 8; the four tensors 16-byte aligned; output overlaps
  * no input. batch stays below 2^16, batch * query_tokens * heads below
  * 2^32 - 256, batch * kv_heads below 2^23. scratch as for
- * dav2_hip_attention_cache_i8. */
+ * dav2_hip_attention_cache_i8; its size goes by the sizes alone, a key mask's
+ * part included. A call without a mask whose keys are not split touches none
+ * and may leave it NULL. */
 typedef struct dav2_cross_attention_args {
     const void* query;           /* [batch][query_tokens][heads][head_dim]         */
     const void* keys;            /* [batch][key_tokens][kv_heads][head_dim]        */

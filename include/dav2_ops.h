@@ -230,7 +230,8 @@ DAV2_API dav2_status DAV2_CALL dav2_ops_attention_cache_int8(dav2_ops* ops, dav2
                                                              dav2_device_buffer lengths, dav2_device_buffer scratch,
                                                              const dav2_attention_cache_i8_args* sizes);
 /* key_lengths (batch int32) and key_mask (batch x key_tokens bytes) may be
- * left out; scratch as above, dav2_hip_cross_attention_scratch_bytes(). */
+ * left out; scratch as above, dav2_hip_cross_attention_scratch_bytes(sizes),
+ * which is enough with a mask and without. */
 DAV2_API dav2_status DAV2_CALL dav2_ops_cross_attention(dav2_ops* ops, dav2_device_buffer output,
                                                         dav2_device_buffer query, dav2_device_buffer keys,
                                                         dav2_device_buffer values, dav2_device_buffer key_lengths,

@@ -8,7 +8,8 @@ import math
 import pytest
 
 import decoder_ref as ref
-from test_gpu_decoder import ints, launch, ptr, rand, random_cache, store_args
+from gpu_util import db
+from test_gpu_decoder import cross_args, ints, launch, ops, rand, random_cache, store_args, surface  # noqa: F401
 
 pytestmark = pytest.mark.gpu
 
@@ -76,3 +77,73 @@ def test_store_of_more_pages_than_a_launch_has(gpu, pkg, lib):
     torch.cuda.synchronize()
     for a, b in zip(cache, small):
         assert torch.equal(a, b)
+
+
+# ---- cross attention through the surface -------------------------------------------------
+
+
+def cross_case(torch, pkg, lib, dtype, queries, keys, masked=True, batch=3, heads=4, kv=2, d=64):
+    """Tensors of a call, its buffers in the surface's order without scratch, and a block without pointers."""
+    q = rand(torch, 1, batch, queries, heads, d, dtype=dtype)
+    k, v = (rand(torch, i, batch, keys, kv, d, dtype=dtype) for i in (2, 3))
+    mask = (torch.rand((batch, keys), device="cuda") < 0.5).to(torch.uint8) if masked else None
+    out = torch.full_like(q, math.nan)
+    a, _ = cross_args(torch, pkg, lib, q, k, v, out, None, None, dtype, 0.125)
+    for name, kind in a._fields_:
+        if kind is C.c_void_p:
+            setattr(a, name, None)
+    a.scratch_bytes = 0
+    buffers = [db(pkg, t) for t in (out, q, k, v, None, mask)]
+    want, bound = ref.cross(q, k, v, None, mask, 0.125, dtype)
+    torch.cuda.synchronize()
+    return (q, k, v, mask), out, buffers, a, want, bound
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("queries,keys", [(1, 1370), (600, 200), (5, 0)])
+def test_surface_mask_with_scratch_of_a_bare_block(gpu, pkg, lib, ops, dtype, queries, keys):  # noqa: F811
+    torch = gpu
+    held, out, buffers, a, want, bound = cross_case(torch, pkg, lib, dtype, queries, keys)
+    need = lib.dav2_hip_cross_attention_scratch_bytes(C.byref(a))
+    scratch = torch.full((max(need, 1),), 255, dtype=torch.uint8, device="cuda")
+    for given in (db(pkg, scratch, need), db(pkg, None)):
+        out.fill_(math.nan)
+        torch.cuda.synchronize()
+        surface(lib, lib.dav2_ops_cross_attention(ops, *buffers, given, C.byref(a)))
+        surface(lib, lib.dav2_ops_synchronize(ops))
+        ref.assert_within(out, want, bound)
+    if need:
+        assert lib.dav2_ops_cross_attention(ops, *buffers, db(pkg, scratch, need - 1), C.byref(a)) == 1
+        assert b"scratch" in lib.dav2_ops_last_error()
+
+
+def test_surface_mask_captured(gpu, pkg, lib, ops):  # noqa: F811
+    # a mask or split keys under capture bring a scratch; a call that touches none needs none
+    torch = gpu
+    masked = cross_case(torch, pkg, lib, "f16", 1, 1370)
+    whole = cross_case(torch, pkg, lib, "bf16", 300, 60, masked=False)
+    need = lib.dav2_hip_cross_attention_scratch_bytes(C.byref(masked[3]))
+    scratch = torch.empty(need, dtype=torch.uint8, device="cuda")
+    stream = torch.cuda.ExternalStream(lib.dav2_ops_stream(ops))
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=stream):
+        refused = lib.dav2_ops_cross_attention(ops, *masked[2], db(pkg, None), C.byref(masked[3]))
+        text = lib.dav2_ops_last_error()
+        rc = [lib.dav2_ops_cross_attention(ops, *masked[2], db(pkg, scratch), C.byref(masked[3])),
+              lib.dav2_ops_cross_attention(ops, *whole[2], db(pkg, None), C.byref(whole[3]))]
+    assert refused == 1 and b"scratch" in text and rc == [0, 0]
+    for replay in range(4):
+        for case in (masked, whole):
+            case[1].fill_(math.nan)
+        scratch.fill_(255)
+        torch.cuda.synchronize()
+        with torch.cuda.stream(stream):
+            graph.replay()
+        torch.cuda.synchronize()
+        for case in (masked, whole):
+            ref.assert_within(case[1], case[4], case[5], str(replay))
+        eager = torch.full_like(masked[1], math.nan)
+        torch.cuda.synchronize()
+        surface(lib, lib.dav2_ops_cross_attention(ops, db(pkg, eager), *masked[2][1:], db(pkg, None), C.byref(masked[3])))
+        surface(lib, lib.dav2_ops_synchronize(ops))
+        assert torch.equal(eager, masked[1])
