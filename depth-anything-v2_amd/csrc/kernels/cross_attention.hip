@@ -489,7 +489,8 @@ Plan plan_of(const dav2_cross_attention_args& a) {
     Plan p{128, 1, 1};
     if (a.kv_heads == 0 || a.heads < a.kv_heads || a.batch == 0 || a.query_tokens == 0) return p;
     const uint64_t rows = static_cast<uint64_t>(a.query_tokens) * (a.heads / a.kv_heads);
-    const uint64_t planes = static_cast<uint64_t>(a.kv_heads) * a.batch;
+    // a call's planes are below 2^23; sizes that no call has may not overflow below
+    const uint64_t planes = std::min<uint64_t>(static_cast<uint64_t>(a.kv_heads) * a.batch, 1u << 23);
     const uint64_t most = std::clamp<uint64_t>(a.key_tokens / (a.dtype == DAV2_DTYPE_F32 ? 64 : 128), 1, kMostSplits);
     if (a.head_dim > 64 && a.dtype != DAV2_DTYPE_F32 && (rows + 127) / 128 % 2 == 0 &&
         (rows + 255) / 256 * planes * most >= 256)
