@@ -208,7 +208,11 @@ __global__ __launch_bounds__(256) void rotary_lanes_kernel(dav2_qk_norm_rotary_a
 #pragma unroll
                         for (int i = 0; i < static_cast<int>(U); ++i) squares = fmaf(v[i], v[i], squares);
                         if (!active) squares = 0.0f;
-                        const float factor = __builtin_amdgcn_rsqf(sum_lanes<LANES>(squares) * share + a.epsilon);
+                        const float variance = sum_lanes<LANES>(squares) * share + a.epsilon;
+                        // the instruction takes a subnormal number for zero
+                        const bool small = variance < 0x1p-100f;
+                        const float factor = __builtin_amdgcn_rsqf(small ? variance * 0x1p64f : variance) *
+                                             (small ? 0x1p32f : 1.0f);
 #pragma unroll
                         for (int i = 0; i < static_cast<int>(U); ++i) v[i] *= factor * w[i];
                     }

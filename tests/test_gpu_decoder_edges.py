@@ -9,7 +9,8 @@ import pytest
 
 import decoder_ref as ref
 from gpu_util import db
-from test_gpu_decoder import cross_args, ints, launch, ops, rand, random_cache, store_args, surface  # noqa: F401
+from test_gpu_decoder import (cross_args, ints, launch, ops, qk_args, qk_want, rand, random_cache,  # noqa: F401
+                              store_args, surface)
 
 pytestmark = pytest.mark.gpu
 
@@ -77,6 +78,33 @@ def test_store_of_more_pages_than_a_launch_has(gpu, pkg, lib):
     torch.cuda.synchronize()
     for a, b in zip(cache, small):
         assert torch.equal(a, b)
+
+
+# ---- norms ------------------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("norm", ["rms", "layer"])
+@pytest.mark.parametrize("head_dim", [64, 33])
+@pytest.mark.parametrize("epsilon", [1e-40, 1.2e-38, 1e-30])
+def test_norm_near_the_ends_of_fp32(gpu, pkg, lib, dtype, norm, head_dim, epsilon):
+    # an epsilon that is subnormal in fp32, heads of zeros and of 1e-18 and 1e17 beside it
+    torch = gpu
+    epsilon = float(torch.tensor(epsilon, dtype=torch.float32))
+    q = rand(torch, 1, 6, 2, head_dim, dtype=dtype)
+    q[0] = 0.0
+    q[1:3] *= 1e-18
+    q[3:5] *= 1e17
+    k = q.flip(0).contiguous()
+    w = 1 + 0.3 * rand(torch, 2, head_dim)
+    positions, freq = ints(torch, [0] * 6), None
+    q_out, k_out = torch.full_like(q, math.nan), torch.full_like(k, math.nan)
+    launch(torch, lib, "dav2_hip_qk_norm_rotary",
+           qk_args(pkg, q, k, q_out, k_out, w, w, positions, freq, 0, "halves", norm, dtype, epsilon))
+    torch.cuda.synchronize()
+    for x, out in ((q, q_out), (k, k_out)):
+        want, bound = qk_want(x, w, norm, epsilon, positions, freq, 0, "halves", dtype)
+        ref.assert_within(out, want, bound)
 
 
 # ---- cross attention through the surface -------------------------------------------------
