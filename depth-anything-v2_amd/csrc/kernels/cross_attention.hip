@@ -535,6 +535,7 @@ int dav2_hip_cross_attention(const dav2_cross_attention_args* args, void* stream
         a.head_dim > 128 || a.head_dim % 16 || static_cast<uint64_t>(a.batch) * a.kv_heads > 0x7fffffull ||
         static_cast<uint64_t>(a.query_tokens) * a.heads > 0xffffff00ull / a.batch ||
         (a.query_tokens > 1 && (a.query_stride < row || a.output_stride < row)) ||
+        (a.batch > 1 && a.output_batch_stride < row) ||
         (a.key_tokens > 1 && (a.key_stride < key_row || a.value_stride < key_row)))
         return hipErrorInvalidValue;
     if (cross_attention_uses_scratch(a) && (!a.scratch || !aligned16(a.scratch) ||

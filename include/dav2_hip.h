@@ -617,8 +617,9 @@ DAV2_API int dav2_hip_attention_cache_i8(const dav2_attention_cache_i8_args* arg
  * what is not seen may hold anything, NaN included. A batch that sees nothing
  * gives zeros. heads is a multiple of kv_heads; head h reads key head
  * h / (heads / kv_heads). head_dim a multiple of 16 up to 128; strides in
- * elements, multiples of 8; the four tensors 16-byte aligned; output overlaps
- * no input. batch stays below 2^16, batch * query_tokens * heads below
+ * elements, multiples of 8, those of the inputs between batches may be 0; the
+ * four tensors 16-byte aligned; output overlaps no input, nor a batch's output
+ * another's. batch stays below 2^16, batch * query_tokens * heads below
  * 2^32 - 256, batch * kv_heads below 2^23. scratch as for
  * dav2_hip_attention_cache_i8; its size goes by the sizes alone, a key mask's
  * part included. A call without a mask whose keys are not split touches none
