@@ -114,7 +114,8 @@ struct Tiles {
     static constexpr int kCopies = kTile * kRow / (1024 * WAVES);  // of each wave, for the keys and again for the values
     // rescale when a score passes the running maximum by kSlack: most tiles
     // leave the sums alone. Weights stay below 2^(kBias + kSlack).
-    static constexpr float kSlack = 2.0f, kBias = std::is_same_v<E, _Float16> ? 13.0f : 0.0f;
+    static constexpr bool kHalf = std::is_same_v<E, _Float16>;
+    static constexpr float kSlack = kHalf ? 2.0f : 6.0f, kBias = kHalf ? 13.0f : 0.0f;
     typedef E V __attribute__((ext_vector_type(N)));
 
     // of the workgroup
