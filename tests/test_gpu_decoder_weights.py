@@ -222,3 +222,29 @@ def test_cross_attention_scores_past_2_to_30(gpu, pkg, lib, dtype, sign, batch, 
             want = mean_of_largest(s, v[b, :, h].double())
             bound = want.abs() * (ref.half_step(dtype) + 2.0 ** -8) + v[b, :, h].abs().max().double() * 2.0 ** -20
             ref.assert_within(out[b, :, h], want, bound)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("length", [1, 2, 9, 68, 1580])
+@pytest.mark.parametrize("d", [64, 128])
+def test_cache_attention_of_single_tokens_rounds_once(gpu, pkg, lib, dtype, length, d):
+    # few rows: weights of 22 bits and more for every type, so that the output's own rounding is what is left
+    torch = gpu
+    page_size, heads = 32, 16
+    pages = -(-length // page_size)
+    g = torch.Generator(device="cuda").manual_seed(length + d)
+    keys = torch.randint(-127, 128, (pages, 2, page_size, d), generator=g, dtype=torch.int8, device="cuda")
+    values = torch.randint(-127, 128, (pages, 2, d, page_size), generator=g, dtype=torch.int8, device="cuda")
+    ks, vs = (0.005 + 0.02 * torch.rand((pages, 2), generator=g, device="cuda") for _ in range(2))
+    table = torch.arange(pages, device="cuda", dtype=torch.int32)[None]
+    q = rand(torch, 8, 2, heads, d, dtype=dtype)
+    out = torch.full_like(q, math.nan)
+    a, keep = attend_args(torch, pkg, lib, [keys, values, ks, vs], q, out, table, ints(torch, [0, 2]),
+                          ints(torch, [length]), False, dtype, 0.125)
+    launch(torch, lib, "dav2_hip_attention_cache_i8", a)
+    torch.cuda.synchronize()
+    for h in range(heads):
+        k = (keys[:, h // 8].double() * ks[:, h // 8].double()[:, None, None]).reshape(-1, d)[:length]
+        v = (values[:, h // 8].double() * vs[:, h // 8].double()[:, None, None]).transpose(1, 2).reshape(-1, d)[:length]
+        want, bound = want_of(q[:, h].double(), k, v, 0.125, dtype, 2.0 ** -22, 2.0 ** -47, exponent=8.0)
+        ref.assert_within(out[:, h], want, bound)
