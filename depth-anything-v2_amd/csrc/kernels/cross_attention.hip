@@ -150,8 +150,8 @@ struct Tiles {
         count = __builtin_amdgcn_readfirstlane(LISTED ? lists.counts[b] : length_of(a, b));
         keys = static_cast<const E*>(a.keys) + b * a.key_batch_stride + static_cast<uint64_t>(h) * D;
         values = static_cast<const E*>(a.values) + b * a.value_batch_stride + static_cast<uint64_t>(h) * D;
-        // not 0, for -infinity times it has to stay what it is
-        c = a.scale == 0.0f ? 1.0e-37f : fabsf(a.scale) * kLog2e;
+        // not 0, for -infinity times it has to stay what it is: the query is zeros then
+        c = a.scale == 0.0f ? 1.0f : fabsf(a.scale) * kLog2e;
     }
 
     // Copies: this wave's copy i brings rows kRowsPerCopy (kCopies wave + i) ..;
@@ -215,6 +215,7 @@ struct Tiles {
         for (int k = 0; k < KS; ++k) {
             qf[k] = *reinterpret_cast<const V*>(x + 2 * N * k);
             if (a.scale < 0.0f) qf[k] = -qf[k];
+            if (a.scale == 0.0f) qf[k] *= static_cast<E>(0.0f);
         }
 #pragma unroll
         for (int f = 0; f < FB; ++f)

@@ -248,3 +248,22 @@ def test_cache_attention_of_single_tokens_rounds_once(gpu, pkg, lib, dtype, leng
         v = (values[:, h // 8].double() * vs[:, h // 8].double()[:, None, None]).transpose(1, 2).reshape(-1, d)[:length]
         want, bound = want_of(q[:, h].double(), k, v, 0.125, dtype, 2.0 ** -22, 2.0 ** -47, exponent=8.0)
         ref.assert_within(out[:, h], want, bound)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("queries", [1, 70])
+def test_cross_attention_scale_of_zero(gpu, pkg, lib, dtype, queries):
+    # the mean of the values, however large the products are; what is not finite stays so
+    torch = gpu
+    q, k, v = (rand(torch, i, 2, n, 2, 64, dtype=dtype) for i, n in ((1, queries), (2, 333), (3, 333)))
+    q, k = q * 1e18, k * 1e18
+    q[1, 0, 1, 5] = math.nan
+    out = torch.zeros_like(q)
+    a, keep = cross_args(torch, pkg, lib, q, k, v, out, None, None, dtype, 0.0)
+    launch(torch, lib, "dav2_hip_cross_attention", a)
+    torch.cuda.synchronize()
+    want = v.double().mean(1, keepdim=True).expand(q.shape).clone()
+    want[1, 0, 1] = math.nan
+    size = v.double().abs().mean(1, keepdim=True)
+    # weights of one are exact; sums of 333 values in fp32
+    ref.assert_within(out, want, size * 333 * ref.U + want.abs() * ref.half_step(dtype))
