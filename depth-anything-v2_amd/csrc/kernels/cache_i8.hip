@@ -39,8 +39,9 @@ DAV2_DEV uint32_t byte_of(uint32_t word, uint32_t i, int code) {
 // a thread) and values take from the caches: their pages are feature-major, so
 // a thread needs 16 tokens of one 4-byte piece of features. Codes are written
 // 16 at a time; a value chunk that also holds older or later tokens is read,
-// changed and written back. Bound by memory: 8 prompts of up to 2048 tokens, 8
-// heads of 128, f16 (55 MB): 30 us, 1.8 TB/s.
+// changed and written back. 8 prompts of up to 2048 tokens, 8 heads of 128, f16
+// (55 MB): 30 us, 1.8 TB/s, a third of a copy's rate: the vector units are busy
+// for half of it, the waves wait for loads and stores for two thirds.
 template <typename E, bool ALIGNED>
 __global__ __launch_bounds__(256, 8) void cache_store_kernel(dav2_cache_store_i8_args a) {
     constexpr int kKept = 1;
@@ -535,11 +536,13 @@ __global__ __launch_bounds__(256, 2) void cache_rows_kernel(dav2_attention_cache
 // all waves on their way into LDS (two buffers, one barrier for a tile; the
 // next tile's codes are in registers meanwhile, its places in the table a tile
 // before). Two prompts' last 2048 of up to 8192 tokens, 32 heads of 8, 128
-// features, f16: 441 us, 717 TFLOP/s; 8 times 512 of 4096 770 TFLOP/s; every
-// row all keys 820. A tile shared by eight waves instead of four is worth 10 %
+// features, f16: 451 us, 700 TFLOP/s; 8 times 512 of 4096 750 TFLOP/s; every
+// row all keys 800. A tile shared by eight waves instead of four is worth 10 %
 // there, the staging and the exponentials written between the matrix
 // instructions 8 %. Heads of 64 are held to registers for three waves a SIMD:
-// 16 prompts' last 300 of up to 2048 tokens 74 us, 83 with four registers more.
+// 16 prompts' last 300 of up to 2048 tokens 76 us, 12 % more with four registers
+// more. A slack of 6 with a smaller bias (see above) is 1 % faster, the fp32
+// mode without its factor of 2^11 5 to 9 %.
 //
 // S^T = K Q^T and O^T = V^T P^T on v_mfma_f32_32x32x16_f16. Lane l holds, for
 // query l % 32, the scores of keys 8 (r / 4) + 4 (l / 32) + r % 4 of a 32-key
@@ -943,9 +946,12 @@ bool valid(const dav2_attention_cache_i8_args& a) {
 // How a call is dealt out. cache_rows_kernel for up to 32 rows of a cache head,
 // or little work: the tiles of cache_tiles_kernel have four times its latency,
 // but do the same work in less than two thirds of the time where they fill the
-// chip. us, rows against tiles (32 or 16 heads): 32 rows, 8 sequences of 2048
-// keys 26 / 29; 64 rows, 8 of 4096 (2^26) 23 / 27; 128 rows, 2 of 8192 (2^26)
-// 19 / 25; 72 rows, 32 of 1500 (2^27) 36 / 31; 100 rows, 8 of 4096 (2^28) 52 / 39.
+// chip. us, rows against tiles, bf16, causal: 32 rows of 8 cache heads of 128, 8
+// sequences of 2048 keys 21 / 25; 64 rows of 4 of 128, 8 of 4096 (2^26) 25 / 31;
+// 128 rows of 8 of 64, 2 of 8192 (2^26) 22 / 25; 72 rows of 4 of 128, 32 of 1500
+// (2^27) 37 / 32; 100 rows of 16 of 64, 8 of 4096 (2^28) 58 / 41.
+// The figures below are from before the weights' bias and second part, which
+// cost both sides alike: tiles 2 %, rows 1 to 10 %.
 //
 // cache_rows_kernel: two workgroups share a CU, so up to 512 all run at once:
 // split the keys as far as that goes, down to 128 keys (two waves' blocks) each.

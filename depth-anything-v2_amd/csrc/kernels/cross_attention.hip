@@ -406,16 +406,17 @@ struct Tiles {
 //
 // Bound by the matrix cores and, as long again in 16 bits, the exponentials of
 // the vector units beside them: 8 x 2048 queries of 32 heads of 128 on 4096
-// keys of 8, bf16, 1.15 ms, 956 TFLOP/s, where a large library product runs at
-// 1190 (four waves 1.20 ms); heads of 64 750. fp32: 129 TFLOP/s of 152 at 8 x
-// 1024 queries, 16 heads of 64, 4096 keys; 82 at 2 x 577 queries and 1370 keys,
-// where 160 workgroups are split in three. Tried and not kept: eight waves in
-// two groups that multiply and weigh in turns (barriers between; no
-// difference), a tile's scores one tile ahead among the exponentials (spills),
-// a step's exponentials between the products of the step before (556 -> 563 us
-// at a masked case of 8 prompts), tiles through registers (575 -> 610 us),
-// workgroups of one wave for up to 32 rows (one query each, 1370 keys, 16 heads
-// of 64: 16 in fp32 57 -> 48 us, but 4 in f16 10.3 -> 11.4, 16 20.9 -> 22.7).
+// keys of 8, bf16, 1.12 ms, 980 TFLOP/s, where a large library product runs at
+// 1190 (four waves 4 % more); f16 1.18 ms, whose weights take a bias; heads of
+// 64 in f16 740. fp32: 129 TFLOP/s of 152 at 8 x 1024 queries, 16 heads of 64,
+// 4096 keys; 82 at 2 x 577 queries and 1370 keys, where 160 workgroups are
+// split in three. Tried and not kept: eight waves in two groups that multiply
+// and weigh in turns (barriers between; no difference), a tile's scores one
+// tile ahead among the exponentials (spills), a step's exponentials between the
+// products of the step before (556 -> 563 us at a masked case of 8 prompts),
+// tiles through registers (575 -> 610 us), workgroups of one wave for up to 32
+// rows (one query each, 1370 keys, 16 heads of 64: 16 in fp32 57 -> 48 us, but
+// 4 in f16 10.3 -> 11.4, 16 20.9 -> 22.7).
 template <typename E, int D, bool LISTED, int WAVES>
 __global__ __launch_bounds__(64 * WAVES, 2)
 void cross_tiles_kernel(dav2_cross_attention_args a, Lists lists, uint32_t splits, uint32_t tiles) {

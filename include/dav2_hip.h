@@ -480,7 +480,9 @@ DAV2_API int dav2_hip_finish_tokens(float* tokens, const float* interpolated,
 /* ---- operators of a decoder behind the encoder (no reference counterpart) ----
  *
  * Element types of their activations; sums, norms and softmax statistics are
- * fp32 whatever the type, and a result is rounded once. */
+ * fp32 whatever the type. A result is rounded once; the attentions also round
+ * the softmax's weights on their way into the product with the values, as each
+ * says below. */
 enum { DAV2_DTYPE_F32 = 0, DAV2_DTYPE_F16 = 1, DAV2_DTYPE_BF16 = 2 };
 
 /* Which features of a head form a rotated pair: i and i + rotary_dim/2
@@ -509,7 +511,8 @@ typedef struct dav2_rotary_args {
 DAV2_API int dav2_hip_rotary(const dav2_rotary_args* args, void* stream);
 
 /* Norm of a head: x / sqrt(mean(x^2) + epsilon) * weight (RMS), or
- * (x - mean) / sqrt(variance + epsilon) * weight (LAYER). */
+ * (x - mean) / sqrt(variance + epsilon) * weight (LAYER). There is no bias. The
+ * squares of a head's features are summed in fp32: the sum stays below 2^128. */
 enum { DAV2_QK_NORM_RMS = 0, DAV2_QK_NORM_LAYER = 1 };
 
 /* The norm of every query head and every key head over its head_dim
@@ -563,8 +566,10 @@ typedef struct dav2_cache_i8 {
  * infinity makes the scale of its page NaN or infinite, and with it the
  * page's values, until the page is begun anew. starts must not decrease; rows
  * outside [0, tokens) and positions outside the table are not stored. Pages
- * that get tokens must belong to one sequence only. Other bytes of the cache
- * are left as they were. sequences stays below 2^16. */
+ * that get tokens must belong to one sequence only, once; a sequence without
+ * new rows may name any. Other bytes of the cache are left as they were.
+ * max_new 0 says that nothing is new: nothing is stored. sequences stays below
+ * 2^16. */
 typedef struct dav2_cache_store_i8_args {
     dav2_cache_i8 cache;
     const void* keys;            /* [tokens][kv_heads][head_dim]                   */
@@ -579,20 +584,27 @@ typedef struct dav2_cache_store_i8_args {
 } dav2_cache_store_i8_args;
 DAV2_API int dav2_hip_cache_store_i8(const dav2_cache_store_i8_args* args, void* stream);
 
-/* softmax(scale * q k^T) v over a cache: query rows starts[s] .. starts[s+1]
- * are the last tokens of sequence s, of lengths[s] tokens in all. causal: row
- * i of n sees the first lengths[s] - n + 1 + i tokens; otherwise all. heads is
- * a multiple of kv_heads; head h reads head h / (heads / kv_heads) of the
- * cache. A row that sees nothing gives zeros; output rows of no sequence are
- * left as they were. Scales of pages are not negative. tokens * heads stays
- * below 2^32 - 512, sequences * kv_heads below 2^23, sequences below 2^16.
- * Strides (elements between tokens) are multiples of 8, query and output
- * 16-byte aligned; output overlaps no input. max_query and max_length, the
- * most new and the most tokens of a sequence, size the launch and the scratch;
- * a sequence beyond them is still computed. scratch:
- * dav2_hip_attention_cache_i8_scratch_bytes() bytes (0: none), 16-byte
- * aligned, in use until the call's work is done. That number depends on the
- * sizes, never on the pointers. */
+/* softmax(scale * q k^T) v over a cache: query rows starts[s] .. starts[s+1] are
+ * the last tokens of sequence s, of lengths[s] tokens in all. causal: row i of n
+ * sees the first lengths[s] - n + 1 + i tokens; otherwise all. heads is a
+ * multiple of kv_heads; head h reads head h / (heads / kv_heads) of the cache. A
+ * row that sees nothing gives zeros; output rows of no sequence are left as they
+ * were. Scales of pages are not negative, and a value scale below 2^-80 counts
+ * as that. Scores stay below 2^127 in size, with the scale and without. A query
+ * row enters its product as binary16 times a power of two (exact for f16 and
+ * bf16; f32: two parts, 22 bits), a weight as binary16 (11 bits down to 2^-27 of
+ * the largest) or, in f32 and where a call has few rows, as two parts (22 bits).
+ * tokens * heads stays below 2^32 - 512, sequences * kv_heads below 2^23,
+ * sequences below 2^16. Strides (elements between tokens) are multiples of 8,
+ * query and output 16-byte aligned; output overlaps no input. max_query and
+ * max_length, the most new and the most tokens of a sequence, size the launch
+ * and the scratch; a sequence beyond them is still computed (max_query 0 says
+ * that there are no rows: nothing is). One way of dealing out the work is chosen
+ * for a call by them: prompts and single tokens over long caches are better two
+ * calls, as the tokens of a mixed one walk their caches alone. scratch:
+ * dav2_hip_attention_cache_i8_scratch_bytes() bytes (0: none), 16-byte aligned,
+ * in use until the call's work is done. That number depends on the sizes, never
+ * on the pointers. */
 typedef struct dav2_attention_cache_i8_args {
     dav2_cache_i8 cache;
     const void* query;           /* [tokens][heads][head_dim]                      */
@@ -611,19 +623,21 @@ typedef struct dav2_attention_cache_i8_args {
 DAV2_API uint64_t dav2_hip_attention_cache_i8_scratch_bytes(const dav2_attention_cache_i8_args* args);
 DAV2_API int dav2_hip_attention_cache_i8(const dav2_attention_cache_i8_args* args, void* stream);
 
-/* softmax(scale * q k^T) v of queries against keys and values of another
- * length (an encoder's tokens), batch by batch. Key j of batch b is seen if
- * j < key_lengths[b] (NULL: key_tokens) and key_mask[b][j] != 0 (NULL: all);
- * what is not seen may hold anything, NaN included. A batch that sees nothing
- * gives zeros. heads is a multiple of kv_heads; head h reads key head
- * h / (heads / kv_heads). head_dim a multiple of 16 up to 128; strides in
- * elements, multiples of 8, those of the inputs between batches may be 0; the
- * four tensors 16-byte aligned; output overlaps no input, nor a batch's output
- * another's. batch stays below 2^16, batch * query_tokens * heads below
- * 2^32 - 256, batch * kv_heads below 2^23. scratch as for
+/* softmax(scale * q k^T) v of queries against keys and values of another length
+ * (an encoder's tokens), batch by batch. Key j of batch b is seen if j <
+ * key_lengths[b] (NULL: key_tokens) and key_mask[b][j] != 0 (NULL: all); what is
+ * not seen may hold anything, NaN included. A batch that sees nothing gives
+ * zeros. Scores stay below 2^127 in size, with the scale and without. Weights
+ * are rounded to the tensors' type for the product with the values, f16 ones to
+ * 11 bits down to 2^-27 of the largest. heads is a multiple of kv_heads; head h
+ * reads key head h / (heads / kv_heads). head_dim a multiple of 16 up to 128;
+ * strides in elements, multiples of 8, those of the inputs between batches may
+ * be 0; the four tensors 16-byte aligned; output overlaps no input, nor a
+ * batch's output another's. batch stays below 2^16, batch * query_tokens * heads
+ * below 2^32 - 256, batch * kv_heads below 2^23. scratch as for
  * dav2_hip_attention_cache_i8; its size goes by the sizes alone, a key mask's
- * part included. A call without a mask whose keys are not split touches none
- * and may leave it NULL. */
+ * part included. A call without a mask whose keys are not split touches none and
+ * may leave it NULL. */
 typedef struct dav2_cross_attention_args {
     const void* query;           /* [batch][query_tokens][heads][head_dim]         */
     const void* keys;            /* [batch][key_tokens][kv_heads][head_dim]        */
