@@ -200,9 +200,58 @@ class CrossAttentionArgs(C.Structure):
                 ("scratch_bytes", C.c_uint64)]
 
 
+class CacheI4(C.Structure):
+    _fields_ = [("keys", C.c_void_p), ("values", C.c_void_p), ("key_scales", C.c_void_p),
+                ("value_scales", C.c_void_p), ("pages", C.c_uint32), ("kv_heads", C.c_uint32),
+                ("page_size", C.c_uint32), ("head_dim", C.c_uint32)]
+
+
+class CacheStoreI4Args(C.Structure):
+    _fields_ = [("cache", CacheI4)] + CacheStoreI8Args._fields_[1:]
+
+
+class AttentionCacheI4Args(C.Structure):
+    _fields_ = [("cache", CacheI4)] + AttentionCacheI8Args._fields_[1:]
+
+
+class CachePlanArgs(C.Structure):
+    _fields_ = [("held", C.c_void_p), ("added", C.c_void_p), ("page_table", C.c_void_p), ("free_pages", C.c_void_p),
+                ("free_state", C.c_void_p), ("held_out", C.c_void_p), ("free_state_out", C.c_void_p),
+                ("starts", C.c_void_p), ("lengths", C.c_void_p), ("positions", C.c_void_p), ("owners", C.c_void_p),
+                ("slots", C.c_void_p), ("sequences", C.c_uint32), ("table_pages", C.c_uint32),
+                ("tokens", C.c_uint32), ("pages", C.c_uint32), ("page_size", C.c_uint32), ("scratch", C.c_void_p),
+                ("scratch_bytes", C.c_uint64)]
+
+
+class AddRmsNormArgs(C.Structure):
+    _fields_ = [("input", C.c_void_p), ("residual", C.c_void_p), ("weight", C.c_void_p), ("sum", C.c_void_p),
+                ("output", C.c_void_p), ("codes", C.c_void_p), ("scales", C.c_void_p), ("input_stride", C.c_uint64),
+                ("residual_stride", C.c_uint64), ("sum_stride", C.c_uint64), ("output_stride", C.c_uint64),
+                ("code_stride", C.c_uint64), ("rows", C.c_uint32), ("columns", C.c_uint32), ("dtype", C.c_uint32),
+                ("epsilon", C.c_float)]
+
+
+class SampleArgs(C.Structure):
+    _fields_ = [("logits", C.c_void_p), ("logit_stride", C.c_uint64), ("temperature", C.c_void_p),
+                ("top_k", C.c_void_p), ("top_p", C.c_void_p), ("min_p", C.c_void_p), ("uniform", C.c_void_p),
+                ("tokens", C.c_void_p), ("probabilities", C.c_void_p), ("rows", C.c_uint32),
+                ("vocabulary", C.c_uint32), ("dtype", C.c_uint32), ("scratch", C.c_void_p),
+                ("scratch_bytes", C.c_uint64)]
+
+
 class OpsCacheInt8(C.Structure):
     _fields_ = [("keys", DeviceBuffer), ("values", DeviceBuffer), ("key_scales", DeviceBuffer),
                 ("value_scales", DeviceBuffer)]
+
+
+class OpsCacheInt4(C.Structure):
+    _fields_ = OpsCacheInt8._fields_
+
+
+class OpsCachePlanBuffers(C.Structure):
+    _fields_ = [(name, DeviceBuffer) for name in (
+        "held", "added", "page_table", "free_pages", "free_state", "held_out", "free_state_out", "starts", "lengths",
+        "positions", "owners", "slots")]
 
 
 CONV_RELU_INPUT, CONV_RELU_OUTPUT, CONV_EMIT_ABSMAX, CONV_EMIT_RELU_MAX = 1, 2, 4, 8
@@ -309,6 +358,14 @@ PROTOTYPES = {
     "dav2_hip_attention_cache_i8": (C.c_int, [vp, vp]),
     "dav2_hip_cross_attention_scratch_bytes": (u64, [vp]),
     "dav2_hip_cross_attention": (C.c_int, [vp, vp]),
+    "dav2_hip_cache_store_i4": (C.c_int, [vp, vp]),
+    "dav2_hip_attention_cache_i4_scratch_bytes": (u64, [vp]),
+    "dav2_hip_attention_cache_i4": (C.c_int, [vp, vp]),
+    "dav2_hip_cache_plan_scratch_bytes": (u64, [vp]),
+    "dav2_hip_cache_plan": (C.c_int, [vp, vp]),
+    "dav2_hip_add_rms_norm": (C.c_int, [vp, vp]),
+    "dav2_hip_sample_scratch_bytes": (u64, [vp]),
+    "dav2_hip_sample": (C.c_int, [vp, vp]),
     "dav2_hip_error_string": (C.c_char_p, [C.c_int]),
     # operator surface
     "dav2_ops_create": (vp, [i32]),
@@ -342,6 +399,11 @@ PROTOTYPES = {
     "dav2_ops_cache_store_int8": (C.c_int, [vp, OpsCacheInt8, DB, DB, DB, DB, DB, vp]),
     "dav2_ops_attention_cache_int8": (C.c_int, [vp, DB, DB, OpsCacheInt8, DB, DB, DB, DB, vp]),
     "dav2_ops_cross_attention": (C.c_int, [vp, DB, DB, DB, DB, DB, DB, DB, vp]),
+    "dav2_ops_cache_store_int4": (C.c_int, [vp, OpsCacheInt4, DB, DB, DB, DB, DB, vp]),
+    "dav2_ops_attention_cache_int4": (C.c_int, [vp, DB, DB, OpsCacheInt4, DB, DB, DB, DB, vp]),
+    "dav2_ops_cache_plan": (C.c_int, [vp, vp, DB, vp]),
+    "dav2_ops_add_rms_norm": (C.c_int, [vp, DB, DB, DB, DB, DB, DB, DB, vp]),
+    "dav2_ops_sample": (C.c_int, [vp, DB, DB, DB, DB, DB, DB, DB, DB, DB, vp]),
     "dav2_infer_tensor_f32_device_logits": (C.c_int, [vp, vp, i32, i32, vp, vp, vp]),
 }
 

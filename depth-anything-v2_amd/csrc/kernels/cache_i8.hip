@@ -6,7 +6,7 @@
 #include <algorithm>
 #include <type_traits>
 
-#include "decoder.h"
+#include "cache.h"
 
 using namespace dav2k;
 
@@ -198,43 +198,6 @@ __global__ __launch_bounds__(256, 8) void cache_store_kernel(dav2_cache_store_i8
 // few, has a second part: the rest times 2^11, whose product takes the codes
 // times 2^-11 (exact in binary16), so that it ends 2^11 later: 2^-23 of a weight
 // down to 2^(-14 - kBias), at most 2^(-36 - kBias) below.
-//
-// A score past kFar is rounded to more than the exponentials' range has room
-// for, and kBias would be lost beside it: base is then the maximum itself.
-constexpr float kFar = 1048576.0f;
-constexpr float kSecond = 2048.0f;  // what the second part is multiplied by
-DAV2_DEV h8 for_second(h8 codes) { return codes * static_cast<_Float16>(1.0f / kSecond); }
-
-// Page and slot of a 16-token chunk; magic = ceil(2^32 / chunks per page),
-// which divides every chunk below 2^28 exactly (2 to 16 chunks per page). For
-// one chunk per page that is 0 in 32 bits, and alone adds the chunk itself.
-struct Pages {
-    const int32_t* table;  // of one sequence
-    uint32_t table_pages, pages, per_page, magic, alone;
-    struct Place {
-        uint32_t index, slot;  // of the page in the table, of the chunk in the page
-        int32_t entry;
-    };
-    // A chunk's place; the entry's load is not waited for here.
-    DAV2_DEV Place find(uint32_t chunk) const {
-        Place p;
-        p.index = __umulhi(chunk, magic) + (chunk & alone);
-        p.slot = (chunk - p.index * per_page) * 16u;
-        p.entry = table[min(p.index, table_pages - 1u)];
-        return p;
-    }
-    DAV2_DEV bool exists(const Place& p) const {
-        return p.index < table_pages && static_cast<uint32_t>(p.entry) < pages;
-    }
-    // the page, or one that may be read in its place
-    DAV2_DEV uint32_t page(const Place& p) const { return exists(p) ? static_cast<uint32_t>(p.entry) : 0u; }
-};
-
-DAV2_DEV Pages pages_of(const dav2_attention_cache_i8_args& a, uint32_t s) {
-    const uint32_t per_page = a.cache.page_size / 16u;
-    return {a.page_table + static_cast<uint64_t>(s) * a.table_pages, a.table_pages, a.cache.pages, per_page,
-            static_cast<uint32_t>(((1ull << 32) + per_page - 1u) / per_page), per_page == 1 ? ~0u : 0u};
-}
 
 // Eight codes as binary16: the byte c + 128 below the exponent of 1024 is the
 // number 1152 + c.
@@ -246,18 +209,6 @@ DAV2_DEV h8 widen(uint32_t lo, uint32_t hi) {
     const h2 c = __builtin_bit_cast(h2, __builtin_amdgcn_perm(0x64646464u, y, 0x04010400u)) - shift;
     const h2 d = __builtin_bit_cast(h2, __builtin_amdgcn_perm(0x64646464u, y, 0x04030402u)) - shift;
     return h8{a.x, a.y, b.x, b.y, c.x, c.y, d.x, d.y};
-}
-
-// A page's value scale as 2^e f. Below 2^-80 (a page of zeros with a scale of
-// 0) 2^-80 stands in: the sum of w 2^-e, of up to 2^31 weights of 2^15, stays
-// finite. Infinity and NaN make f NaN.
-DAV2_DEV void split_scale(float scale, float& exponent, float& fraction, float& inverse) {
-    const uint32_t bits = max(__float_as_uint(scale) & 0x7fffffffu, 47u << 23);
-    const int e = static_cast<int>(bits >> 23) - 127;
-    exponent = static_cast<float>(e);
-    fraction = bits >= 0x7f800000u ? __uint_as_float(0x7fc00000u)
-                                   : __uint_as_float((bits & 0x007fffffu) | 0x3f800000u);
-    inverse = ldexpf(1.0f, -e);
 }
 
 DAV2_DEV Parts parts_of(const dav2_attention_cache_i8_args& a, uint32_t splits) {
@@ -914,27 +865,12 @@ void cache_tiles_kernel(dav2_attention_cache_i8_args a, uint32_t splits, uint32_
 // The splits of the sequences' rows joined.
 template <typename E, int FEW>
 __global__ __launch_bounds__(256) void cache_join_kernel(dav2_attention_cache_i8_args a, uint32_t splits) {
-    const Sequence q = sequence_of(a.starts, a.lengths, blockIdx.y, a.tokens);
-    const uint64_t rows = static_cast<uint64_t>(q.end - q.begin) * a.heads;
-    const Parts parts = parts_of(a, splits);
-    const uint32_t d = a.cache.head_dim, heads = a.heads;
-    auto token = [&](uint64_t r) { return q.begin + static_cast<uint64_t>(static_cast<uint32_t>(r) / heads); };
-    auto head = [&](uint64_t r) { return static_cast<uint64_t>(static_cast<uint32_t>(r) % heads); };
-    auto output = [&](uint64_t r) { return static_cast<E*>(a.output) + token(r) * a.output_stride + head(r) * d; };
-    auto slot = [&](uint64_t r) { return (token(r) * heads + head(r)) * splits; };
-    if constexpr (FEW > 0) {
-        const uint32_t lanes = join_lanes_log2(d), each = 256u >> lanes, f4 = threadIdx.x & ((1u << lanes) - 1u);
-        for (uint64_t r = static_cast<uint64_t>(blockIdx.x) * each + (threadIdx.x >> lanes); r < rows;
-             r += static_cast<uint64_t>(gridDim.x) * each)
-            join_few<FEW>(parts, slot(r), splits, d, f4, output(r));
-    } else {
-        for (uint64_t r = blockIdx.x; r < rows; r += gridDim.x) join_row(parts, slot(r), splits, d, output(r));
-    }
+    join_sequence<E, FEW>(a, parts_of(a, splits), splits);
 }
 
 bool valid(const dav2_attention_cache_i8_args& a) {
     const uint64_t row = static_cast<uint64_t>(a.heads) * a.cache.head_dim;
-    return valid_cache(a.cache) && a.query && a.output && aligned16(a.query) && aligned16(a.output) && a.page_table &&
+    return valid_pages(a.cache) && a.query && a.output && aligned16(a.query) && aligned16(a.output) && a.page_table &&
            a.starts && a.lengths && a.dtype <= DAV2_DTYPE_BF16 && a.sequences <= 65535u && a.tokens <= 0x7fffffffu &&
            a.table_pages > 0 && a.table_pages <= 0x7fffffffu && a.heads > 0 && a.heads <= 65535u &&
            a.heads % a.cache.kv_heads == 0 && static_cast<uint64_t>(a.tokens) * a.heads <= 0xfffffe00ull &&
@@ -1011,7 +947,7 @@ int dav2_hip_cache_store_i8(const dav2_cache_store_i8_args* args, void* stream) 
     const dav2_cache_store_i8_args& a = *args;
     if (a.sequences == 0 || a.tokens == 0 || a.max_new == 0) return hipSuccess;
     const uint64_t row = static_cast<uint64_t>(a.cache.kv_heads) * a.cache.head_dim;
-    if (!valid_cache(a.cache) || !a.keys || !a.values || !a.page_table || !a.starts || !a.lengths ||
+    if (!valid_pages(a.cache) || !a.keys || !a.values || !a.page_table || !a.starts || !a.lengths ||
         a.dtype > DAV2_DTYPE_BF16 || a.sequences > 65535u || a.tokens > 0x7fffffffu || a.table_pages == 0 ||
         a.table_pages > 0x7fffffffu || (a.tokens > 1 && (a.key_stride < row || a.value_stride < row)))
         return hipErrorInvalidValue;
@@ -1061,14 +997,11 @@ int dav2_hip_attention_cache_i8(const dav2_attention_cache_i8_args* args, void* 
             else dispatch(cache_rows_kernel<E, D>, grid, dim3(256), 0, s, a, p.splits, p.tiles);
         });
         if (p.splits > 1) {
-            const uint64_t rows = static_cast<uint64_t>(std::min(a.max_query, a.tokens)) * a.heads;
-            const int few = join_kind(rows * a.sequences, p.splits);
-            const uint64_t each = few ? join_rows(a.cache.head_dim) : 1;
-            const dim3 join(static_cast<uint32_t>(std::min<uint64_t>((rows + each - 1) / each, 4096)), a.sequences);
-            dispatch(few == 4   ? cache_join_kernel<E, 4>
-                     : few == 8 ? cache_join_kernel<E, 8>
-                                : cache_join_kernel<E, 0>,
-                     join, dim3(256), 0, s, a, p.splits);
+            const JoinLaunch j = join_launch(a, p.splits);
+            dispatch(j.few == 4   ? cache_join_kernel<E, 4>
+                     : j.few == 8 ? cache_join_kernel<E, 8>
+                                  : cache_join_kernel<E, 0>,
+                     j.grid, dim3(256), 0, s, a, p.splits);
         }
         return hipGetLastError();
     });

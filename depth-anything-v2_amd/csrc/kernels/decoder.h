@@ -110,7 +110,8 @@ DAV2_DEV void lds_turn() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: 
 // selecting its results afterwards.
 DAV2_DEV void stay_in_branch() { asm volatile(""); }
 
-inline bool valid_cache(const dav2_cache_i8& c) {
+template <typename Cache>
+bool valid_pages(const Cache& c) {
     return c.keys && c.values && c.key_scales && c.value_scales && aligned16(c.keys) && aligned16(c.values) &&
            c.pages > 0 && c.pages <= 0x7fffffffu && c.kv_heads > 0 && c.kv_heads <= 32767u && c.page_size >= 16 &&
            c.page_size <= 256 && c.page_size % 16 == 0 && c.head_dim >= 16 && c.head_dim <= 128 &&

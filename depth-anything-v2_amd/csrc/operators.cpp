@@ -383,7 +383,7 @@ void HipOperators::attention_fused(DeviceBuffer& output, const DeviceBuffer& qkv
     require_bytes(output, elements, "attention output");
     require_bytes(qkv, elements * 3, "QKV");
     const std::uint64_t need = attention_fused_scratch_bytes(tokens, heads, batch);
-    if (scratch.size() < need) throw std::invalid_argument("attention scratch device buffer is too small");
+    if (scratch.size() < need) throw std::invalid_argument("scratch device buffer is too small");
     const hipStream_t s = stream();
     // QK^T and PV: 4*T*T*64 flops per head.
     const double flops = 4.0 * batch * heads * double(tokens) * tokens * 64.0;
@@ -1036,19 +1036,24 @@ unsigned __int128 strided(std::uint64_t count, std::uint64_t stride, std::uint64
     return count == 0 ? 0 : static_cast<unsigned __int128>(count - 1) * stride + row;
 }
 
-void require_cache(const HipOperators::CacheBuffers& b, const dav2_cache_i8& c) {
+// codes: of a byte; scales: of a page and head, or of each token in it
+template <typename Cache>
+void require_cache(const HipOperators::CacheBuffers& b, const Cache& c, std::uint32_t codes, std::uint32_t scales) {
     const auto planes = static_cast<unsigned __int128>(c.pages) * c.kv_heads;
-    const std::uint64_t plane = static_cast<std::uint64_t>(c.page_size) * c.head_dim;
+    const std::uint64_t plane = static_cast<std::uint64_t>(c.page_size) * c.head_dim / codes;
     if (planes == 0 || plane == 0) throw std::invalid_argument("invalid cache dimensions");
     require_size(b.keys, planes * plane, 1, "cache keys");
     require_size(b.values, planes * plane, 1, "cache values");
-    require_size(b.key_scales, planes, sizeof(float), "cache key scales");
-    require_size(b.value_scales, planes, sizeof(float), "cache value scales");
+    require_size(b.key_scales, planes * scales, sizeof(float), "cache key scales");
+    require_size(b.value_scales, planes * scales, sizeof(float), "cache value scales");
 }
+void require_cache(const HipOperators::CacheBuffers& b, const dav2_cache_i8& c) { require_cache(b, c, 1, 1); }
+void require_cache(const HipOperators::CacheBuffers& b, const dav2_cache_i4& c) { require_cache(b, c, 2, c.page_size); }
 
-dav2_cache_i8 cache_of(const HipOperators::CacheBuffers& b, dav2_cache_i8 c) {
-    c.keys = b.keys.as<int8_t>();
-    c.values = b.values.as<int8_t>();
+template <typename Cache>
+Cache cache_of(const HipOperators::CacheBuffers& b, Cache c) {
+    c.keys = b.keys.as<std::remove_pointer_t<decltype(c.keys)>>();
+    c.values = b.values.as<std::remove_pointer_t<decltype(c.values)>>();
     c.key_scales = b.key_scales.as<float>();
     c.value_scales = b.value_scales.as<float>();
     return c;
@@ -1137,17 +1142,17 @@ void HipOperators::cache_store_int8(const CacheBuffers& cache, const DeviceBuffe
     launch_check(dav2_hip_cache_store_i8(&a, stream()), "cache store");
 }
 
-void* HipOperators::attention_scratch(const DeviceBuffer& given, std::uint64_t need, std::uint64_t& bytes) {
+void* HipOperators::scratch_of(const DeviceBuffer& given, std::uint64_t need, std::uint64_t& bytes) {
     bytes = need;
     if (need == 0) return nullptr;
     if (given) {
-        if (given.size() < need) throw std::invalid_argument("attention scratch device buffer is too small");
+        if (given.size() < need) throw std::invalid_argument("scratch device buffer is too small");
         return given.data();
     }
     hipStreamCaptureStatus capture = hipStreamCaptureStatusNone;
     hip_check(hipStreamIsCapturing(stream(), &capture), "capture status");
     if (capture != hipStreamCaptureStatusNone)
-        throw std::invalid_argument("attention under graph capture needs a scratch buffer of its own");
+        throw std::invalid_argument("a call under graph capture needs a scratch buffer of its own");
     return grow(decoder_scratch_, need).data();
 }
 
@@ -1169,7 +1174,7 @@ void HipOperators::attention_cache_int8(DeviceBuffer& output, const DeviceBuffer
     a.page_table = page_table.as<std::int32_t>();
     a.starts = starts.as<std::int32_t>();
     a.lengths = lengths.as<std::int32_t>();
-    a.scratch = attention_scratch(scratch, dav2_hip_attention_cache_i8_scratch_bytes(&a), a.scratch_bytes);
+    a.scratch = scratch_of(scratch, dav2_hip_attention_cache_i8_scratch_bytes(&a), a.scratch_bytes);
     // at most: every row sees max_length tokens
     ProfileScope prof(context_.profiler(), "attention_cache_i8", 4.0 * row * a.tokens * a.max_length, "FLOP", stream());
     launch_check(dav2_hip_attention_cache_i8(&a, stream()), "cache attention");
@@ -1201,10 +1206,143 @@ void HipOperators::cross_attention(DeviceBuffer& output, const DeviceBuffer& que
     a.key_lengths = key_lengths.as<std::int32_t>();
     a.key_mask = key_mask.as<std::uint8_t>();
     const std::uint64_t need = dav2k::cross_attention_uses_scratch(a) ? dav2_hip_cross_attention_scratch_bytes(&a) : 0;
-    a.scratch = attention_scratch(scratch, need, a.scratch_bytes);
+    a.scratch = scratch_of(scratch, need, a.scratch_bytes);
     ProfileScope prof(context_.profiler(), "cross_attention",
                       4.0 * row * a.query_tokens * double(a.batch) * a.key_tokens, "FLOP", stream());
     launch_check(dav2_hip_cross_attention(&a, stream()), "cross attention");
+}
+
+void HipOperators::cache_store_int4(const CacheBuffers& cache, const DeviceBuffer& keys, const DeviceBuffer& values,
+                                    const DeviceBuffer& page_table, const DeviceBuffer& starts,
+                                    const DeviceBuffer& lengths, const dav2_cache_store_i4_args& sizes) {
+    dav2_cache_store_i4_args a = sizes;
+    if (a.sequences == 0 || a.tokens == 0 || a.max_new == 0 || a.table_pages == 0)
+        throw std::invalid_argument("invalid cache store dimensions");
+    require_cache(cache, a.cache);
+    require_sequences(page_table, starts, lengths, a.sequences, a.table_pages);
+    const std::uint64_t size = element_bytes(a.dtype), row = std::uint64_t(a.cache.kv_heads) * a.cache.head_dim;
+    require_size(keys, strided(a.tokens, a.key_stride, row), size, "new keys");
+    require_size(values, strided(a.tokens, a.value_stride, row), size, "new values");
+    a.cache = cache_of(cache, a.cache);
+    a.keys = keys.data();
+    a.values = values.data();
+    a.page_table = page_table.as<std::int32_t>();
+    a.starts = starts.as<std::int32_t>();
+    a.lengths = lengths.as<std::int32_t>();
+    ProfileScope prof(context_.profiler(), "cache_store_i4", 2.0 * (size + 0.5) * row * a.tokens, "B", stream());
+    launch_check(dav2_hip_cache_store_i4(&a, stream()), "cache store");
+}
+
+void HipOperators::attention_cache_int4(DeviceBuffer& output, const DeviceBuffer& query, const CacheBuffers& cache,
+                                        const DeviceBuffer& page_table, const DeviceBuffer& starts,
+                                        const DeviceBuffer& lengths, const DeviceBuffer& scratch,
+                                        const dav2_attention_cache_i4_args& sizes) {
+    dav2_attention_cache_i4_args a = sizes;
+    if (a.sequences == 0 || a.tokens == 0 || a.max_query == 0 || a.table_pages == 0 || a.heads == 0)
+        throw std::invalid_argument("invalid cache attention dimensions");
+    require_cache(cache, a.cache);
+    require_sequences(page_table, starts, lengths, a.sequences, a.table_pages);
+    const std::uint64_t size = element_bytes(a.dtype), row = std::uint64_t(a.heads) * a.cache.head_dim;
+    require_size(query, strided(a.tokens, a.query_stride, row), size, "query");
+    require_size(output, strided(a.tokens, a.output_stride, row), size, "attention output");
+    a.cache = cache_of(cache, a.cache);
+    a.query = query.data();
+    a.output = output.data();
+    a.page_table = page_table.as<std::int32_t>();
+    a.starts = starts.as<std::int32_t>();
+    a.lengths = lengths.as<std::int32_t>();
+    a.scratch = scratch_of(scratch, dav2_hip_attention_cache_i4_scratch_bytes(&a), a.scratch_bytes);
+    // at most: every row sees max_length tokens
+    ProfileScope prof(context_.profiler(), "attention_cache_i4", 4.0 * row * a.tokens * a.max_length, "FLOP", stream());
+    launch_check(dav2_hip_attention_cache_i4(&a, stream()), "cache attention");
+}
+
+void HipOperators::cache_plan(const PlanBuffers& b, const DeviceBuffer& scratch, const dav2_cache_plan_args& sizes) {
+    dav2_cache_plan_args a = sizes;
+    if (a.sequences == 0 || a.table_pages == 0 || a.pages == 0 || a.page_size == 0)
+        throw std::invalid_argument("invalid cache plan dimensions");
+    const std::uint64_t size = sizeof(std::int32_t);
+    require_sequences(b.page_table, b.starts, b.lengths, a.sequences, a.table_pages);
+    require_size(b.held, a.sequences, size, "held");
+    require_size(b.added, a.sequences, size, "added");
+    require_size(b.held_out, a.sequences, size, "held output");
+    require_size(b.free_pages, a.pages, size, "free pages");
+    require_size(b.free_state, 2, size, "free state");
+    require_size(b.free_state_out, 2, size, "free state output");
+    if (b.positions) require_size(b.positions, a.tokens, size, "positions");
+    if (b.owners) require_size(b.owners, a.tokens, size, "owners");
+    if (b.slots) require_size(b.slots, a.tokens, sizeof(std::int64_t), "slots");
+    a.held = b.held.as<std::int32_t>();
+    a.added = b.added.as<std::int32_t>();
+    a.page_table = b.page_table.as<std::int32_t>();
+    a.free_pages = b.free_pages.as<std::int32_t>();
+    a.free_state = b.free_state.as<std::int32_t>();
+    a.held_out = b.held_out.as<std::int32_t>();
+    a.free_state_out = b.free_state_out.as<std::int32_t>();
+    a.starts = b.starts.as<std::int32_t>();
+    a.lengths = b.lengths.as<std::int32_t>();
+    a.positions = b.positions.as<std::int32_t>();
+    a.owners = b.owners.as<std::int32_t>();
+    a.slots = b.slots.as<std::int64_t>();
+    a.scratch = scratch_of(scratch, dav2_hip_cache_plan_scratch_bytes(&a), a.scratch_bytes);
+    ProfileScope prof(context_.profiler(), "cache_plan", 16.0 * a.tokens + 20.0 * a.sequences, "B", stream());
+    launch_check(dav2_hip_cache_plan(&a, stream()), "cache plan");
+}
+
+void HipOperators::add_rms_norm(DeviceBuffer& sum, DeviceBuffer& output, DeviceBuffer& codes, DeviceBuffer& scales,
+                                const DeviceBuffer& input, const DeviceBuffer& residual, const DeviceBuffer& weight,
+                                const dav2_add_rms_norm_args& sizes) {
+    dav2_add_rms_norm_args a = sizes;
+    if (a.rows == 0 || a.columns == 0) throw std::invalid_argument("invalid norm dimensions");
+    const std::uint64_t size = element_bytes(a.dtype);
+    require_size(input, strided(a.rows, a.input_stride, a.columns), size, "norm input");
+    if (residual) require_size(residual, strided(a.rows, a.residual_stride, a.columns), size, "residual");
+    if (weight) require_size(weight, a.columns, sizeof(float), "norm weight");
+    if (sum) require_size(sum, strided(a.rows, a.sum_stride, a.columns), size, "sum output");
+    if (output) require_size(output, strided(a.rows, a.output_stride, a.columns), size, "norm output");
+    if (codes) {
+        require_size(codes, static_cast<unsigned __int128>(a.rows) * a.code_stride, 1, "codes");
+        require_size(scales, a.rows, sizeof(float), "scales");
+    }
+    a.input = input.data();
+    a.residual = residual.data();
+    a.weight = weight.as<float>();
+    a.sum = sum.data();
+    a.output = output.data();
+    a.codes = codes.as<std::int8_t>();
+    a.scales = scales.as<float>();
+    const double values = static_cast<double>(a.rows) * a.columns;
+    ProfileScope prof(context_.profiler(), "add_rms_norm",
+                      values * (size * (1.0 + !!residual + !!sum + !!output) + !!codes), "B", stream());
+    launch_check(dav2_hip_add_rms_norm(&a, stream()), "norm");
+}
+
+void HipOperators::sample(DeviceBuffer& tokens, DeviceBuffer& probabilities, const DeviceBuffer& logits,
+                          const DeviceBuffer& temperature, const DeviceBuffer& top_k, const DeviceBuffer& top_p,
+                          const DeviceBuffer& min_p, const DeviceBuffer& uniform, const DeviceBuffer& scratch,
+                          const dav2_sample_args& sizes) {
+    dav2_sample_args a = sizes;
+    if (a.rows == 0 || a.vocabulary == 0) throw std::invalid_argument("invalid sampling dimensions");
+    const std::uint64_t size = element_bytes(a.dtype);
+    require_size(logits, strided(a.rows, a.logit_stride, a.vocabulary), size, "logits");
+    require_size(tokens, a.rows, sizeof(std::int32_t), "tokens");
+    require_size(uniform, a.rows, sizeof(float), "random numbers");
+    if (probabilities) require_size(probabilities, a.rows, sizeof(float), "probabilities");
+    if (temperature) require_size(temperature, a.rows, sizeof(float), "temperatures");
+    if (top_k) require_size(top_k, a.rows, sizeof(std::int32_t), "top-k");
+    if (top_p) require_size(top_p, a.rows, sizeof(float), "top-p");
+    if (min_p) require_size(min_p, a.rows, sizeof(float), "min-p");
+    a.logits = logits.data();
+    a.temperature = temperature.as<float>();
+    a.top_k = top_k.as<std::int32_t>();
+    a.top_p = top_p.as<float>();
+    a.min_p = min_p.as<float>();
+    a.uniform = uniform.as<float>();
+    a.tokens = tokens.as<std::int32_t>();
+    a.probabilities = probabilities.as<float>();
+    a.scratch = scratch_of(scratch, dav2_hip_sample_scratch_bytes(&a), a.scratch_bytes);
+    ProfileScope prof(context_.profiler(), "sample", static_cast<double>(size) * a.rows * a.vocabulary, "B", stream());
+    launch_check(dav2_hip_sample(&a, stream()), "sampling");
 }
 
 }  // namespace dav2

@@ -212,6 +212,27 @@ public:
                          const DeviceBuffer& values, const DeviceBuffer& key_lengths, const DeviceBuffer& key_mask,
                          const DeviceBuffer& scratch, const dav2_cross_attention_args& sizes);
 
+    void cache_store_int4(const CacheBuffers& cache, const DeviceBuffer& keys, const DeviceBuffer& values,
+                          const DeviceBuffer& page_table, const DeviceBuffer& starts, const DeviceBuffer& lengths,
+                          const dav2_cache_store_i4_args& sizes);
+    void attention_cache_int4(DeviceBuffer& output, const DeviceBuffer& query, const CacheBuffers& cache,
+                              const DeviceBuffer& page_table, const DeviceBuffer& starts, const DeviceBuffer& lengths,
+                              const DeviceBuffer& scratch, const dav2_attention_cache_i4_args& sizes);
+    struct PlanBuffers {
+        const DeviceBuffer &held, &added;
+        DeviceBuffer &page_table, &free_pages;
+        const DeviceBuffer& free_state;
+        DeviceBuffer &held_out, &free_state_out, &starts, &lengths, &positions, &owners, &slots;
+    };
+    void cache_plan(const PlanBuffers& buffers, const DeviceBuffer& scratch, const dav2_cache_plan_args& sizes);
+    void add_rms_norm(DeviceBuffer& sum, DeviceBuffer& output, DeviceBuffer& codes, DeviceBuffer& scales,
+                      const DeviceBuffer& input, const DeviceBuffer& residual, const DeviceBuffer& weight,
+                      const dav2_add_rms_norm_args& sizes);
+    void sample(DeviceBuffer& tokens, DeviceBuffer& probabilities, const DeviceBuffer& logits,
+                const DeviceBuffer& temperature, const DeviceBuffer& top_k, const DeviceBuffer& top_p,
+                const DeviceBuffer& min_p, const DeviceBuffer& uniform, const DeviceBuffer& scratch,
+                const dav2_sample_args& sizes);
+
     // ---- fused variants used by the graph drivers ------------------------
     // LayerNorm whose output row is quantized straight into the workspace
     // (layer_norm + quantize_rows of linear_int8); fp32 row optional.
@@ -277,8 +298,8 @@ private:
                             std::uint32_t output_row_offset, std::uint32_t output_row_stride, bool output_transposed,
                             bool has_bias, const DeviceBuffer* residual = nullptr, bool relu_output = false);
 
-    // The scratch of an attention call: the caller's, or decoder_scratch_.
-    void* attention_scratch(const DeviceBuffer& given, std::uint64_t need, std::uint64_t& bytes);
+    // The scratch of a decoder operator's call: the caller's, or decoder_scratch_.
+    void* scratch_of(const DeviceBuffer& given, std::uint64_t need, std::uint64_t& bytes);
 
     HipContext& context_;
     hipStream_t stream_ = nullptr;
@@ -295,7 +316,7 @@ private:
     DeviceBuffer conv_weights_;    // packed weights of a conv2d_int8 call that brought none
     DeviceBuffer conv_act_;        // ReLU of a conv2d_int8 input on the im2col path
     DeviceBuffer gemm_split_;      // int32 slices of split-K channel-major GEMMs
-    DeviceBuffer decoder_scratch_; // parts of attention_cache_int8 / cross_attention split over the keys
+    DeviceBuffer decoder_scratch_; // of the decoder operators' calls that bring none
     DeviceBuffer f32_cols_;        // fp32 im2col rows of the fp32 convolutions
     std::uint32_t workspace_ld_ = 0;  // row stride of the int8 rows currently in the workspace
 };

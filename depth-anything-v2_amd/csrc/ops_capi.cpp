@@ -515,6 +515,65 @@ dav2_status DAV2_CALL dav2_ops_cross_attention(dav2_ops* ops, dav2_device_buffer
     });
 }
 
+dav2_status DAV2_CALL dav2_ops_cache_store_int4(dav2_ops* ops, dav2_ops_cache_int4 cache, dav2_device_buffer keys,
+                                                dav2_device_buffer values, dav2_device_buffer page_table,
+                                                dav2_device_buffer starts, dav2_device_buffer lengths,
+                                                const dav2_cache_store_i4_args* sizes) {
+    return guard(ops, [&](dav2::HipOperators& o) {
+        const auto ck = v(cache.keys), cv = v(cache.values), ks = v(cache.key_scales), vs = v(cache.value_scales);
+        o.cache_store_int4({ck, cv, ks, vs}, v(keys), v(values), v(page_table), v(starts), v(lengths), given(sizes));
+    });
+}
+
+dav2_status DAV2_CALL dav2_ops_attention_cache_int4(dav2_ops* ops, dav2_device_buffer output,
+                                                    dav2_device_buffer query, dav2_ops_cache_int4 cache,
+                                                    dav2_device_buffer page_table, dav2_device_buffer starts,
+                                                    dav2_device_buffer lengths, dav2_device_buffer scratch,
+                                                    const dav2_attention_cache_i4_args* sizes) {
+    return guard(ops, [&](dav2::HipOperators& o) {
+        const auto ck = v(cache.keys), cv = v(cache.values), ks = v(cache.key_scales), vs = v(cache.value_scales);
+        auto out = v(output);
+        o.attention_cache_int4(out, v(query), {ck, cv, ks, vs}, v(page_table), v(starts), v(lengths), v(scratch),
+                               given(sizes));
+    });
+}
+
+dav2_status DAV2_CALL dav2_ops_cache_plan(dav2_ops* ops, const dav2_ops_cache_plan_buffers* buffers,
+                                          dav2_device_buffer scratch, const dav2_cache_plan_args* sizes) {
+    return guard(ops, [&](dav2::HipOperators& o) {
+        const dav2_ops_cache_plan_buffers& b = given(buffers);
+        const auto held = v(b.held), added = v(b.added), free_state = v(b.free_state);
+        auto table = v(b.page_table), free_pages = v(b.free_pages), held_out = v(b.held_out);
+        auto state_out = v(b.free_state_out), starts = v(b.starts), lengths = v(b.lengths);
+        auto positions = v(b.positions), owners = v(b.owners), slots = v(b.slots);
+        o.cache_plan({held, added, table, free_pages, free_state, held_out, state_out, starts, lengths, positions,
+                      owners, slots},
+                     v(scratch), given(sizes));
+    });
+}
+
+dav2_status DAV2_CALL dav2_ops_add_rms_norm(dav2_ops* ops, dav2_device_buffer sum, dav2_device_buffer output,
+                                            dav2_device_buffer codes, dav2_device_buffer scales,
+                                            dav2_device_buffer input, dav2_device_buffer residual,
+                                            dav2_device_buffer weight, const dav2_add_rms_norm_args* sizes) {
+    return guard(ops, [&](dav2::HipOperators& o) {
+        auto h = v(sum), y = v(output), q = v(codes), s = v(scales);
+        o.add_rms_norm(h, y, q, s, v(input), v(residual), v(weight), given(sizes));
+    });
+}
+
+dav2_status DAV2_CALL dav2_ops_sample(dav2_ops* ops, dav2_device_buffer tokens, dav2_device_buffer probabilities,
+                                      dav2_device_buffer logits, dav2_device_buffer temperature,
+                                      dav2_device_buffer top_k, dav2_device_buffer top_p, dav2_device_buffer min_p,
+                                      dav2_device_buffer uniform, dav2_device_buffer scratch,
+                                      const dav2_sample_args* sizes) {
+    return guard(ops, [&](dav2::HipOperators& o) {
+        auto out = v(tokens), share = v(probabilities);
+        o.sample(out, share, v(logits), v(temperature), v(top_k), v(top_p), v(min_p), v(uniform), v(scratch),
+                 given(sizes));
+    });
+}
+
 dav2_status DAV2_CALL dav2_infer_tensor_f32_device_logits(dav2_context* context, const float* input, int32_t width,
                                                          int32_t height, float* depth, float* logits,
                                                          void* stream) {

@@ -656,6 +656,178 @@ typedef struct dav2_cross_attention_args {
 DAV2_API uint64_t dav2_hip_cross_attention_scratch_bytes(const dav2_cross_attention_args* args);
 DAV2_API int dav2_hip_cross_attention(const dav2_cross_attention_args* args, void* stream);
 
+/* A key/value cache in 4 bits: pages as dav2_cache_i8 has them, and one scale
+ * for each token and head, for its keys and for its values. A code c of -7 .. 7
+ * is held as c + 8 in half a byte and stands for c * scale (0 would be -8, which
+ * is read but never stored). A key's features 2 i and 2 i + 1 are the low and
+ * the high half of byte i. Values are held 16 tokens at a time, feature by
+ * feature: the tokens 16 t + 2 i and 16 t + 2 i + 1 of a feature are byte i of
+ * its eight. Limits as for dav2_cache_i8. */
+typedef struct dav2_cache_i4 {
+    uint8_t* keys;               /* [pages][kv_heads][page_size][head_dim / 2]     */
+    uint8_t* values;             /* [pages][kv_heads][page_size / 16][head_dim][8] */
+    float* key_scales;           /* [pages][kv_heads][page_size]                   */
+    float* value_scales;         /* [pages][kv_heads][page_size]                   */
+    uint32_t pages, kv_heads, page_size, head_dim;
+} dav2_cache_i4;
+
+/* Stores new tokens as dav2_hip_cache_store_i8 does, with its rules for rows,
+ * positions, pages and sequences. A head of a token gets the scale
+ * max(absmax / 7, 1e-8) and codes x / scale rounded half to even, quotients
+ * being fp32. Older tokens keep their codes and scales: storing is exact in any
+ * order and number of calls. A NaN or infinity makes the scale of its head and
+ * token NaN or infinite, and with it those values and no others. Bytes of
+ * other slots are left as they were. */
+typedef struct dav2_cache_store_i4_args {
+    dav2_cache_i4 cache;
+    const void* keys;            /* [tokens][kv_heads][head_dim]                   */
+    const void* values;
+    uint64_t key_stride, value_stride;  /* elements between tokens                 */
+    const int32_t* page_table;   /* [sequences][table_pages]                       */
+    const int32_t* starts;       /* [sequences + 1]                                */
+    const int32_t* lengths;      /* [sequences]                                    */
+    uint32_t sequences, table_pages, tokens;
+    uint32_t max_new;            /* most new tokens of a sequence: sizes the launch */
+    uint32_t dtype;
+} dav2_cache_store_i4_args;
+DAV2_API int dav2_hip_cache_store_i4(const dav2_cache_store_i4_args* args, void* stream);
+
+/* dav2_hip_attention_cache_i8 over a cache in 4 bits: its rules, limits, types,
+ * hints and scratch, with scales of tokens in the place of scales of pages. A
+ * token that a row does not see may have any scale, NaN included. */
+typedef struct dav2_attention_cache_i4_args {
+    dav2_cache_i4 cache;
+    const void* query;           /* [tokens][heads][head_dim]                      */
+    void* output;
+    uint64_t query_stride, output_stride;
+    const int32_t* page_table;   /* [sequences][table_pages]                       */
+    const int32_t* starts;       /* [sequences + 1]                                */
+    const int32_t* lengths;      /* [sequences]                                    */
+    uint32_t sequences, table_pages, tokens, heads;
+    uint32_t max_query, max_length;
+    uint32_t causal, dtype;
+    float scale;
+    void* scratch;
+    uint64_t scratch_bytes;
+} dav2_attention_cache_i4_args;
+DAV2_API uint64_t dav2_hip_attention_cache_i4_scratch_bytes(const dav2_attention_cache_i4_args* args);
+DAV2_API int dav2_hip_attention_cache_i4(const dav2_attention_cache_i4_args* args, void* stream);
+
+/* What a step of a paged cache (of either width) needs, from what its sequences
+ * hold and get, so that a captured step needs no host between its replays.
+ *
+ * added[s] >= 0: sequence s gets that many tokens, rows starts[s] .. starts[s+1]
+ * of the step, rows of all sequences one after the other. Pages for them come
+ * from the front of a ring of free ones: free_pages[(first + i) % pages] for i <
+ * count, {first, count} = free_state, go in order to the sequences that need
+ * any, in order. A sequence is served if it needs no page or if the pages that
+ * it and the sequences before it need are there, if its tokens fit the table and
+ * its rows fit `tokens`; one that does not fit needs nothing. If served it has
+ * length held[s] + added[s], and held_out[s] is that; if not, it gets no page,
+ * has length 0, so that nothing is stored or seen in this step, and still holds
+ * what it held. added[s] < 0: the sequence ends. Its pages go to the end of the
+ * ring, for later calls (those beyond `pages` entries are dropped), its length
+ * and held_out[s] are 0. Its table entries stay.
+ *
+ * Row r of sequence s, i-th of its new tokens: positions[r] = held[s] + i,
+ * owners[r] = s, slots[r] = page * page_size + slot where it is stored, -1 where
+ * it is not (not served, or the entry is no page). Rows of no sequence: 0, -1, -1.
+ * starts end at `tokens` at the most. positions, owners and slots may be NULL.
+ *
+ * held counts below 0 are 0. free_state and the ring outside [0, pages) are
+ * brought into it; a ring entry that is no page is handed out and is no page in
+ * the table. The pages of a sequence belong to it alone. held_out may be held
+ * and free_state_out free_state; other outputs overlap nothing. pages up to
+ * 2^31 - 1, page_size 16 .. 256 in steps of 16, sequences below 2^16, tokens and
+ * table_pages below 2^31. scratch: dav2_hip_cache_plan_scratch_bytes() bytes,
+ * 16-byte aligned, in use until the call's work is done. */
+typedef struct dav2_cache_plan_args {
+    const int32_t* held;         /* [sequences]                                    */
+    const int32_t* added;        /* [sequences]                                    */
+    int32_t* page_table;         /* [sequences][table_pages], new pages are added  */
+    int32_t* free_pages;         /* [pages]                                        */
+    const int32_t* free_state;   /* [2]                                            */
+    int32_t* held_out;           /* [sequences]                                    */
+    int32_t* free_state_out;     /* [2]                                            */
+    int32_t* starts;             /* [sequences + 1]                                */
+    int32_t* lengths;            /* [sequences]                                    */
+    int32_t* positions;          /* [tokens] or NULL                               */
+    int32_t* owners;             /* [tokens] or NULL                               */
+    int64_t* slots;              /* [tokens] or NULL                               */
+    uint32_t sequences, table_pages, tokens, pages, page_size;
+    void* scratch;
+    uint64_t scratch_bytes;
+} dav2_cache_plan_args;
+DAV2_API uint64_t dav2_hip_cache_plan_scratch_bytes(const dav2_cache_plan_args* args);
+DAV2_API int dav2_hip_cache_plan(const dav2_cache_plan_args* args, void* stream);
+
+/* The residual's addition, the root-mean-square norm and rows in 8 bits:
+ *   h = input + residual, rounded to the type (residual NULL: h = input);
+ *   y = (h * f) * weight, f = 1 / sqrt(mean(h^2) + epsilon) over a row, formed in
+ *       64 bits and rounded to fp32, each product fp32;
+ *   sum = h, output = y rounded to the type;
+ *   codes = y / scale rounded half to even, scale = max(absmax(y) / 127, 1e-8),
+ *       as dav2_hip_quantize_rows_i8 has them, bytes [columns, code_stride) zero:
+ *       the rows of dav2_hip_gemm_i8.
+ * Each of sum, output and codes (with scales) is left out with NULL, not all
+ * three. weight [columns] fp32, NULL = ones. A row with a NaN or infinity has NaN
+ * in y; its codes mean nothing and its scale is NaN. Strides in elements, at
+ * least columns; code_stride a multiple of 64, codes 16-byte aligned. sum and output
+ * may each be input or residual with the same stride; they overlap nothing
+ * otherwise. columns below 2^20, rows below 2^31. */
+typedef struct dav2_add_rms_norm_args {
+    const void* input;           /* [rows][columns]                                */
+    const void* residual;        /* [rows][columns] or NULL                        */
+    const float* weight;
+    void* sum;                   /* [rows][columns] or NULL                        */
+    void* output;                /* [rows][columns] or NULL                        */
+    int8_t* codes;               /* [rows][code_stride] or NULL                    */
+    float* scales;               /* [rows], with codes                             */
+    uint64_t input_stride, residual_stride, sum_stride, output_stride, code_stride;
+    uint32_t rows, columns;
+    uint32_t dtype;              /* DAV2_DTYPE_* of input, residual, sum, output   */
+    float epsilon;               /* > 0                                            */
+} dav2_add_rms_norm_args;
+DAV2_API int dav2_hip_add_rms_norm(const dav2_add_rms_norm_args* args, void* stream);
+
+/* The next token of each row of logits. The tokens of a row stand in order of
+ * their logits, the largest first, equal ones by index; of this order a prefix is
+ * kept, its weights being e_i = exp((l_i - l_0) / temperature):
+ *   min_p in (0, 1]: tokens with e_i >= min_p;
+ *   top_k > 0: the first top_k;
+ *   top_p < 1: of what these leave, those before which the sum of the weights
+ *       is below top_p of the whole.
+ * The first token always stays. The token drawn is the first at which the sum
+ * of the kept weights is above uniform times the whole; its probability is its
+ * weight over the whole. temperature <= 0 (or NaN) keeps the first token alone.
+ * temperature NULL is 1 for all rows; top_k, top_p, min_p NULL or outside the
+ * ranges above (NaN included) keep all; uniform is taken into [0, 1), NaN is 0.
+ * A NaN logit counts as -infinity; such tokens are never drawn. Where +infinity is
+ * the largest, tokens of it share the weight. A row without a finite logit and
+ * without +infinity has token -1 and probability 0.
+ *
+ * Sums are integers: weights in units of 2^-s, s = 62 - ceil(log2(vocabulary)),
+ * from 64-bit exponentials, so that a result does not depend on their order.
+ * vocabulary 1 .. 2^20, rows below 2^16; logits of a row are contiguous, rows
+ * logit_stride elements apart. scratch: dav2_hip_sample_scratch_bytes() bytes,
+ * 16-byte aligned, in use until the call's work is done. */
+typedef struct dav2_sample_args {
+    const void* logits;          /* [rows][vocabulary]                             */
+    uint64_t logit_stride;
+    const float* temperature;    /* [rows] or NULL                                 */
+    const int32_t* top_k;        /* [rows] or NULL                                 */
+    const float* top_p;          /* [rows] or NULL                                 */
+    const float* min_p;          /* [rows] or NULL                                 */
+    const float* uniform;        /* [rows], in [0, 1)                              */
+    int32_t* tokens;             /* [rows]                                         */
+    float* probabilities;        /* [rows] or NULL                                 */
+    uint32_t rows, vocabulary, dtype;
+    void* scratch;
+    uint64_t scratch_bytes;
+} dav2_sample_args;
+DAV2_API uint64_t dav2_hip_sample_scratch_bytes(const dav2_sample_args* args);
+DAV2_API int dav2_hip_sample(const dav2_sample_args* args, void* stream);
+
 DAV2_API const char* dav2_hip_error_string(int error);
 
 #ifdef __cplusplus

@@ -238,6 +238,50 @@ DAV2_API dav2_status DAV2_CALL dav2_ops_cross_attention(dav2_ops* ops, dav2_devi
                                                         dav2_device_buffer key_mask, dav2_device_buffer scratch,
                                                         const dav2_cross_attention_args* sizes);
 
+/* As dav2_ops_cache_int8 for dav2_cache_i4. */
+typedef struct dav2_ops_cache_int4 {
+    dav2_device_buffer keys, values, key_scales, value_scales;
+} dav2_ops_cache_int4;
+DAV2_API dav2_status DAV2_CALL dav2_ops_cache_store_int4(dav2_ops* ops, dav2_ops_cache_int4 cache,
+                                                         dav2_device_buffer keys, dav2_device_buffer values,
+                                                         dav2_device_buffer page_table, dav2_device_buffer starts,
+                                                         dav2_device_buffer lengths,
+                                                         const dav2_cache_store_i4_args* sizes);
+/* scratch as for dav2_ops_attention_cache_int8, dav2_hip_attention_cache_i4_scratch_bytes(sizes). */
+DAV2_API dav2_status DAV2_CALL dav2_ops_attention_cache_int4(dav2_ops* ops, dav2_device_buffer output,
+                                                             dav2_device_buffer query, dav2_ops_cache_int4 cache,
+                                                             dav2_device_buffer page_table, dav2_device_buffer starts,
+                                                             dav2_device_buffer lengths, dav2_device_buffer scratch,
+                                                             const dav2_attention_cache_i4_args* sizes);
+
+/* held, added, held_out, lengths: sequences int32; free_pages: pages int32;
+ * free_state, free_state_out: 2 int32; starts: sequences + 1 int32; positions and
+ * owners: tokens int32, slots: tokens int64, each of which may be left out.
+ * held_out may be held, free_state_out free_state. scratch as above,
+ * dav2_hip_cache_plan_scratch_bytes(sizes). */
+typedef struct dav2_ops_cache_plan_buffers {
+    dav2_device_buffer held, added, page_table, free_pages, free_state;
+    dav2_device_buffer held_out, free_state_out, starts, lengths, positions, owners, slots;
+} dav2_ops_cache_plan_buffers;
+DAV2_API dav2_status DAV2_CALL dav2_ops_cache_plan(dav2_ops* ops, const dav2_ops_cache_plan_buffers* buffers,
+                                                   dav2_device_buffer scratch, const dav2_cache_plan_args* sizes);
+
+/* residual, weight, sum, output and codes with scales may be left out, as in dav2_add_rms_norm_args. */
+DAV2_API dav2_status DAV2_CALL dav2_ops_add_rms_norm(dav2_ops* ops, dav2_device_buffer sum, dav2_device_buffer output,
+                                                     dav2_device_buffer codes, dav2_device_buffer scales,
+                                                     dav2_device_buffer input, dav2_device_buffer residual,
+                                                     dav2_device_buffer weight, const dav2_add_rms_norm_args* sizes);
+
+/* temperature, top_k, top_p, min_p and uniform: rows values each; all but the
+ * last may be left out, and probabilities. scratch as above,
+ * dav2_hip_sample_scratch_bytes(sizes). */
+DAV2_API dav2_status DAV2_CALL dav2_ops_sample(dav2_ops* ops, dav2_device_buffer tokens,
+                                               dav2_device_buffer probabilities, dav2_device_buffer logits,
+                                               dav2_device_buffer temperature, dav2_device_buffer top_k,
+                                               dav2_device_buffer top_p, dav2_device_buffer min_p,
+                                               dav2_device_buffer uniform, dav2_device_buffer scratch,
+                                               const dav2_sample_args* sizes);
+
 /* Whole-graph variant of dav2_infer_tensor_f32_device that also returns the
  * depth logits before the final ReLU (batch 1); for parity checks where
  * random weights drive most of the ReLU output to zero. No reference
