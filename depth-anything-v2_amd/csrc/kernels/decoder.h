@@ -134,6 +134,36 @@ DAV2_DEV Sequence sequence_of(const int32_t* starts, const int32_t* lengths, uin
     return q;
 }
 
+// A vector of a row, at any address that an element may have.
+template <typename E>
+struct Vec {
+    static constexpr int N = 16 / sizeof(E);
+    typedef E any __attribute__((ext_vector_type(N), aligned(sizeof(E))));
+    // elements c .. c + N - 1 of a row of `columns`, zeros behind it
+    static DAV2_DEV void load(const E* row, uint32_t c, uint32_t columns, float (&v)[N]) {
+        if (c + N <= columns) {
+            const any x = *reinterpret_cast<const any*>(row + c);
+#pragma unroll
+            for (int i = 0; i < N; ++i) v[i] = static_cast<float>(x[i]);
+        } else {
+#pragma unroll
+            for (int i = 0; i < N; ++i) v[i] = c + i < columns ? static_cast<float>(row[c + i]) : 0.0f;
+        }
+    }
+    static DAV2_DEV void store(E* row, uint32_t c, uint32_t columns, const float (&v)[N]) {
+        if (c + N <= columns) {
+            any x;
+#pragma unroll
+            for (int i = 0; i < N; ++i) x[i] = static_cast<E>(v[i]);
+            *reinterpret_cast<any*>(row + c) = x;
+        } else {
+#pragma unroll
+            for (int i = 0; i < N; ++i)
+                if (c + i < columns) row[c + i] = static_cast<E>(v[i]);
+        }
+    }
+};
+
 typedef _Float16 h8 __attribute__((ext_vector_type(8)));
 typedef __bf16 b8 __attribute__((ext_vector_type(8)));
 typedef float v16f __attribute__((ext_vector_type(16)));
