@@ -23,7 +23,7 @@ using namespace dav2k;
 namespace {
 
 constexpr uint32_t kThreads = 1024, kWaves = kThreads / 64, kDigits = 2048;
-constexpr uint32_t kBins = 1024;        // of a row: 48 powers of two, the last one what is further
+constexpr uint32_t kBins = 2048;        // of a row: 48 powers of two, the last one what is further
 constexpr uint32_t kList = 4096;        // tokens of a row's list
 constexpr uint32_t kMostChunks = 64;    // workgroups that share a row
 constexpr uint32_t kChunkThreads = 256;
@@ -63,46 +63,64 @@ DAV2_DEV Asked asked_of(const dav2_sample_args& a, uint32_t row) {
     return q;
 }
 
-// 2^x for x <= 0: x = n + f, |f| <= 1/2, and the Taylor polynomial of e^(f ln 2) of
-// degree 13, whose rest is below 2^-57. Below 2^-100 it is 0.
+// 2^x for -100 < x <= 0: x = n + f, |f| <= 1/2, and the Taylor polynomial of 2^f of
+// degree 11, whose rest is below 2^-47. n is the low word of x + 1.5 * 2^52.
 DAV2_DEV double exp2_of(double x) {
-    constexpr double kLn2 = 0.69314718055994530942;
-    if (!(x > -100.0)) return 0.0;
-    const double n = rint(x), f = (x - n) * kLn2;
-    double p = 1.0 / 6227020800.0;
-    p = fma(p, f, 1.0 / 479001600.0);
-    p = fma(p, f, 1.0 / 39916800.0);
-    p = fma(p, f, 1.0 / 3628800.0);
-    p = fma(p, f, 1.0 / 362880.0);
-    p = fma(p, f, 1.0 / 40320.0);
-    p = fma(p, f, 1.0 / 5040.0);
-    p = fma(p, f, 1.0 / 720.0);
-    p = fma(p, f, 1.0 / 120.0);
-    p = fma(p, f, 1.0 / 24.0);
-    p = fma(p, f, 1.0 / 6.0);
-    p = fma(p, f, 0.5);
+    constexpr double kLn2 = 0.69314718055994530942, kRound = 0x1.8p52;
+    constexpr double c2 = kLn2 * kLn2 / 2, c3 = c2 * kLn2 / 3, c4 = c3 * kLn2 / 4, c5 = c4 * kLn2 / 5,
+                     c6 = c5 * kLn2 / 6, c7 = c6 * kLn2 / 7, c8 = c7 * kLn2 / 8, c9 = c8 * kLn2 / 9,
+                     c10 = c9 * kLn2 / 10, c11 = c10 * kLn2 / 11;
+    const double rounded = x + kRound, f = x - (rounded - kRound);
+    double p = fma(c11, f, c10);
+    p = fma(p, f, c9);
+    p = fma(p, f, c8);
+    p = fma(p, f, c7);
+    p = fma(p, f, c6);
+    p = fma(p, f, c5);
+    p = fma(p, f, c4);
+    p = fma(p, f, c3);
+    p = fma(p, f, c2);
+    p = fma(p, f, kLn2);
     p = fma(p, f, 1.0);
-    p = fma(p, f, 1.0);
-    return ldexp(p, static_cast<int>(n));
+    const int n = static_cast<int>(__double2loint(rounded));
+    return p * __hiloint2double((n + 1023) << 20, 0);
 }
 
 // exp((l - top) / temperature) in 64 bits. An infinite top has weight 1 and all others none.
 DAV2_DEV double weight_of(float l, float top, double per_temperature) {
     if (l == top) return 1.0;
-    if (!(top < INFINITY)) return 0.0;
-    return exp2_of((static_cast<double>(l) - static_cast<double>(top)) * per_temperature);
+    const double x = (static_cast<double>(l) - static_cast<double>(top)) * per_temperature;
+    return x > -100.0 ? exp2_of(x) : 0.0;  // a NaN is infinity less infinity
 }
-// ... in units of 2^-bits, bits <= 62
+// ... in units of 2^-bits, bits <= 46: the sum with 2^52 is rounded to a whole number, in its low 52 bits
 DAV2_DEV uint64_t units_of(double weight, int bits) {
-    const double v = ldexp(weight, bits) + 0.5;
-    const uint32_t hi = static_cast<uint32_t>(v * 0x1p-32);
-    return (static_cast<uint64_t>(hi) << 32) + static_cast<uint32_t>(fma(static_cast<double>(hi), -0x1p32, v));
+    const double v = weight * __hiloint2double((bits + 1023) << 20, 0) + 0x1p52;
+    return static_cast<uint64_t>(__double_as_longlong(v)) & 0xfffffffffffffull;
 }
 
-DAV2_DEV uint64_t wave_sum64(uint64_t v) {
-    for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(static_cast<unsigned long long>(v), o, kWave);
+// The sum over the lanes up to this one: within rows of 16 lanes by row shifts,
+// then a row's last sum into the rows behind it.
+template <int CTRL, int ROWS>
+DAV2_DEV uint64_t moved64(uint64_t v) {
+    const int lo = __builtin_amdgcn_update_dpp(0, static_cast<int>(static_cast<uint32_t>(v)), CTRL, ROWS, 0xf, true);
+    const int hi = __builtin_amdgcn_update_dpp(0, static_cast<int>(static_cast<uint32_t>(v >> 32)), CTRL, ROWS, 0xf, true);
+    return (static_cast<uint64_t>(static_cast<uint32_t>(hi)) << 32) | static_cast<uint32_t>(lo);
+}
+DAV2_DEV uint64_t wave_upto(uint64_t v) {
+    v += moved64<0x111, 0xf>(v);  // row_shr:1
+    v += moved64<0x112, 0xf>(v);
+    v += moved64<0x114, 0xf>(v);
+    v += moved64<0x118, 0xf>(v);  // row_shr:8
+    v += moved64<0x142, 0xa>(v);  // row_bcast:15 into rows 1 and 3
+    v += moved64<0x143, 0xc>(v);  // row_bcast:31 into rows 2 and 3
     return v;
 }
+DAV2_DEV uint64_t lane63(uint64_t v) {
+    const uint32_t lo = __builtin_amdgcn_readlane(static_cast<int>(static_cast<uint32_t>(v)), 63);
+    const uint32_t hi = __builtin_amdgcn_readlane(static_cast<int>(static_cast<uint32_t>(v >> 32)), 63);
+    return (static_cast<uint64_t>(hi) << 32) | lo;
+}
+DAV2_DEV uint64_t wave_sum64(uint64_t v) { return lane63(wave_upto(v)); }
 
 // of the search in the row itself
 struct Shared {
@@ -125,21 +143,20 @@ DAV2_DEV uint64_t group_sum(uint64_t v, uint64_t* of_wave) {
     return v;
 }
 
-// The sum over the threads before this one.
-DAV2_DEV uint64_t group_before(uint64_t v, uint64_t* of_wave) {
-    uint64_t upto = v;
+// The sum over the threads before this one, and over the workgroup.
+DAV2_DEV uint64_t group_before(uint64_t v, uint64_t* of_wave, uint64_t& all) {
+    const uint64_t upto = wave_upto(v);
     const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6;
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-        const uint64_t other = __shfl_up(static_cast<unsigned long long>(upto), o, kWave);
-        if (lane >= static_cast<uint32_t>(o)) upto += other;
-    }
     __syncthreads();
     if (lane == 63u) of_wave[wave] = upto;
     __syncthreads();
     uint64_t before = 0;
+    all = 0;
 #pragma unroll
-    for (uint32_t w = 0; w < kWaves; ++w) before += w < wave ? of_wave[w] : 0;
+    for (uint32_t w = 0; w < kWaves; ++w) {
+        before += w < wave ? of_wave[w] : 0;
+        all += of_wave[w];
+    }
     return before + upto - v;
 }
 
@@ -214,8 +231,9 @@ struct Row {
             // two digits for each thread
             const uint32_t d0 = 2u * threadIdx.x;
             const uint64_t c0 = sh.counts[d0], c1 = sh.counts[d0 + 1], s0 = sh.sums[d0], s1 = sh.sums[d0 + 1];
-            const uint64_t count_before = count + group_before(c0 + c1, sh.of_wave);
-            const uint64_t sum_before = sum + group_before(s0 + s1, sh.of_wave);
+            uint64_t all;
+            const uint64_t count_before = count + group_before(c0 + c1, sh.of_wave, all);
+            const uint64_t sum_before = sum + group_before(s0 + s1, sh.of_wave, all);
             const uint64_t before = BY_SUM ? sum_before : count_before;
             const uint64_t a0 = BY_SUM ? s0 : c0, a1 = BY_SUM ? s1 : c1;
             if (before <= bound && bound < before + a0 + a1) {
@@ -239,8 +257,8 @@ struct Row {
         for (uint32_t first = 0; first < vocabulary; first += kThreads) {
             const uint32_t i = first + threadIdx.x;
             const bool is = i < vocabulary && rank_key(logit(i)) == key && end.after(key, i);
-            const uint64_t before = group_before(is, sh.of_wave);
-            const uint64_t all = group_sum(is, sh.of_wave);
+            uint64_t all;
+            const uint64_t before = group_before(is, sh.of_wave, all);
             if (all > left) {  // the same for all threads
                 if (is && before == left) sh.found = i;
                 __syncthreads();
@@ -288,26 +306,27 @@ struct RowState {
     unsigned long long list[kList];  // rank key, index
 };
 
-// f(logit, index) for the elements [begin, end) of a row, by kChunkThreads threads.
-template <typename E, typename F>
+// f(logit, index) for the elements [begin, end) of a row, by THREADS threads.
+template <uint32_t THREADS, typename E, typename F>
 DAV2_DEV void for_each(const E* row, uint32_t begin, uint32_t end, F&& f) {
     typedef Vec<E> V;
-    constexpr uint32_t N = V::N, kTogether = 4;  // loads that are under way together
-    for (uint32_t c0 = begin + threadIdx.x * N; c0 < end; c0 += kTogether * kChunkThreads * N) {
+    constexpr uint32_t N = V::N, kTogether = 4, kStep = THREADS * N;  // loads that are under way together
+    uint32_t c = begin + threadIdx.x * N;
+    for (; c + (kTogether - 1u) * kStep + N <= end; c += kTogether * kStep) {
         float v[kTogether][N];
 #pragma unroll
-        for (uint32_t t = 0; t < kTogether; ++t) {
-            const uint32_t c = c0 + t * kChunkThreads * N;
-            if (c < end) V::load(row, c, end, v[t]);
-        }
+        for (uint32_t t = 0; t < kTogether; ++t) V::load(row, c + t * kStep, ~0u, v[t]);
 #pragma unroll
-        for (uint32_t t = 0; t < kTogether; ++t) {
-            const uint32_t c = c0 + t * kChunkThreads * N;
-            if (c >= end) break;
+        for (uint32_t t = 0; t < kTogether; ++t)
 #pragma unroll
-            for (uint32_t i = 0; i < N; ++i)
-                if (c + i < end) f(v[t][i], c + i);
-        }
+            for (uint32_t i = 0; i < N; ++i) f(v[t][i], c + t * kStep + i);
+    }
+    for (; c < end; c += kStep) {
+        float v[N];
+        V::load(row, c, end, v);
+#pragma unroll
+        for (uint32_t i = 0; i < N; ++i)
+            if (c + i < end) f(v[i], c + i);
     }
 }
 
@@ -318,6 +337,7 @@ DAV2_DEV Chunk chunk_of(const dav2_sample_args& a, uint32_t length) {
     const uint32_t begin = blockIdx.x * length;
     return {blockIdx.y, min(begin, a.vocabulary), min(begin + length, a.vocabulary)};
 }
+DAV2_DEV unsigned long long list_entry(float l, uint32_t i) { return (static_cast<uint64_t>(rank_key(l)) << 32) | i; }
 template <typename E>
 DAV2_DEV const E* row_of(const dav2_sample_args& a, uint32_t row) {
     return static_cast<const E*>(a.logits) + row * a.logit_stride;
@@ -328,13 +348,14 @@ DAV2_DEV float top_of(const RowState& state, uint32_t chunks) {
 }
 
 // The bin of a logit: no larger for a larger one, as each rounding keeps the order.
+// What the last one has weighs nothing: 2^-48 rounds to 0 in units of 2^-46.
 struct Bins {
-    float top, scale;
-    DAV2_DEV Bins(float top_, const Asked& q) : top(top_), scale(static_cast<float>(q.per_temperature * (kBins / 48.0))) {}
+    float top, scale;  // finite
+    DAV2_DEV Bins(float top_, const Asked& q)
+        : top(fminf(top_, 3.0e38f)), scale(fminf(static_cast<float>(q.per_temperature * (kBins / 48.0)), 3.0e38f)) {}
     DAV2_DEV uint32_t operator()(float l) const {
-        if (l == top) return 0u;
-        const float x = (top - l) * scale;
-        return x < static_cast<float>(kBins - 1u) ? static_cast<uint32_t>(x) : kBins - 1u;  // NaN in the last
+        // NaN is in the last one: no number, or -infinity times nothing
+        return static_cast<uint32_t>(fmaxf(fminf((top - l) * scale, static_cast<float>(kBins - 1u)), 0.0f));
     }
 };
 
@@ -344,7 +365,7 @@ __global__ __launch_bounds__(kChunkThreads) void sample_largest_kernel(dav2_samp
     const Chunk chunk = chunk_of(a, length);
     RowState& state = static_cast<RowState*>(a.scratch)[chunk.row];
     float top = -INFINITY;
-    for_each(row_of<E>(a, chunk.row), chunk.begin, chunk.end, [&](float l, uint32_t) { top = fmaxf(top, l); });
+    for_each<kChunkThreads>(row_of<E>(a, chunk.row), chunk.begin, chunk.end, [&](float l, uint32_t) { top = fmaxf(top, l); });
     top = wave_max(top);
     if ((threadIdx.x & 63u) == 0) of_wave[threadIdx.x >> 6] = top;
     for (uint32_t b = blockIdx.x * kChunkThreads + threadIdx.x; b < kBins; b += gridDim.x * kChunkThreads) {
@@ -356,6 +377,39 @@ __global__ __launch_bounds__(kChunkThreads) void sample_largest_kernel(dav2_samp
     if (threadIdx.x == 0) state.largest[blockIdx.x] = fmaxf(fmaxf(of_wave[0], of_wave[1]), fmaxf(of_wave[2], of_wave[3]));
 }
 
+// By a wave: the first of from .. to that is so, where all behind one that is so
+// are; `to`, if none is before it. 64 of them are asked at a time.
+template <typename F>
+DAV2_DEV uint32_t first_where(uint32_t from, uint32_t to, F&& so) {
+    const uint32_t lane = threadIdx.x & 63u;
+    while (from < to) {
+        const uint32_t step = (to - from - 1u) / 64u + 1u, at = min(from + lane * step, to);
+        const uint32_t before = static_cast<uint32_t>(__popcll(__ballot(at < to && !so(at))));  // lanes before it
+        if (before == 0) return from;
+        to = min(from + before * step, to);
+        from += (before - 1u) * step + 1u;
+    }
+    return to;
+}
+
+// What the elements [begin, end) of a row add to its bins, in LDS: weights
+// where the list may not have all that is kept, counts where there is a top-k.
+template <uint32_t THREADS, typename E>
+DAV2_DEV void fill_bins(const Row<E>& row, uint32_t begin, uint32_t end, uint32_t* counts, unsigned long long* sums) {
+    const Bins bin_of(row.top, row.q);
+    if (row.q.top_k <= kFew) {
+        for_each<THREADS>(row.logits, begin, end, [&](float l, uint32_t) { atomicAdd(&counts[bin_of(l)], 1u); });
+        return;
+    }
+    const bool counted = row.q.top_k < row.vocabulary;
+    for_each<THREADS>(row.logits, begin, end, [&](float l, uint32_t) {
+        const uint32_t b = bin_of(l);
+        if (counted) atomicAdd(&counts[b], 1u);
+        const uint64_t w = row.units(rank_key(l));
+        if (w) atomicAdd(&sums[b], static_cast<unsigned long long>(w));
+    });
+}
+
 template <typename E>
 __global__ __launch_bounds__(kChunkThreads) void sample_bins_kernel(dav2_sample_args a, uint32_t length, int bits) {
     __shared__ uint32_t counts[kBins];
@@ -364,23 +418,13 @@ __global__ __launch_bounds__(kChunkThreads) void sample_bins_kernel(dav2_sample_
     RowState& state = static_cast<RowState*>(a.scratch)[chunk.row];
     const float top = top_of(state, gridDim.x);
     if (!(top > -INFINITY)) return;
-    const Asked q = asked_of(a, chunk.row);
-    const Row<E> row = {row_of<E>(a, chunk.row), a.vocabulary, bits, top, q};
-    const Bins bin_of(top, q);
+    const Row<E> row = {row_of<E>(a, chunk.row), a.vocabulary, bits, top, asked_of(a, chunk.row)};
     for (uint32_t b = threadIdx.x; b < kBins; b += kChunkThreads) {
         counts[b] = 0;
         sums[b] = 0;
     }
     __syncthreads();
-    const bool weighed = q.top_k > kFew;
-    for_each(row.logits, chunk.begin, chunk.end, [&](float l, uint32_t) {
-        const uint32_t b = bin_of(l);
-        atomicAdd(&counts[b], 1u);
-        if (weighed) {
-            const uint64_t w = row.units(rank_key(l));
-            if (w) atomicAdd(&sums[b], static_cast<unsigned long long>(w));
-        }
-    });
+    fill_bins<kChunkThreads>(row, chunk.begin, chunk.end, counts, sums);
     __syncthreads();
     for (uint32_t b = threadIdx.x; b < kBins; b += kChunkThreads) {
         if (counts[b]) atomicAdd(&state.counts[b], counts[b]);
@@ -396,31 +440,25 @@ struct BinScan {
         uint64_t of_wave[2][THREADS / 64];
         uint32_t found[8];
         uint64_t sums[4];  // before and of bins that were found
+        float bounds[6];
     };
     uint32_t counts[N], count_before;
     uint64_t sums[N], sum_before, whole;
     uint32_t low[3], high[3];  // bins of the list, both ends among them
+    float most[3], least[3];   // logits of them
+    int ranges;
 
-    DAV2_DEV void load(const RowState& state, Shared& sh) {
+    DAV2_DEV void load(const uint32_t* of_counts, const unsigned long long* of_sums, Shared& sh) {
         const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6;
         uint64_t count = 0, sum = 0;
 #pragma unroll
         for (uint32_t i = 0; i < N; ++i) {
-            counts[i] = state.counts[threadIdx.x * N + i];
-            sums[i] = state.sums[threadIdx.x * N + i];
+            counts[i] = of_counts[threadIdx.x * N + i];
+            sums[i] = of_sums[threadIdx.x * N + i];
             count += counts[i];
             sum += sums[i];
         }
-        uint64_t c = count, s = sum;
-#pragma unroll
-        for (int o = 1; o < 64; o <<= 1) {
-            const uint64_t c1 = __shfl_up(static_cast<unsigned long long>(c), o, kWave);
-            const uint64_t s1 = __shfl_up(static_cast<unsigned long long>(s), o, kWave);
-            if (lane >= static_cast<uint32_t>(o)) {
-                c += c1;
-                s += s1;
-            }
-        }
+        uint64_t c = wave_upto(count), s = wave_upto(sum);
         if (lane == 63u) {
             sh.of_wave[0][wave] = c;
             sh.of_wave[1][wave] = s;
@@ -458,7 +496,7 @@ struct BinScan {
     // sums that bound the second and third are known as ranges.
     DAV2_DEV void choose(const Asked& q, uint32_t vocabulary, int bits, Shared& sh) {
         const bool by_count = q.top_k < vocabulary;
-        uint64_t least = whole, most = whole;  // what top-k leaves
+        uint64_t lower = whole, upper = whole;  // what top-k leaves
         if (threadIdx.x < 8) sh.found[threadIdx.x] = 0;
         __syncthreads();
         if (by_count) {
@@ -471,8 +509,9 @@ struct BinScan {
             });
             __syncthreads();
             low[0] = high[0] = sh.found[0];
-            least = sh.sums[0];
-            most = sh.sums[1];
+            if (high[0] == kBins - 1u) high[0] -= 1u;  // where that ends does not matter
+            lower = sh.sums[0];
+            upper = sh.sums[1];
         } else {
             low[0] = 1;
             high[0] = 0;
@@ -484,7 +523,7 @@ struct BinScan {
             return;
         }
         const uint64_t one = 1ull << bits;  // the first token's weight, which always stays
-        least = max(least, one);
+        lower = max(lower, one);
         auto range = [&](uint64_t from, uint64_t to, uint32_t which, bool keep_sums) {
             each([&](uint32_t b, uint32_t, uint32_t, uint64_t s, uint64_t m) {
                 if (s <= from && from < s + m) {
@@ -503,200 +542,560 @@ struct BinScan {
         low[1] = 1;
         high[1] = 0;
         if (q.top_p < 1.0) {
-            range(share_of(q.top_p, least), share_of(q.top_p, most), 2, true);
-            least = max(sh.sums[2], one);
-            most = min(sh.sums[3], most);
+            range(share_of(q.top_p, lower), share_of(q.top_p, upper), 2, true);
+            lower = max(sh.sums[2], one);
+            upper = min(sh.sums[3], upper);
         }
-        range(drawn_of(q, least), drawn_of(q, most), 4, false);
+        range(drawn_of(q, lower), drawn_of(q, upper), 4, false);
     }
-    // Tokens of those bins.
-    DAV2_DEV uint32_t listed(Shared& sh) const {
-        each([&](uint32_t b, uint32_t, uint32_t n, uint64_t, uint64_t) {
-            if (n && lists(b)) atomicAdd(&sh.found[7], n);
-        });
+    // The logits of those bins: the largest and the least of each range.
+    DAV2_DEV void bound(const Bins& bin_of, Shared& sh) {
+        for (uint32_t i = threadIdx.x >> 6; i < 6u; i += THREADS / 64u) {
+            const uint32_t which = i / 2u, last = i & 1u;
+            const uint32_t l = which == 0 ? low[0] : which == 1 ? low[1] : low[2];
+            const uint32_t h = which == 0 ? high[0] : which == 1 ? high[1] : high[2];
+            const uint32_t key = first_where(rank_key(INFINITY), rank_key(-INFINITY),
+                                             [&](uint32_t k) { return bin_of(logit_of(k)) >= (last ? h + 1u : l); });
+            if ((threadIdx.x & 63u) == 0)
+                sh.bounds[i] = l > h ? (last ? INFINITY : -INFINITY) : logit_of(last ? key - 1u : key);
+        }
         __syncthreads();
-        return sh.found[7];
+#pragma unroll
+        for (int i = 0; i < 3; ++i) {
+            most[i] = sh.bounds[2 * i];
+            least[i] = sh.bounds[2 * i + 1];
+        }
+        ranges = low[1] <= high[1] ? 3 : low[2] <= high[2] ? 2 : 1;
     }
-    DAV2_DEV bool lists(uint32_t b) const {
-        return (b >= low[0] && b <= high[0]) || (b >= low[1] && b <= high[1]) || (b >= low[2] && b <= high[2]);
+    DAV2_DEV bool lists(float l) const {
+        return (l <= most[0] && l >= least[0]) || (l <= most[1] && l >= least[1]) || (l <= most[2] && l >= least[2]);
     }
 };
+
+// f for the tokens of [begin, end) in those bins, which are few: a branch for
+// the elements that a thread loads together, not for each of them.
+template <uint32_t THREADS, typename E, typename Scan, typename F>
+DAV2_DEV void for_listed(const Row<E>& row, const Scan& scan, uint32_t begin, uint32_t end, F&& f) {
+    typedef Vec<E> V;
+    constexpr uint32_t N = V::N, kTogether = 4, kStep = THREADS * N;
+    auto pass = [&](auto ranges) {
+        auto is = [&](float l) {
+            bool in = l <= scan.most[0] && l >= scan.least[0];
+            if constexpr (decltype(ranges)::value > 1) in = in || (l <= scan.most[2] && l >= scan.least[2]);
+            if constexpr (decltype(ranges)::value > 2) in = in || (l <= scan.most[1] && l >= scan.least[1]);
+            return in;
+        };
+        uint32_t c = begin + threadIdx.x * N;
+        for (; c + (kTogether - 1u) * kStep + N <= end; c += kTogether * kStep) {
+            float v[kTogether][N];
+#pragma unroll
+            for (uint32_t t = 0; t < kTogether; ++t) V::load(row.logits, c + t * kStep, ~0u, v[t]);
+#pragma unroll
+            for (uint32_t t = 0; t < kTogether; ++t) {
+                bool any = false;
+#pragma unroll
+                for (uint32_t i = 0; i < N; ++i) any |= is(v[t][i]);
+                if (__builtin_expect(any, 0)) {
+#pragma unroll
+                    for (uint32_t i = 0; i < N; ++i)
+                        if (is(v[t][i])) f(list_entry(v[t][i], c + t * kStep + i));
+                }
+            }
+        }
+        for (; c < end; c += kStep)
+            for (uint32_t i = c; i < min(c + N, end); ++i) {
+                const float l = static_cast<float>(row.logits[i]);
+                if (is(l)) f(list_entry(l, i));
+            }
+    };
+    if (scan.ranges == 1) pass(std::integral_constant<int, 1>());
+    else if (scan.ranges == 2) pass(std::integral_constant<int, 2>());
+    else pass(std::integral_constant<int, 3>());
+}
 
 template <typename E>
 __global__ __launch_bounds__(kChunkThreads) void sample_list_kernel(dav2_sample_args a, uint32_t length, int bits) {
     __shared__ typename BinScan<kChunkThreads>::Shared sh;
+    __shared__ unsigned long long staged[kList];
+    __shared__ uint32_t here, first;
     const Chunk chunk = chunk_of(a, length);
     RowState& state = static_cast<RowState*>(a.scratch)[chunk.row];
     const float top = top_of(state, gridDim.x);
     if (!(top > -INFINITY)) return;
-    const Asked q = asked_of(a, chunk.row);
-    const Bins bin_of(top, q);
+    if (threadIdx.x == 0) here = 0;
+    const Row<E> row = {row_of<E>(a, chunk.row), a.vocabulary, bits, top, asked_of(a, chunk.row)};
     BinScan<kChunkThreads> scan;
-    scan.load(state, sh);
-    scan.choose(q, a.vocabulary, bits, sh);
-    if (scan.listed(sh) > kList) {
-        if (blockIdx.x == 0 && threadIdx.x == 0) state.listed = kList + 1u;
-        return;
-    }
-    for_each(row_of<E>(a, chunk.row), chunk.begin, chunk.end, [&](float l, uint32_t i) {
-        if (!scan.lists(bin_of(l))) return;
-        state.list[atomicAdd(&state.listed, 1u)] = (static_cast<uint64_t>(rank_key(l)) << 32) | i;
+    scan.load(state.counts, state.sums, sh);
+    scan.choose(row.q, a.vocabulary, bits, sh);
+    scan.bound(Bins(row.top, row.q), sh);
+    for_listed<kChunkThreads>(row, scan, chunk.begin, chunk.end, [&](unsigned long long entry) {
+        const uint32_t at = atomicAdd(&here, 1u);
+        if (at < kList) staged[at] = entry;
     });
+    __syncthreads();
+    if (here == 0) return;
+    if (threadIdx.x == 0) first = atomicAdd(&state.listed, here);
+    __syncthreads();
+    for (uint32_t i = threadIdx.x; first + i < kList && i < here; i += kChunkThreads) state.list[first + i] = staged[i];
 }
 
-// The list of a row sorted, and the searches ended in it: a workgroup for each
-// row. chunks 0: the row is short enough to be its own list.
-template <typename E>
-__global__ __launch_bounds__(kThreads) void sample_pick_kernel(dav2_sample_args a, uint32_t chunks, int bits) {
-    typedef typename Row<E>::Place Place;
-    __shared__ union {
+// A list sorted into LDS: entry(i) is its i-th, all different.
+template <typename F>
+DAV2_DEV void sort_list(unsigned long long* list, uint32_t listed, F&& entry) {
+    constexpr uint32_t kCounted = 512;
+    if (listed <= kCounted) {
+        // how many are before it says where a token goes: two or four threads
+        // for each, and nothing to wait for between
+        typedef unsigned long long U2 __attribute__((ext_vector_type(2)));
+        unsigned long long* const raw = list + kList - kCounted;
+        if (threadIdx.x < kCounted) raw[threadIdx.x] = entry(threadIdx.x);
+        __syncthreads();
+        const uint32_t sharing = listed <= kCounted / 2 ? 2u : 1u;  // log2 of the threads
+        const uint32_t i = threadIdx.x >> sharing, part = threadIdx.x & ((1u << sharing) - 1u);
+        const uint32_t pairs = (((listed + 1u) / 2u) >> sharing) + 1u;  // of each thread
+        const unsigned long long mine = raw[i];
+        uint32_t before = 0;
+#pragma unroll 8
+        for (uint32_t j = 0; j < pairs; ++j) {
+            // past the last the first again, counted by nobody
+            const uint32_t p = part * pairs + j;
+            const U2 x = reinterpret_cast<const U2*>(raw)[min(p, kCounted / 2 - 1u)];
+            before += (x[0] < mine) & (2u * p < listed);
+            before += (x[1] < mine) & (2u * p + 1u < listed);
+        }
+        before += __shfl_xor(static_cast<int>(before), 1, kWave);
+        if (sharing == 2u) before += __shfl_xor(static_cast<int>(before), 2, kWave);
+        if (i < listed && part == 0) list[before] = mine;
+        __syncthreads();
+        return;
+    }
+    uint32_t size = 2 * kCounted;
+    while (size < listed) size *= 2;
+    for (uint32_t i = threadIdx.x; i < size; i += kThreads) list[i] = entry(i);
+    __syncthreads();
+    for (uint32_t k = 2; k <= size; k *= 2)
+        for (uint32_t j = k / 2; j > 0; j /= 2) {
+            for (uint32_t t = threadIdx.x; t < size / 2; t += kThreads) {
+                const uint32_t i = 2 * t - (t & (j - 1)), p = i + j;
+                const unsigned long long x = list[i], y = list[p];
+                if ((x > y) == ((i & k) == 0)) {
+                    list[i] = y;
+                    list[p] = x;
+                }
+            }
+            __syncthreads();
+        }
+}
+
+// What a workgroup that ends a row's searches has in LDS; KEYS: with a count for
+// each number of 16 bits, two of them to a word.
+constexpr uint32_t kKeyWords = 32768;
+template <bool KEYS = false>
+struct Finish {
+    union {
         Shared search;
         unsigned long long list[kList];
-    } sh;
-    __shared__ typename BinScan<kThreads>::Shared bins;
-    __shared__ uint64_t sums_before[kBins];  // of a bin, less the list's sum before it
-    __shared__ uint32_t counts_before[kBins];
-    __shared__ uint64_t of_wave[kWaves], result[2];
-    __shared__ int32_t token;
-    __shared__ float share;
-    constexpr uint32_t kEach = kList / kThreads;
-    const uint32_t r = blockIdx.x;
-    const RowState* state = chunks ? static_cast<const RowState*>(a.scratch) + r : nullptr;
-    Row<E> row = {row_of<E>(a, r), a.vocabulary, bits, 0.0f, asked_of(a, r)};
-    const Asked& q = row.q;
+        uint32_t keys[KEYS ? kKeyWords : 1];
+    };
+    unsigned long long sums[kBins];  // of a bin; then before it, less the list's sum there
+    uint32_t counts[kBins];
+    typename BinScan<kThreads>::Shared bins;
+    uint64_t of_wave[kWaves], result[2];
+    float tops[kWaves];
+    int32_t token;
+    float share;
     uint32_t listed;
-    if (threadIdx.x == 0) {
-        token = -1;
-        share = 0.0f;
-    }
-    if (chunks) {
-        row.top = top_of(*state, chunks);
-        listed = state->listed;
-    } else {
-        float top = -INFINITY;
-        for (uint32_t i = threadIdx.x; i < a.vocabulary; i += kThreads) top = fmaxf(top, row.logit(i));
-        top = wave_max(top);
-        float* tops = reinterpret_cast<float*>(of_wave);
-        if ((threadIdx.x & 63u) == 0) tops[threadIdx.x >> 6] = top;
-        __syncthreads();
-        for (uint32_t w = 0; w < kWaves; ++w) top = fmaxf(top, tops[w]);
-        row.top = top + 0.0f;
-        listed = a.vocabulary;
-    }
+};
+
+// The searches ended in the row's list, whose i-th token is entry(i). gaps: bins
+// lie between those of the list; sums and counts are then those before each bin,
+// and whole the sum of all.
+template <uint32_t kEach, typename E, typename F>
+DAV2_DEV void finish_sorted(const Row<E>& row, F& sh, uint32_t listed, bool gaps, uint64_t whole) {
+    const Asked& q = row.q;
     const Bins bin_of(row.top, q);
-    // whether bins lie between those of the list
-    const bool gaps = chunks && q.top_k > kFew;
-    uint64_t whole = 0;
-    __syncthreads();
-    if (row.top > -INFINITY && listed > kList) {
-        search_row(row, sh.search, &token, &share);
-    } else if (row.top > -INFINITY) {
-        if (gaps) {
-            BinScan<kThreads> scan;
-            scan.load(*state, bins);
-            scan.each([&](uint32_t b, uint32_t c, uint32_t, uint64_t s, uint64_t) {
-                sums_before[b] = s;
-                counts_before[b] = c;
-            });
-            whole = scan.whole;
-        }
-        uint32_t size = 2;
-        while (size < listed) size *= 2;
-        for (uint32_t i = threadIdx.x; i < size; i += kThreads)
-            sh.list[i] = i >= listed ? ~0ull
-                         : chunks    ? state->list[i]
-                                     : (static_cast<uint64_t>(rank_key(row.logit(i))) << 32) | i;
-        __syncthreads();
-        for (uint32_t k = 2; k <= size; k *= 2)
-            for (uint32_t j = k / 2; j > 0; j /= 2) {
-                for (uint32_t t = threadIdx.x; t < size / 2; t += kThreads) {
-                    const uint32_t i = 2 * t - (t & (j - 1)), p = i + j;
-                    const unsigned long long x = sh.list[i], y = sh.list[p];
-                    if ((x > y) == ((i & k) == 0)) {
-                        sh.list[i] = y;
-                        sh.list[p] = x;
-                    }
-                }
-                __syncthreads();
-            }
-        // neighbouring tokens for each thread, and the sums before them
-        uint64_t w[kEach], sum = 0;
-        uint32_t key[kEach], bin[kEach];
+    // neighbouring tokens for each thread, and the sums before them
+    uint64_t w[kEach], sum = 0;
+    uint32_t key[kEach], bin[kEach];
+#pragma unroll
+    for (uint32_t e = 0; e < kEach; ++e) {
+        const uint32_t i = threadIdx.x * kEach + e;
+        key[e] = i < listed ? static_cast<uint32_t>(sh.list[i] >> 32) : ~0u;
+        w[e] = i < listed ? row.units(key[e]) : 0;
+        bin[e] = gaps && i < listed ? bin_of(logit_of(key[e])) : 0u;
+        sum += w[e];
+    }
+    uint64_t all;
+    const uint64_t before = group_before(sum, sh.of_wave, all);
+    if (gaps) {
+        // a bin's first token says where the bin is in the list
+        uint64_t at = before;
 #pragma unroll
         for (uint32_t e = 0; e < kEach; ++e) {
             const uint32_t i = threadIdx.x * kEach + e;
-            key[e] = i < listed ? static_cast<uint32_t>(sh.list[i] >> 32) : ~0u;
-            w[e] = i < listed ? row.units(key[e]) : 0;
-            bin[e] = gaps && i < listed ? bin_of(logit_of(key[e])) : 0u;
-            sum += w[e];
+            if (i < listed && (i == 0 || bin_of(logit_of(static_cast<uint32_t>(sh.list[i - 1] >> 32))) != bin[e])) {
+                sh.sums[bin[e]] -= at;
+                sh.counts[bin[e]] -= i;
+            }
+            at += w[e];
         }
-        uint64_t before = group_before(sum, of_wave);
-        const uint64_t all = group_sum(sum, of_wave);
-        if (!gaps) whole = all;
-        uint64_t at = before;
-        if (gaps) {
-            // a bin's first token says where the bin is in the list
+    } else {
+        whole = all;
+    }
+    // where top-k ends in the last bin, the whole is that of all others
+    if (threadIdx.x == 0) sh.result[0] = whole;
+    __syncthreads();
+    // f(token of the list, its rank, the sum before it)
+    auto each = [&](auto&& f) {
+        uint64_t s = before;
 #pragma unroll
-            for (uint32_t e = 0; e < kEach; ++e) {
-                const uint32_t i = threadIdx.x * kEach + e;
-                if (i < listed && (i == 0 || bin_of(logit_of(static_cast<uint32_t>(sh.list[i - 1] >> 32))) != bin[e])) {
-                    sums_before[bin[e]] -= at;
-                    counts_before[bin[e]] -= i;
-                }
-                at += w[e];
-            }
-            __syncthreads();
+        for (uint32_t e = 0; e < kEach; ++e) {
+            const uint32_t i = threadIdx.x * kEach + e;
+            if (i < listed) f(e, gaps ? i + sh.counts[bin[e]] : i, gaps ? s + sh.sums[bin[e]] : s);
+            s += w[e];
         }
-        // f(token of the list, its rank, the sum before it)
-        auto each = [&](auto&& f) {
-            uint64_t s = before;
-#pragma unroll
-            for (uint32_t e = 0; e < kEach; ++e) {
-                const uint32_t i = threadIdx.x * kEach + e;
-                if (i < listed) f(e, gaps ? i + counts_before[bin[e]] : i, gaps ? s + sums_before[bin[e]] : s);
-                s += w[e];
-            }
-        };
-        if (q.top_k < a.vocabulary) {
-            each([&](uint32_t e, uint32_t rank, uint64_t s) {
-                if (rank == q.top_k - 1u) result[0] = s + w[e];
-            });
-            __syncthreads();
-            whole = result[0];
-        }
-        if (q.top_p < 1.0) {
-            const uint64_t bound = share_of(q.top_p, whole);
-            each([&](uint32_t e, uint32_t, uint64_t s) {
-                if (s <= bound && bound < s + w[e]) result[1] = s + w[e];
-            });
-            __syncthreads();
-            whole = result[1];
-        }
-        const uint64_t drawn = drawn_of(q, whole);
-        each([&](uint32_t e, uint32_t, uint64_t s) {
-            if (s <= drawn && drawn < s + w[e]) {
-                token = static_cast<int32_t>(static_cast<uint32_t>(sh.list[threadIdx.x * kEach + e]));
-                share = row.share(key[e], whole);
-            }
+    };
+    if (q.top_k < row.vocabulary) {
+        each([&](uint32_t e, uint32_t rank, uint64_t s) {
+            if (rank == q.top_k - 1u) sh.result[0] = s + w[e];
         });
+        __syncthreads();
+        whole = sh.result[0];
+    }
+    if (q.top_p < 1.0) {
+        const uint64_t bound = share_of(q.top_p, whole);
+        each([&](uint32_t e, uint32_t, uint64_t s) {
+            if (s <= bound && bound < s + w[e]) sh.result[1] = s + w[e];
+        });
+        __syncthreads();
+        whole = sh.result[1];
+    }
+    const uint64_t drawn = drawn_of(q, whole);
+    each([&](uint32_t e, uint32_t, uint64_t s) {
+        if (s <= drawn && drawn < s + w[e]) {
+            sh.token = static_cast<int32_t>(static_cast<uint32_t>(sh.list[threadIdx.x * kEach + e]));
+            sh.share = row.share(key[e], whole);
+        }
+    });
+}
+
+template <typename E, typename S, typename F>
+DAV2_DEV void finish_row(const Row<E>& row, S& sh, uint32_t listed, bool gaps, uint64_t whole, F&& entry) {
+    sort_list(sh.list, listed, entry);
+    if (listed <= kThreads) finish_sorted<1>(row, sh, listed, gaps, whole);
+    else finish_sorted<kList / kThreads>(row, sh, listed, gaps, whole);
+}
+
+// The sums before each bin in the place of those of each.
+template <typename F>
+DAV2_DEV void put_before(const BinScan<kThreads>& scan, F& sh) {
+    scan.each([&](uint32_t b, uint32_t c, uint32_t, uint64_t s, uint64_t) {
+        sh.sums[b] = s;
+        sh.counts[b] = c;
+    });
+}
+
+template <typename F>
+DAV2_DEV void put_token(const dav2_sample_args& a, const F& sh) {
+    __syncthreads();
+    if (threadIdx.x != 0) return;
+    a.tokens[blockIdx.x] = sh.token;
+    if (a.probabilities) a.probabilities[blockIdx.x] = sh.share;
+}
+
+// The list of a row whose bins have been filled, and the end of its searches.
+template <typename E, typename F>
+DAV2_DEV void list_and_finish(const Row<E>& row, F& sh) {
+    BinScan<kThreads> scan;
+    scan.load(sh.counts, sh.sums, sh.bins);
+    scan.choose(row.q, row.vocabulary, row.bits, sh.bins);
+    scan.bound(Bins(row.top, row.q), sh.bins);
+    put_before(scan, sh);
+    if (threadIdx.x == 0) sh.listed = 0;
+    __syncthreads();
+    for_listed<kThreads>(row, scan, 0u, row.vocabulary, [&](unsigned long long entry) {
+        const uint32_t at = atomicAdd(&sh.listed, 1u);
+        if (at < kList) sh.list[at] = entry;
+    });
+    __syncthreads();
+    const uint32_t listed = sh.listed;
+    if (listed > kList) return search_row(row, sh.search, &sh.token, &sh.share);
+    finish_row(row, sh, listed, row.q.top_k > kFew, scan.whole, [&](uint32_t i) { return i < listed ? sh.list[i] : ~0ull; });
+}
+
+// The end of a row that workgroups have shared.
+template <typename E>
+__global__ __launch_bounds__(kThreads) void sample_pick_kernel(dav2_sample_args a, uint32_t chunks, int bits) {
+    __shared__ Finish<> sh;
+    const RowState& state = static_cast<const RowState*>(a.scratch)[blockIdx.x];
+    const Row<E> row = {row_of<E>(a, blockIdx.x), a.vocabulary, bits, top_of(state, chunks), asked_of(a, blockIdx.x)};
+    if (threadIdx.x == 0) {
+        sh.token = -1;
+        sh.share = 0.0f;
+    }
+    if (!(row.top > -INFINITY)) return put_token(a, sh);
+    const uint32_t listed = state.listed;
+    if (listed > kList) {
+        __syncthreads();
+        search_row(row, sh.search, &sh.token, &sh.share);
+        return put_token(a, sh);
+    }
+    const bool gaps = row.q.top_k > kFew;
+    uint64_t whole = 0;
+    if (gaps) {
+        BinScan<kThreads> scan;
+        scan.load(state.counts, state.sums, sh.bins);
+        put_before(scan, sh);
+        whole = scan.whole;
+    }
+    finish_row(row, sh, listed, gaps, whole, [&](uint32_t i) { return i < listed ? state.list[i] : ~0ull; });
+    put_token(a, sh);
+}
+
+// ---- rows of 16-bit logits by how often each number is there -----------------------
+//
+// Without a top-k a row's bins need every token's weight, but there are only so
+// many numbers of 16 bits: they are counted, and weighed once. The searches go
+// by the bins, by the numbers of a bin, and by the tokens of a number.
+
+// Numbers in order: 0 .. 32767 are the positive ones from the largest pattern
+// down, 32768 .. 65535 the negative ones.
+DAV2_DEV uint32_t pattern_of(uint32_t order) { return order < 32768u ? 32767u - order : order; }
+template <typename E>
+DAV2_DEV float number_of(uint32_t order) {
+    return static_cast<float>(__builtin_bit_cast(E, static_cast<uint16_t>(pattern_of(order))));
+}
+
+// Whether all were counted: 65536 equal ones overflow their half word, and the
+// sum of all counts is then another.
+template <typename E>
+DAV2_DEV bool count_keys(const Row<E>& row, Finish<true>& sh) {
+    typedef uint16_t Raw __attribute__((ext_vector_type(8), aligned(2)));
+    const uint16_t* const raw = reinterpret_cast<const uint16_t*>(row.logits);
+    for (uint32_t i = threadIdx.x; i < kKeyWords / 4u; i += kThreads)
+        reinterpret_cast<uint4*>(sh.keys)[i] = make_uint4(0, 0, 0, 0);
+    __syncthreads();
+    auto add = [&](uint32_t x) { atomicAdd(&sh.keys[x >> 1], 1u << (16u * (x & 1u))); };
+    constexpr uint32_t kTogether = 4, kStep = 8 * kThreads;
+    uint32_t c = 8u * threadIdx.x;
+    for (; c + (kTogether - 1u) * kStep + 8u <= row.vocabulary; c += kTogether * kStep) {
+        Raw v[kTogether];
+#pragma unroll
+        for (uint32_t t = 0; t < kTogether; ++t) v[t] = *reinterpret_cast<const Raw*>(raw + c + t * kStep);
+#pragma unroll
+        for (uint32_t t = 0; t < kTogether; ++t)
+#pragma unroll
+            for (uint32_t i = 0; i < 8; ++i) add(v[t][i]);
+    }
+    for (; c < row.vocabulary; c += kStep)
+        for (uint32_t i = c; i < min(c + 8u, row.vocabulary); ++i) add(raw[i]);
+    __syncthreads();
+    const Bins bin_of(row.top, row.q);
+    uint64_t counted = 0;
+    auto weigh = [&](uint32_t pattern, uint32_t n) {
+        const float l = static_cast<float>(__builtin_bit_cast(E, static_cast<uint16_t>(pattern)));
+        const uint64_t w = row.units(rank_key(l));
+        if (w) atomicAdd(&sh.sums[bin_of(l)], static_cast<unsigned long long>(w * n));
+    };
+    for (uint32_t i = threadIdx.x; i < kKeyWords / 4u; i += kThreads) {
+        const uint4 words = reinterpret_cast<const uint4*>(sh.keys)[i];
+        const uint32_t word[4] = {words.x, words.y, words.z, words.w};
+#pragma unroll
+        for (uint32_t j = 0; j < 4; ++j) {
+            if (word[j] == 0) continue;
+            counted += (word[j] & 0xffffu) + (word[j] >> 16);
+            if (word[j] & 0xffffu) weigh(8u * i + 2u * j, word[j] & 0xffffu);
+            if (word[j] >> 16) weigh(8u * i + 2u * j + 1u, word[j] >> 16);
+        }
+    }
+    return group_sum(counted, sh.of_wave) == row.vocabulary;
+}
+
+// Where the running sum passes `bound`: a number, which of its tokens, and the sum before that one.
+struct Passed {
+    uint32_t order, nth;
+    uint64_t before;
+};
+template <typename E>
+DAV2_DEV Passed search_keys(const Row<E>& row, Finish<true>& sh, const BinScan<kThreads>& scan, uint64_t bound) {
+    const Bins bin_of(row.top, row.q);
+    scan.each([&](uint32_t b, uint32_t, uint32_t, uint64_t s, uint64_t m) {
+        if (s <= bound && bound < s + m) {
+            sh.bins.found[0] = b;
+            sh.bins.sums[0] = s;
+        }
+    });
+    __syncthreads();
+    const uint32_t bin = sh.bins.found[0];
+    const uint32_t infinity = 32767u - (sizeof(E) == 2 && std::is_same_v<E, _Float16> ? 0x7c00u : 0x7f80u);
+    // the bin's numbers, found by each wave alike
+    const uint32_t last = 65535u - infinity;
+    auto first_of = [&](uint32_t b) {
+        return first_where(infinity, last + 1u, [&](uint32_t o) { return bin_of(number_of<E>(o)) >= b; });
+    };
+    const uint32_t end = first_of(bin + 1u);
+    uint64_t before = sh.bins.sums[0];
+    for (uint32_t from = first_of(bin); from < end; from += kThreads) {
+        const uint32_t o = from + threadIdx.x, pattern = pattern_of(o & 0xffffu);
+        uint32_t n = 0;
+        if (o < end) {
+            n = (sh.keys[pattern >> 1] >> (16u * (pattern & 1u))) & 0xffffu;
+            // both zeros are one number
+            if (pattern == 0u) n += sh.keys[0x8000u >> 1] & 0xffffu;
+            if (pattern == 0x8000u) n = 0;
+        }
+        const uint64_t w = n ? row.units(rank_key(number_of<E>(o))) : 0;
+        uint64_t all;
+        const uint64_t mine = before + group_before(w * n, sh.of_wave, all);
+        if (n && mine <= bound && bound < mine + w * n) {
+            const uint64_t nth = (bound - mine) / w;
+            sh.result[0] = mine + nth * w;
+            sh.bins.found[1] = o;
+            sh.bins.found[2] = static_cast<uint32_t>(nth);
+        }
+        before += all;
+        if (before > bound) break;  // the same for all threads
     }
     __syncthreads();
-    if (threadIdx.x == 0) {
-        a.tokens[r] = token;
-        if (a.probabilities) a.probabilities[r] = share;
+    const Passed passed = {sh.bins.found[1], sh.bins.found[2], sh.result[0]};
+    __syncthreads();
+    return passed;
+}
+
+// The index of the nth token of a number, each wave counting a part of the row.
+template <typename E>
+DAV2_DEV void find_nth(const Row<E>& row, Finish<true>& sh, float number, uint32_t nth) {
+    typedef Vec<E> V;
+    constexpr uint32_t N = V::N, kBlock = 64 * N;
+    const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6;
+    const uint32_t length = ((row.vocabulary + kWaves - 1u) / kWaves + kBlock - 1u) / kBlock * kBlock;
+    const uint32_t begin = min(wave * length, row.vocabulary), end = min(begin + length, row.vocabulary);
+    auto count = [&](uint32_t c) {
+        uint32_t n = 0;
+        if (c + N <= end) {
+            float v[N];
+            V::load(row.logits, c, ~0u, v);
+#pragma unroll
+            for (uint32_t i = 0; i < N; ++i) n += v[i] == number;
+        } else {
+            for (uint32_t i = c; i < end; ++i) n += row.logit(i) == number;
+        }
+        return n;
+    };
+    uint32_t n = 0;
+#pragma unroll 4
+    for (uint32_t c = begin + lane * N; c < end; c += kBlock) n += count(c);
+    const uint64_t of_wave = wave_sum64(n);
+    __syncthreads();
+    if (lane == 0) sh.of_wave[wave] = of_wave;
+    __syncthreads();
+    uint64_t before = 0;
+    for (uint32_t w = 0; w < wave; ++w) before += sh.of_wave[w];
+    if (before > nth || nth >= before + of_wave) return;
+    // this wave has it
+    for (uint32_t c0 = begin; c0 < end; c0 += kBlock) {
+        const uint32_t c = c0 + lane * N;
+        const uint32_t mine = c < end ? count(c) : 0u;
+        const uint64_t upto = wave_upto(mine), from = before + upto - mine;
+        if (from <= nth && nth < from + mine) {
+            uint32_t left = nth - static_cast<uint32_t>(from);
+            for (uint32_t i = c; i < end; ++i)
+                if (row.logit(i) == number && left-- == 0) {
+                    sh.token = static_cast<int32_t>(i);
+                    break;
+                }
+        }
+        before += lane63(upto);
+        if (before > nth) break;
     }
+}
+
+template <typename E>
+DAV2_DEV void finish_keys(const Row<E>& row, Finish<true>& sh) {
+    BinScan<kThreads> scan;
+    scan.load(sh.counts, sh.sums, sh.bins);
+    uint64_t whole = scan.whole;
+    if (row.q.top_p < 1.0) {
+        const Passed last = search_keys(row, sh, scan, share_of(row.q.top_p, whole));
+        whole = last.before + row.units(rank_key(number_of<E>(last.order)));
+    }
+    const Passed drawn = search_keys(row, sh, scan, drawn_of(row.q, whole));
+    const float number = number_of<E>(drawn.order);
+    if (threadIdx.x == 0) sh.share = row.share(rank_key(number), whole);
+    find_nth(row, sh, number, drawn.nth);
+}
+
+// A workgroup for each row, from its largest logit to its token: where rows are
+// many, and where they are short, which then are their own list.
+template <typename E, bool KEYS>
+__global__ __launch_bounds__(kThreads) void sample_row_kernel(dav2_sample_args a, int bits) {
+    __shared__ Finish<KEYS> sh;
+    Row<E> row = {row_of<E>(a, blockIdx.x), a.vocabulary, bits, 0.0f, asked_of(a, blockIdx.x)};
+    float top = -INFINITY;
+    for_each<kThreads>(row.logits, 0u, a.vocabulary, [&](float l, uint32_t) { top = fmaxf(top, l); });
+    top = wave_max(top);
+    if ((threadIdx.x & 63u) == 0) sh.tops[threadIdx.x >> 6] = top;
+    if (threadIdx.x == 0) {
+        sh.token = -1;
+        sh.share = 0.0f;
+    }
+    for (uint32_t b = threadIdx.x; b < kBins; b += kThreads) {
+        sh.counts[b] = 0;
+        sh.sums[b] = 0;
+    }
+    __syncthreads();
+    for (uint32_t w = 0; w < kWaves; ++w) top = fmaxf(top, sh.tops[w]);
+    row.top = top + 0.0f;
+    if (!(row.top > -INFINITY)) return put_token(a, sh);
+    if (a.vocabulary <= kList) {
+        finish_row(row, sh, a.vocabulary, false, 0,
+                   [&](uint32_t i) { return i < a.vocabulary ? list_entry(row.logit(i), i) : ~0ull; });
+        return put_token(a, sh);
+    }
+    if constexpr (KEYS) {
+        if (row.q.greedy) {
+            if (threadIdx.x == 0) sh.share = 1.0f;
+            find_nth(row, sh, row.top, 0u);
+            return put_token(a, sh);
+        }
+        if (count_keys(row, sh)) {
+            finish_keys(row, sh);
+            return put_token(a, sh);
+        }
+        for (uint32_t b = threadIdx.x; b < kBins; b += kThreads) sh.sums[b] = 0;
+        __syncthreads();
+    }
+    fill_bins<kThreads>(row, 0u, a.vocabulary, sh.counts, sh.sums);
+    __syncthreads();
+    list_and_finish(row, sh);
+    put_token(a, sh);
 }
 
 // Weights of 2^bits each, summed over a vocabulary, stay below 2^63.
 int weight_bits(uint32_t vocabulary) {
     int log2 = 0;
     while ((1u << log2) < vocabulary) ++log2;
-    return 62 - log2;
+    return std::min(62 - log2, 46);
 }
 
-// Logits of a chunk: 2048 workgroups for the call, of 4096 and more each.
+// Rows that workgroups share: few and long ones, and sooner where every token of
+// the row is weighed. us, a workgroup for each row against four launches, 4, 16
+// and 64 rows: fp32 with top-p alone, 32000 tokens 32 / 31, 35 / 33, 37 / 42, 100003
+// tokens 76 / 34, 93 / 51, 94 / 62; with top-k 32000 tokens 18 / 22, 18 / 24, 19 / 31,
+// 100003 tokens 25 / 22, 25 / 27, 27 / 33; bf16 with top-p alone 100003 tokens 43 / 34,
+// 49 / 46, 49 / 67.
+bool shares_rows(const dav2_sample_args& a) {
+    if (a.vocabulary <= kList) return false;
+    if (a.dtype == DAV2_DTYPE_F32 && !a.top_k) return a.rows <= 96 && a.vocabulary >= 24576u + 512u * a.rows;
+    return a.rows <= 32 && a.vocabulary >= 65536u + 4096u * a.rows;
+}
+
+// Rows whose 16-bit logits are counted by their value.
+bool by_key(const dav2_sample_args& a) { return !a.top_k && a.vocabulary >= 16384u; }
+
+// Logits of a chunk: 512 workgroups for the call, of 4096 and more each.
 uint32_t chunk_length(const dav2_sample_args& a) {
-    const uint32_t chunks = std::clamp(2048u / a.rows, 1u, std::min(kMostChunks, (a.vocabulary + 4095u) / 4096u));
+    const uint32_t chunks = std::clamp(512u / a.rows, 1u, std::min(kMostChunks, (a.vocabulary + 4095u) / 4096u));
     return ((a.vocabulary + chunks - 1u) / chunks + 7u) / 8u * 8u;
 }
 
@@ -705,7 +1104,7 @@ uint32_t chunk_length(const dav2_sample_args& a) {
 extern "C" {
 
 uint64_t dav2_hip_sample_scratch_bytes(const dav2_sample_args* args) {
-    return args && args->vocabulary > kList ? static_cast<uint64_t>(args->rows) * sizeof(RowState) : 0;
+    return args && shares_rows(*args) ? static_cast<uint64_t>(args->rows) * sizeof(RowState) : 0;
 }
 
 int dav2_hip_sample(const dav2_sample_args* args, void* stream) {
@@ -721,16 +1120,22 @@ int dav2_hip_sample(const dav2_sample_args* args, void* stream) {
     const int bits = weight_bits(a.vocabulary);
     return with_dtype(a.dtype, [&](auto* e) -> int {
         typedef std::remove_pointer_t<decltype(e)> E;
-        uint32_t chunks = 0;
-        if (need) {
-            const uint32_t length = chunk_length(a);
-            chunks = (a.vocabulary + length - 1u) / length;
+        if (shares_rows(a)) {
+            const uint32_t length = chunk_length(a), chunks = (a.vocabulary + length - 1u) / length;
             const dim3 grid(chunks, a.rows);
             dispatch(sample_largest_kernel<E>, grid, dim3(kChunkThreads), 0, s, a, length);
             dispatch(sample_bins_kernel<E>, grid, dim3(kChunkThreads), 0, s, a, length, bits);
             dispatch(sample_list_kernel<E>, grid, dim3(kChunkThreads), 0, s, a, length, bits);
+            dispatch(sample_pick_kernel<E>, dim3(a.rows), dim3(kThreads), 0, s, a, chunks, bits);
+        } else {
+            if constexpr (sizeof(E) == 2) {
+                if (by_key(a)) {
+                    dispatch(sample_row_kernel<E, true>, dim3(a.rows), dim3(kThreads), 0, s, a, bits);
+                    return hipGetLastError();
+                }
+            }
+            dispatch(sample_row_kernel<E, false>, dim3(a.rows), dim3(kThreads), 0, s, a, bits);
         }
-        dispatch(sample_pick_kernel<E>, dim3(a.rows), dim3(kThreads), 0, s, a, chunks, bits);
         return hipGetLastError();
     });
 }

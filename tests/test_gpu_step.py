@@ -760,6 +760,35 @@ def test_sample_ties_and_masks(gpu, pkg, lib, dtype, vocabulary):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows,vocabulary", [(97, 4097), (130, 16390), (100, 40000), (98, 70001)])
+def test_sample_many_rows(gpu, pkg, lib, dtype, rows, vocabulary):
+    # rows that have a workgroup each; some of equal logits, masked, or of one number in bulk
+    torch = gpu
+    x = rand(torch, rows, rows, vocabulary, dtype=dtype, scale=2.5)
+    x[1] = 0.5
+    x[2] = -math.inf
+    x[3, 7:] = math.nan
+    x[4, 2:] = -30000.0
+    x[5] = torch.round(x[5])
+    x[6, :60] = math.inf
+    x[7] = torch.where(torch.arange(vocabulary, device="cuda") % 3 == 0, -0.0, 0.0)
+    x[8, : vocabulary // 2] = torch.finfo(x.dtype).min
+    x[9, 1:] = 0.0
+    x[10, 500:] = -math.inf
+    r = np.random.default_rng(rows)
+    u = r.random(rows).tolist()
+    t = (0.4 + r.random(rows)).tolist()
+    t[11], t[12], t[13], t[14] = 0.0, math.nan, 1e-20, 1e30
+    p = (0.3 + 0.69 * r.random(rows)).tolist()
+    check_sample(torch, pkg, lib, x, u, dtype)
+    check_sample(torch, pkg, lib, x, u, dtype, temperature=t, top_p=p)
+    check_sample(torch, pkg, lib, x, u, dtype, temperature=t, min_p=[0.02 * (i % 4) for i in range(rows)])
+    check_sample(torch, pkg, lib, x, u, dtype, temperature=t, top_k=[(1, 50, 2048, 3000, 0)[i % 5] for i in range(rows)],
+                 top_p=p)
+    check_sample(torch, pkg, lib, x[:, 1:vocabulary - 2], u, dtype, temperature=t, top_p=p)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
 def test_sample_strides(gpu, pkg, lib, dtype):
     # rows of a wider matrix at an odd address, in any order of the rows' requests
     torch = gpu
