@@ -359,6 +359,368 @@ __global__ __launch_bounds__(256, 2) void cache4_rows_kernel(dav2_attention_cach
     }
 }
 
+// Many query rows for a cache head (prompts): the tiles, the order of the work
+// and the split of cache_tiles_kernel in cache_i8.hip, with scales of keys: four
+// numbers in LDS for each key of a tile, read four keys at a time.
+//
+// Codes are widened once for all waves: a key's words of eight features in the
+// order of widen4, which the query's features are put in too; the tokens 0-3 and
+// 8-11 of a chunk, then 4-7 and 12-15, which are what a lane holds scores of.
+template <typename E, int D, int WAVES>
+__global__ __launch_bounds__(64 * WAVES, D <= 64 && sizeof(E) == 2 ? 3 : 2)
+void cache4_tiles_kernel(dav2_attention_cache_i4_args a, uint32_t splits, uint32_t tiles) {
+    constexpr bool kFloat = std::is_same_v<E, float>;
+    constexpr int HEAD = D <= 64 ? 64 : 128;  // features of a row in LDS
+    constexpr int KS = D / 16, FB = (D + 31) / 32, NP = kFloat ? 2 : 1;
+    constexpr uint32_t d = D;
+    constexpr uint32_t kThreads = 64 * WAVES, kTileRows = 32 * WAVES;
+    constexpr int kPieces = HEAD * 4 / kThreads;  // of 16 codes, for each thread and tile: keys, and values
+    constexpr int kRow = HEAD * 2;                // bytes of a key row in LDS
+    constexpr float kSlack = 2.0f, kBias = kFloat ? 14.0f - kSlack : 15.0f - kSlack;
+    __shared__ __attribute__((aligned(16))) int8_t lds_keys[2][64 * kRow];
+    __shared__ __attribute__((aligned(16))) int8_t lds_values[2][HEAD * 128];
+    // of a key: its scale, what its value's scale adds to the exponent, the share
+    // of its weight in the sum, and the fraction (fp32); whether its page exists
+    constexpr int kKinds = kFloat ? 4 : 3;
+    __shared__ __attribute__((aligned(16))) float lds_scales[2][kKinds][64];
+    __shared__ uint32_t lds_exists[2][4];
+    const uint32_t lane = threadIdx.x & 63u, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const uint32_t col = lane & 31u, hf = lane >> 5;
+    const uint32_t kv_heads = a.cache.kv_heads, page_size = a.cache.page_size;
+    const uint32_t s = blockIdx.x / kv_heads, h = blockIdx.x - s * kv_heads, group = a.heads / kv_heads;
+    const uint32_t split = blockIdx.y % splits;
+    const Sequence q = sequence_of(a.starts, a.lengths, s, a.tokens);
+    const uint32_t n = static_cast<uint32_t>(q.end - q.begin), rows = n * group;
+    const int64_t span = static_cast<int64_t>(a.table_pages) * page_size;
+    const Pages pages = pages_of(a, s);
+    const Parts parts = parts_of(a, splits);
+    const uint32_t row_tiles = (rows + kTileRows - 1u) / kTileRows;
+    auto seen = [&](uint32_t i) {
+        int64_t t = q.length;
+        if (a.causal) t += 1 + static_cast<int64_t>(i) - n;
+        return static_cast<uint32_t>(max(min(t, span), int64_t(0)));
+    };
+
+    // the last rows first: under a causal mask they see the most keys
+    for (uint32_t turn = blockIdx.y / splits; turn < row_tiles; turn += tiles) {
+        const uint32_t tile = row_tiles - 1u - turn;
+        const uint32_t row0 = tile * kTileRows + wave * 32u;  // of this wave
+        const bool any_row = row0 < rows;
+        const Rows<32> of(any_row ? row0 : tile * kTileRows, group, rows);
+        uint32_t token, head, last_token, last_head;
+        of.find(col, token, head);
+        of.find(31u, last_token, last_head);
+        head += h * group;
+        const uint32_t limit = row0 + col < rows ? seen(token) : 0u;
+        const uint32_t wave_most = any_row ? seen(last_token) : 0u, wave_least = seen(of.token);
+        const uint32_t most = seen((min(tile * kTileRows + kTileRows, rows) - 1u) / group);
+        const uint32_t blocks = (most + 63u) / 64u, per = (blocks + splits - 1u) / splits;
+        const uint32_t first = split * per, last = min(first + per, blocks);
+
+        // Staging. A wave's pieces of a tile are of one chunk of 16 tokens, so
+        // that their places in the table are found once for it.
+        u2_t key_codes[kPieces], value_codes[kPieces];
+        Pages::Place of_key[kPieces]{}, of_value{}, of_scale{};
+        float key_scale = 0.0f, value_scale = 1.0f;
+        bool exists = false;
+        constexpr uint32_t kLanes = HEAD / 16, kWaveKeys = 64 / kLanes, kKeyStep = WAVES * kWaveKeys;
+        constexpr uint32_t kValueStep = kThreads / 4;
+        const uint32_t key_chunk = lane % kLanes, key_row = wave * kWaveKeys + lane / kLanes;
+        const uint32_t value_chunk = wave & 3u, value_row = lane + 64u * (wave >> 2);
+        // features that the head does not have: others in their place, whose
+        // copies in LDS meet no query feature and reach no output
+        const uint32_t key_feature = 16u * key_chunk < d ? 16u * key_chunk : 0u;
+        // Called without a condition, and never past the last block: registers
+        // that are loaded in one branch only are waited for where the branches
+        // meet.
+        auto find = [&](uint32_t block) {
+            block = min(block, last - 1u);
+#pragma unroll
+            for (int i = 0; i < kPieces; ++i)
+                of_key[i] = pages.find(block * 4u + (wave * kWaveKeys + kKeyStep * i) / 16u);
+            of_value = pages.find(block * 4u + value_chunk);
+            of_scale = pages.find(block * 4u + lane / 16u);
+        };
+        auto load_keys = [&] {
+#pragma unroll
+            for (int i = 0; i < kPieces; ++i) {
+                const uint64_t plane = static_cast<uint64_t>(pages.page(of_key[i])) * kv_heads + h;
+                key_codes[i] = *reinterpret_cast<const u2_t*>(
+                    a.cache.keys +
+                    ((plane * page_size + of_key[i].slot + (key_row + kKeyStep * i) % 16u) * d + key_feature) / 2u);
+            }
+        };
+        auto load_values = [&] {
+            const uint64_t plane = static_cast<uint64_t>(pages.page(of_value)) * kv_heads + h;
+#pragma unroll
+            for (int i = 0; i < kPieces; ++i)
+                value_codes[i] = *reinterpret_cast<const u2_t*>(a.cache.values + (plane * page_size + of_value.slot) * (d / 2u) +
+                                                                8u * min(value_row + kValueStep * i, d - 1u));
+            exists = pages.exists(of_scale);
+            const uint64_t at = (static_cast<uint64_t>(pages.page(of_scale)) * kv_heads + h) * page_size + of_scale.slot +
+                                lane % 16u;
+            key_scale = a.cache.key_scales[at];
+            value_scale = a.cache.value_scales[at];
+        };
+        auto store_scales = [&](uint32_t buffer) {
+            if (wave == 0) {
+                float exponent, fraction, inverse;
+                split_scale(value_scale, exponent, fraction, inverse);
+                // a scale that is no number shows in the exponent alone: a token
+                // that a row does not see adds nothing to its sums
+                const bool number = fraction == fraction;
+                if (!number) exponent = fraction;
+                if constexpr (kFloat) {
+                    lds_scales[buffer][3][lane] = number ? fraction : 1.0f;
+                } else {
+                    // the weights take the whole scale, off by half a step of its
+                    // logarithm: below 2^-20 of them for scales of 1e-8 and more
+                    exponent += __builtin_amdgcn_logf(number ? fraction : 1.0f);
+                    inverse = inverse / (number ? fraction : 1.0f);
+                }
+                lds_scales[buffer][0][lane] = exists ? key_scale : 0.0f;
+                lds_scales[buffer][1][lane] = exists ? exponent : -INFINITY;
+                lds_scales[buffer][2][lane] = number ? inverse : 1.0f;
+                if (lane % 16u == 0) lds_exists[buffer][lane / 16u] = exists;
+            }
+        };
+        // Bringing a tile in small steps that fit between matrix instructions.
+        constexpr int kStages = 4 * kPieces + 3;
+        auto stage = [&](int n, uint32_t buffer, uint32_t block) {
+            if (n < 4 * kPieces) {
+                const int i = n / 4, half = n & 1;
+                if (n & 2) {
+                    const u2_t v = value_codes[i];
+                    *reinterpret_cast<h8*>(lds_values[buffer] +
+                                           swz<128>(value_row + kValueStep * i, 2u * value_chunk + half)) =
+                        widen4(__builtin_amdgcn_perm(v[1], v[0], half ? 0x07060302u : 0x05040100u));
+                } else {
+                    *reinterpret_cast<h8*>(lds_keys[buffer] + swz<kRow>(key_row + kKeyStep * i, 2u * key_chunk + half)) =
+                        widen4(key_codes[i][half]);
+                }
+            } else if (n == 4 * kPieces) {
+                load_keys();
+            } else if (n == 4 * kPieces + 1) {
+                load_values();
+            } else if (n == 4 * kPieces + 2) {
+                find(block);
+            }
+        };
+        auto stage_rest = [&](int n, uint32_t buffer, uint32_t block) {
+#pragma unroll
+            for (int i = 0; i < kStages; ++i)
+                if (i >= n) stage(i, buffer, block);
+        };
+        __syncthreads();  // the row tile before has been read
+        if (first < last) {
+            find(first);
+            load_keys();
+            load_values();
+            find(first + 1u);
+        }
+
+        // the right operand of the scores
+        h8 qf[NP][KS];
+        float factor;
+        {
+            const E* x = static_cast<const E*>(a.query) + static_cast<uint64_t>(q.begin + token) * a.query_stride +
+                         static_cast<uint64_t>(head) * d + 8u * hf;
+            typedef E V __attribute__((ext_vector_type(16 / sizeof(E))));
+            constexpr int kVec = 16 / sizeof(E);
+            V raw[KS][8 / kVec];
+            float largest = 0.0f;
+#pragma unroll
+            for (int k = 0; k < KS; ++k)
+#pragma unroll
+                for (int j = 0; j < 8 / kVec; ++j) {
+                    raw[k][j] = *reinterpret_cast<const V*>(x + 16 * k + kVec * j);
+#pragma unroll
+                    for (int i = 0; i < kVec; ++i) largest = fmaxf(largest, fabsf(static_cast<float>(raw[k][j][i])));
+                }
+            largest = over_halves(largest, Larger());
+            const int e = largest > 0.0f && largest < INFINITY ? 14 - ilogbf(largest) : 0;
+            const float sign = a.scale < 0.0f ? -1.0f : 1.0f;
+            factor = ldexpf(fabsf(a.scale) * kLog2e, -e);
+#pragma unroll
+            for (int k = 0; k < KS; ++k)
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    const int from = widened(i);
+                    const float y = keep_fp32(ldexpf(static_cast<float>(raw[k][from / kVec][from % kVec]), e) * sign);
+                    const _Float16 hi = static_cast<_Float16>(y);
+                    qf[0][k][i] = hi;
+                    if constexpr (kFloat) qf[1][k][i] = static_cast<_Float16>(y - static_cast<float>(hi));
+                }
+        }
+
+        v16f o[FB];
+#pragma unroll
+        for (int f = 0; f < FB; ++f)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) o[f][r] = 0.0f;
+        float base = kNoScore, sum = 0.0f;  // sum: this lane's keys only
+        bool far = false;                   // the same for all lanes
+
+        if (first < last) {
+            store_scales(0);
+            stage_rest(0, 0, first + 2u);
+        }
+        __syncthreads();
+        for (uint32_t block = first; block < last; ++block) {
+            const uint32_t buffer = (block - first) & 1u;
+            const uint32_t k0 = block * 64u;
+            // behind the last tile that one is brought again, unread
+            store_scales(buffer ^ 1u);
+            if (k0 >= wave_most) {
+                stage_rest(0, buffer ^ 1u, block + 3u);
+            } else {
+                v16f sc[2];
+#pragma unroll
+                for (int b = 0; b < 2; ++b)
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) sc[b][r] = 0.0f;
+                {
+                    h8 in[2][2];
+                    auto read = [&](int k, h8 (&v)[2]) {
+                        v[0] = *reinterpret_cast<const h8*>(lds_keys[buffer] + swz<kRow>(col, 2u * k + hf));
+                        v[1] = *reinterpret_cast<const h8*>(lds_keys[buffer] + swz<kRow>(col + 32u, 2u * k + hf));
+                    };
+                    read(0, in[0]);
+                    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+                    for (int k = 0; k < KS; ++k) {
+                        if (k + 1 < KS) read(k + 1, in[(k + 1) & 1]);
+#pragma unroll
+                        for (int b = 0; b < 2; ++b) {
+#pragma unroll
+                            for (int p = 0; p < NP; ++p)
+                                sc[b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(in[k & 1][b], qf[p][k], sc[b], 0, 0, 0);
+                            stage(2 * k + b, buffer ^ 1u, block + 3u);
+                            __builtin_amdgcn_sched_barrier(0);
+                        }
+                    }
+                    stage_rest(2 * KS, buffer ^ 1u, block + 3u);
+                }
+                h8 vf[2][FB];
+                auto read_values = [&](int t, h8 (&v)[FB]) {
+#pragma unroll
+                    for (int f = 0; f < FB; ++f)
+                        v[f] = *reinterpret_cast<const h8*>(lds_values[buffer] + swz<128>(32u * f + col, 2u * t + hf));
+                };
+                read_values(0, vf[0]);
+                // four keys of the lane: registers 4 g .. of block b
+                auto read_scales = [&](int kind, int b, int g) {
+                    return *reinterpret_cast<const v4f*>(&lds_scales[buffer][kind][32 * b + 8 * g + 4 * hf]);
+                };
+                __builtin_amdgcn_sched_barrier(0);
+                float largest = kNoScore;
+#pragma unroll
+                for (int b = 0; b < 2; ++b)
+#pragma unroll
+                    for (int g = 0; g < 4; ++g) {
+                        const v4f c = read_scales(0, b, g), shift = read_scales(1, b, g);
+#pragma unroll
+                        for (int r = 0; r < 4; ++r) sc[b][4 * g + r] = fmaf(sc[b][4 * g + r], c[r] * factor, shift[r]);
+                    }
+                const v4i_t pages_exist = *reinterpret_cast<const v4i_t*>(lds_exists[buffer]);
+                if (!(k0 + 64u <= wave_least && pages_exist[0] && pages_exist[1] && pages_exist[2] && pages_exist[3])) {
+                    stay_in_branch();
+#pragma unroll
+                    for (int b = 0; b < 2; ++b)
+#pragma unroll
+                        for (int r = 0; r < 16; ++r) {
+                            const uint32_t key = k0 + 32u * b + 8u * (r >> 2) + 4u * hf + (r & 3);
+                            if (!pages_exist[2 * b + (r >> 3)] || key >= limit) sc[b][r] = -INFINITY;
+                        }
+                }
+#pragma unroll
+                for (int b = 0; b < 2; ++b)
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) largest = fmaxf(largest, sc[b][r]);
+                largest = over_halves(largest, Larger());
+                if (__any(largest > base + (far ? 0.0f : kBias + kSlack))) {
+                    stay_in_branch();
+                    const float grown = fmaxf(base + (far ? 0.0f : kBias), largest);
+                    far = far || __any(fabsf(grown) >= kFar && grown != kNoScore);
+                    const float moved = grown - (far ? 0.0f : kBias);
+                    const float keep = __builtin_amdgcn_exp2f(base - moved);
+                    base = moved;
+                    sum *= keep;
+#pragma unroll
+                    for (int f = 0; f < FB; ++f)
+#pragma unroll
+                        for (int r = 0; r < 16; ++r) o[f][r] *= keep;
+                }
+                // weights of chunk t + 1 between the products of chunk t
+                h8 pf[2][NP];
+                v4f share[2], fraction[2];
+                auto weigh = [&](int t, int r) {
+                    if (r % 4 == 0) {
+                        share[r / 4] = read_scales(2, t >> 1, 2 * (t & 1) + r / 4);
+                        if constexpr (kFloat) fraction[r / 4] = read_scales(3, t >> 1, 2 * (t & 1) + r / 4);
+                    }
+                    const float w = __builtin_amdgcn_exp2f(sc[t >> 1][8 * (t & 1) + r] - base);
+                    sum = fmaf(w, share[r / 4][r % 4], sum);
+                    const int to = 2 * (r & 3) + (r >> 2);  // in the order of widen4
+                    if constexpr (kFloat) {
+                        const float y = keep_fp32(w * fraction[r / 4][r % 4]);  // hi and lo of one rounded product
+                        const _Float16 hi = static_cast<_Float16>(y);
+                        pf[t & 1][0][to] = hi;
+                        pf[t & 1][1][to] = static_cast<_Float16>((y - static_cast<float>(hi)) * kSecond);
+                    } else {
+                        pf[t & 1][0][to] = static_cast<_Float16>(w);
+                    }
+                };
+#pragma unroll
+                for (int r = 0; r < 8; ++r) weigh(0, r);
+#pragma unroll
+                for (int t = 0; t < 4; ++t) {
+                    __builtin_amdgcn_sched_barrier(0);
+                    if (t < 3) read_values(t + 1, vf[(t + 1) & 1]);
+#pragma unroll
+                    for (int f = 0; f < FB; ++f) {
+                        o[f] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf[t & 1][f], pf[t & 1][0], o[f], 0, 0, 0);
+                        if constexpr (kFloat)
+                            o[f] = __builtin_amdgcn_mfma_f32_32x32x16_f16(for_second(vf[t & 1][f]), pf[t & 1][1], o[f], 0,
+                                                                          0, 0);
+                        if (t < 3)
+#pragma unroll
+                            for (int r = 8 * f / FB; r < 8 * (f + 1) / FB; ++r) weigh(t + 1, r);
+                        __builtin_amdgcn_sched_barrier(0);
+                    }
+                }
+            }
+            lds_turn();
+        }
+        sum = over_halves(sum, Plus());
+        // register r of o[f]: feature 32 f + 8 (r / 4) + 4 hf + r % 4 of row col
+        if (row0 + col < rows) {
+            const uint64_t at = static_cast<uint64_t>(q.begin) + token;
+            const uint64_t slot = (at * a.heads + head) * splits + split;
+            const float scale = sum == 0.0f ? 0.0f : 1.0f / sum;
+            typedef E V4 __attribute__((ext_vector_type(4)));
+            E* y = static_cast<E*>(a.output) + at * a.output_stride + static_cast<uint64_t>(head) * d;
+#pragma unroll
+            for (int f = 0; f < FB; ++f)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    const uint32_t feature = 32u * f + 8u * r + 4u * hf;
+                    if (feature >= d) continue;
+                    if (splits > 1) {
+                        *reinterpret_cast<v4f*>(parts.sums + slot * d + feature) =
+                            v4f{o[f][4 * r], o[f][4 * r + 1], o[f][4 * r + 2], o[f][4 * r + 3]};
+                    } else {
+                        V4 out;
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) out[i] = static_cast<E>(o[f][4 * r + i] * scale);
+                        *reinterpret_cast<V4*>(y + feature) = out;
+                    }
+                }
+            if (splits > 1 && hf == 0) parts.stats[slot] = make_float2(base, sum);
+        }
+    }
+}
+
 // The splits of the sequences' rows joined.
 template <typename E, int FEW>
 __global__ __launch_bounds__(256) void cache4_join_kernel(dav2_attention_cache_i4_args a, uint32_t splits) {
@@ -379,7 +741,7 @@ bool valid(const dav2_attention_cache_i4_args& a) {
 }
 
 struct Plan {
-    uint32_t tile;  // rows of a workgroup
+    uint32_t tile;  // rows: 16 of cache4_rows_kernel, 128 or 256 of cache4_tiles_kernel
     uint32_t tiles, splits;
 };
 Plan plan_of(const dav2_attention_cache_i4_args& a) {
@@ -387,6 +749,18 @@ Plan plan_of(const dav2_attention_cache_i4_args& a) {
     if (a.cache.kv_heads == 0 || a.heads < a.cache.kv_heads || a.sequences == 0 || a.max_query == 0) return p;
     const uint64_t rows = static_cast<uint64_t>(std::min(a.max_query, a.tokens)) * (a.heads / a.cache.kv_heads);
     const uint64_t planes = static_cast<uint64_t>(a.cache.kv_heads) * a.sequences;
+    const double work = static_cast<double>((rows + 15) / 16 * planes) * a.max_length * a.cache.head_dim;
+    if (rows > 32 && work > 67108864.0) {
+        uint64_t most = 1;  // splits
+        while (most < kMostSplits && (most + 1) * (most + 1) * 32 <= a.max_length) ++most;
+        const uint64_t wide = (rows + 255) / 256 * planes;
+        const bool unequal = a.causal && a.max_query > a.max_length / 2 && wide < 512;
+        p.tile = a.cache.head_dim > 64 && (rows + 127) / 128 % 2 == 0 && wide * most >= 256 && !unequal ? 256 : 128;
+        p.tiles = static_cast<uint32_t>(std::min<uint64_t>((rows + p.tile - 1) / p.tile, 512));
+        p.splits = static_cast<uint32_t>(
+            std::clamp<uint64_t>((p.tile == 256 ? 256 : 512) / std::max<uint64_t>(1, p.tiles * planes), 1, most));
+        return p;
+    }
     p.tiles = static_cast<uint32_t>(std::min<uint64_t>((rows + 15) / 16, 4096));
     const uint64_t have = std::max<uint64_t>(1, p.tiles * planes);
     const uint64_t resident = std::min<uint64_t>(512 / have, a.max_length / 128);
@@ -436,12 +810,17 @@ int dav2_hip_attention_cache_i4(const dav2_attention_cache_i4_args* args, void* 
     if (need && (!a.scratch || !aligned16(a.scratch) || a.scratch_bytes < need)) return hipErrorInvalidValue;
     const hipStream_t s = static_cast<hipStream_t>(stream);
     const Plan p = plan_of(a);
-    const dim3 grid(p.tiles * p.splits, a.cache.kv_heads, a.sequences);
+    const dim3 grid = p.tile > 16 ? dim3(a.cache.kv_heads * a.sequences, p.tiles * p.splits)
+                                  : dim3(p.tiles * p.splits, a.cache.kv_heads, a.sequences);
     return with_dtype(a.dtype, [&](auto* e) -> int {
         typedef std::remove_pointer_t<decltype(e)> E;
         with_head_dim(a.cache.head_dim, [&](auto dim) {
             constexpr int D = decltype(dim)::value;
-            dispatch(cache4_rows_kernel<E, D>, grid, dim3(256), 0, s, a, p.splits, p.tiles);
+            if constexpr (D > 64) {
+                if (p.tile == 256) return dispatch(cache4_tiles_kernel<E, D, 8>, grid, dim3(512), 0, s, a, p.splits, p.tiles);
+            }
+            if (p.tile == 128) dispatch(cache4_tiles_kernel<E, D, 4>, grid, dim3(256), 0, s, a, p.splits, p.tiles);
+            else dispatch(cache4_rows_kernel<E, D>, grid, dim3(256), 0, s, a, p.splits, p.tiles);
         });
         if (p.splits > 1) {
             const JoinLaunch j = join_launch(a, p.splits);
