@@ -13,8 +13,8 @@ using namespace dav2k;
 
 namespace {
 
-// 16-byte vectors at addresses that are multiples of less
-typedef float v4f_any __attribute__((ext_vector_type(4), aligned(4)));
+// vectors at addresses that are multiples of less
+typedef float v2f_any __attribute__((ext_vector_type(2), aligned(4)));
 typedef uint32_t u4_by8 __attribute__((ext_vector_type(4), aligned(8)));
 typedef uint32_t u4_t __attribute__((ext_vector_type(4)));
 typedef uint32_t u2_t __attribute__((ext_vector_type(2)));
@@ -107,19 +107,44 @@ DAV2_DEV Parts parts_of(const dav2_attention_cache_i4_args& a, uint32_t splits) 
 // Lane l = (col, g) = (l % 16, l / 16) takes F features F g .. of its key for
 // the first product (those past the head's width are others, that meet zeros
 // of the query), and chunk g's 16 keys of two neighbouring features for the
-// second, which so are the even and the odd rows of two tiles.
-template <typename E, int D>
+// second, which so are the even and the odd rows of two tiles. Register r of
+// score tile t is key_of(t, r) of chunk g, so that a tile's four scores are two
+// words of the second product's right operand, in the order of widen4.
+//
+// A tile has COLS rows of 16 columns. With 4 or 8 the columns behind them would
+// have their scores weighed for nothing: the tiles' scores are spread over them
+// first, T tiles for each lane, and the weights gathered again.
+DAV2_DEV constexpr uint32_t key_of(uint32_t t, uint32_t r) { return 8u * (t >> 1) + 2u * (t & 1u) + (r >> 1) + 4u * (r & 1u); }
+
+// Lanes of the banks (of four lanes) in BANKS: x of the lane that CTRL names; the others keep `old`.
+template <int CTRL, int BANKS>
+DAV2_DEV float moved(float old, float x) {
+    return __int_as_float(__builtin_amdgcn_update_dpp(__float_as_int(old), __float_as_int(x), CTRL, 0xf, BANKS, false));
+}
+constexpr int kShl4 = 0x104, kShl8 = 0x108, kShl12 = 0x10c, kShr4 = 0x114, kShr8 = 0x118, kShr12 = 0x11c, kRor4 = 0x124,
+              kRor8 = 0x128;
+
+// op over the lanes of a query, COLS apart and in all groups.
+template <int COLS, typename Op>
+DAV2_DEV float over_query(float v, Op op) {
+    if constexpr (COLS == 4) v = op(v, moved<kRor4, 0xf>(v, v));
+    if constexpr (COLS <= 8) v = op(v, moved<kRor8, 0xf>(v, v));
+    return over_groups(v, op);
+}
+
+template <typename E, int D, int COLS>
 __global__ __launch_bounds__(256, 2) void cache4_rows_kernel(dav2_attention_cache_i4_args a, uint32_t splits,
                                                              uint32_t tiles) {
     constexpr bool kFloat = std::is_same_v<E, float>;
     constexpr int F = D > 64 ? 32 : 16, KS = F / 8, FT = D / 16, FP = FT / 2, NP = kFloat ? 2 : 1;
+    constexpr int T = COLS / 4;  // score tiles that a lane weighs
     constexpr uint32_t d = D;
-    constexpr int kPad = 17;
+    constexpr int kPad = COLS + 1;
     constexpr float kBias = 14.0f;  // a weight times a fraction stays below 2^15
     __shared__ float joined[4][D * kPad];
-    __shared__ float shared_base[4][16], shared_sum[4][16];
+    __shared__ float shared_base[4][COLS], shared_sum[4][COLS];
     const uint32_t lane = threadIdx.x & 63u, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const uint32_t col = lane & 15u, g = lane >> 4;
+    const uint32_t col = lane & 15u, g = lane >> 4, t0 = T * (col / COLS);  // the lane's first tile
     const uint32_t split = blockIdx.x % splits, h = blockIdx.y, s = blockIdx.z;
     const uint32_t page_size = a.cache.page_size, kv_heads = a.cache.kv_heads;
     const uint32_t group = a.heads / kv_heads;
@@ -130,11 +155,11 @@ __global__ __launch_bounds__(256, 2) void cache4_rows_kernel(dav2_attention_cach
     const Pages pages = pages_of(a, s);
     const Parts parts = parts_of(a, splits);
 
-    for (uint32_t tile = blockIdx.x / splits; tile < (rows + 15u) / 16u; tile += tiles) {
-        const Rows<16> of(tile * 16u, group, rows);
-        const uint32_t row = tile * 16u + col;
+    for (uint32_t tile = blockIdx.x / splits; tile < (rows + COLS - 1u) / COLS; tile += tiles) {
+        const Rows<COLS> of(tile * COLS, group, rows);
+        const uint32_t row = tile * COLS + col % COLS;
         uint32_t token, head;
-        of.find(col, token, head);
+        of.find(col % COLS, token, head);
         head += h * group;
         auto seen = [&](uint32_t i) {
             int64_t t = q.length;
@@ -143,7 +168,7 @@ __global__ __launch_bounds__(256, 2) void cache4_rows_kernel(dav2_attention_cach
         };
         const uint32_t limit = row < rows ? seen(token) : 0u;
         uint32_t last_token, last_head;
-        of.find(15u, last_token, last_head);
+        of.find(COLS - 1u, last_token, last_head);
         const uint32_t most = seen(last_token), least = seen(of.token);
         const uint32_t blocks = (most + 63u) / 64u, per = (blocks + splits - 1u) / splits;
         const uint32_t first = split * per, last = min(first + per, blocks);
@@ -156,7 +181,7 @@ __global__ __launch_bounds__(256, 2) void cache4_rows_kernel(dav2_attention_cach
         uint32_t kraw[4][F / 8];
         u4_t vraw[FP > 0 ? FP : 1];
         u2_t vlast{};  // of the last 16 features, where their number is odd
-        v4f key_scale[4], value_scale[4];
+        v4f key_scale[T], value_scale[T];
         Pages::Place of_key{}, of_value{};
         bool exists = false;
         const uint32_t f0 = min(F * g, d - F);  // this lane's features
@@ -166,15 +191,15 @@ __global__ __launch_bounds__(256, 2) void cache4_rows_kernel(dav2_attention_cach
         };
         auto load_keys = [&] {
             const uint8_t* k = a.cache.keys + ((static_cast<uint64_t>(pages.page(of_key)) * kv_heads + h) * page_size +
-                                               of_key.slot + col % 4u) * (d / 2u) + f0 / 2u;
+                                               of_key.slot + key_of(0, col % 4u)) * (d / 2u) + f0 / 2u;
 #pragma unroll
             for (int t = 0; t < 4; ++t) {
                 if constexpr (F == 32) {
-                    const u4_by8 v = *reinterpret_cast<const u4_by8*>(k + 4u * t * (d / 2u));
+                    const u4_by8 v = *reinterpret_cast<const u4_by8*>(k + key_of(t, 0) * (d / 2u));
 #pragma unroll
                     for (int i = 0; i < 4; ++i) kraw[t][i] = v[i];
                 } else {
-                    const u2_t v = *reinterpret_cast<const u2_t*>(k + 4u * t * (d / 2u));
+                    const u2_t v = *reinterpret_cast<const u2_t*>(k + key_of(t, 0) * (d / 2u));
                     kraw[t][0] = v[0], kraw[t][1] = v[1];
                 }
             }
@@ -182,10 +207,14 @@ __global__ __launch_bounds__(256, 2) void cache4_rows_kernel(dav2_attention_cach
         auto load_values = [&] {
             exists = pages.exists(of_value);
             const uint64_t at = (static_cast<uint64_t>(pages.page(of_value)) * kv_heads + h) * page_size + of_value.slot;
+            auto four = [&](const float* x) {
+                const v2f_any lo = *reinterpret_cast<const v2f_any*>(x), hi = *reinterpret_cast<const v2f_any*>(x + 4);
+                return v4f{lo[0], hi[0], lo[1], hi[1]};
+            };
 #pragma unroll
-            for (int t = 0; t < 4; ++t) {
-                key_scale[t] = *reinterpret_cast<const v4f_any*>(a.cache.key_scales + at + 4 * t);
-                value_scale[t] = *reinterpret_cast<const v4f_any*>(a.cache.value_scales + at + 4 * t);
+            for (int t = 0; t < T; ++t) {
+                key_scale[t] = four(a.cache.key_scales + at + key_of(t0 + t, 0));
+                value_scale[t] = four(a.cache.value_scales + at + key_of(t0 + t, 0));
             }
             const uint8_t* v = a.cache.values + at * (d / 2u);
 #pragma unroll
@@ -249,45 +278,85 @@ __global__ __launch_bounds__(256, 2) void cache4_rows_kernel(dav2_attention_cach
                 }
             }
             if constexpr (kMore) load_keys();
-            const uint32_t key0 = block * 64u + 16u * g;  // of this lane's first score
+            v4f x[T];
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                if constexpr (COLS == 16) {
+#pragma unroll
+                    for (int t = 0; t < 4; ++t) x[t][r] = sc[t][r];
+                } else if constexpr (COLS == 8) {
+                    x[0][r] = moved<kShr8, 0xc>(sc[0][r], sc[2][r]);
+                    x[1][r] = moved<kShr8, 0xc>(sc[1][r], sc[3][r]);
+                } else {
+                    x[0][r] = moved<kShr4, 0x2>(sc[0][r], sc[1][r]);
+                    x[0][r] = moved<kShr8, 0x4>(x[0][r], sc[2][r]);
+                    x[0][r] = moved<kShr12, 0x8>(x[0][r], sc[3][r]);
+                }
+            }
+            const uint32_t key0 = block * 64u + 16u * g;  // of this lane's chunk
             const bool whole = (block + 1u) * 64u <= least && __all(exists);
-            float fraction[4][4], inverse[4][4];
+            float fraction[T][4], inverse[T][4];
             float largest = kNoScore;
 #pragma unroll
-            for (int t = 0; t < 4; ++t)
+            for (int t = 0; t < T; ++t)
 #pragma unroll
                 for (int r = 0; r < 4; ++r) {
-                    const bool here = whole || (exists && key0 + 4 * t + r < limit);
+                    const bool here = whole || (exists && key0 + key_of(t0 + t, r) < limit);
                     float exponent;
                     // a token that the row does not see may have any scale, NaN included
                     split_scale(here ? value_scale[t][r] : 1.0f, exponent, fraction[t][r], inverse[t][r]);
-                    const float x = fmaf(sc[t][r], key_scale[t][r] * factor, exponent);
-                    sc[t][r] = here ? x : -INFINITY;
-                    largest = fmaxf(largest, sc[t][r]);
+                    const float y = fmaf(x[t][r], key_scale[t][r] * factor, exponent);
+                    x[t][r] = here ? y : -INFINITY;
+                    largest = fmaxf(largest, x[t][r]);
                 }
-            largest = over_groups(largest, Larger());
+            largest = over_query<COLS>(largest, Larger());
             if (__any(largest > maximum)) {
                 maximum = fmaxf(maximum, largest);
-                const float moved = fabsf(maximum) < kFar ? maximum - kBias : maximum;
-                const float keep = __builtin_amdgcn_exp2f(base - moved);
-                base = moved;
+                const float moved_base = fabsf(maximum) < kFar ? maximum - kBias : maximum;
+                const float keep = __builtin_amdgcn_exp2f(base - moved_base);
+                base = moved_base;
                 sum *= keep;
 #pragma unroll
                 for (int f = 0; f < FT; ++f) o[f] *= keep;
             }
-            h8 pf[2][2];
+            // weights, the first parts and the rest of them, as words of the right operand
+            float words[T][2][2];
 #pragma unroll
-            for (int t = 0; t < 4; ++t)
+            for (int t = 0; t < T; ++t)
 #pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    const float w = __builtin_amdgcn_exp2f(sc[t][r] - base);
-                    sum = fmaf(w, inverse[t][r], sum);
-                    const float y = keep_fp32(w * fraction[t][r]);  // hi and lo of one rounded product
-                    const _Float16 hi = static_cast<_Float16>(y);
-                    // key 4 t + r of the chunk, in the order of widen4
-                    pf[0][t >> 1][2 * r + (t & 1)] = hi;
-                    pf[1][t >> 1][2 * r + (t & 1)] = static_cast<_Float16>((y - static_cast<float>(hi)) * kSecond);
+                for (int r = 0; r < 4; r += 2) {
+                    h2 hi, lo;
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) {
+                        const float w = __builtin_amdgcn_exp2f(x[t][r + i] - base);
+                        sum = fmaf(w, inverse[t][r + i], sum);
+                        const float y = keep_fp32(w * fraction[t][r + i]);  // hi and lo of one rounded product
+                        hi[i] = static_cast<_Float16>(y);
+                        lo[i] = static_cast<_Float16>((y - static_cast<float>(hi[i])) * kSecond);
+                    }
+                    words[t][0][r / 2] = __builtin_bit_cast(float, hi);
+                    words[t][1][r / 2] = __builtin_bit_cast(float, lo);
                 }
+            h8 pf[2][2];  // part, half of the chunk
+#pragma unroll
+            for (int p = 0; p < 2; ++p) {
+                v4f half[2];
+#pragma unroll
+                for (int t = 0; t < 4; ++t)
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) {
+                        // tile t is with the lane COLS (t / T) further
+                        const float own = words[t % T][p][i];
+                        constexpr int kNone = 0;
+                        const float from = COLS == 16 || t / T == kNone ? own
+                                           : COLS == 8 || t / T == 2    ? moved<kShl8, 0xf>(0.0f, own)
+                                           : t / T == 1                 ? moved<kShl4, 0xf>(0.0f, own)
+                                                                        : moved<kShl12, 0xf>(0.0f, own);
+                        half[t >> 1][2 * (t & 1) + i] = from;
+                    }
+                pf[p][0] = __builtin_bit_cast(h8, half[0]);
+                pf[p][1] = __builtin_bit_cast(h8, half[1]);
+            }
             auto add = [&](v4f& sums, uint32_t lo, uint32_t hi) {
                 const h8 v0 = widen4(lo), v1 = widen4(hi);
                 sums = __builtin_amdgcn_mfma_f32_16x16x32_f16(v0, pf[0][0], sums, 0, 0, 0);
@@ -308,18 +377,18 @@ __global__ __launch_bounds__(256, 2) void cache4_rows_kernel(dav2_attention_cach
         };
         for (; block + 4u < last; block += 4u) step(std::true_type());
         if (block < last) step(std::false_type());
-        sum = over_groups(sum, Plus());
+        sum = over_query<COLS>(sum, Plus());
 
         // join the four waves
         __syncthreads();  // the tile before has been read
-        if (g == 0) {
+        if (g == 0 && col < COLS) {
             shared_base[wave][col] = base;
             shared_sum[wave][col] = sum;
         }
         __syncthreads();
         float top = kNoScore;
 #pragma unroll
-        for (int w = 0; w < 4; ++w) top = fmaxf(top, shared_base[w][col]);
+        for (int w = 0; w < 4; ++w) top = fmaxf(top, shared_base[w][col % COLS]);
         const float mine = __builtin_amdgcn_exp2f(base - top);
 #pragma unroll
         for (int f = 0; f < FT; ++f)
@@ -328,12 +397,13 @@ __global__ __launch_bounds__(256, 2) void cache4_rows_kernel(dav2_attention_cach
                 // register r of o[f]: row 4 g + r of tile f
                 const uint32_t i = 4 * g + r;
                 const uint32_t feature = f < 2 * FP ? 32u * (f / 2) + 2u * i + f % 2 : 16u * f + i;
-                joined[wave][feature * kPad + col] = o[f][r] * mine;
+                if (col < COLS) joined[wave][feature * kPad + col] = o[f][r] * mine;
             }
         __syncthreads();
-        // 16 threads for each of the 16 rows
-        const uint32_t out_col = threadIdx.x >> 4, lane16 = threadIdx.x & 15u;
-        if (tile * 16u + out_col < rows) {
+        // the threads shared out to the rows
+        constexpr uint32_t kShare = 256 / COLS;
+        const uint32_t out_col = threadIdx.x / kShare, out_lane = threadIdx.x % kShare;
+        if (tile * COLS + out_col < rows) {
             float all = kNoScore, total = 0.0f;
 #pragma unroll
             for (int w = 0; w < 4; ++w) all = fmaxf(all, shared_base[w][out_col]);
@@ -347,14 +417,14 @@ __global__ __launch_bounds__(256, 2) void cache4_rows_kernel(dav2_attention_cach
             const float scale = splits > 1 ? 1.0f : total == 0.0f ? 0.0f : 1.0f / total;
             E* y = static_cast<E*>(a.output) + at * a.output_stride + static_cast<uint64_t>(out_head) * d;
             const uint64_t slot = (at * a.heads + out_head) * splits + split;
-            for (uint32_t f = lane16; f < d; f += 16u) {
+            for (uint32_t f = out_lane; f < d; f += kShare) {
                 float v = 0.0f;
 #pragma unroll
                 for (int w = 0; w < 4; ++w) v += joined[w][f * kPad + out_col];
                 if (splits > 1) parts.sums[slot * d + f] = v;
                 else y[f] = static_cast<E>(v * scale);
             }
-            if (splits > 1 && lane16 == 0) parts.stats[slot] = make_float2(all, total);
+            if (splits > 1 && out_lane == 0) parts.stats[slot] = make_float2(all, total);
         }
     }
 }
@@ -741,7 +811,7 @@ bool valid(const dav2_attention_cache_i4_args& a) {
 }
 
 struct Plan {
-    uint32_t tile;  // rows: 16 of cache4_rows_kernel, 128 or 256 of cache4_tiles_kernel
+    uint32_t tile;  // rows: 4, 8 or 16 of cache4_rows_kernel, 128 or 256 of cache4_tiles_kernel
     uint32_t tiles, splits;
 };
 Plan plan_of(const dav2_attention_cache_i4_args& a) {
@@ -761,7 +831,8 @@ Plan plan_of(const dav2_attention_cache_i4_args& a) {
             std::clamp<uint64_t>((p.tile == 256 ? 256 : 512) / std::max<uint64_t>(1, p.tiles * planes), 1, most));
         return p;
     }
-    p.tiles = static_cast<uint32_t>(std::min<uint64_t>((rows + 15) / 16, 4096));
+    p.tile = rows <= 4 ? 4 : rows <= 8 ? 8 : 16;
+    p.tiles = static_cast<uint32_t>(std::min<uint64_t>((rows + p.tile - 1) / p.tile, 4096));
     const uint64_t have = std::max<uint64_t>(1, p.tiles * planes);
     const uint64_t resident = std::min<uint64_t>(512 / have, a.max_length / 128);
     const uint64_t even = std::min<uint64_t>(2048 / have, a.max_length / 2048);
@@ -820,7 +891,10 @@ int dav2_hip_attention_cache_i4(const dav2_attention_cache_i4_args* args, void* 
                 if (p.tile == 256) return dispatch(cache4_tiles_kernel<E, D, 8>, grid, dim3(512), 0, s, a, p.splits, p.tiles);
             }
             if (p.tile == 128) dispatch(cache4_tiles_kernel<E, D, 4>, grid, dim3(256), 0, s, a, p.splits, p.tiles);
-            else dispatch(cache4_rows_kernel<E, D>, grid, dim3(256), 0, s, a, p.splits, p.tiles);
+            else dispatch(p.tile == 4   ? cache4_rows_kernel<E, D, 4>
+                          : p.tile == 8 ? cache4_rows_kernel<E, D, 8>
+                                        : cache4_rows_kernel<E, D, 16>,
+                          grid, dim3(256), 0, s, a, p.splits, p.tiles);
         });
         if (p.splits > 1) {
             const JoinLaunch j = join_launch(a, p.splits);
