@@ -88,10 +88,16 @@ DAV2_DEV h8 widen4(uint32_t w) {
     const h2 share = {static_cast<_Float16>(0.0625f), static_cast<_Float16>(0.0625f)};
     const h2 down16 = {static_cast<_Float16>(-72.0f), static_cast<_Float16>(-72.0f)};
     const uint32_t u = w >> 8;
-    const h2 a = __builtin_bit_cast(h2, (w & 0x000f000fu) | 0x64006400u) - down;
-    const h2 b = __builtin_elementwise_fma(__builtin_bit_cast(h2, (w & 0x00f000f0u) | 0x64006400u), share, down16);
-    const h2 c = __builtin_bit_cast(h2, (u & 0x000f000fu) | 0x64006400u) - down;
-    const h2 d = __builtin_elementwise_fma(__builtin_bit_cast(h2, (u & 0x00f000f0u) | 0x64006400u), share, down16);
+    // one operation with the constants in registers, which the compiler makes two
+    auto below = [](uint32_t x, uint32_t mask) {
+        uint32_t y;
+        asm("v_and_or_b32 %0, %1, %2, %3" : "=v"(y) : "v"(x), "s"(mask), "v"(0x64006400u));
+        return __builtin_bit_cast(h2, y);
+    };
+    const h2 a = below(w, 0x000f000fu) - down;
+    const h2 b = __builtin_elementwise_fma(below(w, 0x00f000f0u), share, down16);
+    const h2 c = below(u, 0x000f000fu) - down;
+    const h2 d = __builtin_elementwise_fma(below(u, 0x00f000f0u), share, down16);
     return h8{a.x, a.y, b.x, b.y, c.x, c.y, d.x, d.y};
 }
 // which of eight the i-th of widen4 is
@@ -138,6 +144,10 @@ __global__ __launch_bounds__(256, 2) void cache4_rows_kernel(dav2_attention_cach
     constexpr bool kFloat = std::is_same_v<E, float>;
     constexpr int F = D > 64 ? 32 : 16, KS = F / 8, FT = D / 16, FP = FT / 2, NP = kFloat ? 2 : 1;
     constexpr int T = COLS / 4;  // score tiles that a lane weighs
+    // The second parts' sums in registers of their own save the multiplications
+    // of the codes (see for_second), where that does not cost a wave: 64
+    // sequences of up to 2048 keys, 8 heads of 128, 25 for 27 us; 16 heads of 64, fp32, 32.5 for 28.
+    constexpr bool kApart = D > 64;
     constexpr uint32_t d = D;
     constexpr int kPad = COLS + 1;
     constexpr float kBias = 14.0f;  // a weight times a fraction stays below 2^15
@@ -173,9 +183,9 @@ __global__ __launch_bounds__(256, 2) void cache4_rows_kernel(dav2_attention_cach
         const uint32_t blocks = (most + 63u) / 64u, per = (blocks + splits - 1u) / splits;
         const uint32_t first = split * per, last = min(first + per, blocks);
 
-        v4f o[FT];
+        v4f o[FT], o2[kApart ? FT : 1];  // of the weights' first and second parts
 #pragma unroll
-        for (int f = 0; f < FT; ++f) o[f] = v4f{0.f, 0.f, 0.f, 0.f};
+        for (int f = 0; f < FT; ++f) o[f] = o2[kApart ? f : 0] = v4f{0.f, 0.f, 0.f, 0.f};
         float maximum = kNoScore, base = kNoScore, sum = 0.0f;
 
         uint32_t kraw[4][F / 8];
@@ -317,7 +327,10 @@ __global__ __launch_bounds__(256, 2) void cache4_rows_kernel(dav2_attention_cach
                 base = moved_base;
                 sum *= keep;
 #pragma unroll
-                for (int f = 0; f < FT; ++f) o[f] *= keep;
+                for (int f = 0; f < FT; ++f) {
+                    o[f] *= keep;
+                    if constexpr (kApart) o2[f] *= keep;
+                }
             }
             // weights, the first parts and the rest of them, as words of the right operand
             float words[T][2][2];
@@ -357,19 +370,20 @@ __global__ __launch_bounds__(256, 2) void cache4_rows_kernel(dav2_attention_cach
                 pf[p][0] = __builtin_bit_cast(h8, half[0]);
                 pf[p][1] = __builtin_bit_cast(h8, half[1]);
             }
-            auto add = [&](v4f& sums, uint32_t lo, uint32_t hi) {
+            auto add = [&](int f, uint32_t lo, uint32_t hi) {
                 const h8 v0 = widen4(lo), v1 = widen4(hi);
-                sums = __builtin_amdgcn_mfma_f32_16x16x32_f16(v0, pf[0][0], sums, 0, 0, 0);
-                sums = __builtin_amdgcn_mfma_f32_16x16x32_f16(v1, pf[0][1], sums, 0, 0, 0);
-                sums = __builtin_amdgcn_mfma_f32_16x16x32_f16(for_second(v0), pf[1][0], sums, 0, 0, 0);
-                sums = __builtin_amdgcn_mfma_f32_16x16x32_f16(for_second(v1), pf[1][1], sums, 0, 0, 0);
+                v4f& second = kApart ? o2[kApart ? f : 0] : o[f];
+                o[f] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v0, pf[0][0], o[f], 0, 0, 0);
+                second = __builtin_amdgcn_mfma_f32_16x16x32_f16(kApart ? v0 : for_second(v0), pf[1][0], second, 0, 0, 0);
+                o[f] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v1, pf[0][1], o[f], 0, 0, 0);
+                second = __builtin_amdgcn_mfma_f32_16x16x32_f16(kApart ? v1 : for_second(v1), pf[1][1], second, 0, 0, 0);
             };
 #pragma unroll
             for (int f = 0; f < FP; ++f) {
-                add(o[2 * f], vraw[f][0], vraw[f][1]);
-                add(o[2 * f + 1], vraw[f][2], vraw[f][3]);
+                add(2 * f, vraw[f][0], vraw[f][1]);
+                add(2 * f + 1, vraw[f][2], vraw[f][3]);
             }
-            if constexpr (FT % 2) add(o[FT - 1], vlast[0], vlast[1]);
+            if constexpr (FT % 2) add(FT - 1, vlast[0], vlast[1]);
             if constexpr (kMore) {
                 load_values();
                 find(min(block + 8u, last - 1u));
@@ -397,7 +411,7 @@ __global__ __launch_bounds__(256, 2) void cache4_rows_kernel(dav2_attention_cach
                 // register r of o[f]: row 4 g + r of tile f
                 const uint32_t i = 4 * g + r;
                 const uint32_t feature = f < 2 * FP ? 32u * (f / 2) + 2u * i + f % 2 : 16u * f + i;
-                if (col < COLS) joined[wave][feature * kPad + col] = o[f][r] * mine;
+                if (col < COLS) joined[wave][feature * kPad + col] = (kApart ? fmaf(o2[kApart ? f : 0][r], 1.0f / kSecond, o[f][r]) : o[f][r]) * mine;
             }
         __syncthreads();
         // the threads shared out to the rows
