@@ -168,6 +168,15 @@ typedef _Float16 h8 __attribute__((ext_vector_type(8)));
 typedef __bf16 b8 __attribute__((ext_vector_type(8)));
 typedef float v16f __attribute__((ext_vector_type(16)));
 
+// 64 bits of the lane that a DPP control names; 0 from outside, and for rows of
+// lanes that ROWS leaves out.
+template <int CTRL, int ROWS>
+DAV2_DEV uint64_t moved64(uint64_t v) {
+    const int lo = __builtin_amdgcn_update_dpp(0, static_cast<int>(static_cast<uint32_t>(v)), CTRL, ROWS, 0xf, true);
+    const int hi = __builtin_amdgcn_update_dpp(0, static_cast<int>(static_cast<uint32_t>(v >> 32)), CTRL, ROWS, 0xf, true);
+    return (static_cast<uint64_t>(static_cast<uint32_t>(hi)) << 32) | static_cast<uint32_t>(lo);
+}
+
 // The running maximum of a softmax before its first score. Finite, so that
 // exp2(maximum - larger maximum) is 0 and never the difference of infinities.
 constexpr float kNoScore = -3.0e38f;

@@ -16,16 +16,155 @@ using namespace dav2k;
 
 namespace {
 
+// Over the wave, received by all lanes: sums and maxima run up to lane 63.
+template <int CTRL, int ROWS>
+DAV2_DEV double moved(double v) {
+    return __longlong_as_double(static_cast<long long>(moved64<CTRL, ROWS>(static_cast<uint64_t>(__double_as_longlong(v)))));
+}
 DAV2_DEV double wave_sum(double v) {
-    for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o, kWave);
-    return v;
+    v += moved<0x111, 0xf>(v);  // row_shr:1
+    v += moved<0x112, 0xf>(v);
+    v += moved<0x114, 0xf>(v);
+    v += moved<0x118, 0xf>(v);  // row_shr:8
+    v += moved<0x142, 0xa>(v);  // row_bcast:15
+    v += moved<0x143, 0xc>(v);  // row_bcast:31
+    const long long bits = __double_as_longlong(v);
+    const int lo = __builtin_amdgcn_readlane(static_cast<int>(bits), 63);
+    const int hi = __builtin_amdgcn_readlane(static_cast<int>(bits >> 32), 63);
+    return __hiloint2double(hi, lo);
+}
+template <int CTRL, int ROWS>
+DAV2_DEV uint32_t larger(uint32_t v) {
+    return max(v, static_cast<uint32_t>(__builtin_amdgcn_update_dpp(0, static_cast<int>(v), CTRL, ROWS, 0xf, true)));
 }
 DAV2_DEV uint32_t wave_max_bits(uint32_t v) {
-    for (int o = 32; o > 0; o >>= 1) v = max(v, static_cast<uint32_t>(__shfl_xor(static_cast<int>(v), o, kWave)));
-    return v;
+    v = larger<0x111, 0xf>(v);
+    v = larger<0x112, 0xf>(v);
+    v = larger<0x114, 0xf>(v);
+    v = larger<0x118, 0xf>(v);
+    v = larger<0x142, 0xa>(v);
+    v = larger<0x143, 0xc>(v);
+    return static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(v), 63));
 }
 
-// A workgroup for each row, which is read again for its largest value and for its outputs.
+DAV2_DEV float factor_of(double squares, const dav2_add_rms_norm_args& a) {
+    return static_cast<float>(1.0 / sqrt(squares / a.columns + static_cast<double>(a.epsilon)));
+}
+DAV2_DEV float scale_of(uint32_t most) {  // the largest value's bits
+    return __uint_as_float(max(__float_as_uint(div_rn(__uint_as_float(most), 127.0f)), __float_as_uint(1.0e-8f)));
+}
+
+// N codes of a row from element c on, those past its last zero.
+template <int N>
+DAV2_DEV void store_codes(int8_t* row, uint32_t c, uint32_t columns, const float (&v)[N], float scale, float inverse) {
+    uint32_t words[N / 4] = {};
+    // a value past the last is 0, and so is its code unless the scale is no number
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+        words[i / 4] |= (c + i < columns ? static_cast<uint32_t>(quantize_div(v[i], scale, inverse)) & 0xffu : 0u) << (8 * (i % 4));
+    if constexpr (N == 8) *reinterpret_cast<uint2*>(row + c) = make_uint2(words[0], words[1]);
+    else *reinterpret_cast<uint32_t*>(row + c) = words[0];
+}
+
+// LANES lanes share a row and keep it in registers, PIECES vectors each: one
+// read of the inputs and one write of each output. Bound by memory: 8191 rows of
+// 4096, bf16, sum, norm and codes (302 MB): 55 us, 5.5 TB/s, where a kernel that
+// reads the row again from the caches takes 71. The weights stay in registers
+// from row to row. Rows that are not multiples of 16 bytes are read as they lie:
+// 8191 of 5003 106 us, of 5008 87.
+template <typename E, int LANES, int PIECES>
+__global__ __launch_bounds__(LANES < 256 ? 256 : LANES) void rms_norm_kept_kernel(dav2_add_rms_norm_args a) {
+    typedef Vec<E> V;
+    constexpr int N = V::N, kThreads = LANES < 256 ? 256 : LANES, kRows = kThreads / LANES, kWaves = LANES / 64;
+    __shared__ double sums[2][kThreads / 64];
+    __shared__ uint32_t largest[2][kThreads / 64];
+    const uint32_t columns = a.columns, lane = threadIdx.x % LANES, wave = threadIdx.x >> 6, wave0 = wave / kWaves * kWaves;
+    float weight[PIECES][N];
+#pragma unroll
+    for (int p = 0; p < PIECES; ++p)
+#pragma unroll
+        for (int j = 0; j < N; j += 4) {
+            float w[4] = {1.0f, 1.0f, 1.0f, 1.0f};
+            if (a.weight) Vec<float>::load(a.weight, (p * LANES + lane) * N + j, columns, w);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) weight[p][j + i] = w[i];
+        }
+    uint32_t turn = 0;
+    for (uint64_t first = static_cast<uint64_t>(blockIdx.x) * kRows; first < a.rows;
+         first += static_cast<uint64_t>(gridDim.x) * kRows, turn ^= 1u) {
+        const uint64_t row = min(first + threadIdx.x / LANES, static_cast<uint64_t>(a.rows) - 1u);
+        const bool mine = first + threadIdx.x / LANES < a.rows;
+        const E* x = static_cast<const E*>(a.input) + row * a.input_stride;
+        float v[PIECES][N];
+#pragma unroll
+        for (int p = 0; p < PIECES; ++p) V::load(x, (p * LANES + lane) * N, columns, v[p]);
+        if (a.residual) {
+            const E* r = static_cast<const E*>(a.residual) + row * a.residual_stride;
+            float w[PIECES][N];
+#pragma unroll
+            for (int p = 0; p < PIECES; ++p) V::load(r, (p * LANES + lane) * N, columns, w[p]);
+#pragma unroll
+            for (int p = 0; p < PIECES; ++p)
+#pragma unroll
+                for (int i = 0; i < N; ++i) v[p][i] = static_cast<float>(static_cast<E>(keep_fp32(v[p][i] + w[p][i])));
+        }
+        if (a.sum && mine) {
+            E* sum = static_cast<E*>(a.sum) + row * a.sum_stride;
+#pragma unroll
+            for (int p = 0; p < PIECES; ++p) V::store(sum, (p * LANES + lane) * N, columns, v[p]);
+        }
+        double squares = 0.0;
+#pragma unroll
+        for (int p = 0; p < PIECES; ++p)
+#pragma unroll
+            for (int i = 0; i < N; ++i) squares = fma(static_cast<double>(v[p][i]), static_cast<double>(v[p][i]), squares);
+        squares = wave_sum(squares);
+        if constexpr (kWaves > 1) {
+            if ((threadIdx.x & 63u) == 0) sums[turn][wave] = squares;
+            __syncthreads();
+            squares = 0.0;
+#pragma unroll
+            for (int w = 0; w < kWaves; ++w) squares += sums[turn][wave0 + w];
+        }
+        const float factor = factor_of(squares, a);
+        uint32_t most = 0;
+#pragma unroll
+        for (int p = 0; p < PIECES; ++p)
+#pragma unroll
+            for (int i = 0; i < N; ++i) {
+                v[p][i] = (v[p][i] * factor) * weight[p][i];
+                most = max(most, __float_as_uint(fabsf(v[p][i])));  // NaN above all
+            }
+        if (a.output && mine) {
+            E* y = static_cast<E*>(a.output) + row * a.output_stride;
+#pragma unroll
+            for (int p = 0; p < PIECES; ++p) V::store(y, (p * LANES + lane) * N, columns, v[p]);
+        }
+        if (!a.codes) continue;
+        most = wave_max_bits(most);
+        if constexpr (kWaves > 1) {
+            if ((threadIdx.x & 63u) == 0) largest[turn][wave] = most;
+            __syncthreads();
+#pragma unroll
+            for (int w = 0; w < kWaves; ++w) most = max(most, largest[turn][wave0 + w]);
+        }
+        if (!mine) continue;
+        const float scale = scale_of(most), inverse = div_rn(1.0f, scale);
+        if (lane == 0) a.scales[row] = scale;
+        int8_t* q = a.codes + row * a.code_stride;
+#pragma unroll
+        for (int p = 0; p < PIECES; ++p) {
+            const uint32_t c = (p * LANES + lane) * N;
+            if (c < a.code_stride) store_codes(q, c, columns, v[p], scale, inverse);
+        }
+        for (uint64_t c = static_cast<uint64_t>(PIECES * LANES + lane) * N; c < a.code_stride; c += LANES * N)
+#pragma unroll
+            for (int i = 0; i < N; i += 4) *reinterpret_cast<uint32_t*>(q + c + i) = 0u;
+    }
+}
+
+// Rows that are too long for that: a workgroup for each, which is read again for
+// its largest value and for its outputs.
 template <typename E>
 __global__ __launch_bounds__(256) void rms_norm_kernel(dav2_add_rms_norm_args a) {
     typedef Vec<E> V;
@@ -63,7 +202,7 @@ __global__ __launch_bounds__(256) void rms_norm_kernel(dav2_add_rms_norm_args a)
         if ((threadIdx.x & 63u) == 0) sums[wave] = squares;
         __syncthreads();
         squares = (sums[0] + sums[1]) + (sums[2] + sums[3]);
-        const float factor = static_cast<float>(1.0 / sqrt(squares / columns + static_cast<double>(a.epsilon)));
+        const float factor = factor_of(squares, a);
         auto norm = [&](uint32_t c, float (&v)[N]) {
             load(c, v);
 #pragma unroll
@@ -90,7 +229,7 @@ __global__ __launch_bounds__(256) void rms_norm_kernel(dav2_add_rms_norm_args a)
             if ((threadIdx.x & 63u) == 0) largest[wave] = most;
             __syncthreads();
             most = max(max(largest[0], largest[1]), max(largest[2], largest[3]));
-            scale = __uint_as_float(max(__float_as_uint(div_rn(__uint_as_float(most), 127.0f)), __float_as_uint(1.0e-8f)));
+            scale = scale_of(most);
             inverse = div_rn(1.0f, scale);
             if (threadIdx.x == 0) a.scales[row] = scale;
         }
@@ -98,23 +237,21 @@ __global__ __launch_bounds__(256) void rms_norm_kernel(dav2_add_rms_norm_args a)
         int8_t* q = a.codes ? a.codes + row * a.code_stride : nullptr;
         const uint64_t width = q ? a.code_stride : columns;
         for (uint64_t c = threadIdx.x * N; c < width; c += 256u * N) {
-            uint32_t words[N / 4] = {};
+            float v[N] = {};
             if (c < columns) {
-                float v[N];
                 norm(static_cast<uint32_t>(c), v);
                 if (y) V::store(y, static_cast<uint32_t>(c), columns, v);
-                if (q)
-#pragma unroll
-                    for (int i = 0; i < N; ++i)
-                        if (c + i < columns)
-                            words[i / 4] |= (static_cast<uint32_t>(quantize_div(v[i], scale, inverse)) & 0xffu) << (8 * (i % 4));
             }
-            if (q)
-#pragma unroll
-                for (int i = 0; i < N / 4; ++i) reinterpret_cast<uint32_t*>(q + c)[i] = words[i];
+            if (q) store_codes(q + (c - static_cast<uint32_t>(c)), static_cast<uint32_t>(c), columns, v, scale, inverse);
         }
     }
 }
+
+template <int I>
+using Lanes = std::integral_constant<int, I>;
+constexpr uint32_t kWorkgroups = 4096;  // sixteen for each CU, which go from row to row
+// From this many rows on a wave for each narrow one, instead of a workgroup.
+constexpr uint32_t kNarrowRows = 512;
 
 }  // namespace
 
@@ -137,7 +274,33 @@ int dav2_hip_add_rms_norm(const dav2_add_rms_norm_args* args, void* stream) {
         return hipErrorInvalidValue;
     return with_dtype(a.dtype, [&](auto* e) -> int {
         typedef std::remove_pointer_t<decltype(e)> E;
-        dispatch(rms_norm_kernel<E>, dim3(std::min(a.rows, 1u << 22)), dim3(256), 0, static_cast<hipStream_t>(stream), a);
+        const hipStream_t s = static_cast<hipStream_t>(stream);
+        constexpr uint32_t N = Vec<E>::N;
+        // workgroups that share the rows out
+        auto kept = [&](auto lanes, auto pieces) {
+            constexpr int LANES = decltype(lanes)::value, kThreads = LANES < 256 ? 256 : LANES, kRows = kThreads / LANES;
+            dispatch(rms_norm_kept_kernel<E, LANES, decltype(pieces)::value>,
+                     dim3(std::min((a.rows + kRows - 1u) / kRows, kWorkgroups)), dim3(kThreads), 0, s, a);
+        };
+        const uint32_t vectors = (a.columns + N - 1u) / N;
+        if (vectors <= 128 && a.rows >= kNarrowRows) {
+            if (vectors <= 64) kept(Lanes<64>(), Lanes<1>());
+            else kept(Lanes<64>(), Lanes<2>());
+        } else if (vectors <= 256) {
+            kept(Lanes<256>(), Lanes<1>());
+        } else if (vectors <= 512) {
+            kept(Lanes<256>(), Lanes<2>());
+        } else if (vectors <= 768) {
+            kept(Lanes<256>(), Lanes<3>());
+        } else if (vectors <= 1024) {
+            kept(Lanes<512>(), Lanes<2>());
+        } else if (vectors <= 2048) {
+            kept(Lanes<1024>(), Lanes<2>());
+        } else if (vectors <= 4096) {
+            kept(Lanes<1024>(), Lanes<4>());
+        } else {
+            dispatch(rms_norm_kernel<E>, dim3(std::min(a.rows, 1u << 22)), dim3(256), 0, s, a);
+        }
         return hipGetLastError();
     });
 }

@@ -100,12 +100,6 @@ DAV2_DEV uint64_t units_of(double weight, int bits) {
 
 // The sum over the lanes up to this one: within rows of 16 lanes by row shifts,
 // then a row's last sum into the rows behind it.
-template <int CTRL, int ROWS>
-DAV2_DEV uint64_t moved64(uint64_t v) {
-    const int lo = __builtin_amdgcn_update_dpp(0, static_cast<int>(static_cast<uint32_t>(v)), CTRL, ROWS, 0xf, true);
-    const int hi = __builtin_amdgcn_update_dpp(0, static_cast<int>(static_cast<uint32_t>(v >> 32)), CTRL, ROWS, 0xf, true);
-    return (static_cast<uint64_t>(static_cast<uint32_t>(hi)) << 32) | static_cast<uint32_t>(lo);
-}
 DAV2_DEV uint64_t wave_upto(uint64_t v) {
     v += moved64<0x111, 0xf>(v);  // row_shr:1
     v += moved64<0x112, 0xf>(v);
