@@ -19,58 +19,147 @@ typedef uint32_t u4_by8 __attribute__((ext_vector_type(4), aligned(8)));
 typedef uint32_t u4_t __attribute__((ext_vector_type(4)));
 typedef uint32_t u2_t __attribute__((ext_vector_type(2)));
 
-// A code as it is held, of the rounded and clamped quotient x / scale; NaN is the lowest.
-DAV2_DEV uint32_t nibble(float x, float scale, float inverse) {
-    // x * inverse is within 7 (2^-23 + 2^-24 + 2^-47) < 2^-19 of the rounded
-    // quotient: where it is that near to a border, the quotient itself decides
-    float y = x * inverse;
-    if (__builtin_expect(fabsf(y - __builtin_rintf(y)) > 0.5f - 0x1p-18f, 0)) y = div_rn(x, scale);
-    return static_cast<uint32_t>(static_cast<int>(fminf(fmaxf(__builtin_rintf(y), -7.0f), 7.0f)) + 8);
+// Eight codes as they are held, one to a half byte: x / scale rounded, of which
+// x * inverse is within 7 (2^-23 + 2^-24 + 2^-47) < 2^-19. Where that is as near
+// to a border, which is rare, the quotients themselves decide. Adding 1.5 * 2^23
+// rounds to a whole number, and 8 more are the code in its low bits.
+DAV2_DEV uint32_t half_bytes(const float (&x)[8], float scale, float inverse) {
+    constexpr float kRound = 0x1.8p23f;
+    float y[8];
+    bool border = false;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        y[i] = x[i] * inverse;
+        border |= fabsf(y[i] - ((y[i] + kRound) - kRound)) > 0.5f - 0x1p-18f;
+    }
+    if (__builtin_expect(border, 0))
+#pragma unroll
+        for (int i = 0; i < 8; ++i) y[i] = div_rn(x[i], scale);
+    uint32_t word = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        // no number is 0; |y| is at most 7 (1 + 2^-23)
+        const float whole = (y[i] == y[i] ? y[i] : 0.0f) + (kRound + 8.0f);
+        word |= (__float_as_uint(whole) & 15u) << (4 * i);
+    }
+    return word;
 }
 
-// A wave for each new row (token, head, side).
+// The largest over 16 neighbouring lanes, received by all of them.
+template <int CTRL>
+DAV2_DEV uint32_t larger(uint32_t v) {
+    return max(v, static_cast<uint32_t>(__builtin_amdgcn_update_dpp(0, static_cast<int>(v), CTRL, 0xf, 0xf, true)));
+}
+DAV2_DEV uint32_t largest_of_16(uint32_t v) {
+    v = larger<0x121>(v);  // row_ror:1, 2, 4, 8
+    v = larger<0x122>(v);
+    v = larger<0x124>(v);
+    return larger<0x128>(v);
+}
+
+// A wave for each chunk of 16 tokens, head and side. Lane (t, f) = (l / 16, l %
+// 16) has features 8 f .. of the tokens t, t + 4, t + 8 and t + 12. A key's eight
+// codes are a word as they stand. Values are held the other way round: each lane
+// puts its codes where its tokens are in the eight bytes of their features, and
+// the four lanes of a feature join theirs, each ending with two of the eight
+// features and one store. A chunk that has older or later tokens too is read,
+// changed and written back; nobody else writes it. Bound by memory and by the
+// rounding: 8 prompts of up to 2048 tokens, 8 heads of 128, f16 (46 MB).
 template <typename E>
-__global__ __launch_bounds__(256) void cache4_scale_kernel(dav2_cache_store_i4_args a) {
-    const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6;
-    const uint32_t h = blockIdx.y >> 1, side = blockIdx.y & 1u, s = blockIdx.z;
-    const uint32_t page_size = a.cache.page_size, d = a.cache.head_dim;
+__global__ __launch_bounds__(256) void cache4_store_kernel(dav2_cache_store_i4_args a) {
+    const uint32_t lane = threadIdx.x & 63u, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const uint32_t kv_heads = a.cache.kv_heads, page_size = a.cache.page_size, d = a.cache.head_dim;
+    const uint32_t plane_of = blockIdx.y * 4u + wave, side = plane_of >= kv_heads, h = plane_of - side * kv_heads;
+    if (plane_of >= 2u * kv_heads) return;
+    const uint32_t s = blockIdx.z, t0 = lane >> 4, f = lane & 15u;
     const Sequence q = sequence_of(a.starts, a.lengths, s, a.tokens);
-    const int64_t origin = static_cast<int64_t>(q.length) - (q.end - q.begin);
+    // positions [first, last) are new; in 64 bits, as a length may be anything
+    const int64_t origin = static_cast<int64_t>(q.length) - (q.end - q.begin);  // row r has position origin + r - begin
     const int64_t first = max(origin, int64_t(0));
     const int64_t last = min(static_cast<int64_t>(q.length), static_cast<int64_t>(a.table_pages) * page_size);
     const uint64_t stride = side ? a.value_stride : a.key_stride;
-    const E* x = static_cast<const E*>(side ? a.values : a.keys) + static_cast<uint64_t>(h) * d;
-    // two neighbouring tokens for each wave: their values share bytes
-    for (int64_t pair = first / 2 + blockIdx.x * 4u + wave; 2 * pair < last; pair += gridDim.x * 4u) {
-        for (int64_t t = max(2 * pair, first); t < min(2 * pair + 2, last); ++t) {
-            const int32_t page = a.page_table[static_cast<uint64_t>(s) * a.table_pages + t / page_size];
-            if (page < 0 || static_cast<uint32_t>(page) >= a.cache.pages) continue;
-            const uint32_t slot = static_cast<uint32_t>(t % page_size);
-            const uint64_t plane = static_cast<uint64_t>(page) * a.cache.kv_heads + h;
-            const E* row = x + static_cast<uint64_t>(q.begin + (t - origin)) * stride;
-            float v0 = 0.0f, v1 = 0.0f;  // features 2 lane, 2 lane + 1
-            if (2 * lane < d) {
-                v0 = static_cast<float>(row[2 * lane]);
-                v1 = static_cast<float>(row[2 * lane + 1]);
-            }
-            uint32_t bits = max(__float_as_uint(fabsf(v0)), __float_as_uint(fabsf(v1)));  // NaN above all
-            for (int o = 32; o > 0; o >>= 1)
-                bits = max(bits, static_cast<uint32_t>(__shfl_xor(static_cast<int>(bits), o, kWave)));
-            bits = max(__float_as_uint(div_rn(__uint_as_float(bits), 7.0f)), __float_as_uint(1.0e-8f));
-            const float scale = __uint_as_float(bits), inverse = div_rn(1.0f, scale);
-            if (lane == 0) (side ? a.cache.value_scales : a.cache.key_scales)[plane * page_size + slot] = scale;
-            if (2 * lane >= d) continue;
-            const uint32_t c0 = nibble(v0, scale, inverse), c1 = nibble(v1, scale, inverse);
-            uint8_t* at = (side ? a.cache.values : a.cache.keys) + plane * (page_size / 2u) * d;
-            if (side == 0) {
-                at[slot * (d / 2u) + lane] = static_cast<uint8_t>(c0 | (c1 << 4));
-            } else {
-                at += (slot / 16u) * 8u * d + 16u * lane + (slot % 16u) / 2u;
-                const uint32_t shift = 4u * (slot & 1u), keep = 0xf0u >> shift;
-                at[0] = static_cast<uint8_t>((at[0] & keep) | (c0 << shift));
-                at[8] = static_cast<uint8_t>((at[8] & keep) | (c1 << shift));
+    const E* x = static_cast<const E*>(side ? a.values : a.keys) + static_cast<uint64_t>(h) * d + 8u * f;
+    const bool feature = 8u * f < d;
+    for (int64_t chunk = first / 16 + blockIdx.x; chunk * 16 < last; chunk += gridDim.x) {
+        const int64_t base = chunk * 16;
+        const int32_t page = a.page_table[static_cast<uint64_t>(s) * a.table_pages + base / page_size];
+        if (page < 0 || static_cast<uint32_t>(page) >= a.cache.pages) continue;  // the same for the wave
+        const uint32_t slot0 = static_cast<uint32_t>(base % page_size);
+        const uint32_t from = static_cast<uint32_t>(max(first - base, int64_t(0)));
+        const uint32_t to = static_cast<uint32_t>(min(last - base, int64_t(16)));
+        const uint64_t at = (static_cast<uint64_t>(page) * kv_heads + h) * page_size + slot0;  // of the chunk's first token
+        float v[4][8];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const uint32_t t = t0 + 4 * i;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) v[i][j] = 0.0f;
+            if (feature && t >= from && t < to) {
+                const E* row = x + (q.begin + (base + t - origin)) * static_cast<int64_t>(stride);
+#pragma unroll
+                for (int j = 0; j < 8; j += Vec<E>::N) {
+                    float part[Vec<E>::N];
+                    Vec<E>::load(row, j, 8u, part);
+#pragma unroll
+                    for (int k = 0; k < Vec<E>::N; ++k) v[i][j + k] = part[k];
+                }
             }
         }
+        uint32_t codes[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            codes[i] = 0;
+            if (to <= 4u * i || from >= 4u * i + 4u) continue;  // the same for the wave
+            uint32_t bits = 0;  // NaN above all
+#pragma unroll
+            for (int j = 0; j < 8; ++j) bits = max(bits, __float_as_uint(fabsf(v[i][j])));
+            bits = largest_of_16(bits);
+            bits = max(__float_as_uint(div_rn(__uint_as_float(bits), 7.0f)), __float_as_uint(1.0e-8f));
+            const float scale = __uint_as_float(bits);
+            codes[i] = half_bytes(v[i], scale, div_rn(1.0f, scale));
+            const uint32_t t = t0 + 4 * i;
+            if (f == 0 && t >= from && t < to) (side ? a.cache.value_scales : a.cache.key_scales)[at + t] = scale;
+        }
+        if (side == 0) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const uint32_t t = t0 + 4 * i;
+                if (feature && t >= from && t < to)
+                    *reinterpret_cast<uint32_t*>(a.cache.keys + (at + t) * (d / 2u) + 4u * f) = codes[i];
+            }
+            continue;
+        }
+        // words 2 j and 2 j + 1: tokens 0-7 and 8-15 of feature j
+        uint32_t words[16];
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+#pragma unroll
+            for (int half = 0; half < 2; ++half) {
+                const uint32_t a0 = (codes[2 * half] >> (4 * j)) & 15u, a1 = (codes[2 * half + 1] >> (4 * j)) & 15u;
+                words[2 * j + half] = (a0 | (a1 << 16)) << (4u * t0);
+            }
+        // lanes of the upper half end with the upper half of the words, and so on
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            const auto p = __builtin_amdgcn_permlane32_swap(words[j], words[j + 8], false, false);
+            words[j] = p[0] | p[1];
+        }
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const auto p = __builtin_amdgcn_permlane16_swap(words[j], words[j + 4], false, false);
+            words[j] = p[0] | p[1];
+        }
+        // features 8 f + 4 (t0 / 2) + 2 (t0 % 2) and the next
+        if (!feature) continue;
+        u4_t out = {words[0], words[1], words[2], words[3]};
+        u4_t* const place = reinterpret_cast<u4_t*>(a.cache.values + at * (d / 2u) + 8u * (8u * f + 2u * t0));
+        if (to - from < 16u) {
+            const uint64_t mask = ((to < 16u ? 1ull << (4u * to) : 0ull) - (1ull << (4u * from)));
+            const uint32_t lo = static_cast<uint32_t>(mask), hi = static_cast<uint32_t>(mask >> 32);
+            const u4_t masks = {lo, hi, lo, hi};
+            out = (out & masks) | (*place & ~masks);
+        }
+        *place = out;
     }
 }
 
@@ -867,13 +956,12 @@ int dav2_hip_cache_store_i4(const dav2_cache_store_i4_args* args, void* stream) 
         a.dtype > DAV2_DTYPE_BF16 || a.sequences > 65535u || a.tokens > 0x7fffffffu || a.table_pages == 0 ||
         a.table_pages > 0x7fffffffu || (a.tokens > 1 && (a.key_stride < row || a.value_stride < row)))
         return hipErrorInvalidValue;
-    const uint64_t new_most = std::min(a.max_new, a.tokens);
-    const uint64_t pairs = new_most / 2 + 1;
+    const uint64_t chunks = (std::min(a.max_new, a.tokens) + 14u) / 16u + 1u;
     constexpr uint64_t kMostGroups = 1u << 22;  // workgroups along x: threads of a launch stay below 2^32
-    const dim3 grid(static_cast<uint32_t>(std::min<uint64_t>((pairs + 3) / 4, kMostGroups)), 2 * a.cache.kv_heads, a.sequences);
+    const dim3 grid(static_cast<uint32_t>(std::min(chunks, kMostGroups)), (2u * a.cache.kv_heads + 3u) / 4u, a.sequences);
     with_dtype(a.dtype, [&](auto* e) {
         typedef std::remove_pointer_t<decltype(e)> E;
-        dispatch(cache4_scale_kernel<E>, grid, dim3(256), 0, static_cast<hipStream_t>(stream), a);
+        dispatch(cache4_store_kernel<E>, grid, dim3(256), 0, static_cast<hipStream_t>(stream), a);
     });
     return hipGetLastError();
 }
