@@ -177,6 +177,50 @@ DAV2_DEV uint64_t moved64(uint64_t v) {
     return (static_cast<uint64_t>(static_cast<uint32_t>(hi)) << 32) | static_cast<uint32_t>(lo);
 }
 
+// The sum over the lanes up to this one: within rows of 16 lanes by row shifts,
+// then a row's last sum into the rows behind it.
+DAV2_DEV uint64_t wave_upto(uint64_t v) {
+    v += moved64<0x111, 0xf>(v);  // row_shr:1
+    v += moved64<0x112, 0xf>(v);
+    v += moved64<0x114, 0xf>(v);
+    v += moved64<0x118, 0xf>(v);  // row_shr:8
+    v += moved64<0x142, 0xa>(v);  // row_bcast:15 into rows 1 and 3
+    v += moved64<0x143, 0xc>(v);  // row_bcast:31 into rows 2 and 3
+    return v;
+}
+DAV2_DEV uint64_t lane63(uint64_t v) {
+    const uint32_t lo = __builtin_amdgcn_readlane(static_cast<int>(static_cast<uint32_t>(v)), 63);
+    const uint32_t hi = __builtin_amdgcn_readlane(static_cast<int>(static_cast<uint32_t>(v >> 32)), 63);
+    return (static_cast<uint64_t>(hi) << 32) | lo;
+}
+
+// The sum of what each of WAVES waves put into LDS, and of those before this one.
+template <uint32_t WAVES>
+DAV2_DEV uint64_t waves_before(const uint64_t* of_wave, uint64_t& all) {
+    const uint32_t lane = threadIdx.x & 63u, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const uint64_t upto = wave_upto(lane < WAVES ? of_wave[lane] : 0u);
+    all = lane63(upto);
+    const int before = wave ? static_cast<int>(wave) - 1 : 0;
+    const uint32_t lo = __builtin_amdgcn_readlane(static_cast<int>(static_cast<uint32_t>(upto)), before);
+    const uint32_t hi = __builtin_amdgcn_readlane(static_cast<int>(static_cast<uint32_t>(upto >> 32)), before);
+    return wave ? (static_cast<uint64_t>(hi) << 32) | lo : 0u;
+}
+
+// By a wave: the first of from .. to that is so, where all behind one that is so
+// are; `to`, if none is before it. 64 of them are asked at a time.
+template <typename F>
+DAV2_DEV uint32_t first_where(uint32_t from, uint32_t to, F&& so) {
+    const uint32_t lane = threadIdx.x & 63u;
+    while (from < to) {
+        const uint32_t step = (to - from - 1u) / 64u + 1u, at = min(from + lane * step, to);
+        const uint32_t before = static_cast<uint32_t>(__popcll(__ballot(at < to && !so(at))));  // lanes before it
+        if (before == 0) return from;
+        to = min(from + before * step, to);
+        from += (before - 1u) * step + 1u;
+    }
+    return to;
+}
+
 // The running maximum of a softmax before its first score. Finite, so that
 // exp2(maximum - larger maximum) is 0 and never the difference of infinities.
 constexpr float kNoScore = -3.0e38f;

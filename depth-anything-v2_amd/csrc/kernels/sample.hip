@@ -98,22 +98,6 @@ DAV2_DEV uint64_t units_of(double weight, int bits) {
     return static_cast<uint64_t>(__double_as_longlong(v)) & 0xfffffffffffffull;
 }
 
-// The sum over the lanes up to this one: within rows of 16 lanes by row shifts,
-// then a row's last sum into the rows behind it.
-DAV2_DEV uint64_t wave_upto(uint64_t v) {
-    v += moved64<0x111, 0xf>(v);  // row_shr:1
-    v += moved64<0x112, 0xf>(v);
-    v += moved64<0x114, 0xf>(v);
-    v += moved64<0x118, 0xf>(v);  // row_shr:8
-    v += moved64<0x142, 0xa>(v);  // row_bcast:15 into rows 1 and 3
-    v += moved64<0x143, 0xc>(v);  // row_bcast:31 into rows 2 and 3
-    return v;
-}
-DAV2_DEV uint64_t lane63(uint64_t v) {
-    const uint32_t lo = __builtin_amdgcn_readlane(static_cast<int>(static_cast<uint32_t>(v)), 63);
-    const uint32_t hi = __builtin_amdgcn_readlane(static_cast<int>(static_cast<uint32_t>(v >> 32)), 63);
-    return (static_cast<uint64_t>(hi) << 32) | lo;
-}
 DAV2_DEV uint64_t wave_sum64(uint64_t v) { return lane63(wave_upto(v)); }
 
 // of the search in the row itself
@@ -131,9 +115,7 @@ DAV2_DEV uint64_t group_sum(uint64_t v, uint64_t* of_wave) {
     __syncthreads();
     if ((threadIdx.x & 63u) == 0) of_wave[threadIdx.x >> 6] = v;
     __syncthreads();
-    v = 0;
-#pragma unroll
-    for (uint32_t w = 0; w < kWaves; ++w) v += of_wave[w];
+    waves_before<kWaves>(of_wave, v);
     return v;
 }
 
@@ -144,14 +126,7 @@ DAV2_DEV uint64_t group_before(uint64_t v, uint64_t* of_wave, uint64_t& all) {
     __syncthreads();
     if (lane == 63u) of_wave[wave] = upto;
     __syncthreads();
-    uint64_t before = 0;
-    all = 0;
-#pragma unroll
-    for (uint32_t w = 0; w < kWaves; ++w) {
-        before += w < wave ? of_wave[w] : 0;
-        all += of_wave[w];
-    }
-    return before + upto - v;
+    return waves_before<kWaves>(of_wave, all) + upto - v;
 }
 
 // The sum of weights that the last token of top-p passes: the first at which the
@@ -371,21 +346,6 @@ __global__ __launch_bounds__(kChunkThreads) void sample_largest_kernel(dav2_samp
     if (threadIdx.x == 0) state.largest[blockIdx.x] = fmaxf(fmaxf(of_wave[0], of_wave[1]), fmaxf(of_wave[2], of_wave[3]));
 }
 
-// By a wave: the first of from .. to that is so, where all behind one that is so
-// are; `to`, if none is before it. 64 of them are asked at a time.
-template <typename F>
-DAV2_DEV uint32_t first_where(uint32_t from, uint32_t to, F&& so) {
-    const uint32_t lane = threadIdx.x & 63u;
-    while (from < to) {
-        const uint32_t step = (to - from - 1u) / 64u + 1u, at = min(from + lane * step, to);
-        const uint32_t before = static_cast<uint32_t>(__popcll(__ballot(at < to && !so(at))));  // lanes before it
-        if (before == 0) return from;
-        to = min(from + before * step, to);
-        from += (before - 1u) * step + 1u;
-    }
-    return to;
-}
-
 // What the elements [begin, end) of a row add to its bins, in LDS: weights
 // where the list may not have all that is kept, counts where there is a top-k.
 template <uint32_t THREADS, typename E>
@@ -458,17 +418,9 @@ struct BinScan {
             sh.of_wave[1][wave] = s;
         }
         __syncthreads();
-        c -= count;
-        s -= sum;
-        whole = 0;
-#pragma unroll
-        for (uint32_t w = 0; w < THREADS / 64u; ++w) {
-            if (w < wave) {
-                c += sh.of_wave[0][w];
-                s += sh.of_wave[1][w];
-            }
-            whole += sh.of_wave[1][w];
-        }
+        uint64_t all;
+        c += waves_before<THREADS / 64u>(sh.of_wave[0], all) - count;
+        s += waves_before<THREADS / 64u>(sh.of_wave[1], whole) - sum;
         count_before = static_cast<uint32_t>(c);
         sum_before = s;
     }
