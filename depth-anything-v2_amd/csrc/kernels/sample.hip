@@ -320,11 +320,12 @@ DAV2_DEV float top_of(const RowState& state, uint32_t chunks) {
 // What the last one has weighs nothing: 2^-48 rounds to 0 in units of 2^-46.
 struct Bins {
     float top, scale;  // finite
+    DAV2_DEV float place(float l) const { return (top - l) * scale; }  // whose whole part is the bin
     DAV2_DEV Bins(float top_, const Asked& q)
         : top(fminf(top_, 3.0e38f)), scale(fminf(static_cast<float>(q.per_temperature * (kBins / 48.0)), 3.0e38f)) {}
     DAV2_DEV uint32_t operator()(float l) const {
         // NaN is in the last one: no number, or -infinity times nothing
-        return static_cast<uint32_t>(fmaxf(fminf((top - l) * scale, static_cast<float>(kBins - 1u)), 0.0f));
+        return static_cast<uint32_t>(fmaxf(fminf(place(l), static_cast<float>(kBins - 1u)), 0.0f));
     }
 };
 
@@ -394,25 +395,22 @@ struct BinScan {
         uint64_t of_wave[2][THREADS / 64];
         uint32_t found[8];
         uint64_t sums[4];  // before and of bins that were found
-        float bounds[6];
     };
     uint32_t counts[N], count_before;
     uint64_t sums[N], sum_before, whole;
     uint32_t low[3], high[3];  // bins of the list, both ends among them
-    float most[3], least[3];   // logits of them
-    int ranges;
 
-    DAV2_DEV void load(const uint32_t* of_counts, const unsigned long long* of_sums, Shared& sh) {
+    DAV2_DEV void load(const uint32_t* of_counts, const unsigned long long* of_sums, bool weighed, Shared& sh) {
         const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6;
         uint64_t count = 0, sum = 0;
 #pragma unroll
         for (uint32_t i = 0; i < N; ++i) {
             counts[i] = of_counts[threadIdx.x * N + i];
-            sums[i] = of_sums[threadIdx.x * N + i];
+            sums[i] = weighed ? of_sums[threadIdx.x * N + i] : 0u;
             count += counts[i];
             sum += sums[i];
         }
-        uint64_t c = wave_upto(count), s = wave_upto(sum);
+        uint64_t c = wave_upto(count), s = weighed ? wave_upto(sum) : 0u;
         if (lane == 63u) {
             sh.of_wave[0][wave] = c;
             sh.of_wave[1][wave] = s;
@@ -420,7 +418,8 @@ struct BinScan {
         __syncthreads();
         uint64_t all;
         c += waves_before<THREADS / 64u>(sh.of_wave[0], all) - count;
-        s += waves_before<THREADS / 64u>(sh.of_wave[1], whole) - sum;
+        whole = 0;
+        if (weighed) s += waves_before<THREADS / 64u>(sh.of_wave[1], whole) - sum;
         count_before = static_cast<uint32_t>(c);
         sum_before = s;
     }
@@ -494,28 +493,6 @@ struct BinScan {
         }
         range(drawn_of(q, lower), drawn_of(q, upper), 4, false);
     }
-    // The logits of those bins: the largest and the least of each range.
-    DAV2_DEV void bound(const Bins& bin_of, Shared& sh) {
-        for (uint32_t i = threadIdx.x >> 6; i < 6u; i += THREADS / 64u) {
-            const uint32_t which = i / 2u, last = i & 1u;
-            const uint32_t l = which == 0 ? low[0] : which == 1 ? low[1] : low[2];
-            const uint32_t h = which == 0 ? high[0] : which == 1 ? high[1] : high[2];
-            const uint32_t key = first_where(rank_key(INFINITY), rank_key(-INFINITY),
-                                             [&](uint32_t k) { return bin_of(logit_of(k)) >= (last ? h + 1u : l); });
-            if ((threadIdx.x & 63u) == 0)
-                sh.bounds[i] = l > h ? (last ? INFINITY : -INFINITY) : logit_of(last ? key - 1u : key);
-        }
-        __syncthreads();
-#pragma unroll
-        for (int i = 0; i < 3; ++i) {
-            most[i] = sh.bounds[2 * i];
-            least[i] = sh.bounds[2 * i + 1];
-        }
-        ranges = low[1] <= high[1] ? 3 : low[2] <= high[2] ? 2 : 1;
-    }
-    DAV2_DEV bool lists(float l) const {
-        return (l <= most[0] && l >= least[0]) || (l <= most[1] && l >= least[1]) || (l <= most[2] && l >= least[2]);
-    }
 };
 
 // f for the tokens of [begin, end) in those bins, which are few: a branch for
@@ -524,11 +501,22 @@ template <uint32_t THREADS, typename E, typename Scan, typename F>
 DAV2_DEV void for_listed(const Row<E>& row, const Scan& scan, uint32_t begin, uint32_t end, F&& f) {
     typedef Vec<E> V;
     constexpr uint32_t N = V::N, kTogether = 4, kStep = THREADS * N;
+    const Bins bin_of(row.top, row.q);
+    // in places of the bins; the last bin, where no number is, is in no list
+    float from[3], to[3];
+#pragma unroll
+    for (int i = 0; i < 3; ++i) {
+        const bool none = scan.low[i] > scan.high[i];
+        // an infinite top is before the first place
+        from[i] = none ? INFINITY : scan.low[i] ? static_cast<float>(scan.low[i]) : -INFINITY;
+        to[i] = none ? -INFINITY : static_cast<float>(scan.high[i] + 1u);
+    }
     auto pass = [&](auto ranges) {
         auto is = [&](float l) {
-            bool in = l <= scan.most[0] && l >= scan.least[0];
-            if constexpr (decltype(ranges)::value > 1) in = in || (l <= scan.most[2] && l >= scan.least[2]);
-            if constexpr (decltype(ranges)::value > 2) in = in || (l <= scan.most[1] && l >= scan.least[1]);
+            const float x = bin_of.place(l);
+            bool in = x >= from[0] && x < to[0];
+            if constexpr (decltype(ranges)::value > 1) in = in || (x >= from[2] && x < to[2]);
+            if constexpr (decltype(ranges)::value > 2) in = in || (x >= from[1] && x < to[1]);
             return in;
         };
         uint32_t c = begin + threadIdx.x * N;
@@ -554,9 +542,9 @@ DAV2_DEV void for_listed(const Row<E>& row, const Scan& scan, uint32_t begin, ui
                 if (is(l)) f(list_entry(l, i));
             }
     };
-    if (scan.ranges == 1) pass(std::integral_constant<int, 1>());
-    else if (scan.ranges == 2) pass(std::integral_constant<int, 2>());
-    else pass(std::integral_constant<int, 3>());
+    if (scan.low[1] <= scan.high[1]) pass(std::integral_constant<int, 3>());
+    else if (scan.low[2] <= scan.high[2]) pass(std::integral_constant<int, 2>());
+    else pass(std::integral_constant<int, 1>());
 }
 
 template <typename E>
@@ -571,9 +559,8 @@ __global__ __launch_bounds__(kChunkThreads) void sample_list_kernel(dav2_sample_
     if (threadIdx.x == 0) here = 0;
     const Row<E> row = {row_of<E>(a, chunk.row), a.vocabulary, bits, top, asked_of(a, chunk.row)};
     BinScan<kChunkThreads> scan;
-    scan.load(state.counts, state.sums, sh);
+    scan.load(state.counts, state.sums, row.q.top_k > kFew, sh);
     scan.choose(row.q, a.vocabulary, bits, sh);
-    scan.bound(Bins(row.top, row.q), sh);
     for_listed<kChunkThreads>(row, scan, chunk.begin, chunk.end, [&](unsigned long long entry) {
         const uint32_t at = atomicAdd(&here, 1u);
         if (at < kList) staged[at] = entry;
@@ -753,9 +740,8 @@ DAV2_DEV void put_token(const dav2_sample_args& a, const F& sh) {
 template <typename E, typename F>
 DAV2_DEV void list_and_finish(const Row<E>& row, F& sh) {
     BinScan<kThreads> scan;
-    scan.load(sh.counts, sh.sums, sh.bins);
+    scan.load(sh.counts, sh.sums, row.q.top_k > kFew, sh.bins);
     scan.choose(row.q, row.vocabulary, row.bits, sh.bins);
-    scan.bound(Bins(row.top, row.q), sh.bins);
     put_before(scan, sh);
     if (threadIdx.x == 0) sh.listed = 0;
     __syncthreads();
@@ -790,7 +776,7 @@ __global__ __launch_bounds__(kThreads) void sample_pick_kernel(dav2_sample_args 
     uint64_t whole = 0;
     if (gaps) {
         BinScan<kThreads> scan;
-        scan.load(state.counts, state.sums, sh.bins);
+        scan.load(state.counts, state.sums, true, sh.bins);
         put_before(scan, sh);
         whole = scan.whole;
     }
@@ -810,6 +796,25 @@ DAV2_DEV uint32_t pattern_of(uint32_t order) { return order < 32768u ? 32767u - 
 template <typename E>
 DAV2_DEV float number_of(uint32_t order) {
     return static_cast<float>(__builtin_bit_cast(E, static_cast<uint16_t>(pattern_of(order))));
+}
+
+// f(pattern, how often) for the numbers that are there.
+template <typename F>
+DAV2_DEV void for_keys(const Finish<true>& sh, F&& f) {
+    for (uint32_t i = threadIdx.x; i < kKeyWords / 4u; i += kThreads) {
+        const uint4 words = reinterpret_cast<const uint4*>(sh.keys)[i];
+        const uint32_t word[4] = {words.x, words.y, words.z, words.w};
+#pragma unroll
+        for (uint32_t j = 0; j < 4; ++j) {
+            if (word[j] == 0) continue;
+            if (word[j] & 0xffffu) f(8u * i + 2u * j, word[j] & 0xffffu);
+            if (word[j] >> 16) f(8u * i + 2u * j + 1u, word[j] >> 16);
+        }
+    }
+}
+template <typename E>
+DAV2_DEV float number_at(uint32_t pattern) {
+    return static_cast<float>(__builtin_bit_cast(E, static_cast<uint16_t>(pattern)));
 }
 
 // Whether all were counted: 65536 equal ones overflow their half word, and the
@@ -836,25 +841,32 @@ DAV2_DEV bool count_keys(const Row<E>& row, Finish<true>& sh) {
     for (; c < row.vocabulary; c += kStep)
         for (uint32_t i = c; i < min(c + 8u, row.vocabulary); ++i) add(raw[i]);
     __syncthreads();
-    const Bins bin_of(row.top, row.q);
     uint64_t counted = 0;
-    auto weigh = [&](uint32_t pattern, uint32_t n) {
-        const float l = static_cast<float>(__builtin_bit_cast(E, static_cast<uint16_t>(pattern)));
+    for_keys(sh, [&](uint32_t, uint32_t n) { counted += n; });
+    return group_sum(counted, sh.of_wave) == row.vocabulary;
+}
+
+// The largest logit, by the counts: a third of the row's reads.
+template <typename E>
+DAV2_DEV float top_of_keys(Finish<true>& sh) {
+    float top = -INFINITY;
+    for_keys(sh, [&](uint32_t pattern, uint32_t) { top = fmaxf(top, number_at<E>(pattern)); });
+    top = wave_max(top);
+    if ((threadIdx.x & 63u) == 0) sh.tops[threadIdx.x >> 6] = top;
+    __syncthreads();
+    return wave_max(sh.tops[threadIdx.x & (kWaves - 1u)]) + 0.0f;
+}
+
+// The bins' sums, a weight for each number.
+template <typename E>
+DAV2_DEV void weigh_keys(const Row<E>& row, Finish<true>& sh) {
+    const Bins bin_of(row.top, row.q);
+    for_keys(sh, [&](uint32_t pattern, uint32_t n) {
+        const float l = number_at<E>(pattern);
         const uint64_t w = row.units(rank_key(l));
         if (w) atomicAdd(&sh.sums[bin_of(l)], static_cast<unsigned long long>(w * n));
-    };
-    for (uint32_t i = threadIdx.x; i < kKeyWords / 4u; i += kThreads) {
-        const uint4 words = reinterpret_cast<const uint4*>(sh.keys)[i];
-        const uint32_t word[4] = {words.x, words.y, words.z, words.w};
-#pragma unroll
-        for (uint32_t j = 0; j < 4; ++j) {
-            if (word[j] == 0) continue;
-            counted += (word[j] & 0xffffu) + (word[j] >> 16);
-            if (word[j] & 0xffffu) weigh(8u * i + 2u * j, word[j] & 0xffffu);
-            if (word[j] >> 16) weigh(8u * i + 2u * j + 1u, word[j] >> 16);
-        }
-    }
-    return group_sum(counted, sh.of_wave) == row.vocabulary;
+    });
+    __syncthreads();
 }
 
 // Where the running sum passes `bound`: a number, which of its tokens, and the sum before that one.
@@ -879,28 +891,36 @@ DAV2_DEV Passed search_keys(const Row<E>& row, Finish<true>& sh, const BinScan<k
     auto first_of = [&](uint32_t b) {
         return first_where(infinity, last + 1u, [&](uint32_t o) { return bin_of(number_of<E>(o)) >= b; });
     };
-    const uint32_t end = first_of(bin + 1u);
-    uint64_t before = sh.bins.sums[0];
-    for (uint32_t from = first_of(bin); from < end; from += kThreads) {
-        const uint32_t o = from + threadIdx.x, pattern = pattern_of(o & 0xffffu);
-        uint32_t n = 0;
-        if (o < end) {
-            n = (sh.keys[pattern >> 1] >> (16u * (pattern & 1u))) & 0xffffu;
-            // both zeros are one number
-            if (pattern == 0u) n += sh.keys[0x8000u >> 1] & 0xffffu;
-            if (pattern == 0x8000u) n = 0;
+    const uint32_t begin = first_of(bin), end = first_of(bin + 1u);
+    // a run of neighbours for each thread: a bin about zero has thousands, few of which are there
+    const uint32_t each = (end - begin + kThreads - 1u) / kThreads;
+    const uint32_t from = min(begin + threadIdx.x * each, end), to = min(from + each, end);
+    auto count = [&](uint32_t o) {
+        const uint32_t pattern = pattern_of(o), n = (sh.keys[pattern >> 1] >> (16u * (pattern & 1u))) & 0xffffu;
+        // both zeros are one number
+        if (pattern == 0u) return n + (sh.keys[0x8000u >> 1] & 0xffffu);
+        return pattern == 0x8000u ? 0u : n;
+    };
+    auto weight = [&](uint32_t o) { return row.units(rank_key(number_of<E>(o))); };
+    uint64_t sum = 0;
+    for (uint32_t o = from; o < to; ++o)
+        if (const uint32_t n = count(o)) sum += n * weight(o);
+    uint64_t all;
+    uint64_t before = sh.bins.sums[0] + group_before(sum, sh.of_wave, all);
+    if (before <= bound && bound < before + sum) {
+        for (uint32_t o = from; o < to; ++o) {
+            const uint32_t n = count(o);
+            if (n == 0) continue;
+            const uint64_t w = weight(o);
+            if (bound < before + n * w) {
+                const uint64_t nth = (bound - before) / w;
+                sh.result[0] = before + nth * w;
+                sh.bins.found[1] = o;
+                sh.bins.found[2] = static_cast<uint32_t>(nth);
+                break;
+            }
+            before += n * w;
         }
-        const uint64_t w = n ? row.units(rank_key(number_of<E>(o))) : 0;
-        uint64_t all;
-        const uint64_t mine = before + group_before(w * n, sh.of_wave, all);
-        if (n && mine <= bound && bound < mine + w * n) {
-            const uint64_t nth = (bound - mine) / w;
-            sh.result[0] = mine + nth * w;
-            sh.bins.found[1] = o;
-            sh.bins.found[2] = static_cast<uint32_t>(nth);
-        }
-        before += all;
-        if (before > bound) break;  // the same for all threads
     }
     __syncthreads();
     const Passed passed = {sh.bins.found[1], sh.bins.found[2], sh.result[0]};
@@ -959,7 +979,7 @@ DAV2_DEV void find_nth(const Row<E>& row, Finish<true>& sh, float number, uint32
 template <typename E>
 DAV2_DEV void finish_keys(const Row<E>& row, Finish<true>& sh) {
     BinScan<kThreads> scan;
-    scan.load(sh.counts, sh.sums, sh.bins);
+    scan.load(sh.counts, sh.sums, true, sh.bins);
     uint64_t whole = scan.whole;
     if (row.q.top_p < 1.0) {
         const Passed last = search_keys(row, sh, scan, share_of(row.q.top_p, whole));
@@ -977,10 +997,6 @@ template <typename E, bool KEYS>
 __global__ __launch_bounds__(kThreads) void sample_row_kernel(dav2_sample_args a, int bits) {
     __shared__ Finish<KEYS> sh;
     Row<E> row = {row_of<E>(a, blockIdx.x), a.vocabulary, bits, 0.0f, asked_of(a, blockIdx.x)};
-    float top = -INFINITY;
-    for_each<kThreads>(row.logits, 0u, a.vocabulary, [&](float l, uint32_t) { top = fmaxf(top, l); });
-    top = wave_max(top);
-    if ((threadIdx.x & 63u) == 0) sh.tops[threadIdx.x >> 6] = top;
     if (threadIdx.x == 0) {
         sh.token = -1;
         sh.share = 0.0f;
@@ -989,27 +1005,31 @@ __global__ __launch_bounds__(kThreads) void sample_row_kernel(dav2_sample_args a
         sh.counts[b] = 0;
         sh.sums[b] = 0;
     }
+    if constexpr (KEYS) {
+        if (count_keys(row, sh)) {
+            row.top = top_of_keys<E>(sh);
+            if (!(row.top > -INFINITY)) return put_token(a, sh);
+            if (row.q.greedy) {
+                if (threadIdx.x == 0) sh.share = 1.0f;
+                find_nth(row, sh, row.top, 0u);
+            } else {
+                weigh_keys(row, sh);
+                finish_keys(row, sh);
+            }
+            return put_token(a, sh);
+        }
+    }
+    float top = -INFINITY;
+    for_each<kThreads>(row.logits, 0u, a.vocabulary, [&](float l, uint32_t) { top = fmaxf(top, l); });
+    top = wave_max(top);
+    if ((threadIdx.x & 63u) == 0) sh.tops[threadIdx.x >> 6] = top;
     __syncthreads();
-    for (uint32_t w = 0; w < kWaves; ++w) top = fmaxf(top, sh.tops[w]);
-    row.top = top + 0.0f;
+    row.top = wave_max(sh.tops[threadIdx.x & (kWaves - 1u)]) + 0.0f;
     if (!(row.top > -INFINITY)) return put_token(a, sh);
     if (a.vocabulary <= kList) {
         finish_row(row, sh, a.vocabulary, false, 0,
                    [&](uint32_t i) { return i < a.vocabulary ? list_entry(row.logit(i), i) : ~0ull; });
         return put_token(a, sh);
-    }
-    if constexpr (KEYS) {
-        if (row.q.greedy) {
-            if (threadIdx.x == 0) sh.share = 1.0f;
-            find_nth(row, sh, row.top, 0u);
-            return put_token(a, sh);
-        }
-        if (count_keys(row, sh)) {
-            finish_keys(row, sh);
-            return put_token(a, sh);
-        }
-        for (uint32_t b = threadIdx.x; b < kBins; b += kThreads) sh.sums[b] = 0;
-        __syncthreads();
     }
     fill_bins<kThreads>(row, 0u, a.vocabulary, sh.counts, sh.sums);
     __syncthreads();
