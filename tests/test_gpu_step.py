@@ -981,6 +981,68 @@ def test_two_graphs_and_streams(gpu, pkg, lib):
                 assert torch.equal(a, b), (step, i)
 
 
+def test_long_calls_captured(gpu, pkg, lib):
+    # the calls of several launches with a workspace: each replay on other inputs gives the bits of the eager call
+    torch = gpu
+    rows, wide = rand(torch, 1, 3, 100003, scale=2.5), rand(torch, 2, 100, 40000, dtype="bf16", scale=2.5)
+    u = torch.zeros(100, device="cuda")
+    top_p = floats(torch, [0.9] * 100)
+    cache = random_cache(torch, 3, 200, 2, 32, 64)
+    table = shuffled_table(torch, 4, 2, 100, 200)
+    q = rand(torch, 5, 2 * 200, 8, 64, dtype="f16")
+    starts, lengths = ints(torch, [0, 200, 400]), ints(torch, [3001, 2500])
+    held, added = ints(torch, [0] * 300), ints(torch, [7] * 300)
+    x = rand(torch, 6, 70, 5000, dtype="f16")
+
+    def make():
+        t = [torch.zeros(n, dtype=torch.int32, device="cuda") for n in (3, 100)]
+        p = [torch.zeros(n, device="cuda") for n in (3, 100)]
+        o, y = torch.zeros_like(q), torch.zeros_like(x)
+        codes, scales = torch.zeros((70, 5056), dtype=torch.int8, device="cuda"), torch.zeros(70, device="cuda")
+        pages = torch.zeros((300, 4), dtype=torch.int32, device="cuda")
+        ring = torch.arange(1000, dtype=torch.int32, device="cuda")
+        state = ints(torch, [3, 1000])
+        plan_out = [torch.zeros(n, dtype=torch.int32, device="cuda") for n in (300, 2, 301, 300, 2500, 2500)]
+        slots = torch.zeros(2500, dtype=torch.int64, device="cuda")
+        calls = []
+        for logits, tokens, share, dtype in ((rows, t[0], p[0], "f32"), (wide, t[1], p[1], "bf16")):
+            a, s = sample_args(torch, pkg, lib, logits, u, tokens, share, dtype, top_p=top_p)
+            calls.append(("dav2_hip_sample", a, s))
+        a, s = attend_args(torch, pkg, lib, cache, q, o, table, starts, lengths, True, "f16", 0.125)
+        calls.append(("dav2_hip_attention_cache_i4", a, s))
+        plan = pkg.CachePlanArgs(held=ptr(held), added=ptr(added), page_table=ptr(pages), free_pages=ptr(ring),
+                                 free_state=ptr(state), held_out=ptr(plan_out[0]), free_state_out=ptr(plan_out[1]),
+                                 starts=ptr(plan_out[2]), lengths=ptr(plan_out[3]), positions=ptr(plan_out[4]),
+                                 owners=ptr(plan_out[5]), slots=ptr(slots), sequences=300, table_pages=4, tokens=2500,
+                                 pages=1000, page_size=16)
+        calls.append(("dav2_hip_cache_plan", plan, with_scratch(torch, lib, "dav2_hip_cache_plan", plan)))
+        calls.append(("dav2_hip_add_rms_norm", norm_args(pkg, x, None, None, None, y, codes, scales, "f16"), None))
+        return calls, [*t, *p, o, y, codes, scales, pages, ring, *plan_out, slots, state]
+
+    (eager, want), (captured, got) = make(), make()
+    assert all(c[2] is not None for c in (captured[0], captured[2], captured[3]))
+    graph = torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph, stream=torch.cuda.Stream()):
+        for entry, args, _ in captured:
+            launch(torch, lib, entry, args)
+    for replay in range(4):
+        u.copy_(floats(torch, np.random.default_rng(replay).random(100).tolist()))
+        rows.mul_(-1.0)
+        wide.copy_(wide.flip(1))
+        q.mul_(0.9)
+        x.copy_(x.flip(0) * 1.1)
+        added.copy_(ints(torch, [(i * (replay + 3)) % 9 - 1 for i in range(300)]))
+        held.copy_(ints(torch, [(i * 5) % 30 for i in range(300)]))
+        torch.cuda.synchronize()
+        graph.replay()
+        for entry, args, _ in eager:
+            launch(torch, lib, entry, args)
+        torch.cuda.synchronize()
+        for i, (a, b) in enumerate(zip(want, got)):
+            assert torch.equal(a, b), (replay, i)
+
+
 def test_decoding_by_surface(gpu, pkg, lib, ops):
     # the same kernels through the operator surface, with the instance's own scratch
     torch = gpu
