@@ -64,7 +64,9 @@ DAV2_DEV uint32_t largest_of_16(uint32_t v) {
 // the four lanes of a feature join theirs, each ending with two of the eight
 // features and one store. A chunk that has older or later tokens too is read,
 // changed and written back; nobody else writes it. Bound by memory and by the
-// rounding: 8 prompts of up to 2048 tokens, 8 heads of 128, f16 (46 MB).
+// rounding: 8 prompts of up to 2048 tokens, 8 heads of 128, f16 (46 MB), 19 us,
+// 2.4 TB/s (41 with a workgroup for a page that reads its rows twice); a token
+// for each of 64 sequences 4.0 us, the call.
 template <typename E>
 __global__ __launch_bounds__(256) void cache4_store_kernel(dav2_cache_store_i4_args a) {
     const uint32_t lane = threadIdx.x & 63u, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -208,7 +210,9 @@ DAV2_DEV Parts parts_of(const dav2_attention_cache_i4_args& a, uint32_t splits) 
 //
 // A tile has COLS rows of 16 columns. With 4 or 8 the columns behind them would
 // have their scores weighed for nothing: the tiles' scores are spread over them
-// first, T tiles for each lane, and the weights gathered again.
+// first, T tiles for each lane, and the weights gathered again. Bound by memory
+// where the cache is long: 32 sequences of up to 32768 tokens, 32 heads of 8, 128
+// features, bf16 (651 MB) 143 us, 4.6 TB/s, in 4 columns; 179 in 16.
 DAV2_DEV constexpr uint32_t key_of(uint32_t t, uint32_t r) { return 8u * (t >> 1) + 2u * (t & 1u) + (r >> 1) + 4u * (r & 1u); }
 
 // Lanes of the banks (of four lanes) in BANKS: x of the lane that CTRL names; the others keep `old`.
@@ -539,6 +543,10 @@ __global__ __launch_bounds__(256, 2) void cache4_rows_kernel(dav2_attention_cach
 // Codes are widened once for all waves: a key's words of eight features in the
 // order of widen4, which the query's features are put in too; the tokens 0-3 and
 // 8-11 of a chunk, then 4-7 and 12-15, which are what a lane holds scores of.
+// Bound by LDS reads (scales are 24 of a wave's 56 of a tile) and vector units, beside one
+// another: 2 prompts of 2048 tokens at the end of 8192, 32 heads of 8, 128
+// features, f16 (316 GFLOP) 566 us, 560 TFLOP/s; 1125 with a scale read for
+// each score.
 template <typename E, int D, int WAVES>
 __global__ __launch_bounds__(64 * WAVES, D <= 64 && sizeof(E) == 2 ? 3 : 2)
 void cache4_tiles_kernel(dav2_attention_cache_i4_args a, uint32_t splits, uint32_t tiles) {
@@ -913,6 +921,31 @@ bool valid(const dav2_attention_cache_i4_args& a) {
            (a.tokens == 1 || (a.query_stride >= row && a.output_stride >= row));
 }
 
+// Which kernel, and how its keys are split. us; 32 heads of 8, 128 features, bf16,
+// unless it says otherwise.
+//
+// Tiles widen a key once for up to 256 rows, and leave waves without rows where
+// there are few: rows are faster up to a work of 2^26 (one sequence, 64 tokens
+// over 2048 19.0 / 25.1, over 4096 25.8 / 31.5; 4 of 128 over 512 22.1 / 30.1),
+// tiles beyond (128 over 8192 49.5 / 68.2).
+//
+// Rows: as few columns as hold them (32 of up to 4096 keys: 30.5 in 4 columns,
+// 38.8 in 16). Two workgroups share a CU, so up to 512 run at once: keys are split as
+// far as that goes, to 128 keys each (8 of 4096: 14.5 in 8, 19.9 in 2, 18.8 in 16; one
+// token over 1370, 16 heads of 64, f32: 9.2 in 10, 10.0 in 5, 11.3 in 2; 40 of 300: 9.4
+// whole, 13.8 in two). Beyond it a split only evens out sequences of different
+// lengths, and pays for long ones: up to 2048 workgroups of at least 2048 keys (32
+// of up to 32768: 142 in 8, 148 in 4, 159 in 2, 153 in 16).
+//
+// Tiles: splitting n keys s times costs n / s tiles one after the other and s
+// parts to join, so s grows as sqrt(n / 32) (128 tokens over 32768, 8 heads: 56.6;
+// sqrt(n / 64) 72.5, sqrt(n / 16) 58.9), and to one workgroup of 256 rows or two
+// of 128 a CU. 256 rows widen the keys once for twice the rows (566 against
+// 585 above; 512 tokens over 32768 336 against 363), if the head is so wide that
+// three waves of the smaller ones do not fit a SIMD instead, if they add no rows
+// that do not exist (2 of 577 tokens, 16 heads of 16: 36.0 against 33.8), and if
+// there are enough of them, one for each CU and two where a causal mask makes them
+// unequal (4096 tokens, 8 heads of 8: 103.9 against 94.8).
 struct Plan {
     uint32_t tile;  // rows: 4, 8 or 16 of cache4_rows_kernel, 128 or 256 of cache4_tiles_kernel
     uint32_t tiles, splits;

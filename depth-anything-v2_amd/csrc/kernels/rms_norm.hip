@@ -71,7 +71,7 @@ DAV2_DEV void store_codes(int8_t* row, uint32_t c, uint32_t columns, const float
 // 4096, bf16, sum, norm and codes (302 MB): 55 us, 5.5 TB/s, where a kernel that
 // reads the row again from the caches takes 71. The weights stay in registers
 // from row to row. Rows that are not multiples of 16 bytes are read as they lie:
-// 8191 of 5003 106 us, of 5008 87.
+// 8191 of 5003 100 us, of 5008 81.
 template <typename E, int LANES, int PIECES>
 __global__ __launch_bounds__(LANES < 256 ? 256 : LANES) void rms_norm_kept_kernel(dav2_add_rms_norm_args a) {
     typedef Vec<E> V;
@@ -249,8 +249,20 @@ __global__ __launch_bounds__(256) void rms_norm_kernel(dav2_add_rms_norm_args a)
 
 template <int I>
 using Lanes = std::integral_constant<int, I>;
-constexpr uint32_t kWorkgroups = 4096;  // sixteen for each CU, which go from row to row
-// From this many rows on a wave for each narrow one, instead of a workgroup.
+// Workgroups of a kernel for `groups` groups of rows. Wide rows: as many as run at
+// once, LANES * PIECES of 1024 and less by four to a CU (against a workgroup for
+// each row, us, bf16 with sum, norm and codes: 8191 of 6144 87 / 94, of 8192 115 /
+// 126, 4096 of 16384 125 / 135, 2048 of 32768 140 / 172). Others: two groups each,
+// and sixteen workgroups a CU before that (30000 of 4096 199 with one or two
+// groups each, 208 with sixteen workgroups a CU; 8191 of 4096 55 with two, 58 with
+// one; 32768 of 1024 54 with two, 58 with one).
+constexpr uint32_t workgroups_of(uint32_t groups, uint32_t lanes, uint32_t pieces) {
+    if (lanes * pieces > 512u) return std::min(groups, lanes * pieces <= 1024u ? 1024u : 1048576u / (lanes * pieces));
+    return std::min(groups, std::max(4096u, (groups + 1u) / 2u));
+}
+// From this many rows on a wave for each narrow one, instead of a workgroup: us,
+// 512 wide 1024 rows 3.9 / 5.1, 32768 rows 26 / 64, 256 rows alike; 1024 wide 256
+// rows 4.4 / 4.1, 32768 rows 55 / 85.
 constexpr uint32_t kNarrowRows = 512;
 
 }  // namespace
@@ -279,10 +291,14 @@ int dav2_hip_add_rms_norm(const dav2_add_rms_norm_args* args, void* stream) {
         // workgroups that share the rows out
         auto kept = [&](auto lanes, auto pieces) {
             constexpr int LANES = decltype(lanes)::value, kThreads = LANES < 256 ? 256 : LANES, kRows = kThreads / LANES;
-            dispatch(rms_norm_kept_kernel<E, LANES, decltype(pieces)::value>,
-                     dim3(std::min((a.rows + kRows - 1u) / kRows, kWorkgroups)), dim3(kThreads), 0, s, a);
+            constexpr int PIECES = decltype(pieces)::value;
+            dispatch(rms_norm_kept_kernel<E, LANES, PIECES>,
+                     dim3(workgroups_of((a.rows + kRows - 1u) / kRows, LANES, PIECES)), dim3(kThreads), 0, s, a);
         };
         const uint32_t vectors = (a.columns + N - 1u) / N;
+        // a lane's vectors: rows of 8192 in bf16, 8191 of them, us: 512 lanes of two 121,
+        // 256 of four 137, 1024 of one 144; 4096 of 16384 in 1024 of two 135, 512 of
+        // four 179; 2048 of 32768 in registers 172, read again 192
         if (vectors <= 128 && a.rows >= kNarrowRows) {
             if (vectors <= 64) kept(Lanes<64>(), Lanes<1>());
             else kept(Lanes<64>(), Lanes<2>());

@@ -12,7 +12,12 @@
 // tokens and what weight; and for the tokens of those few bins in which the three
 // searches can end, as a list. A workgroup for each row then sorts the list and
 // ends them. Where the list has no room (thousands of equal logits), it searches
-// the row itself.
+// the row itself. Rows of 16 bits without a top-k are counted number by number
+// instead, in one pass, and need no list.
+//
+// Bound by one CU's work on its rows, not by memory: a token's count is an atomic
+// operation in LDS, its weight a polynomial in 64 bits beside one. 4 rows of
+// 32000, fp32, every filter 13.9 us; 256 of 100003, bf16, top-p 39 us (51 MB).
 
 #include <algorithm>
 
@@ -1046,10 +1051,10 @@ int weight_bits(uint32_t vocabulary) {
 
 // Rows that workgroups share: few and long ones, and sooner where every token of
 // the row is weighed. us, a workgroup for each row against four launches, 4, 16
-// and 64 rows: fp32 with top-p alone, 32000 tokens 32 / 31, 35 / 33, 37 / 42, 100003
-// tokens 76 / 34, 93 / 51, 94 / 62; with top-k 32000 tokens 18 / 22, 18 / 24, 19 / 31,
-// 100003 tokens 25 / 22, 25 / 27, 27 / 33; bf16 with top-p alone 100003 tokens 43 / 34,
-// 49 / 46, 49 / 67.
+// and 64 rows: fp32 with top-p alone, 32000 tokens 30 / 28, 32 / 30, 34 / 39, 100003
+// tokens 75 / 31, 90 / 47, 90 / 59; with top-k 32000 tokens 14 / 20, 15 / 21, 15 / 25,
+// 100003 tokens 20 / 20, 21 / 23, 21 / 27; bf16 with top-p alone 100003 tokens 35 / 31,
+// 37 / 42, 37 / 63. One row of 262144: fp32 top-k 37 / 16, top-p 177 / 29, bf16 53 / 27.
 bool shares_rows(const dav2_sample_args& a) {
     if (a.vocabulary <= kList) return false;
     if (a.dtype == DAV2_DTYPE_F32 && !a.top_k) return a.rows <= 96 && a.vocabulary >= 24576u + 512u * a.rows;
@@ -1057,7 +1062,8 @@ bool shares_rows(const dav2_sample_args& a) {
 }
 
 // Rows whose 16-bit logits are counted by their value.
-bool by_key(const dav2_sample_args& a) { return !a.top_k && a.vocabulary >= 16384u; }
+// us, 64 rows, counted / not: 12000 tokens 27 / 18, 24000 30 / 28, 64000 33 / 67.
+bool by_key(const dav2_sample_args& a) { return !a.top_k && a.vocabulary >= 24576u; }
 
 // Logits of a chunk: 512 workgroups for the call, of 4096 and more each.
 uint32_t chunk_length(const dav2_sample_args& a) {

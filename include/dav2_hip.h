@@ -722,7 +722,8 @@ DAV2_API int dav2_hip_attention_cache_i4(const dav2_attention_cache_i4_args* arg
  * count, {first, count} = free_state, go in order to the sequences that need
  * any, in order. A sequence is served if it needs no page or if the pages that
  * it and the sequences before it need are there, if its tokens fit the table and
- * its rows fit `tokens`; one that does not fit needs nothing. If served it has
+ * are below 2^31, and if the step's rows up to its last one fit `tokens`; one that
+ * does not fit needs nothing. If served it has
  * length held[s] + added[s], and held_out[s] is that; if not, it gets no page,
  * has length 0, so that nothing is stored or seen in this step, and still holds
  * what it held. added[s] < 0: the sequence ends. Its pages go to the end of the
@@ -739,7 +740,8 @@ DAV2_API int dav2_hip_attention_cache_i4(const dav2_attention_cache_i4_args* arg
  * the table. The pages of a sequence belong to it alone. held_out may be held
  * and free_state_out free_state; other outputs overlap nothing. pages up to
  * 2^31 - 1, page_size 16 .. 256 in steps of 16, sequences below 2^16, tokens and
- * table_pages below 2^31. scratch: dav2_hip_cache_plan_scratch_bytes() bytes,
+ * table_pages below 2^31; with sequences 0 nothing is written. scratch:
+ * dav2_hip_cache_plan_scratch_bytes() bytes,
  * 16-byte aligned, in use until the call's work is done. */
 typedef struct dav2_cache_plan_args {
     const int32_t* held;         /* [sequences]                                    */
@@ -806,8 +808,9 @@ DAV2_API int dav2_hip_add_rms_norm(const dav2_add_rms_norm_args* args, void* str
  * the largest, tokens of it share the weight. A row without a finite logit and
  * without +infinity has token -1 and probability 0.
  *
- * Sums are integers: weights in units of 2^-s, s = 62 - ceil(log2(vocabulary)),
- * from 64-bit exponentials, so that a result does not depend on their order.
+ * Sums are integers: weights in units of 2^-s, s = 46 or, for 2^17 tokens and more,
+ * 62 - ceil(log2(vocabulary)), from 64-bit exponentials, so that a result does
+ * not depend on their order; a token below 2^-s-1 of the first weighs nothing.
  * vocabulary 1 .. 2^20, rows below 2^16; logits of a row are contiguous, rows
  * logit_stride elements apart. scratch: dav2_hip_sample_scratch_bytes() bytes,
  * 16-byte aligned, in use until the call's work is done. */

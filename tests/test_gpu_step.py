@@ -557,6 +557,15 @@ def test_norm(gpu, pkg, lib, dtype, rows, columns):
     check_norm(torch, pkg, lib, x, r, w, dtype, which=(True, False, True), epsilon=0.3)
 
 
+@pytest.mark.parametrize("dtype,rows,columns", [("bf16", 1100, 5003), ("f16", 1100, 8192), ("bf16", 600, 16384),
+                                                ("f32", 300, 16384), ("f16", 20000, 520), ("f32", 8203, 1024)])
+def test_norm_rows_in_turns(gpu, pkg, lib, dtype, rows, columns):
+    # more rows than are worked on at once
+    torch = gpu
+    x, r = rand(torch, 1, rows, columns, dtype=dtype), rand(torch, 2, rows, columns, dtype=dtype, scale=3.0)
+    check_norm(torch, pkg, lib, x, r, 1 + 0.3 * rand(torch, 3, columns), dtype)
+
+
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("columns", [100, 1024, 5000, 40000])
 def test_norm_in_place(gpu, pkg, lib, dtype, columns):
@@ -760,7 +769,8 @@ def test_sample_ties_and_masks(gpu, pkg, lib, dtype, vocabulary):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
-@pytest.mark.parametrize("rows,vocabulary", [(97, 4097), (130, 16390), (100, 40000), (98, 70001)])
+@pytest.mark.parametrize("rows,vocabulary", [(97, 4097), (130, 16390), (100, 40000), (98, 70001),
+                                             (40, 24580)])
 def test_sample_many_rows(gpu, pkg, lib, dtype, rows, vocabulary):
     # rows that have a workgroup each; some of equal logits, masked, or of one number in bulk
     torch = gpu
