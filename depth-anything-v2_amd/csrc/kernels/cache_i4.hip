@@ -543,10 +543,11 @@ __global__ __launch_bounds__(256, 2) void cache4_rows_kernel(dav2_attention_cach
 // Codes are widened once for all waves: a key's words of eight features in the
 // order of widen4, which the query's features are put in too; the tokens 0-3 and
 // 8-11 of a chunk, then 4-7 and 12-15, which are what a lane holds scores of.
-// Bound by LDS reads (scales are 24 of a wave's 56 of a tile) and vector units, beside one
-// another: 2 prompts of 2048 tokens at the end of 8192, 32 heads of 8, 128
-// features, f16 (316 GFLOP) 566 us, 560 TFLOP/s; 1125 with a scale read for
-// each score.
+// Bound by vector units (53 % busy), LDS (39 %; 24 of a wave's 56 reads of a tile
+// are scales) and matrix cores (34 %), partly beside one another: 2 prompts of
+// 2048 tokens at the end of 8192, 32 heads of 8, 128 features, f16 (316 GFLOP)
+// 566 us, 560 TFLOP/s; 1125 with a scale read for each score, 723 with 64 rows
+// a wave.
 template <typename E, int D, int WAVES>
 __global__ __launch_bounds__(64 * WAVES, D <= 64 && sizeof(E) == 2 ? 3 : 2)
 void cache4_tiles_kernel(dav2_attention_cache_i4_args a, uint32_t splits, uint32_t tiles) {
