@@ -188,6 +188,20 @@ DAV2_DEV uint64_t wave_upto(uint64_t v) {
     v += moved64<0x143, 0xc>(v);  // row_bcast:31 into rows 2 and 3
     return v;
 }
+DAV2_DEV uint32_t wave_upto32(uint32_t v) {
+    auto moved = [](uint32_t x, auto control, auto rows) {
+        return static_cast<uint32_t>(__builtin_amdgcn_update_dpp(0, static_cast<int>(x), decltype(control)::value,
+                                                                 decltype(rows)::value, 0xf, true));
+    };
+    using std::integral_constant;
+    v += moved(v, integral_constant<int, 0x111>(), integral_constant<int, 0xf>());
+    v += moved(v, integral_constant<int, 0x112>(), integral_constant<int, 0xf>());
+    v += moved(v, integral_constant<int, 0x114>(), integral_constant<int, 0xf>());
+    v += moved(v, integral_constant<int, 0x118>(), integral_constant<int, 0xf>());
+    v += moved(v, integral_constant<int, 0x142>(), integral_constant<int, 0xa>());
+    v += moved(v, integral_constant<int, 0x143>(), integral_constant<int, 0xc>());
+    return v;
+}
 DAV2_DEV uint64_t lane63(uint64_t v) {
     const uint32_t lo = __builtin_amdgcn_readlane(static_cast<int>(static_cast<uint32_t>(v)), 63);
     const uint32_t hi = __builtin_amdgcn_readlane(static_cast<int>(static_cast<uint32_t>(v >> 32)), 63);

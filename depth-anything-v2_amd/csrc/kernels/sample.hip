@@ -30,9 +30,12 @@ namespace {
 constexpr uint32_t kThreads = 1024, kWaves = kThreads / 64, kDigits = 2048;
 constexpr uint32_t kBins = 2048;        // of a row: 48 powers of two, the last one what is further
 constexpr uint32_t kList = 4096;        // tokens of a row's list
+// A row of so many is its own list: us, 64 rows of 60 tokens 5 against 9 with bins,
+// of 250 8.4 / 9.4, of 500 15.8 / 9.4, of 4000 41 / 10.
+constexpr uint32_t kSorted = 256;
 constexpr uint32_t kMostChunks = 64;    // workgroups that share a row
 constexpr uint32_t kChunkThreads = 256;
-constexpr uint32_t kFew = 2048;         // a top-k up to this many: the list has all of it, and the bins need no weights
+constexpr uint32_t kFew = 2048;         // a top-k up to this many is few
 
 // A logit's place in the order, 0 for the largest number there is: floats as
 // whole numbers that grow as they fall. -0 is 0, NaN is -infinity.
@@ -53,6 +56,7 @@ struct Asked {
     uint32_t top_k;  // at least 1
     float uniform;
     bool greedy;
+    bool few;  // the list has all that top-k leaves, and the bins need no weights
 };
 DAV2_DEV Asked asked_of(const dav2_sample_args& a, uint32_t row) {
     Asked q;
@@ -64,13 +68,14 @@ DAV2_DEV Asked asked_of(const dav2_sample_args& a, uint32_t row) {
     q.top_p = top_p < 1.0f ? fmaxf(top_p, 0.0f) : 1.0;  // NaN keeps all
     const int32_t k = a.top_k ? a.top_k[row] : 0;
     q.top_k = q.greedy ? 1u : k > 0 && static_cast<uint32_t>(k) < a.vocabulary ? static_cast<uint32_t>(k) : a.vocabulary;
+    q.few = q.top_k <= kFew && q.top_k < a.vocabulary;
     q.uniform = fminf(fmaxf(a.uniform[row], 0.0f), 0x1.fffffep-1f);  // fmaxf drops a NaN
     return q;
 }
 
-// 2^x for -100 < x <= 0: x = n + f, |f| <= 1/2, and the Taylor polynomial of 2^f of
-// degree 11, whose rest is below 2^-47. n is the low word of x + 1.5 * 2^52.
-DAV2_DEV double exp2_of(double x) {
+// 2^x over 2^n for -100 <= x <= 0: x = n + f, |f| <= 1/2, and the Taylor polynomial
+// of 2^f of degree 11, whose rest is below 2^-47. n is the low word of x + 1.5 * 2^52.
+DAV2_DEV double exp2_of(double x, int& n) {
     constexpr double kLn2 = 0.69314718055994530942, kRound = 0x1.8p52;
     constexpr double c2 = kLn2 * kLn2 / 2, c3 = c2 * kLn2 / 3, c4 = c3 * kLn2 / 4, c5 = c4 * kLn2 / 5,
                      c6 = c5 * kLn2 / 6, c7 = c6 * kLn2 / 7, c8 = c7 * kLn2 / 8, c9 = c8 * kLn2 / 9,
@@ -86,16 +91,18 @@ DAV2_DEV double exp2_of(double x) {
     p = fma(p, f, c3);
     p = fma(p, f, c2);
     p = fma(p, f, kLn2);
-    p = fma(p, f, 1.0);
-    const int n = static_cast<int>(__double2loint(rounded));
-    return p * __hiloint2double((n + 1023) << 20, 0);
+    n = static_cast<int>(__double2loint(rounded));
+    return fma(p, f, 1.0);
 }
 
 // exp((l - top) / temperature) in 64 bits. An infinite top has weight 1 and all others none.
 DAV2_DEV double weight_of(float l, float top, double per_temperature) {
     if (l == top) return 1.0;
     const double x = (static_cast<double>(l) - static_cast<double>(top)) * per_temperature;
-    return x > -100.0 ? exp2_of(x) : 0.0;  // a NaN is infinity less infinity
+    if (!(x > -100.0)) return 0.0;  // a NaN is infinity less infinity
+    int n;
+    const double p = exp2_of(x, n);
+    return ldexp(p, n);
 }
 // ... in units of 2^-bits, bits <= 46: the sum with 2^52 is rounded to a whole number, in its low 52 bits
 DAV2_DEV uint64_t units_of(double weight, int bits) {
@@ -166,6 +173,21 @@ struct Row {
         const double w = weight_of(l, top, q.per_temperature);
         return l > -INFINITY && w >= q.min_p ? units_of(w, bits) : 0;
     }
+
+    // units() of any logit under a largest one that is finite: what is below 2^-100
+    // or no number rounds to 0 by itself
+    struct Weigher {
+        double top, per_temperature, least;
+        int bits;
+        DAV2_DEV uint64_t operator()(float l) const {
+            const double x = fmax((static_cast<double>(l) - top) * per_temperature, -100.0);
+            int n;
+            const double v = ldexp(exp2_of(x, n), n + bits);
+            const uint64_t u = static_cast<uint64_t>(__double_as_longlong(v + 0x1p52)) & 0xfffffffffffffull;
+            return v >= least ? u : 0;
+        }
+    };
+    DAV2_DEV Weigher weigher() const { return {top, q.per_temperature, ldexp(q.min_p, bits), bits}; }
 
     // a token's weight over the whole
     DAV2_DEV float share(uint32_t key, uint64_t whole) const {
@@ -357,17 +379,21 @@ __global__ __launch_bounds__(kChunkThreads) void sample_largest_kernel(dav2_samp
 template <uint32_t THREADS, typename E>
 DAV2_DEV void fill_bins(const Row<E>& row, uint32_t begin, uint32_t end, uint32_t* counts, unsigned long long* sums) {
     const Bins bin_of(row.top, row.q);
-    if (row.q.top_k <= kFew) {
+    if (row.q.few) {
         for_each<THREADS>(row.logits, begin, end, [&](float l, uint32_t) { atomicAdd(&counts[bin_of(l)], 1u); });
         return;
     }
     const bool counted = row.q.top_k < row.vocabulary;
-    for_each<THREADS>(row.logits, begin, end, [&](float l, uint32_t) {
-        const uint32_t b = bin_of(l);
-        if (counted) atomicAdd(&counts[b], 1u);
-        const uint64_t w = row.units(rank_key(l));
-        if (w) atomicAdd(&sums[b], static_cast<unsigned long long>(w));
-    });
+    auto fill = [&](auto&& units) {
+        for_each<THREADS>(row.logits, begin, end, [&](float l, uint32_t) {
+            const uint32_t b = bin_of(l);
+            if (counted) atomicAdd(&counts[b], 1u);
+            const uint64_t w = units(l);
+            if (w) atomicAdd(&sums[b], static_cast<unsigned long long>(w));
+        });
+    };
+    if (row.top < INFINITY) fill(row.weigher());
+    else fill([&](float l) { return l == INFINITY ? 1ull << row.bits : 0ull; });
 }
 
 template <typename E>
@@ -466,7 +492,7 @@ struct BinScan {
             low[0] = 1;
             high[0] = 0;
         }
-        if (q.top_k <= kFew) {  // all that top-k keeps
+        if (q.few) {  // all that top-k keeps
             low[0] = 0;
             low[1] = low[2] = 1;
             high[1] = high[2] = 0;
@@ -500,10 +526,11 @@ struct BinScan {
     }
 };
 
-// f for the tokens of [begin, end) in those bins, which are few: a branch for
-// the elements that a thread loads together, not for each of them.
+// put(place, entry) for the tokens of [begin, end) in those bins, places being
+// counted in `listed`. A thread marks which of its elements are, and a wave
+// counts for all of its own at once.
 template <uint32_t THREADS, typename E, typename Scan, typename F>
-DAV2_DEV void for_listed(const Row<E>& row, const Scan& scan, uint32_t begin, uint32_t end, F&& f) {
+DAV2_DEV void for_listed(const Row<E>& row, const Scan& scan, uint32_t begin, uint32_t end, uint32_t* listed, F&& put) {
     typedef Vec<E> V;
     constexpr uint32_t N = V::N, kTogether = 4, kStep = THREADS * N;
     const Bins bin_of(row.top, row.q);
@@ -520,32 +547,38 @@ DAV2_DEV void for_listed(const Row<E>& row, const Scan& scan, uint32_t begin, ui
         auto is = [&](float l) {
             const float x = bin_of.place(l);
             bool in = x >= from[0] && x < to[0];
-            if constexpr (decltype(ranges)::value > 1) in = in || (x >= from[2] && x < to[2]);
-            if constexpr (decltype(ranges)::value > 2) in = in || (x >= from[1] && x < to[1]);
+            if constexpr (decltype(ranges)::value > 1) in |= x >= from[2] && x < to[2];
+            if constexpr (decltype(ranges)::value > 2) in |= x >= from[1] && x < to[1];
             return in;
         };
-        uint32_t c = begin + threadIdx.x * N;
-        for (; c + (kTogether - 1u) * kStep + N <= end; c += kTogether * kStep) {
-            float v[kTogether][N];
+        for (uint32_t c0 = begin; c0 < end; c0 += kTogether * kStep) {  // the same for all threads
+            const uint32_t c = c0 + threadIdx.x * N;
+            uint32_t marks = 0;
+            if (c + (kTogether - 1u) * kStep + N <= end) {
+                float v[kTogether][N];
 #pragma unroll
-            for (uint32_t t = 0; t < kTogether; ++t) V::load(row.logits, c + t * kStep, ~0u, v[t]);
+                for (uint32_t t = 0; t < kTogether; ++t) V::load(row.logits, c + t * kStep, ~0u, v[t]);
 #pragma unroll
-            for (uint32_t t = 0; t < kTogether; ++t) {
-                bool any = false;
+                for (uint32_t t = 0; t < kTogether; ++t)
 #pragma unroll
-                for (uint32_t i = 0; i < N; ++i) any |= is(v[t][i]);
-                if (__builtin_expect(any, 0)) {
-#pragma unroll
-                    for (uint32_t i = 0; i < N; ++i)
-                        if (is(v[t][i])) f(list_entry(v[t][i], c + t * kStep + i));
-                }
+                    for (uint32_t i = 0; i < N; ++i) marks |= is(v[t][i]) ? 1u << (t * N + i) : 0u;
+            } else {
+                for (uint32_t t = 0; t < kTogether; ++t)
+                    for (uint32_t i = 0; i < N; ++i) {
+                        const uint32_t at = c + t * kStep + i;
+                        if (at < end && is(row.logit(at))) marks |= 1u << (t * N + i);
+                    }
+            }
+            if (!__any(marks != 0u)) continue;
+            const uint32_t count = static_cast<uint32_t>(__popc(marks)), upto = wave_upto32(count);
+            uint32_t first = 0;
+            if ((threadIdx.x & 63u) == 63u) first = atomicAdd(listed, upto);
+            uint32_t at = static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(first), 63)) + upto - count;
+            for (; marks; marks &= marks - 1u) {
+                const uint32_t bit = static_cast<uint32_t>(__builtin_ctz(marks)), i = c + bit / N * kStep + bit % N;
+                put(at++, list_entry(row.logit(i), i));
             }
         }
-        for (; c < end; c += kStep)
-            for (uint32_t i = c; i < min(c + N, end); ++i) {
-                const float l = static_cast<float>(row.logits[i]);
-                if (is(l)) f(list_entry(l, i));
-            }
     };
     if (scan.low[1] <= scan.high[1]) pass(std::integral_constant<int, 3>());
     else if (scan.low[2] <= scan.high[2]) pass(std::integral_constant<int, 2>());
@@ -564,10 +597,9 @@ __global__ __launch_bounds__(kChunkThreads) void sample_list_kernel(dav2_sample_
     if (threadIdx.x == 0) here = 0;
     const Row<E> row = {row_of<E>(a, chunk.row), a.vocabulary, bits, top, asked_of(a, chunk.row)};
     BinScan<kChunkThreads> scan;
-    scan.load(state.counts, state.sums, row.q.top_k > kFew, sh);
+    scan.load(state.counts, state.sums, !row.q.few, sh);
     scan.choose(row.q, a.vocabulary, bits, sh);
-    for_listed<kChunkThreads>(row, scan, chunk.begin, chunk.end, [&](unsigned long long entry) {
-        const uint32_t at = atomicAdd(&here, 1u);
+    for_listed<kChunkThreads>(row, scan, chunk.begin, chunk.end, &here, [&](uint32_t at, unsigned long long entry) {
         if (at < kList) staged[at] = entry;
     });
     __syncthreads();
@@ -745,19 +777,18 @@ DAV2_DEV void put_token(const dav2_sample_args& a, const F& sh) {
 template <typename E, typename F>
 DAV2_DEV void list_and_finish(const Row<E>& row, F& sh) {
     BinScan<kThreads> scan;
-    scan.load(sh.counts, sh.sums, row.q.top_k > kFew, sh.bins);
+    scan.load(sh.counts, sh.sums, !row.q.few, sh.bins);
     scan.choose(row.q, row.vocabulary, row.bits, sh.bins);
     put_before(scan, sh);
     if (threadIdx.x == 0) sh.listed = 0;
     __syncthreads();
-    for_listed<kThreads>(row, scan, 0u, row.vocabulary, [&](unsigned long long entry) {
-        const uint32_t at = atomicAdd(&sh.listed, 1u);
+    for_listed<kThreads>(row, scan, 0u, row.vocabulary, &sh.listed, [&](uint32_t at, unsigned long long entry) {
         if (at < kList) sh.list[at] = entry;
     });
     __syncthreads();
     const uint32_t listed = sh.listed;
     if (listed > kList) return search_row(row, sh.search, &sh.token, &sh.share);
-    finish_row(row, sh, listed, row.q.top_k > kFew, scan.whole, [&](uint32_t i) { return i < listed ? sh.list[i] : ~0ull; });
+    finish_row(row, sh, listed, !row.q.few, scan.whole, [&](uint32_t i) { return i < listed ? sh.list[i] : ~0ull; });
 }
 
 // The end of a row that workgroups have shared.
@@ -777,7 +808,7 @@ __global__ __launch_bounds__(kThreads) void sample_pick_kernel(dav2_sample_args 
         search_row(row, sh.search, &sh.token, &sh.share);
         return put_token(a, sh);
     }
-    const bool gaps = row.q.top_k > kFew;
+    const bool gaps = !row.q.few;
     uint64_t whole = 0;
     if (gaps) {
         BinScan<kThreads> scan;
@@ -1031,7 +1062,7 @@ __global__ __launch_bounds__(kThreads) void sample_row_kernel(dav2_sample_args a
     __syncthreads();
     row.top = wave_max(sh.tops[threadIdx.x & (kWaves - 1u)]) + 0.0f;
     if (!(row.top > -INFINITY)) return put_token(a, sh);
-    if (a.vocabulary <= kList) {
+    if (a.vocabulary <= kSorted) {
         finish_row(row, sh, a.vocabulary, false, 0,
                    [&](uint32_t i) { return i < a.vocabulary ? list_entry(row.logit(i), i) : ~0ull; });
         return put_token(a, sh);
@@ -1050,20 +1081,22 @@ int weight_bits(uint32_t vocabulary) {
 }
 
 // Rows that workgroups share: few and long ones, and sooner where every token of
-// the row is weighed. us, a workgroup for each row against four launches, 4, 16
-// and 64 rows: fp32 with top-p alone, 32000 tokens 30 / 28, 32 / 30, 34 / 39, 100003
-// tokens 75 / 31, 90 / 47, 90 / 59; with top-k 32000 tokens 14 / 20, 15 / 21, 15 / 25,
-// 100003 tokens 20 / 20, 21 / 23, 21 / 27; bf16 with top-p alone 100003 tokens 35 / 31,
-// 37 / 42, 37 / 63. One row of 262144: fp32 top-k 37 / 16, top-p 177 / 29, bf16 53 / 27.
-bool shares_rows(const dav2_sample_args& a) {
-    if (a.vocabulary <= kList) return false;
-    if (a.dtype == DAV2_DTYPE_F32 && !a.top_k) return a.rows <= 96 && a.vocabulary >= 24576u + 512u * a.rows;
-    return a.rows <= 32 && a.vocabulary >= 65536u + 4096u * a.rows;
+// the row is weighed. us, a workgroup for each row against four launches, 1, 4, 16
+// and 64 rows: fp32 with top-p alone, 32000 tokens 22 / 24, 22 / 24, 23 / 26, 25 / 34,
+// 64000 35 / 25, 36 / 26, 37 / 28, 44 / 45, 100003 47 / 25, 50 / 27, 60 / 42, 60 / 50;
+// with top-k 64000 tokens 16 / 18, 19 / 20, 19 / 20, 20 / 26, 100003 19 / 18, 22 / 20,
+// 23 / 23, 24 / 28, 200000 32 / 18, 35 / 20, 37 / 25, 44 / 42; bf16 with top-p alone, 1, 4
+// and 16 rows, 100003 tokens 28 / 25, 35 / 30, 37 / 40, 200000 38 / 25, 46 / 36, 45 / 49.
+bool shares_rows(const dav2_sample_args& a, bool top_k) {
+    if (top_k) return a.rows <= 64 && a.vocabulary >= 73728u + 2048u * a.rows;
+    if (a.dtype == DAV2_DTYPE_F32) return a.rows <= 96 && a.vocabulary >= 36864u + 512u * a.rows;
+    return a.rows <= 8 && a.vocabulary >= 65536u + 4096u * a.rows;
 }
 
 // Rows whose 16-bit logits are counted by their value.
-// us, 64 rows, counted / not: 12000 tokens 27 / 18, 24000 30 / 28, 64000 33 / 67.
-bool by_key(const dav2_sample_args& a) { return !a.top_k && a.vocabulary >= 24576u; }
+// us, 64 rows, counted / not: 12000 tokens 26 / 16, 24000 30 / 24, 32000 29 / 30, 64000
+// 33 / 46, 100003 37 / 65.
+bool by_key(const dav2_sample_args& a) { return !a.top_k && a.vocabulary >= 28672u; }
 
 // Logits of a chunk: 512 workgroups for the call, of 4096 and more each.
 uint32_t chunk_length(const dav2_sample_args& a) {
@@ -1076,14 +1109,16 @@ uint32_t chunk_length(const dav2_sample_args& a) {
 extern "C" {
 
 uint64_t dav2_hip_sample_scratch_bytes(const dav2_sample_args* args) {
-    return args && shares_rows(*args) ? static_cast<uint64_t>(args->rows) * sizeof(RowState) : 0;
+    return args && (shares_rows(*args, false) || shares_rows(*args, true))
+               ? static_cast<uint64_t>(args->rows) * sizeof(RowState) : 0;
 }
 
 int dav2_hip_sample(const dav2_sample_args* args, void* stream) {
     if (!args) return hipErrorInvalidValue;
     const dav2_sample_args& a = *args;
     if (a.rows == 0) return hipSuccess;
-    const uint64_t need = dav2_hip_sample_scratch_bytes(args);
+    const bool shared = shares_rows(a, a.top_k != nullptr);
+    const uint64_t need = shared ? static_cast<uint64_t>(a.rows) * sizeof(RowState) : 0;
     if (!a.logits || !a.uniform || !a.tokens || a.rows > 65535u || a.vocabulary == 0 || a.vocabulary > (1u << 20) ||
         a.dtype > DAV2_DTYPE_BF16 || (a.rows > 1 && a.logit_stride < a.vocabulary) ||
         (need && (!a.scratch || !aligned16(a.scratch) || a.scratch_bytes < need)))
@@ -1092,7 +1127,7 @@ int dav2_hip_sample(const dav2_sample_args* args, void* stream) {
     const int bits = weight_bits(a.vocabulary);
     return with_dtype(a.dtype, [&](auto* e) -> int {
         typedef std::remove_pointer_t<decltype(e)> E;
-        if (shares_rows(a)) {
+        if (shared) {
             const uint32_t length = chunk_length(a), chunks = (a.vocabulary + length - 1u) / length;
             const dim3 grid(chunks, a.rows);
             dispatch(sample_largest_kernel<E>, grid, dim3(kChunkThreads), 0, s, a, length);

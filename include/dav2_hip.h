@@ -812,9 +812,9 @@ DAV2_API int dav2_hip_add_rms_norm(const dav2_add_rms_norm_args* args, void* str
  * ceil(log2(vocabulary))), from 64-bit exponentials, so that a result does not
  * depend on their order; a token below 2^-s-1 of the first weighs nothing.
  * vocabulary 1 .. 2^20, rows below 2^16; logits of a row are contiguous, rows
- * logit_stride elements apart. scratch: dav2_hip_sample_scratch_bytes() bytes (from
- * rows, vocabulary, dtype and whether top_k is NULL, where it is as much or
- * more), 16-byte aligned, in use until the call's work is done. */
+ * logit_stride elements apart. scratch: dav2_hip_sample_scratch_bytes() bytes, from
+ * rows, vocabulary and dtype alone, 16-byte aligned, in use until the call's work
+ * is done. */
 typedef struct dav2_sample_args {
     const void* logits;          /* [rows][vocabulary]                             */
     uint64_t logit_stride;

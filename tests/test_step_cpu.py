@@ -123,14 +123,13 @@ def test_scratch_is_checked(pkg, lib, block, entry):
             assert getattr(lib, entry)(C.byref(a), None) == 1
 
 
-def test_sample_scratch_without_top_k_is_enough(pkg, lib):
-    # a size asked for without a top-k serves calls with one
+def test_sample_scratch_by_sizes_alone(pkg, lib):
     for dtype in (0, 1, 2):
         for rows in (1, 2, 7, 16, 31, 32, 33, 64, 96, 97, 200):
             for vocabulary in (1, 4096, 4097, 25088, 32000, 65536, 69632, 100003, 131072, 200000, 1 << 20):
                 sizes = [lib.dav2_hip_sample_scratch_bytes(C.byref(pkg.SampleArgs(
                     rows=rows, vocabulary=vocabulary, dtype=dtype, top_k=k))) for k in (None, P)]
-                assert sizes[0] >= sizes[1], (dtype, rows, vocabulary)
+                assert sizes[0] == sizes[1], (dtype, rows, vocabulary)
 
 
 def test_argument_blocks_match_the_headers(pkg):
