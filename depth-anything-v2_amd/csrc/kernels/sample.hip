@@ -17,7 +17,7 @@
 //
 // Bound by one CU's work on its rows, not by memory: a token's count is an atomic
 // operation in LDS, its weight a polynomial in 64 bits beside one. 4 rows of
-// 32000, fp32, every filter 13.9 us; 256 of 100003, bf16, top-p 39 us (51 MB).
+// 32000, fp32, every filter 13.0 us; 256 of 100003, bf16, top-p 39 us (51 MB).
 
 #include <algorithm>
 
@@ -30,8 +30,8 @@ namespace {
 constexpr uint32_t kThreads = 1024, kWaves = kThreads / 64, kDigits = 2048;
 constexpr uint32_t kBins = 2048;        // of a row: 48 powers of two, the last one what is further
 constexpr uint32_t kList = 4096;        // tokens of a row's list
-// A row of so many is its own list: us, 64 rows of 60 tokens 5 against 9 with bins,
-// of 250 8.4 / 9.4, of 500 15.8 / 9.4, of 4000 41 / 10.
+// A row of so many is its own list: us, 64 rows of 60 tokens 5.7 against 9.5 with
+// bins, of 250 8.9 / 9.5, of 500 16.2 / 9.5, of 4000 41 / 11.
 constexpr uint32_t kSorted = 256;
 constexpr uint32_t kMostChunks = 64;    // workgroups that share a row
 constexpr uint32_t kChunkThreads = 256;
@@ -302,28 +302,53 @@ struct RowState {
     unsigned long long list[kList];  // rank key, index
 };
 
-// f(logit, index) for the elements [begin, end) of a row, by THREADS threads.
+// f(logit, index, bit) for the elements [begin, end) of a row, by THREADS threads
+// and up to 32 elements at a time, and next(c) after these: bit b of a thread is
+// the element index_of(c, b, end). Loads behind the end are of the last
+// elements instead, so that all are under way together. A row shorter than a
+// vector has no bits.
+template <typename E, uint32_t THREADS>
+struct Elements {
+    typedef Vec<E> V;
+    static constexpr uint32_t N = V::N, kTogether = 4, kStep = THREADS * N;
+    static DAV2_DEV uint32_t index_of(uint32_t c, uint32_t bit, uint32_t end) {
+        return min(c + bit / N * kStep, end - N) + bit % N;
+    }
+    template <typename F, typename G>
+    static DAV2_DEV void each(const E* row, uint32_t begin, uint32_t end, F&& f, G&& next) {
+        if (end < N) {
+            if (threadIdx.x == 0)
+                for (uint32_t i = begin; i < end; ++i) f(static_cast<float>(row[i]), i, i);
+            return;
+        }
+        for (uint32_t c0 = begin; c0 < end; c0 += kTogether * kStep) {  // the same for all threads
+            const uint32_t c = c0 + threadIdx.x * N;
+            float v[kTogether][N];
+#pragma unroll
+            for (uint32_t t = 0; t < kTogether; ++t) V::load(row, index_of(c, t * N, end), ~0u, v[t]);
+            if (c0 + kTogether * kStep <= end) {
+#pragma unroll
+                for (uint32_t t = 0; t < kTogether; ++t)
+#pragma unroll
+                    for (uint32_t i = 0; i < N; ++i) f(v[t][i], c + t * kStep + i, t * N + i);
+            } else {
+#pragma unroll
+                for (uint32_t t = 0; t < kTogether; ++t) {
+                    if (c0 + t * kStep >= end) break;
+#pragma unroll
+                    for (uint32_t i = 0; i < N; ++i) {
+                        const uint32_t at = index_of(c, t * N + i, end);
+                        if (at >= c + t * kStep) f(v[t][i], at, t * N + i);
+                    }
+                }
+            }
+            next(c);
+        }
+    }
+};
 template <uint32_t THREADS, typename E, typename F>
 DAV2_DEV void for_each(const E* row, uint32_t begin, uint32_t end, F&& f) {
-    typedef Vec<E> V;
-    constexpr uint32_t N = V::N, kTogether = 4, kStep = THREADS * N;  // loads that are under way together
-    uint32_t c = begin + threadIdx.x * N;
-    for (; c + (kTogether - 1u) * kStep + N <= end; c += kTogether * kStep) {
-        float v[kTogether][N];
-#pragma unroll
-        for (uint32_t t = 0; t < kTogether; ++t) V::load(row, c + t * kStep, ~0u, v[t]);
-#pragma unroll
-        for (uint32_t t = 0; t < kTogether; ++t)
-#pragma unroll
-            for (uint32_t i = 0; i < N; ++i) f(v[t][i], c + t * kStep + i);
-    }
-    for (; c < end; c += kStep) {
-        float v[N];
-        V::load(row, c, end, v);
-#pragma unroll
-        for (uint32_t i = 0; i < N; ++i)
-            if (c + i < end) f(v[i], c + i);
-    }
+    Elements<E, THREADS>::each(row, begin, end, [&](float l, uint32_t i, uint32_t) { f(l, i); }, [](uint32_t) {});
 }
 
 struct Chunk {
@@ -531,8 +556,6 @@ struct BinScan {
 // counts for all of its own at once.
 template <uint32_t THREADS, typename E, typename Scan, typename F>
 DAV2_DEV void for_listed(const Row<E>& row, const Scan& scan, uint32_t begin, uint32_t end, uint32_t* listed, F&& put) {
-    typedef Vec<E> V;
-    constexpr uint32_t N = V::N, kTogether = 4, kStep = THREADS * N;
     const Bins bin_of(row.top, row.q);
     // in places of the bins; the last bin, where no number is, is in no list
     float from[3], to[3];
@@ -551,34 +574,21 @@ DAV2_DEV void for_listed(const Row<E>& row, const Scan& scan, uint32_t begin, ui
             if constexpr (decltype(ranges)::value > 2) in |= x >= from[1] && x < to[1];
             return in;
         };
-        for (uint32_t c0 = begin; c0 < end; c0 += kTogether * kStep) {  // the same for all threads
-            const uint32_t c = c0 + threadIdx.x * N;
-            uint32_t marks = 0;
-            if (c + (kTogether - 1u) * kStep + N <= end) {
-                float v[kTogether][N];
-#pragma unroll
-                for (uint32_t t = 0; t < kTogether; ++t) V::load(row.logits, c + t * kStep, ~0u, v[t]);
-#pragma unroll
-                for (uint32_t t = 0; t < kTogether; ++t)
-#pragma unroll
-                    for (uint32_t i = 0; i < N; ++i) marks |= is(v[t][i]) ? 1u << (t * N + i) : 0u;
-            } else {
-                for (uint32_t t = 0; t < kTogether; ++t)
-                    for (uint32_t i = 0; i < N; ++i) {
-                        const uint32_t at = c + t * kStep + i;
-                        if (at < end && is(row.logit(at))) marks |= 1u << (t * N + i);
-                    }
-            }
-            if (!__any(marks != 0u)) continue;
-            const uint32_t count = static_cast<uint32_t>(__popc(marks)), upto = wave_upto32(count);
-            uint32_t first = 0;
-            if ((threadIdx.x & 63u) == 63u) first = atomicAdd(listed, upto);
-            uint32_t at = static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(first), 63)) + upto - count;
-            for (; marks; marks &= marks - 1u) {
-                const uint32_t bit = static_cast<uint32_t>(__builtin_ctz(marks)), i = c + bit / N * kStep + bit % N;
-                put(at++, list_entry(row.logit(i), i));
-            }
-        }
+        typedef Elements<E, THREADS> All;
+        uint32_t marks = 0;
+        All::each(
+            row.logits, begin, end, [&](float l, uint32_t, uint32_t bit) { marks |= is(l) ? 1u << bit : 0u; },
+            [&](uint32_t c) {
+                if (!__any(marks != 0u)) return;
+                const uint32_t count = static_cast<uint32_t>(__popc(marks)), upto = wave_upto32(count);
+                uint32_t first = 0;
+                if ((threadIdx.x & 63u) == 63u) first = atomicAdd(listed, upto);
+                uint32_t at = static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(first), 63)) + upto - count;
+                for (; marks; marks &= marks - 1u) {
+                    const uint32_t i = All::index_of(c, static_cast<uint32_t>(__builtin_ctz(marks)), end);
+                    put(at++, list_entry(row.logit(i), i));
+                }
+            });
     };
     if (scan.low[1] <= scan.high[1]) pass(std::integral_constant<int, 3>());
     else if (scan.low[2] <= scan.high[2]) pass(std::integral_constant<int, 2>());
@@ -1082,21 +1092,21 @@ int weight_bits(uint32_t vocabulary) {
 
 // Rows that workgroups share: few and long ones, and sooner where every token of
 // the row is weighed. us, a workgroup for each row against four launches, 1, 4, 16
-// and 64 rows: fp32 with top-p alone, 32000 tokens 22 / 24, 22 / 24, 23 / 26, 25 / 34,
-// 64000 35 / 25, 36 / 26, 37 / 28, 44 / 45, 100003 47 / 25, 50 / 27, 60 / 42, 60 / 50;
-// with top-k 64000 tokens 16 / 18, 19 / 20, 19 / 20, 20 / 26, 100003 19 / 18, 22 / 20,
-// 23 / 23, 24 / 28, 200000 32 / 18, 35 / 20, 37 / 25, 44 / 42; bf16 with top-p alone, 1, 4
-// and 16 rows, 100003 tokens 28 / 25, 35 / 30, 37 / 40, 200000 38 / 25, 46 / 36, 45 / 49.
+// and 64 rows: fp32 with top-p alone, 32000 tokens 23 / 21, 23 / 22, 24 / 23, 25 / 31,
+// 64000 36 / 22, 37 / 23, 38 / 26, 45 / 43, 100003 51 / 22, 53 / 24, 63 / 38, 63 / 52;
+// with top-k 64000 tokens 15 / 16, 18 / 18, 18 / 19, 19 / 24, 100003 20 / 16, 23 / 18,
+// 24 / 21, 24 / 27, 200000 32 / 16, 37 / 19, 37 / 24, 44 / 42; bf16 with top-p alone, 1, 4
+// and 16 rows, 100003 tokens 29 / 24, 35 / 29, 38 / 39, 200000 39 / 25, 46 / 35, 46 / 44.
 bool shares_rows(const dav2_sample_args& a, bool top_k) {
-    if (top_k) return a.rows <= 64 && a.vocabulary >= 73728u + 2048u * a.rows;
-    if (a.dtype == DAV2_DTYPE_F32) return a.rows <= 96 && a.vocabulary >= 36864u + 512u * a.rows;
+    if (top_k) return a.rows <= 64 && a.vocabulary >= 65536u + 2048u * a.rows;
+    if (a.dtype == DAV2_DTYPE_F32) return a.rows <= 96 && a.vocabulary >= 28672u + 640u * a.rows;
     return a.rows <= 8 && a.vocabulary >= 65536u + 4096u * a.rows;
 }
 
 // Rows whose 16-bit logits are counted by their value.
-// us, 64 rows, counted / not: 12000 tokens 26 / 16, 24000 30 / 24, 32000 29 / 30, 64000
-// 33 / 46, 100003 37 / 65.
-bool by_key(const dav2_sample_args& a) { return !a.top_k && a.vocabulary >= 28672u; }
+// us, 64 rows, counted / not: 12000 tokens 27 / 16, 32000 29 / 26, 64000 33 / 49,
+// 100003 37 / 67.
+bool by_key(const dav2_sample_args& a) { return !a.top_k && a.vocabulary >= 40960u; }
 
 // Logits of a chunk: 512 workgroups for the call, of 4096 and more each.
 uint32_t chunk_length(const dav2_sample_args& a) {

@@ -770,7 +770,7 @@ def test_sample_ties_and_masks(gpu, pkg, lib, dtype, vocabulary):
 
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("rows,vocabulary", [(97, 4097), (130, 16390), (100, 40000), (98, 70001),
-                                             (40, 24580)])
+                                             (40, 40970)])
 def test_sample_many_rows(gpu, pkg, lib, dtype, rows, vocabulary):
     # rows that have a workgroup each; some of equal logits, masked, or of one number in bulk
     torch = gpu
@@ -994,7 +994,7 @@ def test_two_graphs_and_streams(gpu, pkg, lib):
 def test_long_calls_captured(gpu, pkg, lib):
     # the calls of several launches with a workspace: each replay on other inputs gives the bits of the eager call
     torch = gpu
-    rows, wide = rand(torch, 1, 3, 100003, scale=2.5), rand(torch, 2, 100, 40000, dtype="bf16", scale=2.5)
+    rows, wide = rand(torch, 1, 3, 100003, scale=2.5), rand(torch, 2, 100, 42000, dtype="bf16", scale=2.5)
     u = torch.zeros(100, device="cuda")
     top_p = floats(torch, [0.9] * 100)
     cache = random_cache(torch, 3, 200, 2, 32, 64)
