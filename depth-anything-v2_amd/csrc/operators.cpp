@@ -383,7 +383,7 @@ void HipOperators::attention_fused(DeviceBuffer& output, const DeviceBuffer& qkv
     require_bytes(output, elements, "attention output");
     require_bytes(qkv, elements * 3, "QKV");
     const std::uint64_t need = attention_fused_scratch_bytes(tokens, heads, batch);
-    if (scratch.size() < need) throw std::invalid_argument("scratch device buffer is too small");
+    if (scratch.size() < need) throw std::invalid_argument("attention scratch device buffer is too small");
     const hipStream_t s = stream();
     // QK^T and PV: 4*T*T*64 flops per head.
     const double flops = 4.0 * batch * heads * double(tokens) * tokens * 64.0;
@@ -1142,17 +1142,17 @@ void HipOperators::cache_store_int8(const CacheBuffers& cache, const DeviceBuffe
     launch_check(dav2_hip_cache_store_i8(&a, stream()), "cache store");
 }
 
-void* HipOperators::scratch_of(const DeviceBuffer& given, std::uint64_t need, std::uint64_t& bytes) {
+void* HipOperators::scratch_of(const DeviceBuffer& given, std::uint64_t need, std::uint64_t& bytes, const std::string& of) {
     bytes = need;
     if (need == 0) return nullptr;
     if (given) {
-        if (given.size() < need) throw std::invalid_argument("scratch device buffer is too small");
+        if (given.size() < need) throw std::invalid_argument(of + " scratch device buffer is too small");
         return given.data();
     }
     hipStreamCaptureStatus capture = hipStreamCaptureStatusNone;
     hip_check(hipStreamIsCapturing(stream(), &capture), "capture status");
     if (capture != hipStreamCaptureStatusNone)
-        throw std::invalid_argument("a call under graph capture needs a scratch buffer of its own");
+        throw std::invalid_argument(of + " under graph capture needs a scratch buffer of its own");
     return grow(decoder_scratch_, need).data();
 }
 
@@ -1174,7 +1174,7 @@ void HipOperators::attention_cache_int8(DeviceBuffer& output, const DeviceBuffer
     a.page_table = page_table.as<std::int32_t>();
     a.starts = starts.as<std::int32_t>();
     a.lengths = lengths.as<std::int32_t>();
-    a.scratch = scratch_of(scratch, dav2_hip_attention_cache_i8_scratch_bytes(&a), a.scratch_bytes);
+    a.scratch = scratch_of(scratch, dav2_hip_attention_cache_i8_scratch_bytes(&a), a.scratch_bytes, "attention");
     // at most: every row sees max_length tokens
     ProfileScope prof(context_.profiler(), "attention_cache_i8", 4.0 * row * a.tokens * a.max_length, "FLOP", stream());
     launch_check(dav2_hip_attention_cache_i8(&a, stream()), "cache attention");
@@ -1206,7 +1206,7 @@ void HipOperators::cross_attention(DeviceBuffer& output, const DeviceBuffer& que
     a.key_lengths = key_lengths.as<std::int32_t>();
     a.key_mask = key_mask.as<std::uint8_t>();
     const std::uint64_t need = dav2k::cross_attention_uses_scratch(a) ? dav2_hip_cross_attention_scratch_bytes(&a) : 0;
-    a.scratch = scratch_of(scratch, need, a.scratch_bytes);
+    a.scratch = scratch_of(scratch, need, a.scratch_bytes, "attention");
     ProfileScope prof(context_.profiler(), "cross_attention",
                       4.0 * row * a.query_tokens * double(a.batch) * a.key_tokens, "FLOP", stream());
     launch_check(dav2_hip_cross_attention(&a, stream()), "cross attention");
@@ -1251,7 +1251,7 @@ void HipOperators::attention_cache_int4(DeviceBuffer& output, const DeviceBuffer
     a.page_table = page_table.as<std::int32_t>();
     a.starts = starts.as<std::int32_t>();
     a.lengths = lengths.as<std::int32_t>();
-    a.scratch = scratch_of(scratch, dav2_hip_attention_cache_i4_scratch_bytes(&a), a.scratch_bytes);
+    a.scratch = scratch_of(scratch, dav2_hip_attention_cache_i4_scratch_bytes(&a), a.scratch_bytes, "attention");
     // at most: every row sees max_length tokens
     ProfileScope prof(context_.profiler(), "attention_cache_i4", 4.0 * row * a.tokens * a.max_length, "FLOP", stream());
     launch_check(dav2_hip_attention_cache_i4(&a, stream()), "cache attention");
@@ -1284,7 +1284,7 @@ void HipOperators::cache_plan(const PlanBuffers& b, const DeviceBuffer& scratch,
     a.positions = b.positions.as<std::int32_t>();
     a.owners = b.owners.as<std::int32_t>();
     a.slots = b.slots.as<std::int64_t>();
-    a.scratch = scratch_of(scratch, dav2_hip_cache_plan_scratch_bytes(&a), a.scratch_bytes);
+    a.scratch = scratch_of(scratch, dav2_hip_cache_plan_scratch_bytes(&a), a.scratch_bytes, "cache plan");
     ProfileScope prof(context_.profiler(), "cache_plan", 16.0 * a.tokens + 20.0 * a.sequences, "B", stream());
     launch_check(dav2_hip_cache_plan(&a, stream()), "cache plan");
 }
@@ -1340,7 +1340,7 @@ void HipOperators::sample(DeviceBuffer& tokens, DeviceBuffer& probabilities, con
     a.uniform = uniform.as<float>();
     a.tokens = tokens.as<std::int32_t>();
     a.probabilities = probabilities.as<float>();
-    a.scratch = scratch_of(scratch, dav2_hip_sample_scratch_bytes(&a), a.scratch_bytes);
+    a.scratch = scratch_of(scratch, dav2_hip_sample_scratch_bytes(&a), a.scratch_bytes, "sampling");
     ProfileScope prof(context_.profiler(), "sample", static_cast<double>(size) * a.rows * a.vocabulary, "B", stream());
     launch_check(dav2_hip_sample(&a, stream()), "sampling");
 }

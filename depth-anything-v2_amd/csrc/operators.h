@@ -299,7 +299,7 @@ private:
                             bool has_bias, const DeviceBuffer* residual = nullptr, bool relu_output = false);
 
     // The scratch of a decoder operator's call: the caller's, or decoder_scratch_.
-    void* scratch_of(const DeviceBuffer& given, std::uint64_t need, std::uint64_t& bytes);
+    void* scratch_of(const DeviceBuffer& given, std::uint64_t need, std::uint64_t& bytes, const std::string& of);
 
     HipContext& context_;
     hipStream_t stream_ = nullptr;
