@@ -17,7 +17,7 @@
 //
 // Bound by one CU's work on its rows, not by memory: a token's count is an atomic
 // operation in LDS, its weight a polynomial in 64 bits beside one. 4 rows of
-// 32000, fp32, every filter 13.0 us; 256 of 100003, bf16, top-p 39 us (51 MB).
+// 32000, fp32, every filter 13.0 us; 256 of 100003, bf16, top-p 35 us (51 MB).
 
 #include <algorithm>
 
@@ -551,9 +551,26 @@ struct BinScan {
     }
 };
 
-// put(place, entry) for the tokens of [begin, end) in those bins, places being
+// put(place, index) for the elements of [begin, end) that are so, places being
 // counted in `listed`. A thread marks which of its elements are, and a wave
-// counts for all of its own at once.
+// counts for all of its own at once. The row is no shorter than a vector.
+template <uint32_t THREADS, typename E, typename Is, typename F>
+DAV2_DEV void gather(const E* row, uint32_t begin, uint32_t end, uint32_t* listed, Is&& is, F&& put) {
+    typedef Elements<E, THREADS> All;
+    uint32_t marks = 0;
+    All::each(
+        row, begin, end, [&](float l, uint32_t, uint32_t bit) { marks |= is(l) ? 1u << bit : 0u; },
+        [&](uint32_t c) {
+            if (!__any(marks != 0u)) return;
+            const uint32_t count = static_cast<uint32_t>(__popc(marks)), upto = wave_upto32(count);
+            uint32_t first = 0;
+            if ((threadIdx.x & 63u) == 63u) first = atomicAdd(listed, upto);
+            uint32_t at = static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(first), 63)) + upto - count;
+            for (; marks; marks &= marks - 1u) put(at++, All::index_of(c, static_cast<uint32_t>(__builtin_ctz(marks)), end));
+        });
+}
+
+// put(place, entry) for the tokens of [begin, end) in those bins.
 template <uint32_t THREADS, typename E, typename Scan, typename F>
 DAV2_DEV void for_listed(const Row<E>& row, const Scan& scan, uint32_t begin, uint32_t end, uint32_t* listed, F&& put) {
     const Bins bin_of(row.top, row.q);
@@ -574,21 +591,8 @@ DAV2_DEV void for_listed(const Row<E>& row, const Scan& scan, uint32_t begin, ui
             if constexpr (decltype(ranges)::value > 2) in |= x >= from[1] && x < to[1];
             return in;
         };
-        typedef Elements<E, THREADS> All;
-        uint32_t marks = 0;
-        All::each(
-            row.logits, begin, end, [&](float l, uint32_t, uint32_t bit) { marks |= is(l) ? 1u << bit : 0u; },
-            [&](uint32_t c) {
-                if (!__any(marks != 0u)) return;
-                const uint32_t count = static_cast<uint32_t>(__popc(marks)), upto = wave_upto32(count);
-                uint32_t first = 0;
-                if ((threadIdx.x & 63u) == 63u) first = atomicAdd(listed, upto);
-                uint32_t at = static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(first), 63)) + upto - count;
-                for (; marks; marks &= marks - 1u) {
-                    const uint32_t i = All::index_of(c, static_cast<uint32_t>(__builtin_ctz(marks)), end);
-                    put(at++, list_entry(row.logit(i), i));
-                }
-            });
+        gather<THREADS>(row.logits, begin, end, listed, is,
+                        [&](uint32_t at, uint32_t i) { put(at, list_entry(row.logit(i), i)); });
     };
     if (scan.low[1] <= scan.high[1]) pass(std::integral_constant<int, 3>());
     else if (scan.low[2] <= scan.high[2]) pass(std::integral_constant<int, 2>());
@@ -844,17 +848,21 @@ DAV2_DEV float number_of(uint32_t order) {
     return static_cast<float>(__builtin_bit_cast(E, static_cast<uint16_t>(pattern_of(order))));
 }
 
-// f(pattern, how often) for the numbers that are there.
+// f(pattern, how often) for the numbers that are there. Neighbouring numbers are
+// of neighbouring threads: those of a row lie close together.
 template <typename F>
 DAV2_DEV void for_keys(const Finish<true>& sh, F&& f) {
-    for (uint32_t i = threadIdx.x; i < kKeyWords / 4u; i += kThreads) {
-        const uint4 words = reinterpret_cast<const uint4*>(sh.keys)[i];
-        const uint32_t word[4] = {words.x, words.y, words.z, words.w};
+    constexpr uint32_t kTogether = 8;
+    for (uint32_t i0 = threadIdx.x; i0 < kKeyWords; i0 += kTogether * kThreads) {
+        uint32_t word[kTogether];
 #pragma unroll
-        for (uint32_t j = 0; j < 4; ++j) {
+        for (uint32_t j = 0; j < kTogether; ++j) word[j] = sh.keys[i0 + j * kThreads];
+#pragma unroll
+        for (uint32_t j = 0; j < kTogether; ++j) {
+            const uint32_t i = i0 + j * kThreads;
             if (word[j] == 0) continue;
-            if (word[j] & 0xffffu) f(8u * i + 2u * j, word[j] & 0xffffu);
-            if (word[j] >> 16) f(8u * i + 2u * j + 1u, word[j] >> 16);
+            if (word[j] & 0xffffu) f(2u * i, word[j] & 0xffffu);
+            if (word[j] >> 16) f(2u * i + 1u, word[j] >> 16);
         }
     }
 }
@@ -864,9 +872,9 @@ DAV2_DEV float number_at(uint32_t pattern) {
 }
 
 // Whether all were counted: 65536 equal ones overflow their half word, and the
-// sum of all counts is then another.
+// sum of all counts is then another. The largest logit goes into row.top.
 template <typename E>
-DAV2_DEV bool count_keys(const Row<E>& row, Finish<true>& sh) {
+DAV2_DEV bool count_keys(Row<E>& row, Finish<true>& sh) {
     typedef uint16_t Raw __attribute__((ext_vector_type(8), aligned(2)));
     const uint16_t* const raw = reinterpret_cast<const uint16_t*>(row.logits);
     for (uint32_t i = threadIdx.x; i < kKeyWords / 4u; i += kThreads)
@@ -888,19 +896,16 @@ DAV2_DEV bool count_keys(const Row<E>& row, Finish<true>& sh) {
         for (uint32_t i = c; i < min(c + 8u, row.vocabulary); ++i) add(raw[i]);
     __syncthreads();
     uint64_t counted = 0;
-    for_keys(sh, [&](uint32_t, uint32_t n) { counted += n; });
-    return group_sum(counted, sh.of_wave) == row.vocabulary;
-}
-
-// The largest logit, by the counts: a third of the row's reads.
-template <typename E>
-DAV2_DEV float top_of_keys(Finish<true>& sh) {
     float top = -INFINITY;
-    for_keys(sh, [&](uint32_t pattern, uint32_t) { top = fmaxf(top, number_at<E>(pattern)); });
+    for_keys(sh, [&](uint32_t pattern, uint32_t n) {
+        counted += n;
+        top = fmaxf(top, number_at<E>(pattern));
+    });
     top = wave_max(top);
     if ((threadIdx.x & 63u) == 0) sh.tops[threadIdx.x >> 6] = top;
-    __syncthreads();
-    return wave_max(sh.tops[threadIdx.x & (kWaves - 1u)]) + 0.0f;
+    const bool all = group_sum(counted, sh.of_wave) == row.vocabulary;
+    row.top = wave_max(sh.tops[threadIdx.x & (kWaves - 1u)]) + 0.0f;
+    return all;
 }
 
 // The bins' sums, a weight for each number.
@@ -974,9 +979,28 @@ DAV2_DEV Passed search_keys(const Row<E>& row, Finish<true>& sh, const BinScan<k
     return passed;
 }
 
-// The index of the nth token of a number, each wave counting a part of the row.
+// The index of the nth token of a number: by a list of all of them or, if they
+// are many, each wave counting a part of the row.
 template <typename E>
 DAV2_DEV void find_nth(const Row<E>& row, Finish<true>& sh, float number, uint32_t nth) {
+    constexpr uint32_t kMost = 256;
+    if (threadIdx.x == 0) sh.listed = 0;
+    __syncthreads();  // the keys, in whose place the list is, have been read
+    gather<kThreads>(row.logits, 0u, row.vocabulary, &sh.listed, [&](float l) { return l == number; },
+                     [&](uint32_t at, uint32_t i) {
+                         if (at < kMost) sh.list[at] = i;
+                     });
+    __syncthreads();
+    const uint32_t listed = sh.listed;
+    if (listed <= kMost) {
+        if (threadIdx.x >= listed) return;
+        const unsigned long long mine = sh.list[threadIdx.x];
+        uint32_t before_mine = 0;
+#pragma unroll 4
+        for (uint32_t j = 0; j < listed; ++j) before_mine += sh.list[j] < mine;
+        if (before_mine == nth) sh.token = static_cast<int32_t>(mine);
+        return;
+    }
     typedef Vec<E> V;
     constexpr uint32_t N = V::N, kBlock = 64 * N;
     const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6;
@@ -1053,7 +1077,6 @@ __global__ __launch_bounds__(kThreads) void sample_row_kernel(dav2_sample_args a
     }
     if constexpr (KEYS) {
         if (count_keys(row, sh)) {
-            row.top = top_of_keys<E>(sh);
             if (!(row.top > -INFINITY)) return put_token(a, sh);
             if (row.q.greedy) {
                 if (threadIdx.x == 0) sh.share = 1.0f;
@@ -1096,17 +1119,18 @@ int weight_bits(uint32_t vocabulary) {
 // 64000 36 / 22, 37 / 23, 38 / 26, 45 / 43, 100003 51 / 22, 53 / 24, 63 / 38, 63 / 52;
 // with top-k 64000 tokens 15 / 16, 18 / 18, 18 / 19, 19 / 24, 100003 20 / 16, 23 / 18,
 // 24 / 21, 24 / 27, 200000 32 / 16, 37 / 19, 37 / 24, 44 / 42; bf16 with top-p alone, 1, 4
-// and 16 rows, 100003 tokens 29 / 24, 35 / 29, 38 / 39, 200000 39 / 25, 46 / 35, 46 / 44.
+// and 16 rows, 64000 tokens 24 / 22, 26 / 24, 27 / 30, 100003 26 / 24, 29 / 29, 32 / 39,
+// 200000 35 / 24, 40 / 35, 41 / 44, 400000 52 / 33, 86 / 46, 83 / 72.
 bool shares_rows(const dav2_sample_args& a, bool top_k) {
     if (top_k) return a.rows <= 64 && a.vocabulary >= 65536u + 2048u * a.rows;
     if (a.dtype == DAV2_DTYPE_F32) return a.rows <= 96 && a.vocabulary >= 28672u + 640u * a.rows;
-    return a.rows <= 8 && a.vocabulary >= 65536u + 4096u * a.rows;
+    return a.rows <= 16 && a.vocabulary >= 65536u + 16384u * a.rows;
 }
 
 // Rows whose 16-bit logits are counted by their value.
-// us, 64 rows, counted / not: 12000 tokens 27 / 16, 32000 29 / 26, 64000 33 / 49,
-// 100003 37 / 67.
-bool by_key(const dav2_sample_args& a) { return !a.top_k && a.vocabulary >= 40960u; }
+// us, 64 rows, counted / not: 12000 tokens 23 / 16, 24000 26 / 22, 32000 25 / 26, 64000
+// 28 / 48, 100003 32 / 68.
+bool by_key(const dav2_sample_args& a) { return !a.top_k && a.vocabulary >= 28672u; }
 
 // Logits of a chunk: 512 workgroups for the call, of 4096 and more each.
 uint32_t chunk_length(const dav2_sample_args& a) {
