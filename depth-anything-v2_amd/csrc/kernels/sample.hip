@@ -12,8 +12,8 @@
 // tokens and what weight; and for the tokens of those few bins in which the three
 // searches can end, as a list. A workgroup for each row then sorts the list and
 // ends them. Where the list has no room (thousands of equal logits), it searches
-// the row itself. Rows of 16 bits without a top-k are counted number by number
-// instead, in one pass, and need no list.
+// the row itself. Long rows of 16 bits without a top-k are counted number by
+// number instead, in one pass, and read again for the places of the number drawn.
 //
 // Bound by one CU's work on its rows, not by memory: a token's count is an atomic
 // operation in LDS, its weight a polynomial in 64 bits beside one. 4 rows of
