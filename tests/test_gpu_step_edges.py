@@ -1,0 +1,59 @@
+"""Calls of a decoding step's operators at the edges of what their argument blocks
+say: sequences that get nothing."""
+
+import math
+
+import pytest
+
+import step_ref
+from test_gpu_step import ints, launch, rand, random_cache, store_args
+
+pytestmark = pytest.mark.gpu
+
+DTYPES = ["f32", "f16", "bf16"]
+
+
+# ---- storing ------------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("d", [64, 48])
+def test_store_of_nothing_leaves_the_page(gpu, pkg, lib, dtype, d):
+    # sequences without new rows, or whose rows are behind the last one, whose last page is begun
+    torch = gpu
+    cache = random_cache(torch, 3, 8, 2, 16, d)
+    for scales in cache[2:]:
+        scales[0], scales[1], scales[2], scales[3] = 0.0, 1e-9, math.nan, -1.0
+    before = [t.clone() for t in cache]
+    table = ints(torch, [[4, 0], [5, 1], [6, 2], [7, 3]])
+    k = rand(torch, 1, 6, 2, d, dtype=dtype)
+    for starts in ([2, 2, 2, 2, 2], [6, 9, 9, 11, 20]):
+        launch(torch, lib, "dav2_hip_cache_store_i4",
+               store_args(pkg, cache, k, k, table, ints(torch, starts), ints(torch, [17, 21, 31, 25]), 9, dtype))
+        torch.cuda.synchronize()
+        for a, b in zip(cache, before):
+            assert torch.equal(a.view(torch.uint8), b.view(torch.uint8))
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("behind", [0, 3])
+def test_store_beside_idle_sequences(gpu, pkg, lib, dtype, behind):
+    # lengths and table entries of idle sequences are stale: their pages belong to those that store now; the rows of
+    # those behind the last busy one, if they have any, do not exist
+    torch = gpu
+    sequences, page_size = 96, 32
+    cache = random_cache(torch, 3, 8, 2, page_size, 64)
+    table = ints(torch, [[i % 4, 4 + i % 4] for i in range(sequences)])
+    lengths = [33 + i % 31 for i in range(sequences)]
+    busy = {40: (0, 6), 41: (6, 7), 42: (7, 40), 43: (40, 43)}
+    starts, at = [], 0
+    for i in range(sequences + 1):
+        starts.append(at)
+        at = busy.get(i, (0, at))[1] + (behind if i > 43 else 0)
+    k, v = rand(torch, 1, 43, 2, 64, dtype=dtype), rand(torch, 2, 43, 2, 64, dtype=dtype, scale=3.0)
+    starts, lengths = ints(torch, starts), ints(torch, lengths)
+    want = step_ref.store(*cache, k, v, table, starts, lengths)
+    launch(torch, lib, "dav2_hip_cache_store_i4", store_args(pkg, cache, k, v, table, starts, lengths, 33, dtype))
+    torch.cuda.synchronize()
+    for got, w in zip(cache, want):
+        assert torch.equal(got.cpu(), w)
