@@ -369,14 +369,18 @@ DAV2_DEV float top_of(const RowState& state, uint32_t chunks) {
 }
 
 // The bin of a logit: no larger for a larger one, as each rounding keeps the order.
-// What the last one has weighs nothing: 2^-48 rounds to 0 in units of 2^-46.
+// What the last one has weighs nothing: 2^-48 rounds to 0 in units of 2^-46. A
+// distance is formed as its half, which no two finite numbers take past fp32, and
+// counts for something at any temperature: an infinite one stays infinite.
 struct Bins {
-    float top, scale;  // finite
-    DAV2_DEV float place(float l) const { return (top - l) * scale; }  // whose whole part is the bin
-    DAV2_DEV Bins(float top_, const Asked& q)
-        : top(fminf(top_, 3.0e38f)), scale(fminf(static_cast<float>(q.per_temperature * (kBins / 48.0)), 3.0e38f)) {}
+    float half_top, scale;  // finite, and not 0
+    // whose whole part is the bin
+    DAV2_DEV float place(float l) const { return fmaf(-0.5f, l, half_top) * scale; }
+    DAV2_DEV Bins(float top, const Asked& q)
+        : half_top(0.5f * fminf(top, 3.0e38f)),
+          scale(fminf(fmaxf(static_cast<float>(q.per_temperature * (2 * kBins / 48.0)), 0x1p-126f), 3.0e38f)) {}
     DAV2_DEV uint32_t operator()(float l) const {
-        // NaN is in the last one: no number, or -infinity times nothing
+        // NaN is in the last one
         return static_cast<uint32_t>(fmaxf(fminf(place(l), static_cast<float>(kBins - 1u)), 0.0f));
     }
 };

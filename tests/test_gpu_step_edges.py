@@ -1,12 +1,12 @@
 """Calls of a decoding step's operators at the edges of what their argument blocks
-say: sequences that get nothing."""
+say: sequences that get nothing, temperatures without end."""
 
 import math
 
 import pytest
 
 import step_ref
-from test_gpu_step import ints, launch, rand, random_cache, store_args
+from test_gpu_step import check_sample, ints, launch, rand, random_cache, store_args
 
 pytestmark = pytest.mark.gpu
 
@@ -57,3 +57,40 @@ def test_store_beside_idle_sequences(gpu, pkg, lib, dtype, behind):
     torch.cuda.synchronize()
     for got, w in zip(cache, want):
         assert torch.equal(got.cpu(), w)
+
+
+# ---- sampling ---------------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("vocabulary", [70, 5000, 40000, 270000])
+def test_sample_high_temperatures(gpu, pkg, lib, dtype, vocabulary):
+    # temperatures at which any finite logit has a weight, infinite ones too: beside logits further apart than fp32
+    # holds, masks of the lowest value, infinities; in lists, counted by value, with rows shared and not
+    torch = gpu
+    n = 12
+    x = rand(torch, vocabulary, n, vocabulary, dtype=dtype, scale=3.0)
+    f = torch.finfo(x.dtype)
+    x[1, 5] = x[1, vocabulary - 1] = math.inf
+    x[2, vocabulary // 2:] = f.min
+    x[3, ::2], x[3, 1::2] = f.max, f.min
+    x[4, : vocabulary // 3] = -math.inf
+    x[5, ::2] = math.nan
+    x[6] = f.min
+    x[7] = f.max
+    x[8] = f.min
+    x[8, vocabulary // 2] = f.max
+    x[9] = f.min
+    x[9, ::3] = math.inf
+    x[10] = (torch.linspace(-1.0, 1.0, vocabulary, device="cuda", dtype=torch.float64) * f.max).to(x.dtype)
+    x[11] = -math.inf
+    x[11, 7], x[11, 9] = f.min, f.max
+    hot = [math.inf, 3e38, 1e38, 1e37, 1e36]
+    for turn in range(len(hot)):
+        t = [hot[(i + turn) % len(hot)] for i in range(n)]
+        u = [(0.0, 0.31, 0.5, 0.77, 0.9999999)[(3 * i + turn) % 5] for i in range(n)]
+        check_sample(torch, pkg, lib, x, u, dtype, temperature=t)
+        check_sample(torch, pkg, lib, x, u, dtype, temperature=t, top_p=[0.6] * n)
+        check_sample(torch, pkg, lib, x, u, dtype, temperature=t, top_k=[vocabulary // 2] * n, top_p=[0.83] * n,
+                     min_p=[0.01] * n)
+        check_sample(torch, pkg, lib, x, u, dtype, temperature=t, top_k=[33] * n)
