@@ -255,10 +255,12 @@ using Lanes = std::integral_constant<int, I>;
 // 126, 4096 of 16384 125 / 135, 2048 of 32768 140 / 172). Others: two groups each,
 // and sixteen workgroups a CU before that (30000 of 4096 199 with one or two
 // groups each, 208 with sixteen workgroups a CU; 8191 of 4096 55 with two, 58 with
-// one; 32768 of 1024 54 with two, 58 with one).
+// one; 32768 of 1024 54 with two, 58 with one). Never more than 2^22: threads of a
+// launch stay below 2^32.
+constexpr uint32_t kMostGroups = 1u << 22;
 constexpr uint32_t workgroups_of(uint32_t groups, uint32_t lanes, uint32_t pieces) {
     if (lanes * pieces > 512u) return std::min(groups, lanes * pieces <= 1024u ? 1024u : 1048576u / (lanes * pieces));
-    return std::min(groups, std::max(4096u, (groups + 1u) / 2u));
+    return std::min({groups, std::max(4096u, (groups + 1u) / 2u), kMostGroups});
 }
 // From this many rows on a wave for each narrow one, instead of a workgroup: us,
 // 512 wide 1024 rows 3.9 / 5.1, 32768 rows 26 / 64, 256 rows alike; 1024 wide 256
@@ -292,6 +294,7 @@ int dav2_hip_add_rms_norm(const dav2_add_rms_norm_args* args, void* stream) {
         auto kept = [&](auto lanes, auto pieces) {
             constexpr int LANES = decltype(lanes)::value, kThreads = LANES < 256 ? 256 : LANES, kRows = kThreads / LANES;
             constexpr int PIECES = decltype(pieces)::value;
+            static_assert(uint64_t(workgroups_of(0x7fffffffu / kRows + 1u, LANES, PIECES)) * kThreads < 1ull << 32);
             dispatch(rms_norm_kept_kernel<E, LANES, PIECES>,
                      dim3(workgroups_of((a.rows + kRows - 1u) / kRows, LANES, PIECES)), dim3(kThreads), 0, s, a);
         };
@@ -315,7 +318,7 @@ int dav2_hip_add_rms_norm(const dav2_add_rms_norm_args* args, void* stream) {
         } else if (vectors <= 4096) {
             kept(Lanes<1024>(), Lanes<4>());
         } else {
-            dispatch(rms_norm_kernel<E>, dim3(std::min(a.rows, 1u << 22)), dim3(256), 0, s, a);
+            dispatch(rms_norm_kernel<E>, dim3(std::min(a.rows, kMostGroups)), dim3(256), 0, s, a);
         }
         return hipGetLastError();
     });

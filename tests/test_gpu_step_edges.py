@@ -1,12 +1,13 @@
 """Calls of a decoding step's operators at the edges of what their argument blocks
-say: sequences that get nothing, temperatures without end."""
+say: sequences that get nothing, more rows than a launch has, temperatures without
+end."""
 
 import math
 
 import pytest
 
 import step_ref
-from test_gpu_step import check_sample, ints, launch, rand, random_cache, store_args
+from test_gpu_step import check_sample, ints, launch, norm_args, rand, random_cache, store_args
 
 pytestmark = pytest.mark.gpu
 
@@ -57,6 +58,30 @@ def test_store_beside_idle_sequences(gpu, pkg, lib, dtype, behind):
     torch.cuda.synchronize()
     for got, w in zip(cache, want):
         assert torch.equal(got.cpu(), w)
+
+
+# ---- the norm ---------------------------------------------------------------------------
+
+
+def test_norm_of_more_rows_than_a_launch_has(gpu, pkg, lib):
+    # 2^27 rows and five more, of 4096 different ones
+    torch = gpu
+    rows, columns = (1 << 27) + 5, 8
+    x, r = rand(torch, 1, 4096, columns, dtype="bf16"), rand(torch, 2, 4096, columns, dtype="bf16", scale=3.0)
+    w = 1 + 0.3 * rand(torch, 3, columns)
+    h, y, s, c = (t.cuda() for t in step_ref.add_rms_norm(x, r, w, 1e-6))
+    c = torch.cat([c, torch.zeros((4096, 64 - columns), dtype=torch.int8, device="cuda")], dim=1)
+
+    def repeated(t):
+        return torch.cat([t[None].expand(rows // 4096, *t.shape).flatten(0, 1), t[:5]])
+
+    total, out = repeated(x), repeated(r)  # in place
+    codes, scales = torch.empty((rows, 64), dtype=torch.int8, device="cuda"), torch.empty(rows, device="cuda")
+    launch(torch, lib, "dav2_hip_add_rms_norm",
+           norm_args(pkg, total, out, w, total, out, codes, scales, "bf16"))
+    torch.cuda.synchronize()
+    for got, want in ((total, h), (out, y.to(x.dtype)), (codes, c), (scales, s)):
+        assert (got[:rows - 5].unflatten(0, (-1, 4096)) == want).all() and torch.equal(got[rows - 5:], want[:5])
 
 
 # ---- sampling ---------------------------------------------------------------------------
