@@ -545,17 +545,26 @@ __global__ __launch_bounds__(256, 2) void cache4_rows_kernel(dav2_attention_cach
 // Codes are widened once for all waves: a key's words of eight features in the
 // order of widen4, which the query's features are put in too; the tokens 0-3 and
 // 8-11 of a chunk, then 4-7 and 12-15, which are what a lane holds scores of.
+// A weight is one binary16 number for bf16, whose rounding of the output hides
+// 2^-12. For f16 it added as much error as that rounding does (2.7e-4 of the
+// output against 64 bits, where a 32-bit softmax has 2.1e-4): two parts, cut
+// rather than rounded, 2^-20 of a weight and 2^-38 of the largest at most. The
+// rest needs no factor as in for_second: it loses what a single part loses.
+//
 // Bound by vector units (53 % busy), LDS (39 %; 24 of a wave's 56 reads of a tile
 // are scales) and matrix cores (34 %), partly beside one another: 2 prompts of
-// 2048 tokens at the end of 8192, 32 heads of 8, 128 features, f16 (316 GFLOP)
-// 566 us, 560 TFLOP/s; 1125 with a scale read for each score, 723 with 64 rows
-// a wave.
+// 2048 tokens at the end of 8192, 32 heads of 8, 128 features (316 GFLOP), bf16
+// 561 us, 563 TFLOP/s; f16, with half as many products again, 658. One part for
+// f16: 566, 1125 with a scale read for each score, 723 with 64 rows a wave.
 template <typename E, int D, int WAVES>
 __global__ __launch_bounds__(64 * WAVES, D <= 64 && sizeof(E) == 2 ? 3 : 2)
 void cache4_tiles_kernel(dav2_attention_cache_i4_args a, uint32_t splits, uint32_t tiles) {
     constexpr bool kFloat = std::is_same_v<E, float>;
     constexpr int HEAD = D <= 64 ? 64 : 128;  // features of a row in LDS
     constexpr int KS = D / 16, FB = (D + 31) / 32, NP = kFloat ? 2 : 1;
+    constexpr int WP = std::is_same_v<E, __bf16> ? 1 : 2;  // parts of a weight
+    constexpr bool kPairs = WP == 2 && !kFloat;
+    constexpr int kSteps = kFloat ? FB : WP * FB;          // of the second product, for 16 keys
     constexpr uint32_t d = D;
     constexpr uint32_t kThreads = 64 * WAVES, kTileRows = 32 * WAVES;
     constexpr int kPieces = HEAD * 4 / kThreads;  // of 16 codes, for each thread and tile: keys, and values
@@ -658,7 +667,8 @@ void cache4_tiles_kernel(dav2_attention_cache_i4_args a, uint32_t splits, uint32
                     lds_scales[buffer][3][lane] = number ? fraction : 1.0f;
                 } else {
                     // the weights take the whole scale, off by half a step of its
-                    // logarithm: below 2^-20 of them for scales of 1e-8 and more
+                    // logarithm: below 2^-20 of them for scales of 1e-8 to 2^32,
+                    // 2^-18 for any
                     exponent += __builtin_amdgcn_logf(number ? fraction : 1.0f);
                     inverse = inverse / (number ? fraction : 1.0f);
                 }
@@ -836,10 +846,12 @@ void cache4_tiles_kernel(dav2_attention_cache_i4_args a, uint32_t splits, uint32
                         for (int r = 0; r < 16; ++r) o[f][r] *= keep;
                 }
                 // weights of chunk t + 1 between the products of chunk t
-                h8 pf[2][NP];
+                h8 pf[2][WP];
                 v4f share[2], fraction[2];
-                auto weigh = [&](int t, int r) {
-                    if (r % 4 == 0) {
+                float before = 0.0f;  // a weight that waits for its neighbour
+                auto weigh = [&](int t, int i) {
+                    const int r = kPairs ? 4 * (i & 1) + i / 2 : i;
+                    if (kPairs ? i < 2 : r % 4 == 0) {
                         share[r / 4] = read_scales(2, t >> 1, 2 * (t & 1) + r / 4);
                         if constexpr (kFloat) fraction[r / 4] = read_scales(3, t >> 1, 2 * (t & 1) + r / 4);
                     }
@@ -851,6 +863,16 @@ void cache4_tiles_kernel(dav2_attention_cache_i4_args a, uint32_t splits, uint32
                         const _Float16 hi = static_cast<_Float16>(y);
                         pf[t & 1][0][to] = hi;
                         pf[t & 1][1][to] = static_cast<_Float16>((y - static_cast<float>(hi)) * kSecond);
+                    } else if constexpr (kPairs) {
+                        if (i % 2 == 0) {
+                            before = w;
+                        } else {
+                            const h2 hi = __builtin_bit_cast(h2, __builtin_amdgcn_cvt_pkrtz(before, w));
+                            const h2 lo = __builtin_bit_cast(h2, __builtin_amdgcn_cvt_pkrtz(before - static_cast<float>(hi[0]),
+                                                                                            w - static_cast<float>(hi[1])));
+                            pf[t & 1][0][to - 1] = hi[0], pf[t & 1][0][to] = hi[1];
+                            pf[t & 1][1][to - 1] = lo[0], pf[t & 1][1][to] = lo[1];
+                        }
                     } else {
                         pf[t & 1][0][to] = static_cast<_Float16>(w);
                     }
@@ -862,15 +884,16 @@ void cache4_tiles_kernel(dav2_attention_cache_i4_args a, uint32_t splits, uint32
                     __builtin_amdgcn_sched_barrier(0);
                     if (t < 3) read_values(t + 1, vf[(t + 1) & 1]);
 #pragma unroll
-                    for (int f = 0; f < FB; ++f) {
-                        o[f] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf[t & 1][f], pf[t & 1][0], o[f], 0, 0, 0);
+                    for (int i = 0; i < kSteps; ++i) {
+                        const int f = i % FB;
+                        o[f] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf[t & 1][f], pf[t & 1][i / FB], o[f], 0, 0, 0);
                         if constexpr (kFloat)
                             o[f] = __builtin_amdgcn_mfma_f32_32x32x16_f16(for_second(vf[t & 1][f]), pf[t & 1][1], o[f], 0,
                                                                           0, 0);
                         if (t < 3)
 #pragma unroll
-                            for (int r = 8 * f / FB; r < 8 * (f + 1) / FB; ++r) weigh(t + 1, r);
-                        __builtin_amdgcn_sched_barrier(0);
+                            for (int r = 8 * i / kSteps; r < 8 * (i + 1) / kSteps; ++r) weigh(t + 1, r);
+                        if (!kPairs || i % 2) __builtin_amdgcn_sched_barrier(0);
                     }
                 }
             }
@@ -943,12 +966,13 @@ bool valid(const dav2_attention_cache_i4_args& a) {
 // Tiles: splitting n keys s times costs n / s tiles one after the other and s
 // parts to join, so s grows as sqrt(n / 32) (128 tokens over 32768, 8 heads: 56.6;
 // sqrt(n / 64) 72.5, sqrt(n / 16) 58.9), and to one workgroup of 256 rows or two
-// of 128 a CU. 256 rows widen the keys once for twice the rows (566 against
-// 585 above; 512 tokens over 32768 336 against 363), if the head is so wide that
-// three waves of the smaller ones do not fit a SIMD instead, if they add no rows
-// that do not exist (2 of 577 tokens, 16 heads of 16: 36.0 against 33.8), and if
-// there are enough of them, one for each CU and two where a causal mask makes them
-// unequal (4096 tokens, 8 heads of 8: 103.9 against 94.8).
+// of 128 a CU. 256 rows widen the keys once for twice the rows (2 of 2048 over
+// 8192 561 against 583, f16 661 / 679; 512 over 32768 334 / 361, f16 417 / 446),
+// if the head is so wide that three waves of the smaller ones do not fit a SIMD
+// instead, if they add no rows that do not exist (2 of 577 tokens, 16 heads of 16:
+// 36.0 against 33.8), and if there are enough of them, one for each CU and two
+// where a causal mask makes them unequal (4096 tokens, 8 heads of 8: 103.9 against
+// 94.8).
 struct Plan {
     uint32_t tile;  // rows: 4, 8 or 16 of cache4_rows_kernel, 128 or 256 of cache4_tiles_kernel
     uint32_t tiles, splits;

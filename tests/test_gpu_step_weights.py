@@ -9,7 +9,7 @@ import pytest
 import decoder_ref as ref
 import step_ref
 from test_gpu_decoder_weights import CACHE_STEPS, mean_of_largest, sink_query, want_of
-from test_gpu_step import attend_args, ints, launch
+from test_gpu_step import attend_args, ints, launch, rand
 
 pytestmark = pytest.mark.gpu
 
@@ -118,3 +118,32 @@ def test_scores_past_2_to_30(gpu, pkg, lib, dtype, sign, queries, sequences, mos
         # equal weights: the sums of n products, the quotient, the output's rounding
         bound = v.abs().max() * (64 + n / 32) * ref.U + want.abs() * ref.half_step(dtype) + ref.floor_of(dtype)
         ref.assert_within(out[:, h], want, bound + 0 * want)
+
+
+@pytest.mark.parametrize("dtype,queries", [("f32", 1), ("f16", 1), ("bf16", 1), ("f32", 32), ("f16", 32), ("f32", 40),
+                                           ("f16", 40)])
+@pytest.mark.parametrize("sequences,most", [(4, 2 ** 22), (128, 255)])
+@pytest.mark.parametrize("length", [40, 68, 1580])
+@pytest.mark.parametrize("d", [48, 64, 96, 128])
+def test_outputs_round_once(gpu, pkg, lib, dtype, queries, sequences, most, length, d):
+    # weights of 20 bits and more, so that the output's own rounding is what is left: rows and tiles of both heights,
+    # the keys whole and split, scales of values far apart
+    torch = gpu
+    page_size, heads, kv = 32, 16, 2
+    pages = -(-length // page_size)
+    g = torch.Generator(device="cuda").manual_seed(length + d)
+    keys, values = (torch.randint(-8, 8, (pages, kv, page_size, d), generator=g, dtype=torch.int8, device="cuda")
+                    for _ in range(2))
+    ks, vs = (0.02 + 0.2 * torch.rand((pages, kv, page_size), generator=g, device="cuda") for _ in range(2))
+    vs *= 2.0 ** -torch.randint(0, 8, vs.shape, generator=g, device="cuda")
+    cache = [step_ref.pack(keys), step_ref.pack_values(values), ks, vs]
+    table = torch.randperm(pages, generator=g, device="cuda").to(torch.int32)
+    q = rand(torch, 8, queries, heads, d, dtype=dtype)
+    out = attend(torch, pkg, lib, cache, q, table, length, queries, sequences, most, dtype, 0.02)
+    for h in range(heads):
+        k, v = ((c[table.long(), h // 8].double() * s[table.long(), h // 8].double()[..., None]).reshape(-1, d)[:length]
+                for c, s in ((keys, ks), (values, vs)))
+        # a weight's two parts, 2^-20 of it, and its exponent with a scale's logarithm, 2^-20 at most, which is in
+        # the sum of the weights too
+        want, bound = want_of(q[:, h].double(), k, v, 0.02, dtype, 2.0 ** -19, 2.0 ** -37, exponent=8.0)
+        ref.assert_within(out[:, h], want, bound + want.abs() * 2.0 ** -20)
