@@ -13,7 +13,8 @@ using namespace dav2k;
 
 namespace {
 
-// vectors at addresses that are multiples of less
+// vectors, `any` and `by` at addresses that are multiples of less
+typedef float v2f __attribute__((ext_vector_type(2)));
 typedef float v2f_any __attribute__((ext_vector_type(2), aligned(4)));
 typedef uint32_t u4_by8 __attribute__((ext_vector_type(4), aligned(8)));
 typedef uint32_t u4_t __attribute__((ext_vector_type(4)));
@@ -547,15 +548,16 @@ __global__ __launch_bounds__(256, 2) void cache4_rows_kernel(dav2_attention_cach
 // 8-11 of a chunk, then 4-7 and 12-15, which are what a lane holds scores of.
 // A weight is one binary16 number for bf16, whose rounding of the output hides
 // 2^-12. For f16 it added as much error as that rounding does (2.7e-4 of the
-// output against 64 bits, where a 32-bit softmax has 2.1e-4): two parts, cut
-// rather than rounded, 2^-20 of a weight and 2^-38 of the largest at most. The
-// rest needs no factor as in for_second: it loses what a single part loses.
+// output against 64 bits, where a 32-bit softmax has 2.1e-4): two parts, 2^-22 of
+// a weight and 2^-38 of the largest at most. The rest needs no factor as in
+// for_second: it loses what a single part loses.
 //
-// Bound by vector units (53 % busy), LDS (39 %; 24 of a wave's 56 reads of a tile
-// are scales) and matrix cores (34 %), partly beside one another: 2 prompts of
-// 2048 tokens at the end of 8192, 32 heads of 8, 128 features (316 GFLOP), bf16
-// 561 us, 563 TFLOP/s; f16, with half as many products again, 658. One part for
-// f16: 566, 1125 with a scale read for each score, 723 with 64 rows a wave.
+// Bound by vector units and matrix cores, partly beside one another, and by the
+// clock that falls under both: 2 prompts of 2048 tokens at the end of 8192, 32
+// heads of 8, 128 features (316 GFLOP), bf16 561 us, 563 TFLOP/s (vector units 53 %
+// busy, LDS 39 %, of whose 56 reads of a wave and tile 24 are scales, matrix cores
+// 34 %); f16, with half as many products again, 641. With one part for f16: 566,
+// 1125 with a scale read for each score, 723 with 64 rows a wave.
 template <typename E, int D, int WAVES>
 __global__ __launch_bounds__(64 * WAVES, D <= 64 && sizeof(E) == 2 ? 3 : 2)
 void cache4_tiles_kernel(dav2_attention_cache_i4_args a, uint32_t splits, uint32_t tiles) {
@@ -867,9 +869,13 @@ void cache4_tiles_kernel(dav2_attention_cache_i4_args a, uint32_t splits, uint32
                         if (i % 2 == 0) {
                             before = w;
                         } else {
-                            const h2 hi = __builtin_bit_cast(h2, __builtin_amdgcn_cvt_pkrtz(before, w));
-                            const h2 lo = __builtin_bit_cast(h2, __builtin_amdgcn_cvt_pkrtz(before - static_cast<float>(hi[0]),
-                                                                                            w - static_cast<float>(hi[1])));
+                            const h2 hi = __builtin_convertvector((v2f{before, w}), h2);
+                            float rest0, rest1;  // w less its first part, in one operation: 641 us for 656 above
+                            asm("v_fma_mix_f32 %0, -%1, 1.0, %2 op_sel_hi:[1,0,0]" : "=v"(rest0) : "v"(hi), "v"(before));
+                            asm("v_fma_mix_f32 %0, -%1, 1.0, %2 op_sel:[1,0,0] op_sel_hi:[1,0,0]"
+                                : "=v"(rest1)
+                                : "v"(hi), "v"(w));
+                            const h2 lo = __builtin_convertvector((v2f{rest0, rest1}), h2);
                             pf[t & 1][0][to - 1] = hi[0], pf[t & 1][0][to] = hi[1];
                             pf[t & 1][1][to - 1] = lo[0], pf[t & 1][1][to] = lo[1];
                         }
@@ -967,7 +973,7 @@ bool valid(const dav2_attention_cache_i4_args& a) {
 // parts to join, so s grows as sqrt(n / 32) (128 tokens over 32768, 8 heads: 56.6;
 // sqrt(n / 64) 72.5, sqrt(n / 16) 58.9), and to one workgroup of 256 rows or two
 // of 128 a CU. 256 rows widen the keys once for twice the rows (2 of 2048 over
-// 8192 561 against 583, f16 661 / 679; 512 over 32768 334 / 361, f16 417 / 446),
+// 8192 561 against 583, f16 641 / 665; 512 over 32768 334 / 361, f16 406 / 438),
 // if the head is so wide that three waves of the smaller ones do not fit a SIMD
 // instead, if they add no rows that do not exist (2 of 577 tokens, 16 heads of 16:
 // 36.0 against 33.8), and if there are enough of them, one for each CU and two

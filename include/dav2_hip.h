@@ -695,8 +695,8 @@ DAV2_API int dav2_hip_cache_store_i4(const dav2_cache_store_i4_args* args, void*
 /* dav2_hip_attention_cache_i8 over a cache in 4 bits: its rules, limits, types,
  * hints and scratch, with scales of tokens in the place of scales of pages. A
  * token that a row does not see may have any scale, NaN included. A weight is
- * binary16 (11 bits) where a bf16 call has many rows, and two parts (20 bits and
- * more) else; with many rows of 16 bits a value's scale goes with its weight by
+ * binary16 (11 bits) where a bf16 call has many rows, and two parts (22 bits)
+ * else; with many rows of 16 bits a value's scale goes with its weight by
  * its logarithm, to 2^-20 of the weight for scales of 1e-8 to 2^32, 2^-18 for any. */
 typedef struct dav2_attention_cache_i4_args {
     dav2_cache_i4 cache;

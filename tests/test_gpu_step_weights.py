@@ -126,7 +126,7 @@ def test_scores_past_2_to_30(gpu, pkg, lib, dtype, sign, queries, sequences, mos
 @pytest.mark.parametrize("length", [40, 68, 1580])
 @pytest.mark.parametrize("d", [48, 64, 96, 128])
 def test_outputs_round_once(gpu, pkg, lib, dtype, queries, sequences, most, length, d):
-    # weights of 20 bits and more, so that the output's own rounding is what is left: rows and tiles of both heights,
+    # weights of 20 bits, so that the output's own rounding is what is left: rows and tiles of both heights,
     # the keys whole and split, scales of values far apart
     torch = gpu
     page_size, heads, kv = 32, 16, 2
@@ -143,7 +143,7 @@ def test_outputs_round_once(gpu, pkg, lib, dtype, queries, sequences, most, leng
     for h in range(heads):
         k, v = ((c[table.long(), h // 8].double() * s[table.long(), h // 8].double()[..., None]).reshape(-1, d)[:length]
                 for c, s in ((keys, ks), (values, vs)))
-        # a weight's two parts, 2^-20 of it, and its exponent with a scale's logarithm, 2^-20 at most, which is in
+        # a weight's two parts, 2^-22 of it, and its exponent with a scale's logarithm, 2^-20 at most, which is in
         # the sum of the weights too
-        want, bound = want_of(q[:, h].double(), k, v, 0.02, dtype, 2.0 ** -19, 2.0 ** -37, exponent=8.0)
+        want, bound = want_of(q[:, h].double(), k, v, 0.02, dtype, 2.0 ** -22 + 2.0 ** -20, 2.0 ** -37, exponent=8.0)
         ref.assert_within(out[:, h], want, bound + want.abs() * 2.0 ** -20)
