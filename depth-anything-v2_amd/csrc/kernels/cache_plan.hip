@@ -229,7 +229,8 @@ DAV2_DEV void plan_given(const dav2_cache_plan_args& a, const Ring& ring, const 
 
 // Both in one workgroup: the records stay in LDS, and starts beside them for the
 // search. Up to 64 sequences are one wave's, which waits for nobody. us, against two
-// launches: 48 sequences of a token each 5.6 / 9.2, 16 of 128 rows 5.1 / 9.6.
+// launches: 48 sequences of a token each 6.2 / 9.4, 16 of 128 rows 5.6 / 9.2, 128 of a
+// token 9.7 / 10.0.
 constexpr uint32_t kSmallThreads = 512;
 template <bool WAVE>
 __global__ __launch_bounds__(kSmallThreads) void plan_small_kernel(dav2_cache_plan_args a) {

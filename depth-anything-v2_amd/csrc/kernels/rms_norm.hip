@@ -3,9 +3,10 @@
 //   h = x + r in the type, f = fp32(1 / sqrt(mean h^2 + epsilon)), y = (h f) w,
 //   code = rint(y / s), s = max(absmax y / 127, 1e-8).
 //
-// The squares are summed in 64 bits, which costs nothing beside the loads: f is
-// then the same for any order of the sum, and a code next to a border does not
-// go by how many lanes share a row.
+// The squares are summed in 64 bits, which costs nothing beside the loads: orders
+// of the sum differ by some 2^-52, so that f is the same for any of them unless
+// the root lies that near to a border of fp32, one row in 2^28. A code next to a
+// border then hardly ever goes by how many lanes share a row.
 
 #include <algorithm>
 #include <type_traits>
